@@ -538,6 +538,160 @@ int pdm_cross_hash_fwd(const int64_t* const* keys, const int64_t* key_strides,
                        int32_t num_keys, int64_t n, uint64_t table_size,
                        uint64_t salt, int64_t* out, pdm_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Cached attention: queries and keys normed and rotated, keys and values
+ * appended to an 8-bit paged cache, and attention over it.  No counterpart in
+ * the reference, whose attention (primus_dlrm/models/onetrans.py:85-169)
+ * recomputes the keys and values of all tokens in every call and takes
+ * positions from an embedding added to the tokens; for serving models that
+ * keep a user's history between requests.
+ * ------------------------------------------------------------------------ */
+
+typedef struct {
+  int64_t tokens;        /* T */
+  int32_t n_q_heads;     /* 0: no q */
+  int32_t n_k_heads;     /* 0: no k */
+  int32_t head_dim;      /* D: a multiple of 16, 16..1024 */
+  int32_t rotary_dim;    /* R: a multiple of 16, 0..D; the first R elements of a head are rotated */
+  int32_t dtype;         /* PDM_F32 | PDM_F16 | PDM_BF16: q, k, outputs and their gradients */
+  int32_t position_bits; /* 32 | 64 */
+  int32_t interleaved;   /* 0: pairs (i, i + R/2); 1: pairs (2i, 2i + 1) */
+  float eps;
+  int64_t table_rows;    /* rows of cos and sin */
+  int64_t q_stride_t, q_stride_h; /* element (t, h, d) of q at q[t * q_stride_t + h * q_stride_h + d] */
+  int64_t k_stride_t, k_stride_h;
+} pdm_qk_rope_desc;
+
+/* Per (token, head): n = x * (mean(x^2) + eps)^(-1/2) * weight (n = x when the
+ * weights are NULL), then the pairs (a, b) of the first R elements become
+ * (n_a cos - n_b sin, n_b cos + n_a sin) with entry i of the token's row of
+ * cos and sin for pair i.  fp32, rounded once.
+ * positions: device [T]; cos, sin: device fp32 [table_rows, R/2]; weights:
+ *            device fp32 [D], both or neither.
+ * q_out, k_out: device, contiguous [T, heads, D].
+ * cos, sin, weights and outputs are 16-byte aligned; q and k need not be.
+ * A token with a negative position is padding: its rows are zeros.  A position
+ * >= table_rows gives zeros too and sets err_flag (optional device int32).
+ * T * heads < 2^31. */
+int pdm_qk_norm_rope_fwd(const pdm_qk_rope_desc* desc, const void* q,
+                         const void* k, const void* positions,
+                         const float* cos, const float* sin,
+                         const float* q_weight, const float* k_weight,
+                         void* q_out, void* k_out, int32_t* err_flag,
+                         pdm_stream_t stream);
+
+/* Backward of pdm_qk_norm_rope_fwd: gradients of q and k (contiguous [T,
+ * heads, D] of dtype) and of the weights (fp32 [D], each may be NULL) from
+ * contiguous grad_q_out / grad_k_out.  Rows of padding have zero gradients.
+ * q and k may be NULL when there are no weights.  Sums run in one fixed order:
+ * the same inputs give the same bits.  workspace: 16-byte aligned, the size
+ * below, no initialisation needed (unused without weights). */
+int64_t pdm_qk_norm_rope_bwd_workspace_size(const pdm_qk_rope_desc* desc);
+
+int pdm_qk_norm_rope_bwd(const pdm_qk_rope_desc* desc, const void* q,
+                         const void* k, const void* positions,
+                         const float* cos, const float* sin,
+                         const float* q_weight, const float* k_weight,
+                         const void* grad_q_out, const void* grad_k_out,
+                         void* grad_q, void* grad_k, float* grad_q_weight,
+                         float* grad_k_weight, void* workspace,
+                         int64_t workspace_bytes, pdm_stream_t stream);
+
+/* A cache of 8-bit keys and values.  Codes are OCP e4m3; value = code * scale
+ * of its (page, head), scale = 2^e with e in [-117, 119]. */
+typedef struct {
+  uint8_t* k_codes; /* device [num_pages, n_kv_heads, page_size, head_dim], 16-byte aligned */
+  uint8_t* v_codes;
+  float* k_scale;   /* device [num_pages, n_kv_heads] */
+  float* v_scale;
+  int64_t num_pages;
+  int32_t n_kv_heads;
+  int32_t page_size; /* 16, 32, 64 or 128 */
+  int32_t head_dim;  /* 64, 128 or 256 */
+  int32_t reserved;
+} pdm_kv_cache;
+
+/* The sequences of a call.  Sequence b's new tokens are rows cu_seqlens[b] ..
+ * cu_seqlens[b + 1] of the batch; it holds seq_lens[b] tokens with them, so
+ * they are its last ones; its token i lies in slot i % page_size of page
+ * page_table[b * table_stride + i / page_size].  Everything is read on the
+ * device: nothing here makes the host wait.  What does not fit (spans outside
+ * [0, tokens], more new tokens than seq_lens, a page outside [0, num_pages), a
+ * length beyond table_width pages) is left out and sets err_flag. */
+typedef struct {
+  const int32_t* cu_seqlens; /* device [num_seqs + 1] */
+  const int32_t* seq_lens;   /* device [num_seqs] */
+  const int32_t* page_table; /* device, row stride table_stride entries */
+  int64_t table_stride;
+  int64_t tokens;            /* rows of the batch (may exceed cu_seqlens[num_seqs]) */
+  int32_t num_seqs;
+  int32_t table_width;       /* entries of a row of page_table */
+} pdm_kv_batch;
+
+typedef struct {
+  int32_t dtype;         /* PDM_F32 | PDM_F16 | PDM_BF16: k and v */
+  int32_t rotary_dim;    /* as in pdm_qk_rope_desc; 0: keys are not rotated */
+  int32_t position_bits; /* 32 | 64 */
+  int32_t interleaved;
+  float eps;
+  int32_t reserved;
+  int64_t table_rows;
+  int64_t k_stride_t, k_stride_h;
+  int64_t v_stride_t, v_stride_h;
+} pdm_kv_append_desc;
+
+/* Writes the batch's new keys and values into their pages; the keys are normed
+ * (k_weight not NULL) and rotated (rotary_dim > 0) first as in
+ * pdm_qk_norm_rope_fwd, by positions[row] or, when positions is NULL, by the
+ * token's index in its sequence (a position outside the tables: a zero key,
+ * and err_flag).
+ * Of the new values x on a page (keys and values apart, each head by itself),
+ * e is the smallest exponent with max |x| <= 448 * 2^e; where the page already
+ * holds tokens of the sequence, e is not below the page's own, and their codes
+ * are brought to the new scale.  code = e4m3(x * 2^-e), nearest even,
+ * saturating; NaN and infinities become NaN and do not count for the maximum.
+ * Only the new tokens' slots, and the codes before them on a page whose scale
+ * grows, are written.  A page that a call writes must belong to one sequence
+ * of the call; appending the same tokens again leaves the same cache. */
+int pdm_kv_append(const pdm_kv_append_desc* desc, const pdm_kv_cache* cache,
+                  const pdm_kv_batch* batch, const void* k, const void* v,
+                  const void* positions, const float* cos, const float* sin,
+                  const float* k_weight, int32_t* err_flag,
+                  pdm_stream_t stream);
+
+typedef struct {
+  int32_t dtype;      /* PDM_F16 | PDM_BF16: q and out */
+  int32_t n_q_heads;  /* a multiple of n_kv_heads: query head h reads key head h / (n_q_heads / n_kv_heads) */
+  int32_t causal;     /* 1: a query sees keys up to its own token */
+  int32_t window;     /* w > 0: and none of w or more tokens before it; 0: no window */
+  float scale;        /* of the scores */
+  int32_t max_q_len;  /* no sequence has more new tokens (one that has is left out) */
+  int64_t q_stride_t, q_stride_h;
+} pdm_kv_attention_desc;
+
+/* Attention of the batch's new tokens over the cache, their own keys and values
+ * included (append first).  Row i of sequence b's n new tokens is its token p =
+ * seq_lens[b] - n + i and sees the keys j with j < seq_lens[b], j <= p (causal)
+ * and j > p - window (window > 0):
+ *   out = sum_j softmax_j(scale * q . k_j) v_j,  lse = log sum_j exp(scale * q . k_j)
+ * Scores, softmax and sums are fp32 (the products take bf16 or f16 operands:
+ * codes are exact in both; weights are rounded to bf16).  A row that sees no
+ * key, a row left out and a row behind the last sequence is zeros, lse -inf.
+ * Keys that a row does not see do not reach it, whatever they hold.
+ * out: device, contiguous [tokens, n_q_heads, D] of dtype, 16-byte aligned;
+ * lse: optional device fp32 [tokens, n_q_heads].  workspace: 256-byte aligned,
+ * the size below (it depends on sizes alone), no initialisation needed; calls
+ * that share one must not overlap. */
+int64_t pdm_kv_attention_workspace_size(const pdm_kv_attention_desc* desc,
+                                        const pdm_kv_cache* cache,
+                                        const pdm_kv_batch* batch);
+
+int pdm_kv_attention_fwd(const pdm_kv_attention_desc* desc,
+                         const pdm_kv_cache* cache, const pdm_kv_batch* batch,
+                         const void* q, void* out, float* lse, void* workspace,
+                         int64_t workspace_bytes, int32_t* err_flag,
+                         pdm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -2,8 +2,10 @@
 
 Drop-ins for the reference's TorchRec EmbeddingBagCollection /
 EmbeddingCollection lookups, the OneTrans S-token build, the OneTrans
-block and the cross-feature id hashing, running hand-written HIP kernels
-through the C ABI of libpdm.so.
+block and the cross-feature id hashing, and cached attention for serving
+(query / key norms with rotation, an 8-bit paged key-value cache and the
+attention over it), running hand-written HIP kernels through the C ABI of
+libpdm.so.
 """
 from . import _lib
 from .embedding import (DataType, EmbeddingBagCollection, EmbeddingBagConfig, EmbeddingCollection,
@@ -11,6 +13,7 @@ from .embedding import (DataType, EmbeddingBagCollection, EmbeddingBagConfig, Em
 from .kjt import JaggedTensor, KeyedJaggedTensor, KeyedTensor
 from .onetrans import (AutoSplitTokenizer, FusedNSTokenizer, FusedSequenceTokenizer, MixedAttention, MixedFFN, OneTransBlock, OneTransStack, RMSNorm,
                        SequentialTokenizer, build_pyramid_mask, pyramid_schedule)
+from .kv_cache import PagedKVCache, QKNormRope, kv_append, kv_attention, qk_norm_rope, rotary_tables
 from . import ops
 from . import hashing
 from . import synthetic
@@ -22,5 +25,6 @@ __all__ = [
     "KeyedJaggedTensor", "KeyedTensor", "MixedAttention", "MixedFFN", "OneTransBlock", "OneTransStack",
     "SequentialTokenizer", "FusedSequenceTokenizer", "AutoSplitTokenizer", "FusedNSTokenizer",
     "RMSNorm", "build_pyramid_mask", "pyramid_schedule", "ops", "hashing", "EmbOptimType",
-    "FusedEmbeddingOptimizer", "RowWiseAdagrad", "WeightDecayMode",
+    "FusedEmbeddingOptimizer", "RowWiseAdagrad", "WeightDecayMode", "PagedKVCache", "QKNormRope", "kv_append",
+    "kv_attention", "qk_norm_rope", "rotary_tables",
 ]

@@ -64,6 +64,12 @@ EXPORTED_SYMBOLS = (
     "pdm_onetrans_block_fwd",
     "pdm_onetrans_stack_workspace_size",
     "pdm_onetrans_stack_fwd",
+    "pdm_qk_norm_rope_fwd",
+    "pdm_qk_norm_rope_bwd_workspace_size",
+    "pdm_qk_norm_rope_bwd",
+    "pdm_kv_append",
+    "pdm_kv_attention_workspace_size",
+    "pdm_kv_attention_fwd",
 )
 
 
@@ -174,6 +180,83 @@ class BlockWeights(ctypes.Structure):
     ]
 
 
+class QkRopeDesc(ctypes.Structure):
+    """pdm_qk_rope_desc: the heads, types and strides of a norm + rotation."""
+    _fields_ = [
+        ("tokens", ctypes.c_int64),
+        ("n_q_heads", ctypes.c_int32),
+        ("n_k_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("position_bits", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("table_rows", ctypes.c_int64),
+        ("q_stride_t", ctypes.c_int64),
+        ("q_stride_h", ctypes.c_int64),
+        ("k_stride_t", ctypes.c_int64),
+        ("k_stride_h", ctypes.c_int64),
+    ]
+
+
+class KvCacheDesc(ctypes.Structure):
+    """pdm_kv_cache: the pages of an 8-bit cache."""
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p),
+        ("v_codes", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int64),
+        ("n_kv_heads", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class KvBatchDesc(ctypes.Structure):
+    """pdm_kv_batch: the sequences of a call."""
+    _fields_ = [
+        ("cu_seqlens", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("num_seqs", ctypes.c_int32),
+        ("table_width", ctypes.c_int32),
+    ]
+
+
+class KvAppendDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("position_bits", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("table_rows", ctypes.c_int64),
+        ("k_stride_t", ctypes.c_int64),
+        ("k_stride_h", ctypes.c_int64),
+        ("v_stride_t", ctypes.c_int64),
+        ("v_stride_h", ctypes.c_int64),
+    ]
+
+
+class KvAttentionDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("n_q_heads", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("max_q_len", ctypes.c_int32),
+        ("q_stride_t", ctypes.c_int64),
+        ("q_stride_h", ctypes.c_int64),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -247,6 +330,21 @@ def _declare(lib: ctypes.CDLL) -> None:
                                                vp, vp]
     lib.pdm_kjt_permute.restype = ctypes.c_int
     lib.pdm_kjt_permute.argtypes = [vp, i32, vp, i32, i64, ctypes.POINTER(i32), i32, vp, vp, vp, vp, i64, vp]
+    lib.pdm_qk_norm_rope_fwd.restype = ctypes.c_int
+    lib.pdm_qk_norm_rope_fwd.argtypes = [ctypes.POINTER(QkRopeDesc)] + [vp] * 11
+    lib.pdm_qk_norm_rope_bwd_workspace_size.restype = i64
+    lib.pdm_qk_norm_rope_bwd_workspace_size.argtypes = [ctypes.POINTER(QkRopeDesc)]
+    lib.pdm_qk_norm_rope_bwd.restype = ctypes.c_int
+    lib.pdm_qk_norm_rope_bwd.argtypes = [ctypes.POINTER(QkRopeDesc)] + [vp] * 14 + [i64, vp]
+    lib.pdm_kv_append.restype = ctypes.c_int
+    lib.pdm_kv_append.argtypes = [ctypes.POINTER(KvAppendDesc), ctypes.POINTER(KvCacheDesc),
+                                  ctypes.POINTER(KvBatchDesc)] + [vp] * 8
+    lib.pdm_kv_attention_workspace_size.restype = i64
+    lib.pdm_kv_attention_workspace_size.argtypes = [ctypes.POINTER(KvAttentionDesc), ctypes.POINTER(KvCacheDesc),
+                                                    ctypes.POINTER(KvBatchDesc)]
+    lib.pdm_kv_attention_fwd.restype = ctypes.c_int
+    lib.pdm_kv_attention_fwd.argtypes = [ctypes.POINTER(KvAttentionDesc), ctypes.POINTER(KvCacheDesc),
+                                         ctypes.POINTER(KvBatchDesc), vp, vp, vp, vp, i64, vp, vp]
     lib.pdm_cross_hash_fwd.restype = ctypes.c_int
     lib.pdm_cross_hash_fwd.argtypes = [ctypes.POINTER(vp), ctypes.POINTER(i64), i32, i64, ctypes.c_uint64,
                                        ctypes.c_uint64, vp, vp]

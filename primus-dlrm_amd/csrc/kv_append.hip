@@ -1,0 +1,278 @@
+// New keys and values into the pages of an 8-bit cache, keys normed and rotated on the way.
+//
+// Codes are e4m3, [pages][heads][page_size][D] for keys and for values, with one fp32 scale 2^e per (page,
+// head).  Of the values x that a call puts on a page, e is the smallest exponent with max|x| <= 448 * 2^e,
+// and at least the page's exponent where the page already holds tokens of the sequence; those are then
+// brought to the new scale.  Powers of two cost a floating-point code no precision: code = rne(x * 2^-e) has
+// the relative error it would have under any scale, and a rescaled code is exact until it becomes subnormal,
+// so a page filled token by token ends up as one filled at once, but for values 2^-14 below its largest.
+//
+// Bound by HBM (2 bytes read and 1 written per bf16 element) for prompts, by latency for single tokens.
+#include "kv_common.h"
+
+namespace pdm {
+namespace {
+
+struct AppendArgs {
+  const void* x[2];           // new keys, new values: element (t, h, d) at t * stride_t + h * stride_h + d
+  int64_t stride_t[2], stride_h[2];
+  uint8_t* codes[2];
+  float* scale[2];
+  const int32_t *cu, *table, *lens;
+  const void* positions;      // null: the token's index in its sequence
+  const float *cos, *sin, *w;
+  int32_t* err;
+  int64_t tokens, table_stride, table_rows, num_pages;
+  int32_t seqs, heads, D, R, page_log2, table_width, bits, width_log2;
+  float eps;
+};
+
+// Where one page's share of a call's tokens lies.
+struct Segment {
+  int64_t row0;     // token row of its first token
+  int64_t index0;   // that token's index in the sequence
+  int64_t page_id;
+  int slot0, n;     // first slot and number of tokens
+};
+
+// Item i of the list of (sequence, touched page): sequence b's span begins at cu[b] / page + 2 b and is never
+// shorter than the pages it touches, (n_b - 2) / page + 2 at most, so the list needs no prefix sum.
+__device__ __forceinline__ bool find_segment(const AppendArgs& a, int64_t item, Segment& g) {
+  const int lg = a.page_log2;
+  const int b = find_sequence(a.seqs, item, [&](int i) { return ((int64_t)a.cu[i] >> lg) + 2 * (int64_t)i; });
+  const int64_t c0 = a.cu[b], c1 = a.cu[b + 1], len = a.lens[b];
+  const int64_t n = c1 - c0;
+  const int64_t j = item - ((c0 >> lg) + 2 * (int64_t)b);
+  if (j < 0 || n <= 0) {
+    if (n < 0 && a.err) *a.err = 1;
+    return false;
+  }
+  if (c0 < 0 || c1 > a.tokens || n > len) {
+    if (a.err) *a.err = 1;
+    return false;
+  }
+  const int64_t start = len - n;
+  const int64_t page = (start >> lg) + j;
+  if (page > (len - 1) >> lg) return false;
+  if (page >= a.table_width) {
+    if (a.err) *a.err = 1;
+    return false;
+  }
+  const int64_t id = a.table[(int64_t)b * a.table_stride + page];
+  if (id < 0 || id >= a.num_pages) {
+    if (a.err) *a.err = 1;
+    return false;
+  }
+  const int64_t lo = start > (page << lg) ? start : page << lg;
+  const int64_t hi = len < ((page + 1) << lg) ? len : (page + 1) << lg;
+  g.row0 = c0 + (lo - start);
+  g.index0 = lo;
+  g.page_id = id;
+  g.slot0 = (int)(lo - (page << lg));
+  g.n = (int)(hi - lo);
+  return true;
+}
+
+// One (page, head, keys or values) per W waves, NI rows of a page per lane group: the values stay in
+// registers between the maximum and the codes.
+template <int DT, bool NORM, bool INTER, bool VEC, int W, int NI>
+__global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a, int64_t items) {
+  __shared__ float red[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int parts = 2 * a.heads;
+  // work list: items x heads x {keys, values}
+  const int64_t unit = (linear_block() * 4 + wave) / W;
+  const int64_t item = unit / parts;
+  if (item >= items) return;  // W == 4: the same for the whole block
+  const int part = (int)(unit - item * parts);
+  const int kv = part >= a.heads, h = kv ? part - a.heads : part;
+  Segment g;
+  if (!find_segment(a, item, g)) return;
+
+  const int width = 1 << a.width_log2;
+  const int j = lane & (width - 1);
+  const int per_wave = 64 >> a.width_log2;
+  const int group = (W == 4 ? wave * per_wave : 0) + (lane >> a.width_log2);
+  const int groups = W * per_wave;
+  const int R = kv ? 0 : a.R;
+  const RowPlace pl = row_place<INTER>(j, a.D, R);
+  float v[NI][16];
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int r = group + i * groups;
+    if (r < g.n) {
+      const int64_t at = (g.row0 + r) * a.stride_t[kv] + h * a.stride_h[kv];
+      load8<DT, VEC>(a.x[kv], at + pl.lo, v[i]);
+      load8<DT, VEC>(a.x[kv], at + pl.hi, v[i] + 8);
+    }
+  }
+  if (!kv) {
+    float w[16];
+    if (NORM) {
+      load8f(a.w + pl.lo, w);
+      load8f(a.w + pl.hi, w + 8);
+    }
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = group + i * groups;
+      const bool ok = r < g.n;
+      if (NORM) {
+        float ss = 0.0f;
+        if (ok) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) ss = __builtin_fmaf(v[i][e], v[i][e], ss);
+        }
+        ss = group_sum(ss, width);
+        if (ok) {
+          const float rs = 1.0f / sqrtf(ss / (float)a.D + a.eps);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[i][e] = v[i][e] * rs * w[e];
+        }
+      }
+      if (ok && pl.turned) {
+        const int64_t p = a.positions ? load_position(a.positions, a.bits, g.row0 + r) : g.index0 + r;
+        if (p < 0 || p >= a.table_rows) {
+          if (a.err) *a.err = 1;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[i][e] = 0.0f;
+        } else {
+          float c[8], s[8];
+          load8f(a.cos + p * (R / 2) + 8 * j, c);
+          load8f(a.sin + p * (R / 2) + 8 * j, s);
+          rotate16<INTER>(v[i], c, s);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    if (group + i * groups < g.n) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float m = fabsf(v[i][e]);
+        amax = fmaxf(amax, m < __builtin_inff() ? m : 0.0f);
+      }
+    }
+  }
+  amax = group_max(amax, 64);
+  if (W == 4) {
+    if (lane == 0) red[wave] = amax;
+    __syncthreads();
+    amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  }
+  int e = scale_exponent(amax);
+  const int64_t entry = g.page_id * a.heads + h;
+  uint8_t* page = a.codes[kv] + ((entry << a.page_log2) * a.D);
+  float* scale = a.scale[kv] + entry;
+  if (g.slot0 > 0) {
+    const int held = scale_exponent_of(*scale);
+    if (W == 4) __syncthreads();  // every wave has read the old scale
+    if (e > held) {
+      // codes of the tokens already there, 16 at a time
+      const float f = exp2_int(held - e > -126 ? held - e : -126);
+      const int n16 = g.slot0 * a.D / 16;
+      for (int i = (W == 4 ? threadIdx.x : lane); i < n16; i += 64 * W) {
+        u32x4_t* p = reinterpret_cast<u32x4_t*>(page) + i;
+        u32x4_t c = *p;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[d], false);
+          const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[d], true);
+          const float x[4] = {lo[0] * f, lo[1] * f, hi[0] * f, hi[1] * f};
+          c[d] = e4m3x4(x);
+        }
+        *p = c;
+      }
+    } else {
+      e = held;
+    }
+  }
+  if (lane == 0 && (W == 1 || wave == 0)) *scale = exp2_int(e);
+  const float inv = exp2_int(-e);
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int r = group + i * groups;
+    if (r < g.n) {
+#pragma unroll
+      for (int d = 0; d < 16; ++d) v[i][d] *= inv;
+      uint8_t* row = page + (int64_t)(g.slot0 + r) * a.D;
+      *reinterpret_cast<u32x2_t*>(row + pl.lo) = u32x2_t{e4m3x4(v[i]), e4m3x4(v[i] + 4)};
+      *reinterpret_cast<u32x2_t*>(row + pl.hi) = u32x2_t{e4m3x4(v[i] + 8), e4m3x4(v[i] + 12)};
+    }
+  }
+}
+
+template <int DT, bool NORM, bool INTER, bool VEC>
+int launch(const AppendArgs& a, hipStream_t st) {
+  const int64_t items = (a.tokens >> a.page_log2) + 2 * (int64_t)a.seqs;
+  const int64_t units = items * 2 * a.heads;
+  // rows of a page per wave-wide step; more than 4 of them take the four waves of a block
+  const int steps = (1 << a.page_log2) * (1 << a.width_log2) / 64;
+  const dim3 g1 = linear_grid((units + 3) / 4), g4 = linear_grid(units);
+  if (steps <= 1) kv_append_kernel<DT, NORM, INTER, VEC, 1, 1><<<g1, 256, 0, st>>>(a, items);
+  else if (steps == 2) kv_append_kernel<DT, NORM, INTER, VEC, 1, 2><<<g1, 256, 0, st>>>(a, items);
+  else if (steps == 4) kv_append_kernel<DT, NORM, INTER, VEC, 1, 4><<<g1, 256, 0, st>>>(a, items);
+  else if (steps == 8) kv_append_kernel<DT, NORM, INTER, VEC, 4, 2><<<g4, 256, 0, st>>>(a, items);
+  else if (steps == 16) kv_append_kernel<DT, NORM, INTER, VEC, 4, 4><<<g4, 256, 0, st>>>(a, items);
+  else kv_append_kernel<DT, NORM, INTER, VEC, 4, 8><<<g4, 256, 0, st>>>(a, items);
+  PDM_CHECK_LAUNCH();
+  return PDM_OK;
+}
+
+template <int DT, bool NORM>
+int launch2(bool inter, bool vec, const AppendArgs& a, hipStream_t st) {
+  if (inter) return vec ? launch<DT, NORM, true, true>(a, st) : launch<DT, NORM, true, false>(a, st);
+  return vec ? launch<DT, NORM, false, true>(a, st) : launch<DT, NORM, false, false>(a, st);
+}
+
+template <int DT>
+int launch1(bool norm, bool inter, bool vec, const AppendArgs& a, hipStream_t st) {
+  return norm ? launch2<DT, true>(inter, vec, a, st) : launch2<DT, false>(inter, vec, a, st);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+}  // namespace pdm
+
+using namespace pdm;
+
+extern "C" int pdm_kv_append(const pdm_kv_append_desc* d, const pdm_kv_cache* cache, const pdm_kv_batch* batch,
+                             const void* k, const void* v, const void* positions, const float* cos, const float* sin,
+                             const float* k_weight, int32_t* err_flag, pdm_stream_t stream) {
+  clear_error();
+  PDM_CHECK_ARG(d && cache && batch, "null descriptor");
+  if (int e = check_cache(__func__, cache, batch)) return e;
+  PDM_CHECK_ARG(d->dtype == PDM_F32 || d->dtype == PDM_F16 || d->dtype == PDM_BF16, "dtype must be F32, F16 or BF16");
+  PDM_CHECK_ARG(d->rotary_dim >= 0 && d->rotary_dim <= cache->head_dim && d->rotary_dim % 16 == 0,
+                "rotary_dim must be a multiple of 16 in [0, head_dim]");
+  PDM_CHECK_ARG(d->position_bits == 32 || d->position_bits == 64, "position_bits must be 32 or 64");
+  PDM_CHECK_ARG(d->table_rows >= 0 && d->eps >= 0, "negative table_rows or eps");
+  if (batch->tokens == 0 || batch->num_seqs == 0) return PDM_OK;
+  PDM_CHECK_ARG(k && v, "null k / v");
+  PDM_CHECK_ARG(!d->rotary_dim || (cos && sin), "null cos / sin");
+  PDM_CHECK_ARG(aligned16(cos) && aligned16(sin) && aligned16(k_weight), "cos, sin and weight must be 16-byte aligned");
+  const int64_t unit = d->dtype == PDM_F32 ? 4 : 8;
+  const bool vec = aligned16(k) && aligned16(v) && d->k_stride_t % unit == 0 && d->k_stride_h % unit == 0 &&
+                   d->v_stride_t % unit == 0 && d->v_stride_h % unit == 0;
+  AppendArgs a{};
+  a.x[0] = k, a.x[1] = v;
+  a.stride_t[0] = d->k_stride_t, a.stride_t[1] = d->v_stride_t;
+  a.stride_h[0] = d->k_stride_h, a.stride_h[1] = d->v_stride_h;
+  a.codes[0] = cache->k_codes, a.codes[1] = cache->v_codes;
+  a.scale[0] = cache->k_scale, a.scale[1] = cache->v_scale;
+  a.cu = batch->cu_seqlens, a.table = batch->page_table, a.lens = batch->seq_lens;
+  a.positions = positions;
+  a.cos = cos, a.sin = sin, a.w = k_weight, a.err = err_flag;
+  a.tokens = batch->tokens, a.table_stride = batch->table_stride, a.table_rows = d->table_rows;
+  a.num_pages = cache->num_pages;
+  a.seqs = batch->num_seqs, a.heads = cache->n_kv_heads, a.D = cache->head_dim, a.R = d->rotary_dim;
+  a.page_log2 = log2_of(cache->page_size), a.table_width = batch->table_width, a.bits = d->position_bits;
+  a.width_log2 = log2_of(cache->head_dim / 16);
+  a.eps = d->eps;
+  const bool norm = k_weight != nullptr, inter = d->interleaved != 0;
+  if (d->dtype == PDM_F32) return launch1<PDM_F32>(norm, inter, vec, a, stream);
+  if (d->dtype == PDM_F16) return launch1<PDM_F16>(norm, inter, vec, a, stream);
+  return launch1<PDM_BF16>(norm, inter, vec, a, stream);
+}

@@ -14,8 +14,10 @@ There is no CPU implementation: called with CPU tensors these ops raise.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import itertools
+import math
 import threading
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -852,3 +854,349 @@ def cross_hash_fwd(keys: List[torch.Tensor], table_size: int, salt: int) -> torc
 def _(keys, table_size, salt):
     n = max(k.numel() for k in keys)
     return keys[0].new_empty(n, dtype=torch.int64)
+
+
+# ---------------------------------------------------------------------------
+# Cached attention: norm and rotation of queries and keys, append to an 8-bit paged cache, attention over it
+# ---------------------------------------------------------------------------
+
+def _on_device(dev: torch.device):
+    """Makes ``dev`` the current device for a launch (nothing to do when it is)."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _check_heads(name: str, t: torch.Tensor) -> None:
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"the elements of a head of {name} must be contiguous")
+    if t.dtype not in TORCH_TO_PDM:
+        raise TypeError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+
+
+def _check_err_flag(err_flag: Optional[torch.Tensor]) -> None:
+    if err_flag is not None and (err_flag.dtype != torch.int32 or err_flag.numel() < 1):
+        raise ValueError("err_flag must be an int32 tensor with at least one element")
+
+
+def _check_rotation(cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], D: int) -> Tuple[int, int]:
+    """(rotary_dim, table rows) of cos / sin [rows, rotary_dim / 2]; (0, 0) without them."""
+    if cos is None and sin is None:
+        return 0, 0
+    if cos is None or sin is None:
+        raise ValueError("cos and sin are given together")
+    if cos.dim() != 2 or cos.shape != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError("cos and sin must be contiguous [positions, rotary_dim / 2] tables of one shape")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise TypeError("cos and sin must be float32")
+    R = 2 * cos.shape[1]
+    if R % 16 or R > D:
+        raise ValueError(f"rotary_dim ({R}) must be a multiple of 16 and at most head_dim ({D})")
+    return R, cos.shape[0]
+
+
+def _check_positions(positions: torch.Tensor, tokens: int) -> None:
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
+    if tuple(positions.shape) != (tokens,) or not positions.is_contiguous():
+        raise ValueError(f"positions must be a contiguous [{tokens}] tensor, got {tuple(positions.shape)}")
+
+
+def _check_norm_weight(name: str, w: Optional[torch.Tensor], D: int) -> None:
+    if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (D,) or not w.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous float32 [{D}] tensor")
+
+
+def _aligned16(t: Optional[torch.Tensor], name: str) -> None:
+    if t is not None and t.data_ptr() % 16:
+        raise ValueError(f"{name} must be 16-byte aligned")
+
+
+def _qk_rope_desc(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved) -> "L.QkRopeDesc":
+    _check_heads("q", q)
+    T, hq, D = q.shape
+    hk, k_st, k_sh = 0, 0, 0
+    if k is not None:
+        _check_heads("k", k)
+        if k.shape[0] != T or k.shape[2] != D or k.dtype != q.dtype:
+            raise ValueError(f"k must be {q.dtype} [{T}, heads, {D}] beside q, got {k.dtype} {tuple(k.shape)}")
+        hk, k_st, k_sh = k.shape[1], k.stride(0), k.stride(1)
+    if D % 16 or not 16 <= D <= 1024:
+        raise ValueError(f"head_dim must be a multiple of 16 in [16, 1024], got {D}")
+    _check_positions(positions, T)
+    R, rows = _check_rotation(cos, sin, D)
+    _check_norm_weight("q_weight", q_weight, D)
+    _check_norm_weight("k_weight", k_weight, D)
+    if k is not None and (q_weight is None) != (k_weight is None):
+        raise ValueError("q_weight and k_weight are given together")
+    if k is None and k_weight is not None:
+        raise ValueError("k_weight without k")
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    return L.QkRopeDesc(T, hq, hk, D, R, TORCH_TO_PDM[q.dtype], 64 if positions.dtype == torch.int64 else 32,
+                        int(interleaved), eps, rows, q.stride(0), q.stride(1), k_st, k_sh)
+
+
+def qk_norm_rope_raw(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
+                     cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
+                     q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                     eps: float = 1e-6, interleaved: bool = False, err_flag: Optional[torch.Tensor] = None
+                     ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Launches pdm_qk_norm_rope_fwd on q [T, Hq, D] and k [T, Hk, D] (any token and head strides)."""
+    desc = _qk_rope_desc(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved)
+    _check_err_flag(err_flag)
+    dev = _require_cuda(q, k, positions, cos, sin, q_weight, k_weight, err_flag)
+    for n, t in (("cos", cos), ("sin", sin), ("q_weight", q_weight), ("k_weight", k_weight)):
+        _aligned16(t, n)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
+    with _on_device(dev):
+        L.check(L.lib().pdm_qk_norm_rope_fwd(
+            ctypes.byref(desc), q.data_ptr(), _ptr(k), positions.data_ptr(), _ptr(cos), _ptr(sin), _ptr(q_weight),
+            _ptr(k_weight), q_out.data_ptr(), _ptr(k_out), _ptr(err_flag), L.stream_ptr(dev)),
+            "pdm_qk_norm_rope_fwd")
+    return q_out, k_out
+
+
+def qk_norm_rope_backward_raw(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
+                              cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
+                              q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                              grad_q_out: torch.Tensor, grad_k_out: Optional[torch.Tensor], eps: float = 1e-6,
+                              interleaved: bool = False):
+    """Launches pdm_qk_norm_rope_bwd: (grad_q, grad_k, grad_q_weight, grad_k_weight), None where there is no input.
+    The output gradients are contiguous and of q's dtype."""
+    desc = _qk_rope_desc(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved)
+    for n, g, x in (("grad_q_out", grad_q_out, q), ("grad_k_out", grad_k_out, k)):
+        if (g is None) != (x is None) or (g is not None and (g.shape != x.shape or g.dtype != x.dtype
+                                                             or not g.is_contiguous())):
+            raise ValueError(f"{n} must be contiguous and of its input's shape and dtype")
+    dev = _require_cuda(q, k, positions, cos, sin, q_weight, k_weight, grad_q_out, grad_k_out)
+    for n, t in (("cos", cos), ("sin", sin), ("q_weight", q_weight), ("k_weight", k_weight)):
+        _aligned16(t, n)
+    lib = L.lib()
+    grad_q = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    grad_k = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
+    grad_qw = None if q_weight is None else torch.empty_like(q_weight)
+    grad_kw = None if k_weight is None else torch.empty_like(k_weight)
+    ws_bytes = 0
+    if q_weight is not None:
+        ws_bytes = int(lib.pdm_qk_norm_rope_bwd_workspace_size(ctypes.byref(desc)))
+        if ws_bytes < 0:
+            raise L.PdmError(ws_bytes, "pdm_qk_norm_rope_bwd_workspace_size", L.last_error())
+    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
+    with _on_device(dev):
+        L.check(lib.pdm_qk_norm_rope_bwd(
+            ctypes.byref(desc), q.data_ptr(), _ptr(k), positions.data_ptr(), _ptr(cos), _ptr(sin), _ptr(q_weight),
+            _ptr(k_weight), grad_q_out.data_ptr(), _ptr(grad_k_out), grad_q.data_ptr(), _ptr(grad_k), _ptr(grad_qw),
+            _ptr(grad_kw), ws.data_ptr(), ws_bytes, L.stream_ptr(dev)), "pdm_qk_norm_rope_bwd")
+    return grad_q, grad_k, grad_qw, grad_kw
+
+
+@torch.library.custom_op("pdm::qk_norm_rope", mutates_args=())
+def qk_norm_rope_op(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, cos: Optional[torch.Tensor],
+                    sin: Optional[torch.Tensor], q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                    eps: float, interleaved: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Without k the second output is empty."""
+    q_out, k_out = qk_norm_rope_raw(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved)
+    return q_out, q.new_empty(0) if k_out is None else k_out
+
+
+@qk_norm_rope_op.register_fake
+def _(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved):
+    return q.new_empty(q.shape), q.new_empty(0) if k is None else k.new_empty(k.shape)
+
+
+@torch.library.custom_op("pdm::qk_norm_rope_backward", mutates_args=())
+def qk_norm_rope_backward_op(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
+                             cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
+                             q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                             grad_q_out: torch.Tensor, grad_k_out: Optional[torch.Tensor], eps: float,
+                             interleaved: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients of q, k, q_weight, k_weight; empty where there is no input."""
+    grads = qk_norm_rope_backward_raw(q, k, positions, cos, sin, q_weight, k_weight, grad_q_out.contiguous(),
+                                      None if grad_k_out is None else grad_k_out.contiguous(), eps, interleaved)
+    return tuple(q.new_empty(0) if g is None else g for g in grads)
+
+
+@qk_norm_rope_backward_op.register_fake
+def _(q, k, positions, cos, sin, q_weight, k_weight, grad_q_out, grad_k_out, eps, interleaved):
+    return tuple(q.new_empty(0) if t is None else t.new_empty(t.shape) for t in (q, k, q_weight, k_weight))
+
+
+def _qk_norm_rope_setup(ctx, inputs, output):
+    q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved = inputs
+    ctx.save_for_backward(q, k, positions, cos, sin, q_weight, k_weight)
+    ctx.eps, ctx.interleaved = eps, interleaved
+
+
+def _qk_norm_rope_backward(ctx, grad_q_out, grad_k_out):
+    q, k, positions, cos, sin, q_weight, k_weight = ctx.saved_tensors
+    if grad_q_out is None:
+        grad_q_out = torch.zeros_like(q)
+    if k is None:
+        grad_k_out = None
+    elif grad_k_out is None:
+        grad_k_out = torch.zeros_like(k)
+    grads = torch.ops.pdm.qk_norm_rope_backward(q, k, positions, cos, sin, q_weight, k_weight, grad_q_out, grad_k_out,
+                                                ctx.eps, ctx.interleaved)
+    need = ctx.needs_input_grad
+    gq, gk, gqw, gkw = (g if need[i] else None for g, i in zip(grads, (0, 1, 5, 6)))
+    return gq, gk, None, None, None, gqw, gkw, None, None
+
+
+qk_norm_rope_op.register_autograd(_qk_norm_rope_backward, setup_context=_qk_norm_rope_setup)
+
+
+def _kv_cache_desc(k_codes, v_codes, k_scale, v_scale) -> "L.KvCacheDesc":
+    if k_codes.dim() != 4 or k_codes.shape != v_codes.shape:
+        raise ValueError("k_codes and v_codes must be [pages, heads, page_size, head_dim] of one shape")
+    for n, t in (("k_codes", k_codes), ("v_codes", v_codes)):
+        if t.dtype not in (torch.float8_e4m3fn, torch.uint8):
+            raise TypeError(f"{n} must be float8_e4m3fn (or its bytes as uint8), got {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"{n} must be contiguous")
+    pages, heads, page, D = k_codes.shape
+    for n, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t.dtype != torch.float32 or tuple(t.shape) != (pages, heads) or not t.is_contiguous():
+            raise ValueError(f"{n} must be a contiguous float32 [{pages}, {heads}] tensor")
+    if page not in (16, 32, 64, 128):
+        raise ValueError(f"page_size must be 16, 32, 64 or 128, got {page}")
+    if D not in (64, 128, 256):
+        raise ValueError(f"head_dim must be 64, 128 or 256, got {D}")
+    return L.KvCacheDesc(k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, heads,
+                         page, D, 0)
+
+
+def _kv_batch_desc(cu_seqlens, page_table, seq_lens, tokens: int) -> "L.KvBatchDesc":
+    for n, t in (("cu_seqlens", cu_seqlens), ("page_table", page_table), ("seq_lens", seq_lens)):
+        if t.dtype != torch.int32:
+            raise TypeError(f"{n} must be int32, got {t.dtype}")
+    if seq_lens.dim() != 1 or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens must be a contiguous [sequences] tensor")
+    B = seq_lens.shape[0]
+    if tuple(cu_seqlens.shape) != (B + 1,) or not cu_seqlens.is_contiguous():
+        raise ValueError(f"cu_seqlens must be a contiguous [{B + 1}] tensor, got {tuple(cu_seqlens.shape)}")
+    if page_table.dim() != 2 or page_table.shape[0] != B or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError(f"page_table must be [{B}, pages] with contiguous rows, got {tuple(page_table.shape)}")
+    return L.KvBatchDesc(cu_seqlens.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), page_table.stride(0),
+                         tokens, B, page_table.shape[1])
+
+
+def kv_append_raw(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
+                  k_scale: torch.Tensor, v_scale: torch.Tensor, cu_seqlens: torch.Tensor, page_table: torch.Tensor,
+                  seq_lens: torch.Tensor, positions: Optional[torch.Tensor] = None,
+                  cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+                  k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+                  err_flag: Optional[torch.Tensor] = None) -> None:
+    """Launches pdm_kv_append: the new keys and values [T, Hk, D] (any token and head strides) into the cache."""
+    cache = _kv_cache_desc(k_codes, v_codes, k_scale, v_scale)
+    _check_heads("k", k)
+    _check_heads("v", v)
+    T, hk, D = k.shape
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError(f"v must be {k.dtype} {tuple(k.shape)} as k is, got {v.dtype} {tuple(v.shape)}")
+    if hk != cache.n_kv_heads or D != cache.head_dim:
+        raise ValueError(f"k has {hk} heads of {D}, the cache {cache.n_kv_heads} of {cache.head_dim}")
+    batch = _kv_batch_desc(cu_seqlens, page_table, seq_lens, T)
+    if positions is not None:
+        _check_positions(positions, T)
+    R, rows = _check_rotation(cos, sin, D)
+    _check_norm_weight("k_weight", k_weight, D)
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    _check_err_flag(err_flag)
+    dev = _require_cuda(k, v, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, positions, cos, sin,
+                        k_weight, err_flag)
+    for n, t in (("cos", cos), ("sin", sin), ("k_weight", k_weight)):
+        _aligned16(t, n)
+    desc = L.KvAppendDesc(TORCH_TO_PDM[k.dtype], R, 32 if positions is not None and positions.dtype == torch.int32 else 64,
+                          int(interleaved), eps, 0, rows, k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+    with _on_device(dev):
+        L.check(L.lib().pdm_kv_append(
+            ctypes.byref(desc), ctypes.byref(cache), ctypes.byref(batch), k.data_ptr(), v.data_ptr(), _ptr(positions),
+            _ptr(cos), _ptr(sin), _ptr(k_weight), _ptr(err_flag), L.stream_ptr(dev)), "pdm_kv_append")
+
+
+@torch.library.custom_op("pdm::kv_append", mutates_args=("k_codes", "v_codes", "k_scale", "v_scale", "err_flag"))
+def kv_append_op(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
+                 k_scale: torch.Tensor, v_scale: torch.Tensor, cu_seqlens: torch.Tensor, page_table: torch.Tensor,
+                 seq_lens: torch.Tensor, positions: Optional[torch.Tensor], cos: Optional[torch.Tensor],
+                 sin: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float, interleaved: bool,
+                 err_flag: Optional[torch.Tensor]) -> None:
+    kv_append_raw(k, v, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, positions, cos, sin,
+                  k_weight, eps, interleaved, err_flag)
+
+
+@kv_append_op.register_fake
+def _(k, v, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, positions, cos, sin, k_weight, eps,
+      interleaved, err_flag):
+    return None
+
+
+def kv_attention_raw(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor,
+                     v_scale: torch.Tensor, cu_seqlens: torch.Tensor, page_table: torch.Tensor,
+                     seq_lens: torch.Tensor, scale: Optional[float] = None, causal: bool = True, window: int = 0,
+                     max_q_len: Optional[int] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None,
+                     err_flag: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Launches pdm_kv_attention_fwd on q [T, Hq, D]; returns (out, lse or None).  ``max_q_len``: no sequence has more
+    new tokens (default: T, which costs a second launch and idle blocks)."""
+    cache = _kv_cache_desc(k_codes, v_codes, k_scale, v_scale)
+    _check_heads("q", q)
+    T, hq, D = q.shape
+    if q.dtype == torch.float32:
+        raise TypeError("q must be float16 or bfloat16")
+    if D != cache.head_dim or hq == 0 or hq % cache.n_kv_heads:
+        raise ValueError(f"q has {hq} heads of {D}, the cache {cache.n_kv_heads} of {cache.head_dim}: the head_dims must "
+                         "be equal and the query heads a multiple of the cache's")
+    batch = _kv_batch_desc(cu_seqlens, page_table, seq_lens, T)
+    if scale is None:
+        scale = D ** -0.5
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    if not 0 <= window < 2 ** 31:
+        raise ValueError(f"window must lie in [0, 2^31), got {window}")
+    if max_q_len is None:
+        max_q_len = T
+    elif max_q_len < 0:
+        raise ValueError("max_q_len must not be negative")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
+        raise ValueError("out must be contiguous and of q's shape and dtype")
+    _check_err_flag(err_flag)
+    dev = _require_cuda(q, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, out, err_flag)
+    if out is None:
+        out = torch.empty((T, hq, D), dtype=q.dtype, device=dev)
+    else:
+        _aligned16(out, "out")
+    lse = torch.empty((T, hq), dtype=torch.float32, device=dev) if return_lse else None
+    desc = L.KvAttentionDesc(TORCH_TO_PDM[q.dtype], hq, int(causal), window, scale, min(max_q_len, T), q.stride(0),
+                             q.stride(1))
+    lib = L.lib()
+    ws_bytes = int(lib.pdm_kv_attention_workspace_size(ctypes.byref(desc), ctypes.byref(cache), ctypes.byref(batch)))
+    if ws_bytes < 0:
+        raise L.PdmError(ws_bytes, "pdm_kv_attention_workspace_size", L.last_error())
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    with _on_device(dev):
+        L.check(lib.pdm_kv_attention_fwd(
+            ctypes.byref(desc), ctypes.byref(cache), ctypes.byref(batch), q.data_ptr(), out.data_ptr(), _ptr(lse),
+            _ptr(ws), ws_bytes, _ptr(err_flag), L.stream_ptr(dev)), "pdm_kv_attention_fwd")
+    return out, lse
+
+
+@torch.library.custom_op("pdm::kv_attention", mutates_args=("err_flag",))
+def kv_attention_op(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor,
+                    v_scale: torch.Tensor, cu_seqlens: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                    scale: float, causal: bool, window: int, max_q_len: int, return_lse: bool,
+                    err_flag: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Without ``return_lse`` the second output is empty."""
+    out, lse = kv_attention_raw(q, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, scale, causal,
+                                window, max_q_len, return_lse, None, err_flag)
+    return out, q.new_empty(0, dtype=torch.float32) if lse is None else lse
+
+
+@kv_attention_op.register_fake
+def _(q, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, scale, causal, window, max_q_len,
+      return_lse, err_flag):
+    return (q.new_empty(q.shape),
+            q.new_empty(q.shape[:2] if return_lse else (0,), dtype=torch.float32))
