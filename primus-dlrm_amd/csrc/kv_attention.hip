@@ -10,6 +10,8 @@
 // page's scale is a factor of the scores in fp32, values are converted with their power-of-two scale, which bf16
 // holds exactly.  Weights are rounded to bf16 (half a step is 2^-8 of a weight, against 2^-4 of an 8-bit value);
 // the running sum takes them before that.
+#include <type_traits>
+
 #include "kv_common.h"
 
 namespace pdm {
@@ -486,103 +488,480 @@ __global__ void __launch_bounds__(256) kv_attn_few_kernel(AttnArgs a, int64_t un
   }
 }
 
-// Joins the splits of a (sequence, key head): one wave per row.
+// Joins the `used` partial results of one row, `step` rows apart from `first`; one wave.
 template <int DT, int D>
-__global__ void __launch_bounds__(256) kv_attn_join_kernel(AttnArgs a, int64_t units, int unit_keys) {
+__device__ __forceinline__ void join_row(const AttnArgs& a, int64_t first, int64_t step, int used, int64_t at) {
   constexpr int E = D / 64;
-  const int64_t x = linear_block() * 4 + (threadIdx.x >> 6);
-  if (x >= units) return;
   const int lane = threadIdx.x & 63;
-  const int row = (int)(x % a.row_stride);
-  const int64_t bh = x / a.row_stride;
-  const int kh = (int)(bh % a.hk), b = (int)(bh / a.hk);
-  Seq sq;
-  if (!seq_of(a, b, sq)) return;
-  const int rows = sq.n * a.group;
-  if (rows > a.few_rows || row >= rows) return;
-  const int size = split_size(sq.hi - sq.lo, a.splits, unit_keys);
-  const int used = sq.hi > sq.lo ? (sq.hi - sq.lo + size - 1) / size : 1;
-  if (used == 1) return;
   float top = -kInf;
-  for (int s = lane; s < used; s += 64) top = fmaxf(top, a.part_ml[2 * ((bh * a.splits + s) * a.row_stride + row)]);
+  for (int s = lane; s < used; s += 64) top = fmaxf(top, a.part_ml[2 * (first + s * step)]);
   top = group_max(top, 64);
   float sum = 0.0f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.0f;
 #pragma unroll 4
   for (int s = 0; s < used; ++s) {
-    const int64_t at = (bh * a.splits + s) * a.row_stride + row;
-    const float m = a.part_ml[2 * at], l = a.part_ml[2 * at + 1];
+    const int64_t pr = first + s * step;
+    const float m = a.part_ml[2 * pr], l = a.part_ml[2 * pr + 1];
     const float f = m == -kInf ? (l != l ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(m - top);
     sum += l * f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += a.part_o[at * D + lane * E + e] * f;
+    for (int e = 0; e < E; ++e) acc[e] += a.part_o[pr * D + lane * E + e] * f;
   }
-  const int i = row / a.group, h = kh * a.group + (row - i * a.group);
-  const int64_t at = (sq.row0 + i) * a.hq + h;
 #pragma unroll
   for (int e = 0; e < E; ++e) store_out(a, DT, at * D + lane * E + e, sum != 0.0f ? acc[e] / sum : 0.0f);
   if (lane == 0 && a.lse) a.lse[at] = sum != 0.0f ? (top + __builtin_amdgcn_logf(sum)) * kLn2 : -kInf;
 }
 
-// Rows of sequences with more than few_rows: one wave per (row, head).
-__device__ __forceinline__ float e4m3_to_f32(uint32_t c) { return __builtin_amdgcn_cvt_f32_fp8((int)c, 0); }
-
+// Joins the splits of the few-rows kernel: one wave per row.
 template <int DT, int D>
-__global__ void __launch_bounds__(64) kv_attn_row_kernel(AttnArgs a) {
-  __shared__ float qs[256];
-  const int64_t unit = linear_block();
-  const int64_t t = unit / a.hq;
-  if (t >= a.tokens || a.seqs == 0) return;
-  const int h = (int)(unit - t * a.hq), kh = h / a.group;
-  const int lane = threadIdx.x;
-  const int b = find_sequence(a.seqs, t, [&](int i) { return (int64_t)a.cu[i]; });
+__global__ void __launch_bounds__(256) kv_attn_join_kernel(AttnArgs a, int64_t units) {
+  const int64_t x = linear_block() * 4 + (threadIdx.x >> 6);
+  if (x >= units) return;
+  const int row = (int)(x % a.row_stride);
+  const int64_t bh = x / a.row_stride;
+  const int kh = (int)(bh % a.hk), b = (int)(bh / a.hk);
   Seq sq;
-  if (t < a.cu[b] || t >= a.cu[b + 1] || !seq_of(a, b, sq) || sq.n * a.group <= a.few_rows) return;
-  const int p0 = sq.len - sq.n + (int)(t - sq.row0);
-  const int hi = a.causal && p0 + 1 < sq.hi ? p0 + 1 : sq.hi;
-  const int lo = a.window > 0 && p0 - a.window + 1 > 0 ? p0 - a.window + 1 : 0;
-  for (int d = lane; d < D; d += 64) {
-    const uint32_t u = static_cast<const uint16_t*>(a.q)[t * a.stride_t + h * a.stride_h + d];
-    qs[d] = DT == PDM_BF16 ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
-  }
-  __syncthreads();
-  float m = -kInf, l = 0.0f, acc[4] = {0, 0, 0, 0};
-  for (int base = lo; base < hi; base += 64) {
-    const int j = base + lane;
-    float s = -kInf;
-    int64_t row = -1;
-    float vs = 0.0f;
-    if (j < hi) {
-      const int64_t id = a.table[(int64_t)b * a.table_stride + (j >> a.page_log2)];
-      if (id < 0 || id >= a.num_pages) {
-        if (a.err) *a.err = 1;
+  if (!seq_of(a, b, sq)) return;
+  const int64_t rows = (int64_t)sq.n * a.group;
+  if (rows > a.few_rows || row >= rows) return;
+  const int size = split_size(sq.hi - sq.lo, a.splits, kFewKeys * kFewWaves);
+  const int used = sq.hi > sq.lo ? (sq.hi - sq.lo + size - 1) / size : 1;
+  if (used == 1) return;
+  const int i = row / a.group, h = kh * a.group + (row - i * a.group);
+  join_row<DT, D>(a, bh * a.splits * a.row_stride + row, a.row_stride, used, (sq.row0 + i) * a.hq + h);
+}
+
+// ---- many rows ---------------------------------------------------------------------
+// 128 rows of a (sequence, key head) against its keys, four waves of 32 rows.  Tiles of KT keys are converted once on
+// their way into LDS: K as rows, two tiles ahead of the values' use, V transposed, one tile ahead, its keys in the order in
+// which the first product leaves P.  The waves meet at one barrier per tile.  A wave computes the scores of tile t + 1
+// beside the exponentials of tile t, and a second workgroup shares the CU: the matrix unit has work while the VALU does
+// a softmax.
+constexpr int kManyRows = 128;
+
+template <int D, int KT>
+struct ManyShared {
+  static constexpr int KS = 2 * D + 16;    // bytes of a K row: 16 rows of a fragment read fall into different banks
+  static constexpr int VS = 2 * KT + 16;   // bytes of a V^T row
+  alignas(16) char k[2][KT * KS];
+  alignas(16) char v[2][D * VS];
+  float sc[4][KT / 16];                    // scale2 * scale of 16 keys; NaN where their page does not exist
+  int odd[4];                              // a wave's share of V held NaN
+};
+
+// Block `item` of the list of (sequence, 128 rows): sequence b's span begins at cu[b] * group / 128 + b.
+__device__ __forceinline__ bool many_block(const AttnArgs& a, int64_t item, Seq& sq, int& b, int& r0) {
+  b = find_sequence(a.seqs, item, [&](int i) { return (int64_t)a.cu[i] * a.group / kManyRows + i; });
+  const int64_t j = item - ((int64_t)a.cu[b] * a.group / kManyRows + b);
+  if (j < 0 || !seq_of(a, b, sq)) return false;
+  const int64_t rows = (int64_t)sq.n * a.group;
+  if (rows <= a.few_rows || j * kManyRows >= rows) return false;
+  r0 = (int)(j * kManyRows);
+  return true;
+}
+
+// The keys that rows r0 .. r0 + 127 may see: [lo, hi), lo a multiple of 32.
+__device__ __forceinline__ void many_keys(const AttnArgs& a, const Seq& sq, int r0, int& lo, int& hi) {
+  const int rows = sq.n * a.group;
+  const int i0 = r0 / a.group, i1 = ((r0 + kManyRows < rows ? r0 + kManyRows : rows) - 1) / a.group;
+  const int p0 = sq.len - sq.n + i0, p1 = sq.len - sq.n + i1;
+  hi = a.causal && p1 + 1 < sq.hi ? p1 + 1 : sq.hi;
+  lo = a.window > 0 && p0 - a.window + 1 > 0 ? (p0 - a.window + 1) & ~31 : 0;
+  if (lo > hi) lo = hi & ~31;
+}
+
+template <int DT>
+__device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+  if constexpr (DT == PDM_BF16) return mfma32x32x16(a, b, c);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+template <int DT, int D, int KT>
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(AttnArgs a, int64_t items) {
+  constexpr int KK = D / 16, DD = D / 32, XX = KT / 32;
+  constexpr int KP = KT * D / 16 / 256;    // 16-byte pieces of a K tile per thread
+  constexpr int VD = D == 64 ? 4 : 8;      // elements of a thread's 4 keys of V
+  constexpr int KS = ManyShared<D, KT>::KS, VS = ManyShared<D, KT>::VS;
+  __shared__ ManyShared<D, KT> sh;
+
+  const int64_t unit = linear_block();
+  const int split = (int)(unit % a.splits);
+  const int64_t ih = unit / a.splits;
+  const int kh = (int)(ih % a.hk);
+  const int64_t item = items - 1 - ih / a.hk;  // later rows see more keys: they begin first
+  if (item < 0) return;
+  Seq sq;
+  int b, r0;
+  if (!many_block(a, item, sq, b, r0)) return;
+  int lo, hi;
+  many_keys(a, sq, r0, lo, hi);
+  const int size = split_size(hi - lo, a.splits, KT);
+  const int begin = lo + split * size;
+  if (split > 0 && begin >= hi) return;
+  const int end = begin + size < hi ? begin + size : hi;
+  const int rows = sq.n * a.group;
+  const int tiles = end > begin ? (end - begin + KT - 1) / KT : 0;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, h = lane >> 5;
+
+  // this lane's row: its query, and the keys that it sees
+  u32x4_t q[KK];
+  int row_lo = 0x7fffffff, row_hi = 0;
+  const int row = r0 + wave * 32 + c;
+  const int tok = row / a.group, head = kh * a.group + (row - tok * a.group);
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) q[kk] = u32x4_t{0, 0, 0, 0};
+  if (row < rows) {
+    const int p = sq.len - sq.n + tok;
+    row_hi = a.causal && p + 1 < sq.hi ? p + 1 : sq.hi;
+    row_lo = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
+    const uint16_t* x = static_cast<const uint16_t*>(a.q) + (sq.row0 + tok) * a.stride_t + head * a.stride_h + 8 * h;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      if (a.vec) {
+        q[kk] = *reinterpret_cast<const u32x4_t*>(x + 16 * kk);
       } else {
-        const int64_t entry = id * a.hk + kh;
-        row = (entry << a.page_log2) + (j & ((1 << a.page_log2) - 1));
-        float dot = 0.0f;
-        const uint8_t* kp = a.k_codes + row * D;
-        for (int d = 0; d < D; ++d) dot += qs[d] * e4m3_to_f32(kp[d]);
-        s = dot * (a.k_scale[entry] * a.scale2);
-        vs = a.v_scale[entry];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[kk][e] = uint32_t(x[16 * kk + 2 * e]) | uint32_t(x[16 * kk + 2 * e + 1]) << 16;
       }
     }
-    const float mn = fmaxf(m, group_max(s, 64));
-    if (mn == -kInf && !__any(s != s)) continue;
-    const float f = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-    const float p = row >= 0 ? __builtin_amdgcn_exp2f(s - mn) : 0.0f;
-    l = l * f + group_sum(p, 64);
-    for (int i = 0; i < 4; ++i) acc[i] *= f;
-    m = mn;
-    for (int x = 0; x < 64; ++x) {
-      const int64_t r = __shfl(row, x);
-      const float px = __shfl(p, x), vx = __shfl(vs, x);
-      if (r < 0) continue;
-      for (int i = 0; i * 64 < D; ++i) acc[i] += px * (vx * e4m3_to_f32(a.v_codes[r * D + i * 64 + lane]));
+  }
+  // keys that every row of this wave sees
+  int all_lo = 0, all_hi = sq.hi;
+  {
+    const int w0 = r0 + wave * 32;
+    if (w0 < rows) {
+      const int w1 = (w0 + 32 < rows ? w0 + 32 : rows) - 1;
+      const int p0 = sq.len - sq.n + w0 / a.group, p1 = sq.len - sq.n + w1 / a.group;
+      if (a.causal && p0 + 1 < all_hi) all_hi = p0 + 1;
+      if (a.window > 0 && p1 - a.window + 1 > 0) all_lo = p1 - a.window + 1;
     }
   }
-  for (int i = 0; i * 64 < D; ++i) store_out(a, DT, (t * a.hq + h) * D + i * 64 + lane, l != 0.0f ? acc[i] / l : 0.0f);
-  if (lane == 0 && a.lse) a.lse[t * a.hq + h] = l != 0.0f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -kInf;
+
+  // ---- staging ----
+  const int32_t* table = a.table + (int64_t)b * a.table_stride;
+  const int mask = (1 << a.page_log2) - 1;
+  constexpr int PER = 1024 / KT;           // tiles of a batch of 1024 keys
+  int ids = -1;                            // lane i: page and scales of keys 16 i .. of the batch
+  float kss = 0.0f, vss = 0.0f;
+  u32x4_t kr[KP];
+  uint32_t vr[4][VD / 4];
+  int v_id = -1;                           // of the V tile that is loaded next
+  float v_sc = 0.0f, v_scale = 0.0f, sc_reg = 0.0f;
+  const int kc = (tid % (D / 16)) * 16, kr0 = tid / (D / 16);       // piece and row of K, 4096 / D rows a pass
+  const int vm = D == 256 ? wave * 8 + (lane & 7) : (wave & 1) * 8 + (lane & 7);
+  const int va = D == 256 ? lane >> 3 : (wave >> 1) * 8 + (lane >> 3);   // four keys of V
+  auto load_k = [&](int t) {
+    const int key0 = begin + t * KT;
+    if (t % PER == 0) {
+      const int key = key0 + 16 * lane;
+      ids = -1, kss = __builtin_nanf(""), vss = 0.0f;
+      if (key < end) {
+        const int id = table[key >> a.page_log2];
+        if (id >= 0 && id < a.num_pages) {
+          ids = id;
+          const int64_t entry = (int64_t)id * a.hk + kh;
+          kss = a.k_scale[entry] * a.scale2;
+          vss = a.v_scale[entry];
+        } else if (a.err) {
+          *a.err = 1;
+        }
+      }
+    }
+    const int g0 = (t % PER) * (KT / 16);
+#pragma unroll
+    for (int p = 0; p < KP; ++p) {
+      const int r = kr0 + p * (4096 / D);
+      const int grp = __builtin_amdgcn_readfirstlane(r >> 4);
+      const int id = __builtin_amdgcn_readlane(ids, g0 + grp);
+      kr[p] = u32x4_t{0, 0, 0, 0};
+      if (id >= 0) {
+        const int64_t at = (((int64_t)id * a.hk + kh) << a.page_log2) + ((key0 + 16 * grp) & mask);
+        kr[p] = *reinterpret_cast<const u32x4_t*>(a.k_codes + at * D + (r & 15) * D + kc);
+      }
+    }
+    v_id = __shfl(ids, g0 + (va >> 2));
+    v_sc = __shfl(vss, g0 + (va >> 2));
+    sc_reg = __shfl(kss, g0 + (lane & (KT / 16 - 1)));
+  };
+  auto load_v = [&](int t) {  // with the page that load_k(t) found
+    v_scale = v_sc;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int e = 0; e < VD / 4; ++e) vr[r][e] = 0;
+    if (v_id >= 0) {
+      const int64_t at = (((int64_t)v_id * a.hk + kh) << a.page_log2) + ((begin + t * KT + 16 * (va >> 2)) & mask) + (va & 3) * 4;
+      const uint8_t* p = a.v_codes + at * D + vm * VD;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (VD == 4) {
+          vr[r][0] = *reinterpret_cast<const uint32_t*>(p + r * D);
+        } else {
+          const u32x2_t w = *reinterpret_cast<const u32x2_t*>(p + r * D);
+          vr[r][0] = w[0], vr[r][1] = w[1];
+        }
+      }
+    }
+  };
+  auto stage_k = [&](int t) {
+    char* kb = sh.k[t & 1];
+#pragma unroll
+    for (int p = 0; p < KP; ++p) {
+      char* dst = kb + (kr0 + p * (4096 / D)) * KS + 2 * kc;
+      u32x4_t w0, w1;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        w0[2 * e] = code_pair<DT>(kr[p][e], false), w0[2 * e + 1] = code_pair<DT>(kr[p][e], true);
+        w1[2 * e] = code_pair<DT>(kr[p][2 + e], false), w1[2 * e + 1] = code_pair<DT>(kr[p][2 + e], true);
+      }
+      *reinterpret_cast<u32x4_t*>(dst) = w0;
+      *reinterpret_cast<u32x4_t*>(dst + 16) = w1;
+    }
+    if (wave == 0 && lane < KT / 16) sh.sc[t & 3][lane] = sc_reg;
+  };
+  // V^T of tile t; NaN codes become zeros here (0 * NaN would reach rows that do not see the key) and are remembered, or,
+  // in MARK, ones where everything else becomes zero.
+  bool odd = false;
+  auto stage_v = [&](int t, auto mark) {
+    // keys 4 va .. + 3: block va % 4 of their 16; blocks 0, 2 belong to lanes h = 0 of the product, 1, 3 to h = 1
+    const int x = va & 3;
+    char* vb = sh.v[t & 1] + 2 * (16 * (va >> 2) + 8 * (x & 1) + 4 * (x >> 1));
+    uint32_t nan = 0;
+#pragma unroll
+    for (int e = 0; e < VD / 4; ++e)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t n = nan_bytes(vr[r][e]);
+        nan |= n;
+        if constexpr (decltype(mark)::value) vr[r][e] = (n >> 7) * 0x38u;  // 0x38: the code of 1
+      }
+    if constexpr (!decltype(mark)::value) {
+      if (__any(nan != 0)) {
+        odd = true;
+#pragma unroll
+        for (int e = 0; e < VD / 4; ++e)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) vr[r][e] &= ~((nan_bytes(vr[r][e]) >> 7) * 0xffu);
+      }
+    }
+    const float f = decltype(mark)::value ? 1.0f : v_scale;
+#pragma unroll
+    for (int e = 0; e < VD / 4; ++e) {
+      const uint32_t w01[2] = {__builtin_amdgcn_perm(vr[1][e], vr[0][e], 0x05010400u), __builtin_amdgcn_perm(vr[1][e], vr[0][e], 0x07030602u)};
+      const uint32_t w23[2] = {__builtin_amdgcn_perm(vr[3][e], vr[2][e], 0x05010400u), __builtin_amdgcn_perm(vr[3][e], vr[2][e], 0x07030602u)};
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const u32x2_t w = d & 1 ? u32x2_t{value_pair_hi(w01[d >> 1], f), value_pair_hi(w23[d >> 1], f)}
+                                : u32x2_t{value_pair_lo(w01[d >> 1], f), value_pair_lo(w23[d >> 1], f)};
+        *reinterpret_cast<u32x2_t*>(vb + (vm * VD + 4 * e + d) * VS) = w;
+      }
+    }
+  };
+
+  // ---- products ----
+  float m = -kInf, l = 0.0f;
+  f32x16_t o[DD], s[XX], n[XX];
+  constexpr f32x16_t zero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+  for (int d = 0; d < DD; ++d) o[d] = zero16;
+  const uint32_t k_at = c * KS + 16 * h, v_at = c * VS + 16 * h;
+  auto scores = [&](int t) {
+    const char* kb = sh.k[t & 1] + k_at;
+#pragma unroll
+    for (int x = 0; x < XX; ++x) {
+      n[x] = zero16;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+        n[x] = mfma32<DT>(*reinterpret_cast<const u32x4_t*>(kb + x * 32 * KS + 32 * kk), q[kk], n[x]);
+    }
+  };
+  // s = the new scores in units of log2, hidden ones at -inf; the running maximum
+  auto settle = [&](int t) {
+    const int key = begin + t * KT;
+    float sc[2 * XX];
+    bool ok = true;
+#pragma unroll
+    for (int x = 0; x < 2 * XX; ++x) {
+      sc[x] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sh.sc[t & 3][x])));
+      ok = ok && sc[x] == sc[x];
+    }
+#pragma unroll
+    for (int x = 0; x < XX; ++x)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[x][e] = n[x][e] * sc[2 * x + (e >> 3)];
+    if (!(ok && key >= all_lo && key + KT <= all_hi)) {
+#pragma unroll
+      for (int x = 0; x < XX; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int j = key + 32 * x + 8 * (e >> 2) + 4 * h + (e & 3);
+          const bool on = sc[2 * x + (e >> 3)] == sc[2 * x + (e >> 3)] && j >= row_lo && j < row_hi;
+          s[x][e] = on ? s[x][e] : -kInf;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int x = 0; x < XX; ++x)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[x][e]);
+    // the maximum moves only where a weight would pass 2^8: sums and products lose nothing by that
+    if (__any(top > m + 8.0f)) {
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float now = top > m + 8.0f ? top : m;  // by row: other rows change nothing
+      const float f = now == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - now);
+      m = now;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < DD; ++d) o[d] *= f;
+    }
+  };
+  u32x4_t p[2 * XX];
+  auto weights = [&]() {
+    const float base = m == -kInf ? 0.0f : m;
+#pragma unroll
+    for (int x = 0; x < XX; ++x) {
+      float v[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = __builtin_amdgcn_exp2f(s[x][e] - base);
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) l += (v[e] + v[e + 1]) + (v[e + 2] + v[e + 3]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        p[2 * x][e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
+        p[2 * x + 1][e] = pack_bf16x2(v[8 + 2 * e], v[8 + 2 * e + 1]);
+      }
+    }
+  };
+  auto values = [&](int t) {
+    const char* vb = sh.v[t & 1] + v_at;
+#pragma unroll
+    for (int y = 0; y < 2 * XX; ++y)
+#pragma unroll
+      for (int d = 0; d < DD; ++d)
+        o[d] = mfma32x32x16(*reinterpret_cast<const u32x4_t*>(vb + d * 32 * VS + 32 * y), p[y], o[d]);
+  };
+  if (tiles > 0) {
+    const std::false_type plain;
+    load_k(0);
+    load_v(0);
+    stage_k(0);
+    stage_v(0, plain);
+    if (tiles > 1) {
+      load_k(1);
+      load_v(1);
+      stage_k(1);
+    }
+    if (tiles > 2) load_k(2);
+    __syncthreads();
+    scores(0);
+    settle(0);
+#pragma unroll 1
+    for (int t = 0; t + 1 < tiles; ++t) {
+      __syncthreads();
+      stage_v(t + 1, plain);
+      if (t + 2 < tiles) {
+        load_v(t + 2);
+        stage_k(t + 2);
+        if (t + 3 < tiles) load_k(t + 3);
+      }
+      scores(t + 1);
+      weights();
+      values(t);
+      settle(t + 1);
+    }
+    __syncthreads();
+    weights();
+    values(tiles - 1);
+
+    // NaN among the values of any wave's share: once more over the tiles, with ones for NaN and for keys that are seen
+    if (lane == 0) sh.odd[wave] = odd;
+    __syncthreads();
+    if (sh.odd[0] | sh.odd[1] | sh.odd[2] | sh.odd[3]) {
+#pragma unroll 1
+      for (int t = 0; t < tiles; ++t) {
+        load_k(t);
+        load_v(t);
+        __syncthreads();  // the tile before is done with
+        stage_v(t, std::true_type());
+        if (wave == 0 && lane < KT / 16) sh.sc[t & 3][lane] = sc_reg;
+        __syncthreads();
+#pragma unroll 1
+        for (int y = 0; y < 2 * XX; ++y) {
+          u32x4_t seen;
+          const bool ok = sh.sc[t & 3][y] == sh.sc[t & 3][y];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = begin + t * KT + 16 * y + 8 * (e >> 1) + 4 * h + 2 * (e & 1);
+            seen[e] = (ok && j >= row_lo && j < row_hi ? 0x3f80u : 0u) | (ok && j + 1 >= row_lo && j + 1 < row_hi ? 0x3f800000u : 0u);
+          }
+#pragma unroll
+          for (int d = 0; d < DD; ++d) {
+            const f32x16_t hits = mfma32x32x16(*reinterpret_cast<const u32x4_t*>(sh.v[t & 1] + v_at + d * 32 * VS + 32 * y), seen, zero16);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] += hits[e] > 0.0f ? __builtin_nanf("") : 0.0f;
+          }
+        }
+      }
+    }
+  }
+
+  const int used = hi > lo ? (hi - lo + size - 1) / size : 1;
+  const float sum = l + __shfl_xor(l, 32);
+  if (row >= rows) return;
+  const int64_t at = (sq.row0 + tok) * a.hq + head;
+  if (used == 1) {
+    const float f = sum != 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int d = 0; d < DD; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const float w[4] = {o[d][e] * f, o[d][e + 1] * f, o[d][e + 2] * f, o[d][e + 3] * f};
+        u32x2_t y;
+        if constexpr (DT == PDM_BF16) {
+          y = u32x2_t{pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3])};
+        } else {
+          y = u32x2_t{f32_to_f16_bits(w[0]) | f32_to_f16_bits(w[1]) << 16, f32_to_f16_bits(w[2]) | f32_to_f16_bits(w[3]) << 16};
+        }
+        *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.out) + at * D + 32 * d + 2 * e + 4 * h) = y;
+      }
+    if (h == 0 && a.lse) a.lse[at] = sum != 0.0f ? (m + __builtin_amdgcn_logf(sum)) * kLn2 : -kInf;
+  } else {
+    const int64_t pr = ((item * a.hk + kh) * a.splits + split) * kManyRows + wave * 32 + c;
+#pragma unroll
+    for (int d = 0; d < DD; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<f32x4_t*>(a.part_o + pr * D + 32 * d + 2 * e + 4 * h) = f32x4_t{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+    if (h == 0) {
+      a.part_ml[2 * pr] = m;
+      a.part_ml[2 * pr + 1] = sum;
+    }
+  }
+}
+
+// Joins the splits of the many-rows kernel: one wave per row.
+template <int DT, int D, int KT>
+__global__ void __launch_bounds__(256) kv_attn_many_join_kernel(AttnArgs a, int64_t items) {
+  const int64_t x = linear_block() * 4 + (threadIdx.x >> 6);
+  const int in = (int)(x % kManyRows);
+  const int64_t ih = x / kManyRows;
+  const int kh = (int)(ih % a.hk);
+  const int64_t item = ih / a.hk;
+  if (item >= items) return;
+  Seq sq;
+  int b, r0, lo, hi;
+  if (!many_block(a, item, sq, b, r0)) return;
+  const int r = r0 + in;
+  if (r >= sq.n * a.group) return;
+  many_keys(a, sq, r0, lo, hi);
+  const int size = split_size(hi - lo, a.splits, KT);
+  const int used = hi > lo ? (hi - lo + size - 1) / size : 1;
+  if (used == 1) return;
+  const int i = r / a.group, h = kh * a.group + (r - i * a.group);
+  join_row<DT, D>(a, ih * a.splits * kManyRows + in, kManyRows, used, (sq.row0 + i) * a.hq + h);
 }
 
 // ---- host -----------------------------------------------------------------------
@@ -609,6 +988,8 @@ struct Plan {
   bool few, many;        // which kernels may have work
   int splits, row_stride;
   int64_t part_rows;
+  int many_splits;
+  int64_t items, many_part_rows;
 };
 
 Plan plan_of(const pdm_kv_attention_desc* d, const pdm_kv_cache* c, const pdm_kv_batch* b) {
@@ -628,10 +1009,23 @@ Plan plan_of(const pdm_kv_attention_desc* d, const pdm_kv_cache* c, const pdm_kv
   p.splits = (int)(splits > 1 ? splits : 1);
   p.row_stride = (int)(rows < 16 * p.mt ? rows : 16 * p.mt);
   p.part_rows = p.few && p.splits > 1 ? pairs * p.splits * p.row_stride : 0;
+  if (p.many) {
+    p.items = b->tokens * group / kManyRows + b->num_seqs;
+    const int64_t blocks = p.items * c->n_kv_heads;
+    int64_t sp = blocks < 256 ? 512 / blocks : 1;
+    const int64_t most_sp = (most + 511) / 512;
+    sp = sp < most_sp ? sp : most_sp;
+    p.many_splits = (int)(sp > 1 ? sp : 1);
+    p.many_part_rows = p.many_splits > 1 ? blocks * p.many_splits * kManyRows : 0;
+  }
   return p;
 }
 
 int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
+
+// The two kernels run one after the other, each with its join: they share the workspace.
+int64_t part_rows_of(const Plan& p) { return p.part_rows > p.many_part_rows ? p.part_rows : p.many_part_rows; }
+int64_t workspace_of(const Plan& p, int D) { return round256(part_rows_of(p) * D * 4) + round256(part_rows_of(p) * 8); }
 
 template <int DT, int D>
 void launch(AttnArgs& a, const Plan& p, hipStream_t st) {
@@ -641,9 +1035,14 @@ void launch(AttnArgs& a, const Plan& p, hipStream_t st) {
   else kv_attn_few_kernel<DT, D, 2><<<grid, 256, 0, st>>>(a, units, guards);
   if (p.part_rows) {
     const int64_t rows = (int64_t)a.seqs * a.hk * a.row_stride;
-    kv_attn_join_kernel<DT, D><<<linear_grid((rows + 3) / 4), 256, 0, st>>>(a, rows, kFewKeys * kFewWaves);
+    kv_attn_join_kernel<DT, D><<<linear_grid((rows + 3) / 4), 256, 0, st>>>(a, rows);
   }
-  if (p.many) kv_attn_row_kernel<DT, D><<<linear_grid(a.tokens * a.hq), 64, 0, st>>>(a);
+  if (!p.many) return;
+  a.splits = p.many_splits;
+  constexpr int KT = D == 256 ? 32 : 64;
+  kv_attn_many_kernel<DT, D, KT><<<linear_grid(p.items * a.hk * a.splits), 256, 0, st>>>(a, p.items);
+  if (p.many_part_rows)
+    kv_attn_many_join_kernel<DT, D, KT><<<linear_grid(p.items * a.hk * (kManyRows / 4)), 256, 0, st>>>(a, p.items);
 }
 
 template <int DT>
@@ -662,8 +1061,7 @@ extern "C" int64_t pdm_kv_attention_workspace_size(const pdm_kv_attention_desc* 
                                                    const pdm_kv_batch* b) {
   clear_error();
   if (int e = check(__func__, d, c, b)) return e;
-  const Plan p = plan_of(d, c, b);
-  return round256(p.part_rows * c->head_dim * 4) + round256(p.part_rows * 8);
+  return workspace_of(plan_of(d, c, b), c->head_dim);
 }
 
 extern "C" int pdm_kv_attention_fwd(const pdm_kv_attention_desc* d, const pdm_kv_cache* c, const pdm_kv_batch* b,
@@ -675,7 +1073,7 @@ extern "C" int pdm_kv_attention_fwd(const pdm_kv_attention_desc* d, const pdm_kv
   PDM_CHECK_ARG(q && out, "null q / out");
   PDM_CHECK_ARG((reinterpret_cast<uintptr_t>(out) & 15) == 0, "out must be 16-byte aligned");
   const Plan p = plan_of(d, c, b);
-  const int64_t o_bytes = round256(p.part_rows * c->head_dim * 4), need = o_bytes + round256(p.part_rows * 8);
+  const int64_t need = workspace_of(p, c->head_dim), o_bytes = round256(part_rows_of(p) * c->head_dim * 4);
   if (need && (!workspace || workspace_bytes < need)) {
     set_error(std::string(__func__) + ": workspace of " + std::to_string(need) + " bytes needed");
     return PDM_ERR_WORKSPACE;
