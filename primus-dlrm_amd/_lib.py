@@ -385,3 +385,10 @@ def stream_ptr(device) -> int:
     import torch
 
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def raw_stream(index: int) -> int:
+    """:func:`stream_ptr` of device ``index`` without a Stream object."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(index)

@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a, int64_t it
       load8<DT, VEC>(a.x[kv], at + pl.hi, v[i] + 8);
     }
   }
-  if (!kv) {
+  if (!kv && (NORM || R > 0)) {
     float w[16];
     if (NORM) {
       load8f(a.w + pl.lo, w);
@@ -117,32 +117,34 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a, int64_t it
     for (int i = 0; i < NI; ++i) {
       const int r = group + i * groups;
       const bool ok = r < g.n;
+      // in 64 bits (as fast as 32 here): the code is the nearest to the key itself, whatever the order of the sum
+      double x[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = ok ? (double)v[i][e] : 0.0;
       if (NORM) {
-        float ss = 0.0f;
-        if (ok) {
+        double ss = 0.0;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) ss = __builtin_fmaf(v[i][e], v[i][e], ss);
-        }
-        ss = group_sum(ss, width);
-        if (ok) {
-          const float rs = 1.0f / sqrtf(ss / (float)a.D + a.eps);
+        for (int e = 0; e < 16; ++e) ss = __builtin_fma(x[e], x[e], ss);
+        for (int o = 1; o < width; o <<= 1) ss += __shfl_xor(ss, o);
+        const double rs = 1.0 / sqrt(ss / (double)a.D + (double)a.eps);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) v[i][e] = v[i][e] * rs * w[e];
-        }
+        for (int e = 0; e < 16; ++e) x[e] = x[e] * rs * (double)w[e];
       }
       if (ok && pl.turned) {
         const int64_t p = a.positions ? load_position(a.positions, a.bits, g.row0 + r) : g.index0 + r;
         if (p < 0 || p >= a.table_rows) {
           if (a.err) *a.err = 1;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) v[i][e] = 0.0f;
+          for (int e = 0; e < 16; ++e) x[e] = 0.0;
         } else {
           float c[8], s[8];
           load8f(a.cos + p * (R / 2) + 8 * j, c);
           load8f(a.sin + p * (R / 2) + 8 * j, s);
-          rotate16<INTER>(v[i], c, s);
+          rotate16<INTER>(x, c, s);
         }
       }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[i][e] = (float)x[e];
     }
   }
 #pragma unroll

@@ -95,16 +95,13 @@ __device__ __forceinline__ void load8f(const float* p, float* v) {
   for (int i = 0; i < 4; ++i) v[i] = a[i], v[i + 4] = b[i];
 }
 
-// The rotation of a lane's 16 elements by the angles of cos / sin: products and sums are rounded one by
-// one (no fused multiply-add), so that a rotated key is quantized from the same fp32 value wherever it is
-// computed.
-template <bool INTER>
-__device__ __forceinline__ void rotate16(float* v, const float* c, const float* s) {
-#pragma clang fp contract(off)
+// The rotation of a lane's 16 elements (F: float or double) by the angles of cos / sin.
+template <bool INTER, typename F>
+__device__ __forceinline__ void rotate16(F* v, const float* c, const float* s) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int a = INTER ? 2 * i : i, b = INTER ? 2 * i + 1 : i + 8;
-    const float x = v[a], y = v[b];
+    const F x = v[a], y = v[b];
     v[a] = x * c[i] - y * s[i];
     v[b] = y * c[i] + x * s[i];
   }

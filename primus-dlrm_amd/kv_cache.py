@@ -22,7 +22,7 @@ import torch
 import torch.nn as nn
 
 from . import ops
-from .onetrans import RMSNorm, _in_graph
+from .onetrans import RMSNorm
 
 __all__ = ["rotary_tables", "qk_norm_rope", "kv_append", "kv_attention", "QKNormRope", "PagedKVCache"]
 
@@ -38,11 +38,20 @@ def rotary_tables(max_positions: int, rotary_dim: int, theta: float = 10000.0, d
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
     """[..., heads, D] -> [tokens, heads, D], a view wherever the strides allow one."""
-    if t.dim() < 3:
-        raise ValueError(f"expected [..., heads, head_dim], got {tuple(t.shape)}")
-    if t.dim() > 3:
+    dims = t.dim()
+    if dims != 3:
+        if dims < 3:
+            raise ValueError(f"expected [..., heads, head_dim], got {tuple(t.shape)}")
         t = t.flatten(0, -3)
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _traced(t: torch.Tensor) -> bool:
+    return torch.compiler.is_compiling() or isinstance(t, torch.fx.Proxy)
+
+
+def _fp32(w: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return w if w is None or (w.dtype == torch.float32 and w.is_contiguous()) else w.float().contiguous()
 
 
 class _QkNormRope(torch.autograd.Function):
@@ -77,22 +86,20 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     gradients are zeros, and so does one beyond the tables, which also sets ``err_flag`` (int32, never cleared).
     cos, sin: fp32 [positions, rotary_dim / 2] (:func:`rotary_tables`); None: no rotation.  ``interleaved``: pairs (2i,
     2i + 1) instead of (i, i + rotary_dim / 2).  q_weight, k_weight: [D], fp32 or q's dtype; None: no norm."""
-    for n, t in (("cos", cos), ("sin", sin)):
-        if t is not None and t.requires_grad:
-            raise ValueError(f"{n} takes no gradient")
-    if tuple(positions.shape) != tuple(q.shape[:-2]):
-        raise ValueError(f"positions must be {tuple(q.shape[:-2])}, one for each token, got {tuple(positions.shape)}")
-    if k is not None and k.shape[:-2] != q.shape[:-2]:
-        raise ValueError(f"k must hold q's tokens {tuple(q.shape[:-2])}, got {tuple(k.shape)}")
+    if (cos is not None and cos.requires_grad) or (sin is not None and sin.requires_grad):
+        raise ValueError("cos and sin take no gradient")
+    lead = q.shape[:-2]
+    if positions.shape != lead:
+        raise ValueError(f"positions must be {tuple(lead)}, one for each token, got {tuple(positions.shape)}")
+    if k is not None and k.shape[:-2] != lead:
+        raise ValueError(f"k must hold q's tokens {tuple(lead)}, got {tuple(k.shape)}")
     for n, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None and w.dtype not in (torch.float32, q.dtype):
             raise TypeError(f"{n} must be float32 or {q.dtype}, got {w.dtype}")
-    lead = q.shape[:-2]
     q3, k3 = _heads(q), None if k is None else _heads(k)
-    pos = positions.reshape(-1).contiguous()
-    qw = None if q_weight is None else q_weight.float().contiguous()
-    kw = None if k_weight is None else k_weight.float().contiguous()
-    if _in_graph(q):
+    pos = positions if len(lead) == 1 and positions.is_contiguous() else positions.reshape(-1).contiguous()
+    qw, kw = _fp32(q_weight), _fp32(k_weight)
+    if _traced(q):
         if err_flag is not None:
             raise ValueError("err_flag is not available in a compiled graph")
         q_out, k_out = torch.ops.pdm.qk_norm_rope(q3, k3, pos, cos, sin, qw, kw, eps, interleaved)
@@ -108,7 +115,9 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
 
 
 def _no_grad(name: str, *tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    for t in tensors:
+        if t is None or not t.requires_grad or not torch.is_grad_enabled():
+            continue
         raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or detach its inputs")
 
 
@@ -135,9 +144,9 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: 
     if kw is not None:
         if kw.dtype not in (torch.float32, k.dtype):
             raise TypeError(f"k_weight must be float32 or {k.dtype}, got {kw.dtype}")
-        kw = kw.detach().float().contiguous()
+        kw = _fp32(kw.detach())
     k, v = _heads(k), _heads(v)
-    run = torch.ops.pdm.kv_append if _in_graph(k) else ops.kv_append_raw
+    run = torch.ops.pdm.kv_append if _traced(k) else ops.kv_append_raw
     run(k, v, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, positions, cos, sin, kw, eps,
         interleaved, err_flag)
 
@@ -158,7 +167,7 @@ def kv_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, 
     width bounds the lengths the work is laid out for."""
     _no_grad("kv_attention", q)
     q = _heads(q)
-    if _in_graph(q):
+    if _traced(q):
         if out is not None:
             raise ValueError("out is not available in a compiled graph")
         out, lse = torch.ops.pdm.kv_attention(q, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens,

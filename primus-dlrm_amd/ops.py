@@ -860,20 +860,41 @@ def _(keys, table_size, salt):
 # Cached attention: norm and rotation of queries and keys, append to an 8-bit paged cache, attention over it
 # ---------------------------------------------------------------------------
 
-def _on_device(dev: torch.device):
-    """Makes ``dev`` the current device for a launch (nothing to do when it is)."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+# The host side of these calls is a large part of a decoding step: checks below take each tensor property once.
+
+_SAME_DEVICE = contextlib.nullcontext()
 
 
-def _check_heads(name: str, t: torch.Tensor) -> None:
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
-    if t.shape[2] > 1 and t.stride(2) != 1:
+def _on_device(index: int):
+    """Makes device ``index`` the current one for a launch (nothing to do when it is)."""
+    return _SAME_DEVICE if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def _gpu_index(*tensors: Optional[torch.Tensor]) -> int:
+    """Index of the one GPU that the given tensors are on; raises as ``_require_cuda`` does."""
+    index = -1
+    for t in tensors:
+        if t is not None:
+            i = t.get_device()
+            if i != index or i < 0:
+                if i < 0 or index >= 0:
+                    _require_cuda(*tensors)
+                index = i
+    return index
+
+
+def _check_heads(name: str, t: torch.Tensor) -> Tuple[int, int, int, int, int, int]:
+    """(tokens, heads, head_dim, token stride, head stride, dtype code) of q, k or v."""
+    shape = t.shape
+    if len(shape) != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], got {tuple(shape)}")
+    st, sh, sd = t.stride()
+    if sd != 1 and shape[2] > 1:
         raise ValueError(f"the elements of a head of {name} must be contiguous")
-    if t.dtype not in TORCH_TO_PDM:
+    code = TORCH_TO_PDM.get(t.dtype)
+    if code is None:
         raise TypeError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+    return shape[0], shape[1], shape[2], st, sh, code
 
 
 def _check_err_flag(err_flag: Optional[torch.Tensor]) -> None:
@@ -915,14 +936,12 @@ def _aligned16(t: Optional[torch.Tensor], name: str) -> None:
 
 
 def _qk_rope_desc(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved) -> "L.QkRopeDesc":
-    _check_heads("q", q)
-    T, hq, D = q.shape
+    T, hq, D, q_st, q_sh, code = _check_heads("q", q)
     hk, k_st, k_sh = 0, 0, 0
     if k is not None:
-        _check_heads("k", k)
-        if k.shape[0] != T or k.shape[2] != D or k.dtype != q.dtype:
+        kT, hk, kD, k_st, k_sh, k_code = _check_heads("k", k)
+        if kT != T or kD != D or k_code != code:
             raise ValueError(f"k must be {q.dtype} [{T}, heads, {D}] beside q, got {k.dtype} {tuple(k.shape)}")
-        hk, k_st, k_sh = k.shape[1], k.stride(0), k.stride(1)
     if D % 16 or not 16 <= D <= 1024:
         raise ValueError(f"head_dim must be a multiple of 16 in [16, 1024], got {D}")
     _check_positions(positions, T)
@@ -935,8 +954,8 @@ def _qk_rope_desc(q, k, positions, cos, sin, q_weight, k_weight, eps, interleave
         raise ValueError("k_weight without k")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
-    return L.QkRopeDesc(T, hq, hk, D, R, TORCH_TO_PDM[q.dtype], 64 if positions.dtype == torch.int64 else 32,
-                        int(interleaved), eps, rows, q.stride(0), q.stride(1), k_st, k_sh)
+    return L.QkRopeDesc(T, hq, hk, D, R, code, 64 if positions.dtype == torch.int64 else 32, int(interleaved), eps, rows,
+                        q_st, q_sh, k_st, k_sh)
 
 
 def qk_norm_rope_raw(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
@@ -947,15 +966,15 @@ def qk_norm_rope_raw(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
     """Launches pdm_qk_norm_rope_fwd on q [T, Hq, D] and k [T, Hk, D] (any token and head strides)."""
     desc = _qk_rope_desc(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved)
     _check_err_flag(err_flag)
-    dev = _require_cuda(q, k, positions, cos, sin, q_weight, k_weight, err_flag)
+    index = _gpu_index(q, k, positions, cos, sin, q_weight, k_weight, err_flag)
     for n, t in (("cos", cos), ("sin", sin), ("q_weight", q_weight), ("k_weight", k_weight)):
         _aligned16(t, n)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
-    with _on_device(dev):
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
+    with _on_device(index):
         L.check(L.lib().pdm_qk_norm_rope_fwd(
             ctypes.byref(desc), q.data_ptr(), _ptr(k), positions.data_ptr(), _ptr(cos), _ptr(sin), _ptr(q_weight),
-            _ptr(k_weight), q_out.data_ptr(), _ptr(k_out), _ptr(err_flag), L.stream_ptr(dev)),
+            _ptr(k_weight), q_out.data_ptr(), _ptr(k_out), _ptr(err_flag), L.raw_stream(index)),
             "pdm_qk_norm_rope_fwd")
     return q_out, k_out
 
@@ -972,12 +991,12 @@ def qk_norm_rope_backward_raw(q: torch.Tensor, k: Optional[torch.Tensor], positi
         if (g is None) != (x is None) or (g is not None and (g.shape != x.shape or g.dtype != x.dtype
                                                              or not g.is_contiguous())):
             raise ValueError(f"{n} must be contiguous and of its input's shape and dtype")
-    dev = _require_cuda(q, k, positions, cos, sin, q_weight, k_weight, grad_q_out, grad_k_out)
+    index = _gpu_index(q, k, positions, cos, sin, q_weight, k_weight, grad_q_out, grad_k_out)
     for n, t in (("cos", cos), ("sin", sin), ("q_weight", q_weight), ("k_weight", k_weight)):
         _aligned16(t, n)
     lib = L.lib()
-    grad_q = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    grad_k = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
+    grad_q = torch.empty_like(q, memory_format=torch.contiguous_format)
+    grad_k = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     grad_qw = None if q_weight is None else torch.empty_like(q_weight)
     grad_kw = None if k_weight is None else torch.empty_like(k_weight)
     ws_bytes = 0
@@ -985,12 +1004,12 @@ def qk_norm_rope_backward_raw(q: torch.Tensor, k: Optional[torch.Tensor], positi
         ws_bytes = int(lib.pdm_qk_norm_rope_bwd_workspace_size(ctypes.byref(desc)))
         if ws_bytes < 0:
             raise L.PdmError(ws_bytes, "pdm_qk_norm_rope_bwd_workspace_size", L.last_error())
-    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
-    with _on_device(dev):
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    with _on_device(index):
         L.check(lib.pdm_qk_norm_rope_bwd(
             ctypes.byref(desc), q.data_ptr(), _ptr(k), positions.data_ptr(), _ptr(cos), _ptr(sin), _ptr(q_weight),
             _ptr(k_weight), grad_q_out.data_ptr(), _ptr(grad_k_out), grad_q.data_ptr(), _ptr(grad_k), _ptr(grad_qw),
-            _ptr(grad_kw), ws.data_ptr(), ws_bytes, L.stream_ptr(dev)), "pdm_qk_norm_rope_bwd")
+            _ptr(grad_kw), _ptr(ws), ws_bytes, L.raw_stream(index)), "pdm_qk_norm_rope_bwd")
     return grad_q, grad_k, grad_qw, grad_kw
 
 
@@ -1049,17 +1068,22 @@ def _qk_norm_rope_backward(ctx, grad_q_out, grad_k_out):
 qk_norm_rope_op.register_autograd(_qk_norm_rope_backward, setup_context=_qk_norm_rope_setup)
 
 
+_CODE_DTYPES = (torch.float8_e4m3fn, torch.uint8)
+
+
 def _kv_cache_desc(k_codes, v_codes, k_scale, v_scale) -> "L.KvCacheDesc":
-    if k_codes.dim() != 4 or k_codes.shape != v_codes.shape:
+    shape = k_codes.shape
+    if len(shape) != 4 or v_codes.shape != shape:
         raise ValueError("k_codes and v_codes must be [pages, heads, page_size, head_dim] of one shape")
-    for n, t in (("k_codes", k_codes), ("v_codes", v_codes)):
-        if t.dtype not in (torch.float8_e4m3fn, torch.uint8):
-            raise TypeError(f"{n} must be float8_e4m3fn (or its bytes as uint8), got {t.dtype}")
-        if not t.is_contiguous():
-            raise ValueError(f"{n} must be contiguous")
-    pages, heads, page, D = k_codes.shape
+    if k_codes.dtype not in _CODE_DTYPES or v_codes.dtype not in _CODE_DTYPES:
+        raise TypeError("k_codes and v_codes must be float8_e4m3fn (or its bytes as uint8), got "
+                        f"{k_codes.dtype} and {v_codes.dtype}")
+    if not (k_codes.is_contiguous() and v_codes.is_contiguous()):
+        raise ValueError("k_codes and v_codes must be contiguous")
+    pages, heads, page, D = shape
+    scales = shape[:2]
     for n, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t.dtype != torch.float32 or tuple(t.shape) != (pages, heads) or not t.is_contiguous():
+        if t.dtype != torch.float32 or t.shape != scales or not t.is_contiguous():
             raise ValueError(f"{n} must be a contiguous float32 [{pages}, {heads}] tensor")
     if page not in (16, 32, 64, 128):
         raise ValueError(f"page_size must be 16, 32, 64 or 128, got {page}")
@@ -1070,18 +1094,19 @@ def _kv_cache_desc(k_codes, v_codes, k_scale, v_scale) -> "L.KvCacheDesc":
 
 
 def _kv_batch_desc(cu_seqlens, page_table, seq_lens, tokens: int) -> "L.KvBatchDesc":
-    for n, t in (("cu_seqlens", cu_seqlens), ("page_table", page_table), ("seq_lens", seq_lens)):
-        if t.dtype != torch.int32:
-            raise TypeError(f"{n} must be int32, got {t.dtype}")
+    if not cu_seqlens.dtype == page_table.dtype == seq_lens.dtype == torch.int32:
+        raise TypeError(f"cu_seqlens, page_table and seq_lens must be int32, got {cu_seqlens.dtype}, {page_table.dtype} "
+                        f"and {seq_lens.dtype}")
     if seq_lens.dim() != 1 or not seq_lens.is_contiguous():
         raise ValueError("seq_lens must be a contiguous [sequences] tensor")
     B = seq_lens.shape[0]
-    if tuple(cu_seqlens.shape) != (B + 1,) or not cu_seqlens.is_contiguous():
+    if cu_seqlens.shape != (B + 1,) or not cu_seqlens.is_contiguous():
         raise ValueError(f"cu_seqlens must be a contiguous [{B + 1}] tensor, got {tuple(cu_seqlens.shape)}")
-    if page_table.dim() != 2 or page_table.shape[0] != B or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise ValueError(f"page_table must be [{B}, pages] with contiguous rows, got {tuple(page_table.shape)}")
+    shape = page_table.shape
+    if len(shape) != 2 or shape[0] != B or (shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError(f"page_table must be [{B}, pages] with contiguous rows, got {tuple(shape)}")
     return L.KvBatchDesc(cu_seqlens.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(), page_table.stride(0),
-                         tokens, B, page_table.shape[1])
+                         tokens, B, shape[1])
 
 
 def kv_append_raw(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
@@ -1092,10 +1117,9 @@ def kv_append_raw(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_cod
                   err_flag: Optional[torch.Tensor] = None) -> None:
     """Launches pdm_kv_append: the new keys and values [T, Hk, D] (any token and head strides) into the cache."""
     cache = _kv_cache_desc(k_codes, v_codes, k_scale, v_scale)
-    _check_heads("k", k)
-    _check_heads("v", v)
-    T, hk, D = k.shape
-    if v.shape != k.shape or v.dtype != k.dtype:
+    T, hk, D, k_st, k_sh, code = _check_heads("k", k)
+    _, _, _, v_st, v_sh, v_code = _check_heads("v", v)
+    if v.shape != k.shape or v_code != code:
         raise ValueError(f"v must be {k.dtype} {tuple(k.shape)} as k is, got {v.dtype} {tuple(v.shape)}")
     if hk != cache.n_kv_heads or D != cache.head_dim:
         raise ValueError(f"k has {hk} heads of {D}, the cache {cache.n_kv_heads} of {cache.head_dim}")
@@ -1107,16 +1131,16 @@ def kv_append_raw(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_cod
     if not eps >= 0:
         raise ValueError("eps must not be negative")
     _check_err_flag(err_flag)
-    dev = _require_cuda(k, v, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, positions, cos, sin,
-                        k_weight, err_flag)
+    index = _gpu_index(k, v, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, positions, cos, sin,
+                       k_weight, err_flag)
     for n, t in (("cos", cos), ("sin", sin), ("k_weight", k_weight)):
         _aligned16(t, n)
-    desc = L.KvAppendDesc(TORCH_TO_PDM[k.dtype], R, 32 if positions is not None and positions.dtype == torch.int32 else 64,
-                          int(interleaved), eps, 0, rows, k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-    with _on_device(dev):
+    desc = L.KvAppendDesc(code, R, 32 if positions is not None and positions.dtype == torch.int32 else 64, int(interleaved),
+                          eps, 0, rows, k_st, k_sh, v_st, v_sh)
+    with _on_device(index):
         L.check(L.lib().pdm_kv_append(
             ctypes.byref(desc), ctypes.byref(cache), ctypes.byref(batch), k.data_ptr(), v.data_ptr(), _ptr(positions),
-            _ptr(cos), _ptr(sin), _ptr(k_weight), _ptr(err_flag), L.stream_ptr(dev)), "pdm_kv_append")
+            _ptr(cos), _ptr(sin), _ptr(k_weight), _ptr(err_flag), L.raw_stream(index)), "pdm_kv_append")
 
 
 @torch.library.custom_op("pdm::kv_append", mutates_args=("k_codes", "v_codes", "k_scale", "v_scale", "err_flag"))
@@ -1143,9 +1167,8 @@ def kv_attention_raw(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tens
     """Launches pdm_kv_attention_fwd on q [T, Hq, D]; returns (out, lse or None).  ``max_q_len``: no sequence has more
     new tokens (default: T, which costs a second launch and idle blocks)."""
     cache = _kv_cache_desc(k_codes, v_codes, k_scale, v_scale)
-    _check_heads("q", q)
-    T, hq, D = q.shape
-    if q.dtype == torch.float32:
+    T, hq, D, q_st, q_sh, code = _check_heads("q", q)
+    if code == L.PDM_F32:
         raise TypeError("q must be float16 or bfloat16")
     if D != cache.head_dim or hq == 0 or hq % cache.n_kv_heads:
         raise ValueError(f"q has {hq} heads of {D}, the cache {cache.n_kv_heads} of {cache.head_dim}: the head_dims must "
@@ -1164,23 +1187,22 @@ def kv_attention_raw(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tens
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
         raise ValueError("out must be contiguous and of q's shape and dtype")
     _check_err_flag(err_flag)
-    dev = _require_cuda(q, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, out, err_flag)
+    index = _gpu_index(q, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, out, err_flag)
     if out is None:
-        out = torch.empty((T, hq, D), dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _aligned16(out, "out")
-    lse = torch.empty((T, hq), dtype=torch.float32, device=dev) if return_lse else None
-    desc = L.KvAttentionDesc(TORCH_TO_PDM[q.dtype], hq, int(causal), window, scale, min(max_q_len, T), q.stride(0),
-                             q.stride(1))
+    lse = torch.empty((T, hq), dtype=torch.float32, device=q.device) if return_lse else None
+    desc = L.KvAttentionDesc(code, hq, int(causal), window, scale, min(max_q_len, T), q_st, q_sh)
     lib = L.lib()
     ws_bytes = int(lib.pdm_kv_attention_workspace_size(ctypes.byref(desc), ctypes.byref(cache), ctypes.byref(batch)))
     if ws_bytes < 0:
         raise L.PdmError(ws_bytes, "pdm_kv_attention_workspace_size", L.last_error())
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    with _on_device(dev):
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    with _on_device(index):
         L.check(lib.pdm_kv_attention_fwd(
             ctypes.byref(desc), ctypes.byref(cache), ctypes.byref(batch), q.data_ptr(), out.data_ptr(), _ptr(lse),
-            _ptr(ws), ws_bytes, _ptr(err_flag), L.stream_ptr(dev)), "pdm_kv_attention_fwd")
+            _ptr(ws), ws_bytes, _ptr(err_flag), L.raw_stream(index)), "pdm_kv_attention_fwd")
     return out, lse
 
 

@@ -1,35 +1,16 @@
 """kv_append against its definition in 64 bits: codes, scales, untouched slots; every dtype, head width, page size; pages
 filled at once and token by token; scales that grow; NaN and infinities; bad spans, lengths, pages and positions.
 
-Keys that are not normed, and values, are quantized from exact products and sums that are rounded one by one, so their
-codes have to be the reference's bit for bit (the reference rotates in fp32 too, product by product).  Normed keys carry
-up to 24 u (|n1| + |n2|), u = 2^-24, before the quantizer: a code may be the other neighbour of a value that close to
-the middle of two, never more."""
+Values, and keys that are neither normed nor rotated, have to get the reference's codes bit for bit.  Keys that are
+computed on the way (in 64 bits, then rounded to fp32 and from there to their codes) may get the other neighbour where
+the fp32 rounding moves them onto the middle of two codes: within 2^-24 of it, a chance of 2^-19 for a code.
+"""
 import pytest
 import torch
 
 from oracle import cached_attention as ref
 
 pytestmark = pytest.mark.gpu
-
-U = 2.0 ** -24
-
-
-def _rotate32(x, positions, cos, sin, inter):
-    """The rotation in fp32 with every product and sum rounded by itself."""
-    if cos is None:
-        return x
-    y, R = x.clone(), 2 * cos.shape[1]
-    ok = (positions >= 0) & (positions < len(cos))
-    p = positions.clamp(0, len(cos) - 1).long()
-    c, s = cos[p][:, None], sin[p][:, None]
-    ia = torch.arange(0, R, 2) if inter else torch.arange(R // 2)
-    ib = ia + 1 if inter else ia + R // 2
-    y[..., ia] = x[..., ia] * c - x[..., ib] * s
-    y[..., ib] = x[..., ib] * c + x[..., ia] * s
-    y[~ok] = 0
-    return y
-
 
 class Pool:
     """A cache on both sides, and sequences that own pages of it."""
@@ -54,7 +35,7 @@ class Pool:
         for x, codes, scale in ((k64, self.codes[0], self.scale[0]), (v64, self.codes[1], self.scale[1])):
             ref.append(x, codes, scale, cu, table, lens)
 
-    def check(self, exact=(True, True), slack=None):
+    def check(self, exact=(True, True)):
         for i, (c, s) in enumerate(((self.cache.k_codes, self.cache.k_scale), (self.cache.v_codes, self.cache.v_scale))):
             assert torch.equal(s.cpu().double(), self.scale[i])
             got = c.cpu().double()
@@ -64,8 +45,7 @@ class Pool:
             bad = got != self.codes[i]
             assert torch.equal(got.isnan(), self.codes[i].isnan())
             bad &= ~got.isnan()
-            # neighbours, and few: the chance that a value lies within 24 u of a middle is below 2^-13
-            assert bad.double().mean().item() <= 2.0 ** -10
+            assert bad.double().mean().item() <= 2.0 ** -15  # in 2^13 to 2^16 codes: one or two at most
             step = torch.exp2(torch.floor(torch.log2(got[bad].abs().clamp(min=2.0 ** -6))) - 3)
             assert ((got[bad] - self.codes[i][bad]).abs() <= 2 * step).all()
 
@@ -134,12 +114,10 @@ def test_rotated_and_normed_keys(pdm, dev, D, R, inter, norm, explicit):
             pos = torch.randint(0, 300, pos.shape, generator=g)
             kw["positions"] = pos.to(dev)
         if norm:
-            k64 = ref.norm_rope(k, w, pos, cos, sin, 1e-6, inter)
             kw["k_weight"] = w.to(dev)
-        else:
-            k64 = _rotate32(k.float(), pos, cos, sin, inter).double()
+        k64 = ref.norm_rope(k, w if norm else None, pos, cos, sin, 1e-6, inter)
         pool.append(k, v, _cu(more), table, lens, k64, v.double(), cos=cos.to(dev), sin=sin.to(dev), interleaved=inter, **kw)
-        pool.check(exact=(not norm, True))
+        pool.check(exact=(False, True))
     pool.cache.check()
 
 
