@@ -29,9 +29,11 @@ struct AttnArgs {
   const int32_t *cu, *table, *lens;
   int32_t* err;
   float *part_o, *part_ml;   // partial results of a split: rows of D floats, and (maximum, sum)
+  int32_t* joins;            // dealt: the pair that each workgroup began and did not end (sequence, key head, parts)
   int64_t tokens, table_stride, num_pages, stride_t, stride_h;
   int32_t seqs, hq, hk, group, page_log2, table_width, max_q, causal, window;
   int32_t splits;            // of the keys of a (sequence, key head)
+  int32_t workers;           // workgroups that the keys of all sequences are dealt to; 0: equal splits
   int32_t row_stride;        // rows of a partial result
   int32_t few_rows;          // sequences of at most so many rows are kv_attn_few_kernel's
   int32_t vec;               // q takes 16-byte loads
@@ -52,6 +54,13 @@ __device__ __forceinline__ bool seq_fits(const AttnArgs& a, int64_t c0, int64_t 
   return c0 >= 0 && c1 <= a.tokens && c1 - c0 <= a.max_q && c1 - c0 <= len;
 }
 
+__device__ __forceinline__ void seq_keys(const AttnArgs& a, Seq& s) {
+  const int64_t most = (int64_t)a.table_width << a.page_log2;
+  s.hi = s.len < most ? s.len : (int)most;
+  const int64_t first = (int64_t)s.len - s.n - a.window + 1;
+  s.lo = a.window > 0 && first > 0 ? (int)first & ~31 : 0;
+}
+
 // False for a sequence without rows, and for one that does not fit (which sets the flag).
 __device__ __forceinline__ bool seq_of(const AttnArgs& a, int b, Seq& s) {
   const int64_t c0 = a.cu[b], c1 = a.cu[b + 1], len = a.lens[b];
@@ -63,11 +72,8 @@ __device__ __forceinline__ bool seq_of(const AttnArgs& a, int b, Seq& s) {
   s.row0 = c0;
   s.n = (int)(c1 - c0);
   s.len = (int)len;
-  const int64_t most = (int64_t)a.table_width << a.page_log2;
-  s.hi = (int)(len < most ? len : most);
-  if (len > most && a.err) *a.err = 1;
-  const int64_t first = len - s.n - a.window + 1;
-  s.lo = a.window > 0 && first > 0 ? (int)first & ~31 : 0;
+  if (len > (int64_t)a.table_width << a.page_log2 && a.err) *a.err = 1;
+  seq_keys(a, s);
   return true;
 }
 
@@ -105,6 +111,13 @@ __device__ __forceinline__ f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c) {
 // NaN codes of a dword: bit 7 of each byte that holds one.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
+template <int DT>
+__device__ __forceinline__ void store4(void* base, int64_t at, float x, float y, float z, float w) {
+  const u32x2_t v = DT == PDM_BF16 ? u32x2_t{pack_bf16x2(x, y), pack_bf16x2(z, w)}
+                                   : u32x2_t{f32_to_f16_bits(x) | f32_to_f16_bits(y) << 16, f32_to_f16_bits(z) | f32_to_f16_bits(w) << 16};
+  *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(base) + at) = v;
+}
+
 __device__ __forceinline__ void store_out(const AttnArgs& a, int dt, int64_t at, float v) {
   static_cast<uint16_t*>(a.out)[at] = (uint16_t)(dt == PDM_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v));
 }
@@ -127,7 +140,7 @@ __device__ __forceinline__ void clear_rows(const AttnArgs& a, int64_t first) {
     covered = c0 <= t && t < c1 && seq_fits(a, c0, c1, a.lens[lo]);
   }
   bad[threadIdx.x] = t < a.tokens && !covered;
-  __syncthreads();
+  if (!__syncthreads_or(t < a.tokens && !covered)) return;
   const int64_t left = a.tokens - first;
   const int rows = left < 256 ? (int)left : 256;
   for (int r = 0; r < rows; ++r) {
@@ -143,98 +156,150 @@ __device__ __forceinline__ void clear_rows(const AttnArgs& a, int64_t first) {
 // Up to 16 MT rows against a split of the keys.  Four waves take tiles of 32 keys in turn, each with its own
 // maximum, sum and O, and join in LDS; splits join in kv_attn_join_kernel.  Bound by the bytes of the codes: a wave
 // has the next tile's loads (8 KB at D = 128) in flight while it works on one.
-constexpr int kFewKeys = 32, kFewWaves = 4;
+constexpr int kFewKeys = 32, kFewWaves = 4, kFewStep = kFewKeys * kFewWaves;
+constexpr int kDealt = 256;   // sequences of a call that is dealt
 
-template <int D>
-struct FewTile {
-  static constexpr int KC = D / 64;       // 16-byte pieces of a key row per lane
-  static constexpr int VW = D / 64;       // dwords of a value row per lane
-  u32x4_t k[2][KC];                       // 16 keys each
-  uint32_t v[2][4][VW];                   // rows 4 g + i of the 16 keys
-  float ks[2], vs[2];
-  bool ok[2];
+// What a workgroup works on: the keys [begin, end) of a (sequence, key head).
+struct FewUnit {
+  Seq sq;
+  int b, kh, begin, end;
+  bool alone;       // these are all keys of the pair
+  int64_t slot;     // else the place of the partial result
 };
 
+__device__ __forceinline__ int steps_of(const Seq& s) { return s.hi > s.lo ? (s.hi - s.lo + kFewStep - 1) / kFewStep : 1; }
+
+// Dealt: the steps of 128 keys of all (sequence, key head) pairs, in order, are dealt to `workers` workgroups in equal
+// runs, so that a batch of long and short sequences keeps every CU busy to the end.  A run ends some pairs and begins
+// one: a workgroup leaves at most two partial results, that of a pair which it did not begin (slot 2 w) and that of one which
+// it did not end (2 w + 1).  Every workgroup computes the plan itself, a sequence per thread.
+struct FewDeal {
+  int64_t first[kDealt + 1];  // steps before a sequence, of all its heads
+  int64_t sums[4];
+  int row0[kDealt], n[kDealt], len[kDealt];
+  int found;
+};
+
+__device__ __forceinline__ int64_t few_deal(const AttnArgs& a, FewDeal& sh) {  // steps of a run
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  Seq s;
+  int64_t steps = 0;
+  if (tid < a.seqs && seq_of(a, tid, s) && (int64_t)s.n * a.group <= a.few_rows) {
+    steps = (int64_t)steps_of(s) * a.hk;
+    sh.row0[tid] = (int)s.row0, sh.n[tid] = s.n, sh.len[tid] = s.len;
+  }
+  int64_t upto = steps;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t v = __shfl_up(upto, o);
+    upto += lane >= o ? v : 0;
+  }
+  if (lane == 63) sh.sums[wave] = upto;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) upto += sh.sums[w];
+  sh.first[tid] = upto - steps;
+  if (tid == kDealt - 1) sh.first[kDealt] = upto;
+  __syncthreads();
+  return (sh.first[kDealt] + a.workers - 1) / a.workers;
+}
+
+// The part of run [x, to) that belongs to the pair at x; returns the steps taken.  FIRST: the run's first pair (a barrier);
+// else u holds the pair before it.
+template <bool FIRST>
+__device__ __forceinline__ int64_t few_next(const AttnArgs& a, FewDeal& sh, int64_t x, int64_t from, int64_t to, int64_t worker,
+                                            FewUnit& u) {
+  if (FIRST) {
+    if (sh.first[threadIdx.x] <= x && x < sh.first[threadIdx.x + 1]) sh.found = threadIdx.x;
+    __syncthreads();
+    u.b = __builtin_amdgcn_readfirstlane(sh.found);
+  } else {
+    while (sh.first[u.b + 1] <= x) ++u.b;  // x is below the last entry
+  }
+  u.sq.row0 = __builtin_amdgcn_readfirstlane(sh.row0[u.b]);
+  u.sq.n = __builtin_amdgcn_readfirstlane(sh.n[u.b]);
+  u.sq.len = __builtin_amdgcn_readfirstlane(sh.len[u.b]);
+  seq_keys(a, u.sq);
+  const int steps = steps_of(u.sq);
+  const int64_t local = x - sh.first[u.b];
+  u.kh = (int)(local / steps);
+  const int s0 = (int)(local - (int64_t)u.kh * steps);
+  const int n = to - x < steps - s0 ? (int)(to - x) : steps - s0;
+  u.begin = u.sq.lo + s0 * kFewStep;
+  u.end = s0 + n < steps ? u.begin + n * kFewStep : u.sq.hi;
+  u.alone = n == steps;
+  u.slot = 2 * worker + (x - s0 < from ? 0 : 1);
+  return n;
+}
+
+// Not dealt: `splits` equal parts of each pair.
+__device__ __forceinline__ bool few_split(const AttnArgs& a, int64_t unit, FewUnit& u) {
+  const int split = (int)(unit % a.splits);
+  const int64_t bh = unit / a.splits;
+  u.kh = (int)(bh % a.hk), u.b = (int)(bh / a.hk);
+  if (!seq_of(a, u.b, u.sq) || (int64_t)u.sq.n * a.group > a.few_rows) return false;
+  const int size = split_size(u.sq.hi - u.sq.lo, a.splits, kFewStep);
+  u.begin = u.sq.lo + split * size;
+  if (split > 0 && u.begin >= u.sq.hi) return false;
+  u.end = u.begin + size < u.sq.hi ? u.begin + size : u.sq.hi;
+  u.alone = u.sq.hi - u.sq.lo <= size;
+  u.slot = unit;
+  return true;
+}
+
 template <int DT, int D, int MT>
-__global__ void __launch_bounds__(256) kv_attn_few_kernel(AttnArgs a, int64_t units, int64_t guards) {
+__global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D * MT <= 256 ? 2 : 1) kv_attn_few_kernel(AttnArgs a, int64_t units, int64_t guards) {
   constexpr int KK = D / 32;              // steps of the first product
   constexpr int DD = D / 16;              // tiles of the second: O^T row m of tile dd is element DD m + dd
   __shared__ float red[kFewWaves][16][D + 4];
-  __shared__ float ml[kFewWaves][2][16 * MT];
+  __shared__ float ml[kFewWaves + 1][2][16 * MT];
+  __shared__ FewDeal deal;
   const int64_t unit = linear_block();
   if (unit >= units) {
     if (unit < units + guards) clear_rows<D>(a, (unit - units) * 256);
     return;
   }
-  const int split = (int)(unit % a.splits);
-  const int64_t bh = unit / a.splits;
-  const int kh = (int)(bh % a.hk), b = (int)(bh / a.hk);
-  Seq sq;
-  if (!seq_of(a, b, sq)) return;
-  const int rows = sq.n * a.group;
-  if (rows > a.few_rows) return;
-  const int size = split_size(sq.hi - sq.lo, a.splits, kFewKeys * kFewWaves);
-  const int begin = sq.lo + split * size;
-  if (split > 0 && begin >= sq.hi) return;
-  const int end = begin + size < sq.hi ? begin + size : sq.hi;
+  int64_t x = 0, from = 0, to = 0;
+  FewUnit fu;
+  if (a.workers) {
+    const int64_t per = few_deal(a, deal);
+    from = x = unit * per;
+    to = x + per < deal.first[kDealt] ? x + per : deal.first[kDealt];
+    if (threadIdx.x == 0) {
+      int parts = 0;
+      if (x < to && to < deal.first[kDealt]) {  // the pair of the last step, and where it ends
+        int b = 0, n = kDealt;
+        while (n > 1) {
+          const int half = n >> 1;
+          if (deal.first[b + half] < to) b += half, n -= half;
+          else n = half;
+        }
+        Seq s;
+        s.n = deal.n[b], s.len = deal.len[b];
+        seq_keys(a, s);
+        const int steps = steps_of(s);
+        const int64_t kh = (to - 1 - deal.first[b]) / steps, begin = deal.first[b] + kh * steps;
+        if (begin >= from && begin + steps > to) parts = (int)((begin + steps - 1) / per - unit) + 1;
+        a.joins[4 * unit] = b, a.joins[4 * unit + 1] = (int)kh;
+      }
+      a.joins[4 * unit + 2] = parts;
+    }
+    if (x >= to) return;
+  }
+  if (a.workers) x += few_next<true>(a, deal, x, from, to, unit, fu);
+  else if (!few_split(a, unit, fu)) return;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-
-  // this lane's rows: queries, and the keys that they see
-  u32x4_t q[MT][KK];
+  u32x4_t q[MT][KK];                      // this lane's rows: queries, and the keys that they see
   int row_lo[MT], row_hi[MT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int r = mt * 16 + c;
-    const int i = r / a.group, h = kh * a.group + (r - i * a.group);
-    row_lo[mt] = 0x7fffffff, row_hi[mt] = 0;
-    if (r < rows) {
-      const int p = sq.len - sq.n + i;
-      row_hi[mt] = a.causal && p + 1 < sq.hi ? p + 1 : sq.hi;
-      row_lo[mt] = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
-      const uint16_t* x = static_cast<const uint16_t*>(a.q) + (sq.row0 + i) * a.stride_t + h * a.stride_h;
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const uint16_t* p8 = x + 64 * (kk >> 1) + 16 * g + 8 * (kk & 1);
-        if (a.vec) {
-          q[mt][kk] = *reinterpret_cast<const u32x4_t*>(p8);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) q[mt][kk][e] = uint32_t(p8[2 * e]) | uint32_t(p8[2 * e + 1]) << 16;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) q[mt][kk] = u32x4_t{0, 0, 0, 0};
-    }
-  }
-  // keys that every row sees (rows that are not there do not count)
-  int all_lo = 0, all_hi = sq.hi;
-  {
-    const int p0 = sq.len - sq.n, p1 = sq.len - 1;
-    if (a.causal && p0 + 1 < all_hi) all_hi = p0 + 1;
-    if (a.window > 0 && p1 - a.window + 1 > 0) all_lo = p1 - a.window + 1;
-  }
-
-  float m[MT], l[MT];
-  f32x4_t o[MT][DD];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    m[mt] = -kInf, l[mt] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DD; ++d) o[mt][d] = f32x4_t{0, 0, 0, 0};
-  }
-
-  const int32_t* table = a.table + (int64_t)b * a.table_stride;
-  const int tiles = (end - begin + kFewKeys - 1) / kFewKeys;
-  const int mine = tiles > wave ? (tiles - wave + kFewWaves - 1) / kFewWaves : 0;
-
-  // lane i of a batch of 32 tiles: page and scales of the 16 keys i % 2 of tile i / 2
+  int all_lo, all_hi;                     // keys that every row sees (rows that are not there do not count)
+  int kh, begin, end, mine;               // of the pair whose tiles are loaded; tiles of this wave
+  const int32_t* table;
+  // lane x of a batch of 32 tiles: page and scales of the 16 keys x % 2 of tile x / 2
   int ids = -1;
   float kss = 0.0f, vss = 0.0f;
+  auto key_of = [&](int i) { return begin + (wave + kFewWaves * i) * kFewKeys; };
   auto look_up = [&](int first) {
-    const int key = begin + (wave + kFewWaves * (first + (lane >> 1))) * kFewKeys + (lane & 1) * 16;
+    const int key = key_of(first + (lane >> 1)) + (lane & 1) * 16;
     ids = -1;
     if (key < end) {
       const int id = table[key >> a.page_log2];
@@ -248,50 +313,120 @@ __global__ void __launch_bounds__(256) kv_attn_few_kernel(AttnArgs a, int64_t un
       }
     }
   };
+  // byte of the first of the 16 keys s of tile i (a page that does not exist: some page, its keys are not seen)
+  auto place = [&](int i, int s) {
+    const int id = __builtin_amdgcn_readlane(ids, (i & 31) * 2 + s);
+    const int slot = (key_of(i) + 16 * s) & ((1 << a.page_log2) - 1);
+    return (((((int64_t)(id < 0 ? 0 : id)) * a.hk + kh) << a.page_log2) + slot) * D;
+  };
+  u32x4_t k[2][D / 64];                   // 16 bytes of a key row, 64 apart
+  uint32_t v[2][4][D / 64];               // rows 4 g + i of 16 keys
   const uint32_t k_off = (uint32_t)(c * D + 16 * g);
   const uint32_t v_off = (uint32_t)(4 * g * D + (D / 16) * c);
-  auto load = [&](FewTile<D>& t, int i) {
-    if ((i & 31) == 0) look_up(i);
-    const int key = begin + (wave + kFewWaves * i) * kFewKeys;
+  auto load_k = [&](int i) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int x = (i & 31) * 2 + s;
-      const int id = __builtin_amdgcn_readlane(ids, x);
-      t.ok[s] = id >= 0;
-      t.ks[s] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, kss), x));
-      t.vs[s] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vss), x));
-      if (!t.ok[s]) {
+      const uint8_t* p = a.k_codes + place(i, s);
 #pragma unroll
-        for (int e = 0; e < FewTile<D>::KC; ++e) t.k[s][e] = u32x4_t{0, 0, 0, 0};
+      for (int e = 0; e < D / 64; ++e) k[s][e] = *reinterpret_cast<const u32x4_t*>(p + k_off + 64 * e);
+    }
+  };
+  auto load_v = [&](int i) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int e = 0; e < FewTile<D>::VW; ++e) t.v[s][r][e] = 0;
-        continue;
-      }
-      const int64_t row = (((int64_t)id * a.hk + kh) << a.page_log2) + ((key + 16 * s) & ((1 << a.page_log2) - 1));
-      const uint8_t* kp = a.k_codes + row * D + k_off;
-      const uint8_t* vp = a.v_codes + row * D + v_off;
-#pragma unroll
-      for (int e = 0; e < FewTile<D>::KC; ++e) t.k[s][e] = *reinterpret_cast<const u32x4_t*>(kp + 64 * e);
+    for (int s = 0; s < 2; ++s) {
+      const uint8_t* p = a.v_codes + place(i, s);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if constexpr (D == 64) {
-          t.v[s][r][0] = *reinterpret_cast<const uint32_t*>(vp + r * D);
+          v[s][r][0] = *reinterpret_cast<const uint32_t*>(p + v_off + r * D);
         } else if constexpr (D == 128) {
-          const u32x2_t w = *reinterpret_cast<const u32x2_t*>(vp + r * D);
-          t.v[s][r][0] = w[0], t.v[s][r][1] = w[1];
+          const u32x2_t w = *reinterpret_cast<const u32x2_t*>(p + v_off + r * D);
+          v[s][r][0] = w[0], v[s][r][1] = w[1];
         } else {
-          const u32x4_t w = *reinterpret_cast<const u32x4_t*>(vp + r * D);
+          const u32x4_t w = *reinterpret_cast<const u32x4_t*>(p + v_off + r * D);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) t.v[s][r][e] = w[e];
+          for (int e = 0; e < 4; ++e) v[s][r][e] = w[e];
         }
       }
     }
   };
+  // 4 x 4 bytes (keys x elements) of dword h of both halves, turned to pairs of keys: element tile x of it
+  auto value_tile = [&](int h, int x, float s0, float s1) {
+    const uint32_t sel = x < 2 ? 0x05010400u : 0x07030602u;
+    const uint32_t w[4] = {__builtin_amdgcn_perm(v[0][1][h], v[0][0][h], sel), __builtin_amdgcn_perm(v[0][3][h], v[0][2][h], sel),
+                           __builtin_amdgcn_perm(v[1][1][h], v[1][0][h], sel), __builtin_amdgcn_perm(v[1][3][h], v[1][2][h], sel)};
+    return x & 1 ? u32x4_t{value_pair_hi(w[0], s0), value_pair_hi(w[1], s0), value_pair_hi(w[2], s1), value_pair_hi(w[3], s1)}
+                 : u32x4_t{value_pair_lo(w[0], s0), value_pair_lo(w[1], s0), value_pair_lo(w[2], s1), value_pair_lo(w[3], s1)};
+  };
+  auto whole_tile = [&](int i, bool ok) { return ok && key_of(i) >= all_lo && key_of(i) + kFewKeys <= all_hi; };
+  // What comes before a unit's first tile, and that tile's loads.
+  auto start = [&]() {
+    const Seq& sq = fu.sq;
+    const int rows = sq.n * a.group;
+    kh = fu.kh, begin = fu.begin, end = fu.end;
+    table = a.table + (int64_t)fu.b * a.table_stride;
+    int tiles = end > begin ? (end - begin + kFewKeys - 1) / kFewKeys : 0;
+    if (tiles && a.num_pages == 0) {
+      tiles = 0;
+      if (a.err) *a.err = 1;
+    }
+    mine = tiles > wave ? (tiles - wave + kFewWaves - 1) / kFewWaves : 0;
+    if (mine > 0) look_up(0);
+    all_lo = 0, all_hi = sq.hi;
+    const int p0 = sq.len - sq.n, p1 = sq.len - 1;
+    if (a.causal && p0 + 1 < all_hi) all_hi = p0 + 1;
+    if (a.window > 0 && p1 - a.window + 1 > 0) all_lo = p1 - a.window + 1;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int r = mt * 16 + c;
+      const int i = r / a.group, h = kh * a.group + (r - i * a.group);
+      row_lo[mt] = 0x7fffffff, row_hi[mt] = 0;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) q[mt][kk] = u32x4_t{0, 0, 0, 0};
+      if (r < rows) {
+        const int p = sq.len - sq.n + i;
+        row_hi[mt] = a.causal && p + 1 < sq.hi ? p + 1 : sq.hi;
+        row_lo[mt] = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
+        const uint16_t* y = static_cast<const uint16_t*>(a.q) + (sq.row0 + i) * a.stride_t + h * a.stride_h;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          const uint16_t* p8 = y + 64 * (kk >> 1) + 16 * g + 8 * (kk & 1);
+          if (a.vec) {
+            q[mt][kk] = *reinterpret_cast<const u32x4_t*>(p8);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[mt][kk][e] = uint32_t(p8[2 * e]) | uint32_t(p8[2 * e + 1]) << 16;
+          }
+        }
+      }
+    }
+    if (mine > 0) {
+      load_k(0);
+      load_v(0);
+    }
+  };
+  start();
 
-  auto work = [&](FewTile<D>& t, int i) {
-    const int key = begin + (wave + kFewWaves * i) * kFewKeys;
+#pragma unroll 1
+  for (;;) {
+  float m[MT], l[MT];
+  f32x4_t o[MT][DD];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    m[mt] = -kInf, l[mt] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DD; ++d) o[mt][d] = f32x4_t{0, 0, 0, 0};
+  }
+  // A NaN value must not reach rows that do not see its key (0 * NaN).  Where some row sees a tile in part, NaN codes are
+  // taken out here and brought to the rows that see them after the loop.
+  bool odd = false;
+#pragma unroll 1
+  for (int i = 0; i < mine; ++i) {
+    const int x0 = (i & 31) * 2;
+    auto lane_f = [&](float f, int x) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), x)); };
+    const bool ok[2] = {__builtin_amdgcn_readlane(ids, x0) >= 0, __builtin_amdgcn_readlane(ids, x0 + 1) >= 0};
+    const float ks[2] = {a.scale2 * lane_f(kss, x0), a.scale2 * lane_f(kss, x0 + 1)};
+    const float vs[2] = {lane_f(vss, x0), lane_f(vss, x0 + 1)};
     f32x4_t s[MT][2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -299,36 +434,34 @@ __global__ void __launch_bounds__(256) kv_attn_few_kernel(AttnArgs a, int64_t un
       for (int mt = 0; mt < MT; ++mt) s[mt][x] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
-        const uint32_t w0 = t.k[x][kk >> 1][2 * (kk & 1)], w1 = t.k[x][kk >> 1][2 * (kk & 1) + 1];
+        const uint32_t w0 = k[x][kk >> 1][2 * (kk & 1)], w1 = k[x][kk >> 1][2 * (kk & 1) + 1];
         const u32x4_t kf = {code_pair<DT>(w0, false), code_pair<DT>(w0, true), code_pair<DT>(w1, false), code_pair<DT>(w1, true)};
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) s[mt][x] = mfma16<DT>(kf, q[mt][kk], s[mt][x]);
       }
     }
-    const bool whole = t.ok[0] && t.ok[1] && key >= all_lo && key + kFewKeys <= all_hi;
-    u32x4_t p[MT], seen[MT];
+    if (i + 1 < mine) {
+      if (((i + 1) & 31) == 0) look_up(i + 1);
+      load_k(i + 1);
+    }
+    const int key = key_of(i);
+    const bool whole = whole_tile(i, ok[0] && ok[1]);
+    u32x4_t p[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      float v[8];
+      float w[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = s[mt][e >> 2][e & 3] * (a.scale2 * t.ks[e >> 2]);
-      uint32_t sees = 0xffu;
+      for (int e = 0; e < 8; ++e) w[e] = s[mt][e >> 2][e & 3] * ks[e >> 2];
       if (!whole) {
-        sees = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int j = key + 16 * (e >> 2) + 4 * g + (e & 3);
-          const bool on = t.ok[e >> 2] && j >= row_lo[mt] && j < row_hi[mt];
-          v[e] = on ? v[e] : -kInf;
-          sees |= on ? 1u << e : 0u;
+          w[e] = ok[e >> 2] && j >= row_lo[mt] && j < row_hi[mt] ? w[e] : -kInf;
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          seen[mt][e] = ((sees >> (2 * e)) & 1u ? 0x3f80u : 0u) | ((sees >> (2 * e + 1)) & 1u ? 0x3f800000u : 0u);
       }
-      float top = v[0];
+      float top = w[0];
 #pragma unroll
-      for (int e = 1; e < 8; ++e) top = fmaxf(top, v[e]);
+      for (int e = 1; e < 8; ++e) top = fmaxf(top, w[e]);
       // the maximum moves only where a weight would pass 2^8: sums and products lose nothing by that
       if (__any(top > m[mt] + 8.0f)) {
         top = fmaxf(top, __shfl_xor(top, 16));
@@ -342,13 +475,10 @@ __global__ void __launch_bounds__(256) kv_attn_few_kernel(AttnArgs a, int64_t un
       }
       const float base = m[mt] == -kInf ? 0.0f : m[mt];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = __builtin_amdgcn_exp2f(v[e] - base);
-      l[mt] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-      p[mt] = u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+      for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(w[e] - base);
+      l[mt] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+      p[mt] = u32x4_t{pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]), pack_bf16x2(w[4], w[5]), pack_bf16x2(w[6], w[7])};
     }
-    // a NaN value must not reach rows that do not see it (0 * NaN): in a tile that some row sees in part, NaN codes are
-    // taken out and counted by a product of their own
-    bool odd = false;
     if (!whole) {
       uint32_t any = 0;
 #pragma unroll
@@ -356,31 +486,50 @@ __global__ void __launch_bounds__(256) kv_attn_few_kernel(AttnArgs a, int64_t un
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-          for (int e = 0; e < FewTile<D>::VW; ++e) any |= nan_bytes(t.v[x][r][e]);
-      odd = __any(any != 0);
+          for (int e = 0; e < D / 64; ++e) {
+            const uint32_t n = nan_bytes(v[x][r][e]);
+            any |= n;
+            v[x][r][e] &= ~((n >> 7) * 0xffu);
+          }
+      odd = odd || __any(any != 0);
     }
 #pragma unroll
-    for (int h = 0; h < FewTile<D>::VW; ++h) {
-      // 4 x 4 bytes (keys x elements) of each 16 keys, turned to pairs of keys
-      uint32_t w01[2][2], w23[2][2];
+    for (int h = 0; h < D / 64; ++h)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        w01[x][0] = __builtin_amdgcn_perm(t.v[x][1][h], t.v[x][0][h], 0x05010400u);
-        w01[x][1] = __builtin_amdgcn_perm(t.v[x][1][h], t.v[x][0][h], 0x07030602u);
-        w23[x][0] = __builtin_amdgcn_perm(t.v[x][3][h], t.v[x][2][h], 0x05010400u);
-        w23[x][1] = __builtin_amdgcn_perm(t.v[x][3][h], t.v[x][2][h], 0x07030602u);
+      for (int x = 0; x < 4; ++x) {
+        const u32x4_t vf = value_tile(h, x, vs[0], vs[1]);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) o[mt][4 * h + x] = mfma16x16x32(vf, p[mt], o[mt][4 * h + x]);
       }
-      if (odd) {
+    if (i + 1 < mine) load_v(i + 1);
+  }
+  if (odd) {  // once more over the tiles that are seen in part: ones for NaN, ones for seen keys
+#pragma unroll 1
+    for (int i = 0; i < mine; ++i) {
+      if ((i & 31) == 0) look_up(i);
+      const bool ok[2] = {__builtin_amdgcn_readlane(ids, (i & 31) * 2) >= 0, __builtin_amdgcn_readlane(ids, (i & 31) * 2 + 1) >= 0};
+      if (whole_tile(i, ok[0] && ok[1])) continue;
+      load_v(i);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int e = 0; e < D / 64; ++e) v[x][r][e] = (nan_bytes(v[x][r][e]) >> 7) * 0x38u;  // the code of 1
+      u32x4_t seen[MT];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = key_of(i) + 16 * (e >> 1) + 4 * g + 2 * (e & 1);
+          seen[mt][e] = (ok[e >> 1] && j >= row_lo[mt] && j < row_hi[mt] ? 0x3f80u : 0u) |
+                        (ok[e >> 1] && j + 1 >= row_lo[mt] && j + 1 < row_hi[mt] ? 0x3f800000u : 0u);
+        }
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          u32x4_t ones;
-          const bool hi = x & 1;
-          const uint32_t src[4] = {w01[0][x >> 1], w23[0][x >> 1], w01[1][x >> 1], w23[1][x >> 1]};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t nb = nan_bytes(src[e]) >> (hi ? 16 : 0);
-            ones[e] = (nb & 0x80u ? 0x3f80u : 0u) | (nb & 0x8000u ? 0x3f800000u : 0u);
-          }
+          const u32x4_t ones = value_tile(h, x, 1.0f, 1.0f);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
             const f32x4_t hits = mfma16x16x32(ones, seen[mt], f32x4_t{0, 0, 0, 0});
@@ -388,48 +537,18 @@ __global__ void __launch_bounds__(256) kv_attn_few_kernel(AttnArgs a, int64_t un
             for (int e = 0; e < 4; ++e) o[mt][4 * h + x][e] += hits[e] > 0.0f ? __builtin_nanf("") : 0.0f;
           }
         }
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t n0 = nan_bytes(w01[x][e]), n1 = nan_bytes(w23[x][e]);
-            w01[x][e] &= ~((n0 >> 7) * 0xffu);
-            w23[x][e] &= ~((n1 >> 7) * 0xffu);
-          }
-      }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int hf = x >> 1;
-        const u32x4_t vf = x & 1 ? u32x4_t{value_pair_hi(w01[0][hf], t.vs[0]), value_pair_hi(w23[0][hf], t.vs[0]),
-                                           value_pair_hi(w01[1][hf], t.vs[1]), value_pair_hi(w23[1][hf], t.vs[1])}
-                                 : u32x4_t{value_pair_lo(w01[0][hf], t.vs[0]), value_pair_lo(w23[0][hf], t.vs[0]),
-                                           value_pair_lo(w01[1][hf], t.vs[1]), value_pair_lo(w23[1][hf], t.vs[1])};
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) o[mt][4 * h + x] = mfma16x16x32(vf, p[mt], o[mt][4 * h + x]);
-      }
-    }
-  };
-
-  if constexpr (D * MT > 256) {  // the registers hold one tile
-    for (int i = 0; i < mine; ++i) {
-      FewTile<D> t0;
-      load(t0, i);
-      work(t0, i);
-    }
-  } else if (mine > 0) {
-    FewTile<D> t0, t1;
-    load(t0, 0);
-    for (int i = 0; i < mine; i += 2) {
-      if (i + 1 < mine) load(t1, i + 1);
-      work(t0, i);
-      if (i + 1 < mine) {
-        if (i + 2 < mine) load(t0, i + 2);
-        work(t1, i + 1);
-      }
     }
   }
 
-  // join the waves: the sums of a row are spread over its four lanes
+  // the next pair's first loads are in flight while this one's waves join
+  const FewUnit cur = fu;
+  const int rows = cur.sq.n * a.group;
+  const bool more = x < to;
+  if (more) {
+    x += few_next<false>(a, deal, x, from, to, unit, fu);
+    start();
+  }
+  // the sums of a row are spread over its four lanes
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     l[mt] += __shfl_xor(l[mt], 16);
@@ -440,7 +559,6 @@ __global__ void __launch_bounds__(256) kv_attn_few_kernel(AttnArgs a, int64_t un
     }
   }
   __syncthreads();
-  const int used = sq.hi > sq.lo ? (sq.hi - sq.lo + size - 1) / size : 1;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     const int r = mt * 16 + c;
@@ -448,6 +566,13 @@ __global__ void __launch_bounds__(256) kv_attn_few_kernel(AttnArgs a, int64_t un
 #pragma unroll
     for (int w = 1; w < kFewWaves; ++w) top = fmaxf(top, ml[w][0][r]);
     const float f = m[mt] == -kInf ? (l[mt] != l[mt] ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(m[mt] - top);
+    if (wave == 0 && g == 0) {  // maximum and sum of the row
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kFewWaves; ++w)
+        sum += ml[w][1][r] * (ml[w][0][r] == -kInf ? 1.0f : __builtin_amdgcn_exp2f(ml[w][0][r] - top));
+      ml[kFewWaves][0][r] = top, ml[kFewWaves][1][r] = sum;
+    }
     if (mt) __syncthreads();
     if (r < rows) {
 #pragma unroll
@@ -458,27 +583,22 @@ __global__ void __launch_bounds__(256) kv_attn_few_kernel(AttnArgs a, int64_t un
               f32x4_t{o[mt][d][e] * f, o[mt][d + 1][e] * f, o[mt][d + 2][e] * f, o[mt][d + 3][e] * f};
     }
     __syncthreads();
-    for (int x = threadIdx.x; x < 16 * D; x += 256) {
-      const int rr = x / D, d = x - rr * D, row = mt * 16 + rr;
-      if (row >= rows) break;
-      float top_r = ml[0][0][row];
+    const int here = rows - mt * 16 < 16 ? rows - mt * 16 : 16;
+    for (int i4 = threadIdx.x; i4 < here * (D / 4); i4 += 256) {
+      const int rr = i4 / (D / 4), d = 4 * (i4 - rr * (D / 4)), row = mt * 16 + rr;
+      f32x4_t acc = {0, 0, 0, 0};
 #pragma unroll
-      for (int w = 1; w < kFewWaves; ++w) top_r = fmaxf(top_r, ml[w][0][row]);
-      float sum = 0.0f, acc = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kFewWaves; ++w) {
-        const float lw = ml[w][1][row];
-        sum += lw * (ml[w][0][row] == -kInf ? 1.0f : __builtin_amdgcn_exp2f(ml[w][0][row] - top_r));
-        acc += red[w][rr][d];
-      }
-      if (used == 1) {
-        const int i = row / a.group, h = kh * a.group + (row - i * a.group);
-        const int64_t at = (sq.row0 + i) * a.hq + h;
-        store_out(a, DT, at * D + d, sum != 0.0f ? acc / sum : 0.0f);
+      for (int w = 0; w < kFewWaves; ++w) acc += *reinterpret_cast<const f32x4_t*>(&red[w][rr][d]);
+      const float top_r = ml[kFewWaves][0][row], sum = ml[kFewWaves][1][row];
+      if (cur.alone) {
+        const int i = row / a.group, h = cur.kh * a.group + (row - i * a.group);
+        const int64_t at = (cur.sq.row0 + i) * a.hq + h;
+        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+        store4<DT>(a.out, at * D + d, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
         if (d == 0 && a.lse) a.lse[at] = sum != 0.0f ? (top_r + __builtin_amdgcn_logf(sum)) * kLn2 : -kInf;
       } else {
-        const int64_t at = unit * a.row_stride + row;
-        a.part_o[at * D + d] = acc;
+        const int64_t at = cur.slot * a.row_stride + row;
+        *reinterpret_cast<f32x4_t*>(a.part_o + at * D + d) = acc;
         if (d == 0) {
           a.part_ml[2 * at] = top_r;
           a.part_ml[2 * at + 1] = sum;
@@ -486,37 +606,77 @@ __global__ void __launch_bounds__(256) kv_attn_few_kernel(AttnArgs a, int64_t un
       }
     }
   }
+  if (!more) return;
+  __syncthreads();
+  }
 }
 
-// Joins the `used` partial results of one row, `step` rows apart from `first`; one wave.
-template <int DT, int D>
-__device__ __forceinline__ void join_row(const AttnArgs& a, int64_t first, int64_t step, int used, int64_t at) {
+// Joins the `used` partial results of one row, in the workspace rows at(0 .. used - 1), in a wave (W = 1) or by the W waves of
+// a block.  A lane holds the maximum and sum of one split, so that only the rows of O are read one after the other.
+template <int DT, int D, int W, typename F>
+__device__ __forceinline__ void join_row(const AttnArgs& a, int used, int64_t out, F at) {
   constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
-  float top = -kInf;
-  for (int s = lane; s < used; s += 64) top = fmaxf(top, a.part_ml[2 * (first + s * step)]);
-  top = group_max(top, 64);
-  float sum = 0.0f, acc[E];
+  __shared__ float part[W][D + 1];
+  __shared__ float tops[W];
+  const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6;
+  const int s0 = (int)((int64_t)used * wave / W), s1 = (int)((int64_t)used * (wave + 1) / W);
+  float top = -kInf, sum = 0.0f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-#pragma unroll 4
-  for (int s = 0; s < used; ++s) {
-    const int64_t pr = first + s * step;
-    const float m = a.part_ml[2 * pr], l = a.part_ml[2 * pr + 1];
-    const float f = m == -kInf ? (l != l ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(m - top);
-    sum += l * f;
+  for (int base = s0; base < s1; base += 64) {
+    float m = -kInf, l = 0.0f;
+    if (base + lane < s1) {
+      const int64_t pr = at(base + lane);
+      m = a.part_ml[2 * pr], l = a.part_ml[2 * pr + 1];
+    }
+    const float now = fmaxf(top, group_max(m, 64));
+    const float back = top == -kInf ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+    const float f = m == -kInf ? (l != l ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(m - now);
+    sum = sum * back + group_sum(l * f, 64);
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += a.part_o[pr * D + lane * E + e] * f;
+    for (int e = 0; e < E; ++e) acc[e] *= back;
+    top = now;
+    const int n = s1 - base < 64 ? s1 - base : 64;
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) {
+      const float fs = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s));
+      const float* o = a.part_o + at(base + s) * D + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(o[e], fs, acc[e]);
+    }
+  }
+  if constexpr (W > 1) {
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+    float all = tops[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) all = fmaxf(all, tops[w]);
+    const float f = top == -kInf ? (sum != sum ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(top - all);
+#pragma unroll
+    for (int e = 0; e < E; ++e) part[wave][lane * E + e] = acc[e] * f;
+    if (lane == 0) part[wave][D] = sum * f;
+    __syncthreads();
+    if (wave) return;
+    sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      sum += part[w][D];
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += part[w][lane * E + e];
+    }
+    top = all;
   }
 #pragma unroll
-  for (int e = 0; e < E; ++e) store_out(a, DT, at * D + lane * E + e, sum != 0.0f ? acc[e] / sum : 0.0f);
-  if (lane == 0 && a.lse) a.lse[at] = sum != 0.0f ? (top + __builtin_amdgcn_logf(sum)) * kLn2 : -kInf;
+  for (int e = 0; e < E; ++e) store_out(a, DT, out * D + lane * E + e, sum != 0.0f ? acc[e] / sum : 0.0f);
+  if (lane == 0 && a.lse) a.lse[out] = sum != 0.0f ? (top + __builtin_amdgcn_logf(sum)) * kLn2 : -kInf;
 }
 
-// Joins the splits of the few-rows kernel: one wave per row.
-template <int DT, int D>
+// Joins the equal parts of the few-rows kernel's pairs: W waves per row.
+template <int DT, int D, int W>
 __global__ void __launch_bounds__(256) kv_attn_join_kernel(AttnArgs a, int64_t units) {
-  const int64_t x = linear_block() * 4 + (threadIdx.x >> 6);
+  const int64_t x = W == 1 ? linear_block() * 4 + (threadIdx.x >> 6) : linear_block();
   if (x >= units) return;
   const int row = (int)(x % a.row_stride);
   const int64_t bh = x / a.row_stride;
@@ -525,11 +685,26 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(AttnArgs a, int64_t u
   if (!seq_of(a, b, sq)) return;
   const int64_t rows = (int64_t)sq.n * a.group;
   if (rows > a.few_rows || row >= rows) return;
-  const int size = split_size(sq.hi - sq.lo, a.splits, kFewKeys * kFewWaves);
+  const int size = split_size(sq.hi - sq.lo, a.splits, kFewStep);
   const int used = sq.hi > sq.lo ? (sq.hi - sq.lo + size - 1) / size : 1;
   if (used == 1) return;
   const int i = row / a.group, h = kh * a.group + (row - i * a.group);
-  join_row<DT, D>(a, bh * a.splits * a.row_stride + row, a.row_stride, used, (sq.row0 + i) * a.hq + h);
+  join_row<DT, D, W>(a, used, (sq.row0 + i) * a.hq + h, [&](int s) { return (bh * a.splits + s) * a.row_stride + row; });
+}
+
+// Joins the dealt pairs: a workgroup for each that began a pair and did not end it, a wave per row in turn.
+template <int DT, int D>
+__global__ void __launch_bounds__(256) kv_attn_dealt_join_kernel(AttnArgs a) {
+  const int64_t w = blockIdx.x;
+  const int parts = a.joins[4 * w + 2];
+  if (parts < 2) return;
+  const int b = a.joins[4 * w], kh = a.joins[4 * w + 1];
+  const int64_t row0 = a.cu[b];
+  const int rows = (int)(a.cu[b + 1] - row0) * a.group;
+  for (int row = threadIdx.x >> 6; row < rows; row += 4) {
+    const int i = row / a.group, h = kh * a.group + (row - i * a.group);
+    join_row<DT, D, 1>(a, parts, (row0 + i) * a.hq + h, [&](int s) { return (2 * (w + s) + (s == 0)) * a.row_stride + row; });
+  }
 }
 
 // ---- many rows ---------------------------------------------------------------------
@@ -917,16 +1092,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
 #pragma unroll
     for (int d = 0; d < DD; ++d)
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const float w[4] = {o[d][e] * f, o[d][e + 1] * f, o[d][e + 2] * f, o[d][e + 3] * f};
-        u32x2_t y;
-        if constexpr (DT == PDM_BF16) {
-          y = u32x2_t{pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3])};
-        } else {
-          y = u32x2_t{f32_to_f16_bits(w[0]) | f32_to_f16_bits(w[1]) << 16, f32_to_f16_bits(w[2]) | f32_to_f16_bits(w[3]) << 16};
-        }
-        *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.out) + at * D + 32 * d + 2 * e + 4 * h) = y;
-      }
+      for (int e = 0; e < 16; e += 4)
+        store4<DT>(a.out, at * D + 32 * d + 2 * e + 4 * h, o[d][e] * f, o[d][e + 1] * f, o[d][e + 2] * f, o[d][e + 3] * f);
     if (h == 0 && a.lse) a.lse[at] = sum != 0.0f ? (m + __builtin_amdgcn_logf(sum)) * kLn2 : -kInf;
   } else {
     const int64_t pr = ((item * a.hk + kh) * a.splits + split) * kManyRows + wave * 32 + c;
@@ -961,7 +1128,7 @@ __global__ void __launch_bounds__(256) kv_attn_many_join_kernel(AttnArgs a, int6
   const int used = hi > lo ? (hi - lo + size - 1) / size : 1;
   if (used == 1) return;
   const int i = r / a.group, h = kh * a.group + (r - i * a.group);
-  join_row<DT, D>(a, ih * a.splits * kManyRows + in, kManyRows, used, (sq.row0 + i) * a.hq + h);
+  join_row<DT, D, 1>(a, used, (sq.row0 + i) * a.hq + h, [&](int x) { return (ih * a.splits + x) * kManyRows + in; });
 }
 
 // ---- host -----------------------------------------------------------------------
@@ -986,8 +1153,8 @@ int check(const char* fn, const pdm_kv_attention_desc* d, const pdm_kv_cache* c,
 struct Plan {
   int mt;                // tiles of 16 rows of the few-rows kernel
   bool few, many;        // which kernels may have work
-  int splits, row_stride;
-  int64_t part_rows;
+  int splits, workers, row_stride;
+  int64_t units, part_rows;
   int many_splits;
   int64_t items, many_part_rows;
 };
@@ -997,18 +1164,21 @@ Plan plan_of(const pdm_kv_attention_desc* d, const pdm_kv_cache* c, const pdm_kv
   const int64_t group = d->n_q_heads / c->n_kv_heads;
   const int64_t max_q = d->max_q_len < b->tokens ? d->max_q_len : b->tokens;
   const int64_t rows = max_q * group;
-  p.mt = group <= 16 && (rows <= 16 || rows > 32) ? 1 : 2;
+  p.mt = c->head_dim == 256 || (group <= 16 && (rows <= 16 || rows > 32)) ? 1 : 2;
   p.few = group <= 16 * p.mt;
   p.many = rows > 16 * p.mt;
   const int64_t most = (int64_t)b->table_width * c->page_size;
   const int64_t pairs = (int64_t)(b->num_seqs > 0 ? b->num_seqs : 1) * c->n_kv_heads;
-  int64_t splits = (2048 + pairs - 1) / pairs;
-  const int64_t cap = (most + 127) / 128;
+  const int64_t cap = (most + kFewStep - 1) / kFewStep;  // steps of a pair
+  const int resident = 256 * (c->head_dim * p.mt <= 64 ? 4 : c->head_dim * p.mt <= 128 ? 3 : 2);
+  p.workers = p.few && b->num_seqs > 1 && b->num_seqs <= kDealt && pairs >= 256 && pairs < 2048 && rows <= 8 && pairs * cap > resident
+                  ? resident : 0;
+  int64_t splits = p.workers || pairs >= 1024 ? 1 : resident / pairs;
   splits = splits < cap ? splits : cap;
-  splits = splits < 256 ? splits : 256;
   p.splits = (int)(splits > 1 ? splits : 1);
+  p.units = p.workers ? p.workers : pairs * p.splits;
   p.row_stride = (int)(rows < 16 * p.mt ? rows : 16 * p.mt);
-  p.part_rows = p.few && p.splits > 1 ? pairs * p.splits * p.row_stride : 0;
+  p.part_rows = !p.few ? 0 : p.workers ? 2 * p.workers * p.row_stride : p.splits > 1 ? p.units * p.row_stride : 0;
   if (p.many) {
     p.items = b->tokens * group / kManyRows + b->num_seqs;
     const int64_t blocks = p.items * c->n_kv_heads;
@@ -1025,17 +1195,20 @@ int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 
 // The two kernels run one after the other, each with its join: they share the workspace.
 int64_t part_rows_of(const Plan& p) { return p.part_rows > p.many_part_rows ? p.part_rows : p.many_part_rows; }
-int64_t workspace_of(const Plan& p, int D) { return round256(part_rows_of(p) * D * 4) + round256(part_rows_of(p) * 8); }
+int64_t workspace_of(const Plan& p, int D) { return round256(part_rows_of(p) * D * 4) + round256(part_rows_of(p) * 8) + round256((int64_t)p.workers * 16); }
 
 template <int DT, int D>
 void launch(AttnArgs& a, const Plan& p, hipStream_t st) {
-  const int64_t units = p.few ? (int64_t)a.seqs * a.hk * a.splits : 0, guards = (a.tokens + 255) / 256;
+  const int64_t units = p.few && a.seqs ? p.units : 0, guards = (a.tokens + 255) / 256;
   const dim3 grid = linear_grid(units + guards);
   if (p.mt == 1) kv_attn_few_kernel<DT, D, 1><<<grid, 256, 0, st>>>(a, units, guards);
-  else kv_attn_few_kernel<DT, D, 2><<<grid, 256, 0, st>>>(a, units, guards);
-  if (p.part_rows) {
+  else if constexpr (D < 256) kv_attn_few_kernel<DT, D, 2><<<grid, 256, 0, st>>>(a, units, guards);  // more rows of 256 spill
+  if (p.workers) {
+    kv_attn_dealt_join_kernel<DT, D><<<(unsigned)p.workers, 256, 0, st>>>(a);
+  } else if (p.part_rows) {
     const int64_t rows = (int64_t)a.seqs * a.hk * a.row_stride;
-    kv_attn_join_kernel<DT, D><<<linear_grid((rows + 3) / 4), 256, 0, st>>>(a, rows);
+    if (rows < 4096) kv_attn_join_kernel<DT, D, 4><<<linear_grid(rows), 256, 0, st>>>(a, rows);
+    else kv_attn_join_kernel<DT, D, 1><<<linear_grid((rows + 3) / 4), 256, 0, st>>>(a, rows);
   }
   if (!p.many) return;
   a.splits = p.many_splits;
@@ -1085,13 +1258,14 @@ extern "C" int pdm_kv_attention_fwd(const pdm_kv_attention_desc* d, const pdm_kv
   a.cu = b->cu_seqlens, a.table = b->page_table, a.lens = b->seq_lens, a.err = err_flag;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + o_bytes);
+  a.joins = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + o_bytes + round256(part_rows_of(p) * 8));
   a.tokens = b->tokens, a.table_stride = b->table_stride, a.num_pages = c->num_pages;
   a.stride_t = d->q_stride_t, a.stride_h = d->q_stride_h;
   a.seqs = b->num_seqs, a.hq = d->n_q_heads, a.hk = c->n_kv_heads, a.group = d->n_q_heads / c->n_kv_heads;
   a.page_log2 = log2_of(c->page_size), a.table_width = b->table_width;
   a.max_q = d->max_q_len;
   a.causal = d->causal != 0, a.window = d->window;
-  a.splits = p.splits, a.row_stride = p.row_stride, a.few_rows = p.few ? 16 * p.mt : 0;
+  a.splits = p.splits, a.workers = p.workers, a.row_stride = p.row_stride, a.few_rows = p.few ? 16 * p.mt : 0;
   a.vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && d->q_stride_t % 8 == 0 && d->q_stride_h % 8 == 0;
   a.scale2 = d->scale * 1.44269504088896341f;
   if (d->dtype == PDM_BF16) launch_dt<PDM_BF16>(a, c->head_dim, p, stream);

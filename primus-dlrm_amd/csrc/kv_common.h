@@ -192,7 +192,7 @@ inline int check_cache(const char* fn, const pdm_kv_cache* c, const pdm_kv_batch
   if (b->tokens < 0 || b->num_seqs < 0 || b->table_width < 0 || b->table_stride < 0) return bad("negative sizes");
   if (b->tokens >= (int64_t(1) << 31)) return bad("tokens must be below 2^31");
   if (b->num_seqs > (1 << 24)) return bad("num_seqs must not exceed 2^24");
-  if ((int64_t)b->table_width * c->page_size > 0x7fffffff) return bad("table_width * page_size must be below 2^31");
+  if ((int64_t)b->table_width * c->page_size > (1 << 30)) return bad("table_width * page_size must not exceed 2^30");
   if (c->num_pages && !(c->k_codes && c->v_codes && c->k_scale && c->v_scale)) return bad("null cache");
   if (((reinterpret_cast<uintptr_t>(c->k_codes) | reinterpret_cast<uintptr_t>(c->v_codes)) & 15) != 0)
     return bad("codes must be 16-byte aligned");
