@@ -29,10 +29,10 @@ struct AppendArgs {
 
 // Where one page's share of a call's tokens lies.
 struct Segment {
-  int64_t row0;     // token row of its first token
-  int64_t index0;   // that token's index in the sequence
-  int64_t page_id;
-  int slot0, n;     // first slot and number of tokens
+  int64_t row0;          // token row of its first token
+  int64_t index0;        // that token's index in the sequence
+  const int32_t* entry;  // its page
+  int slot0, n;          // first slot and number of tokens
 };
 
 // Item i of the list of (sequence, touched page): sequence b's span begins at cu[b] / page + 2 b and is never
@@ -58,163 +58,282 @@ __device__ __forceinline__ bool find_segment(const AppendArgs& a, int64_t item, 
     if (a.err) *a.err = 1;
     return false;
   }
-  const int64_t id = a.table[(int64_t)b * a.table_stride + page];
-  if (id < 0 || id >= a.num_pages) {
-    if (a.err) *a.err = 1;
-    return false;
-  }
   const int64_t lo = start > (page << lg) ? start : page << lg;
   const int64_t hi = len < ((page + 1) << lg) ? len : (page + 1) << lg;
   g.row0 = c0 + (lo - start);
   g.index0 = lo;
-  g.page_id = id;
+  g.entry = a.table + (int64_t)b * a.table_stride + page;
   g.slot0 = (int)(lo - (page << lg));
   g.n = (int)(hi - lo);
   return true;
 }
 
-// One (page, head, keys or values) per W waves, NI rows of a page per lane group: the values stay in
-// registers between the maximum and the codes.
+// The segment's page, -1 where it does not exist.  (Looked up after the rows' loads have been issued.)
+__device__ __forceinline__ int64_t page_of(const AppendArgs& a, const Segment& g) {
+  const int64_t id = *g.entry;
+  if (id >= 0 && id < a.num_pages) return id;
+  if (a.err) *a.err = 1;
+  return -1;
+}
+
+// A lane's 16 elements of a row as they are stored, and as fp32.
+template <int DT>
+struct Row {
+  u32x4_t w[DT == PDM_F32 ? 4 : 2];
+};
+
+template <int DT, bool VEC>
+__device__ __forceinline__ void load_row(const AppendArgs& a, int kv, int h, int64_t row, const RowPlace& pl, Row<DT>& x) {
+  const int64_t at = row * a.stride_t[kv] + h * a.stride_h[kv];
+  load8_raw<DT, VEC>(a.x[kv], at + pl.lo, x.w);
+  load8_raw<DT, VEC>(a.x[kv], at + pl.hi, x.w + (DT == PDM_F32 ? 2 : 1));
+}
+
+template <int DT>
+__device__ __forceinline__ void to_float(const Row<DT>& x, float* v) {
+  raw_to_float<DT>(x.w, v);
+  raw_to_float<DT>(x.w + (DT == PDM_F32 ? 2 : 1), v + 8);
+}
+
+// A key row normed and rotated, in 64 bits (as fast as 32 here): its code is the nearest to the key itself, whatever the
+// order of the sum.  Called by the row's whole group; `ok`: this row exists.
+template <bool NORM, bool INTER>
+__device__ __forceinline__ void key_row(const AppendArgs& a, const Segment& g, int r, bool ok, int j, const RowPlace& pl, float* v) {
+  double rs = 1.0;
+  if (NORM) {
+    double ss = 0.0;
+    if (ok) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) ss = __builtin_fma((double)v[e], (double)v[e], ss);
+    }
+    for (int o = 1; o < 1 << a.width_log2; o <<= 1) ss += __shfl_xor(ss, o);
+    rs = 1.0 / sqrt(ss / (double)a.D + (double)a.eps);
+  }
+  if (!ok) return;
+  float w[16], c[8], s[8];
+  if (NORM) {
+    load8f(a.w + pl.lo, w);
+    load8f(a.w + pl.hi, w + 8);
+  }
+  bool zero = false;
+  if (pl.turned) {
+    const int64_t p = a.positions ? load_position(a.positions, a.bits, g.row0 + r) : g.index0 + r;
+    zero = p < 0 || p >= a.table_rows;
+    if (zero) {
+      if (a.err) *a.err = 1;
+    } else {
+      load8f(a.cos + p * (a.R / 2) + 8 * j, c);
+      load8f(a.sin + p * (a.R / 2) + 8 * j, s);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int ia = INTER ? 2 * i : i, ib = INTER ? 2 * i + 1 : i + 8;
+    double x = v[ia], y = v[ib];
+    if (NORM) x = x * rs * (double)w[ia], y = y * rs * (double)w[ib];
+    if (pl.turned) {
+      const double t = x * (double)c[i] - y * (double)s[i];
+      y = y * (double)c[i] + x * (double)s[i];
+      x = t;
+    }
+    v[ia] = zero ? 0.0f : (float)x;
+    v[ib] = zero ? 0.0f : (float)y;
+  }
+}
+
+// Largest finite magnitude.  (fmaxf passes over NaN; an infinity is rare.)
+__device__ __forceinline__ float row_max(const float* v) {
+  float m = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(v[e]));
+  if (m == __builtin_inff()) {
+    m = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(v[e]) < __builtin_inff() ? fabsf(v[e]) : 0.0f);
+  }
+  return m;
+}
+
+// The exponent of a page's head for new values of at most `amax`, its own if that is larger (`slot0` tokens are there already
+// and `held` is their exponent); codes that are there are brought to a larger one, thread `tid` of `threads`.
+__device__ __forceinline__ int settle_scale(float amax, int slot0, int held, uint8_t* page, int D, int tid, int threads) {
+  const int e = scale_exponent(amax);
+  if (slot0 == 0) return e;
+  if (e <= held) return held;
+  const float f = exp2_int(held - e > -126 ? held - e : -126);
+  for (int i = tid; i < slot0 * D / 16; i += threads) {
+    u32x4_t* p = reinterpret_cast<u32x4_t*>(page) + i;
+    u32x4_t c = *p;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[d], false);
+      const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[d], true);
+      const float x[4] = {lo[0] * f, lo[1] * f, hi[0] * f, hi[1] * f};
+      c[d] = e4m3x4(x);
+    }
+    *p = c;
+  }
+  return e;
+}
+
+__device__ __forceinline__ void store_codes(uint8_t* row, const RowPlace& pl, float* v, int e) {
+  const float inv = exp2_int(-e);
+#pragma unroll
+  for (int d = 0; d < 16; ++d) v[d] *= inv;
+  if (e == kScaleExpMax) {
+#pragma unroll
+    for (int d = 0; d < 16; ++d) v[d] = e4m3_saturated(v[d]);
+  }
+  *reinterpret_cast<u32x2_t*>(row + pl.lo) = u32x2_t{e4m3x4(v), e4m3x4(v + 4)};
+  *reinterpret_cast<u32x2_t*>(row + pl.hi) = u32x2_t{e4m3x4(v + 8), e4m3x4(v + 12)};
+}
+
+// Pages with many new tokens: a page and head, its keys and then its values, per W waves; a lane group takes NI rows.  The loads
+// of both are in flight together, and the values stay in registers between the maximum and the codes.
 template <int DT, bool NORM, bool INTER, bool VEC, int W, int NI>
 __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a, int64_t items) {
-  __shared__ float red[4];
+  __shared__ float red[2][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int parts = 2 * a.heads;
-  // work list: items x heads x {keys, values}
   const int64_t unit = (linear_block() * 4 + wave) / W;
-  const int64_t item = unit / parts;
+  const int64_t item = unit / a.heads;
   if (item >= items) return;  // W == 4: the same for the whole block
-  const int part = (int)(unit - item * parts);
-  const int kv = part >= a.heads, h = kv ? part - a.heads : part;
+  const int h = (int)(unit - item * a.heads);
   Segment g;
   if (!find_segment(a, item, g)) return;
 
   const int width = 1 << a.width_log2;
   const int j = lane & (width - 1);
   const int per_wave = 64 >> a.width_log2;
-  const int group = (W == 4 ? wave * per_wave : 0) + (lane >> a.width_log2);
-  const int groups = W * per_wave;
-  const int R = kv ? 0 : a.R;
-  const RowPlace pl = row_place<INTER>(j, a.D, R);
-  float v[NI][16];
-  float amax = 0.0f;
+  const int group = (W == 4 ? wave * per_wave : 0) + (lane >> a.width_log2), groups = W * per_wave;
+  const RowPlace pk = row_place<INTER>(j, a.D, a.R), pv = row_place<false>(j, a.D, a.D);
+  Row<DT> xk[NI], xv[NI];
 #pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int r = group + i * groups;
-    if (r < g.n) {
-      const int64_t at = (g.row0 + r) * a.stride_t[kv] + h * a.stride_h[kv];
-      load8<DT, VEC>(a.x[kv], at + pl.lo, v[i]);
-      load8<DT, VEC>(a.x[kv], at + pl.hi, v[i] + 8);
+  for (int i = 0; i < NI; ++i)
+    if (group + i * groups < g.n) load_row<DT, VEC>(a, 0, h, g.row0 + group + i * groups, pk, xk[i]);
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+    if (group + i * groups < g.n) load_row<DT, VEC>(a, 1, h, g.row0 + group + i * groups, pv, xv[i]);
+  const int64_t id = page_of(a, g);
+  if (id < 0) return;
+  const int64_t entry = id * a.heads + h;
+  int held[2] = {0, 0};
+  if (g.slot0 > 0) held[0] = scale_exponent_of(a.scale[0][entry]), held[1] = scale_exponent_of(a.scale[1][entry]);
+  // the exponent of keys (0) or values (1)
+  auto settle = [&](int kv, float amax) {
+    amax = group_max(amax, 64);
+    if (W == 4) {  // (and every wave has read the old scale)
+      if (lane == 0) red[kv][wave] = amax;
+      __syncthreads();
+      amax = fmaxf(fmaxf(red[kv][0], red[kv][1]), fmaxf(red[kv][2], red[kv][3]));
     }
-  }
-  if (!kv && (NORM || R > 0)) {
-    float w[16];
-    if (NORM) {
-      load8f(a.w + pl.lo, w);
-      load8f(a.w + pl.hi, w + 8);
-    }
+    const int e = settle_scale(amax, g.slot0, held[kv], a.codes[kv] + ((entry << a.page_log2) * a.D), a.D,
+                               W == 4 ? threadIdx.x : lane, 64 * W);
+    if (lane == 0 && (W == 1 || wave == 0)) a.scale[kv][entry] = exp2_int(e);
+    return e;
+  };
+  const int64_t slots = (entry << a.page_log2) + g.slot0;
+  {
+    float v[NI][16], amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int r = group + i * groups;
-      const bool ok = r < g.n;
-      // in 64 bits (as fast as 32 here): the code is the nearest to the key itself, whatever the order of the sum
-      double x[16];
+      to_float(xk[i], v[i]);
+      if (NORM || a.R > 0) key_row<NORM, INTER>(a, g, r, r < g.n, j, pk, v[i]);
+      if (r < g.n) amax = fmaxf(amax, row_max(v[i]));
+    }
+    const int e = settle(0, amax);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = ok ? (double)v[i][e] : 0.0;
-      if (NORM) {
-        double ss = 0.0;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) ss = __builtin_fma(x[e], x[e], ss);
-        for (int o = 1; o < width; o <<= 1) ss += __shfl_xor(ss, o);
-        const double rs = 1.0 / sqrt(ss / (double)a.D + (double)a.eps);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = x[e] * rs * (double)w[e];
-      }
-      if (ok && pl.turned) {
-        const int64_t p = a.positions ? load_position(a.positions, a.bits, g.row0 + r) : g.index0 + r;
-        if (p < 0 || p >= a.table_rows) {
-          if (a.err) *a.err = 1;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] = 0.0;
-        } else {
-          float c[8], s[8];
-          load8f(a.cos + p * (R / 2) + 8 * j, c);
-          load8f(a.sin + p * (R / 2) + 8 * j, s);
-          rotate16<INTER>(x, c, s);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) v[i][e] = (float)x[e];
+    for (int i = 0; i < NI; ++i) {
+      const int r = group + i * groups;
+      if (r < g.n) store_codes(a.codes[0] + (slots + r) * a.D, pk, v[i], e);
     }
   }
+  float amax = 0.0f;
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    if (group + i * groups < g.n) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float m = fabsf(v[i][e]);
-        amax = fmaxf(amax, m < __builtin_inff() ? m : 0.0f);
-      }
-    }
+    float v[16];
+    to_float(xv[i], v);
+    if (group + i * groups < g.n) amax = fmaxf(amax, row_max(v));
   }
-  amax = group_max(amax, 64);
-  if (W == 4) {
-    if (lane == 0) red[wave] = amax;
-    __syncthreads();
-    amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  }
-  int e = scale_exponent(amax);
-  const int64_t entry = g.page_id * a.heads + h;
-  uint8_t* page = a.codes[kv] + ((entry << a.page_log2) * a.D);
-  float* scale = a.scale[kv] + entry;
-  if (g.slot0 > 0) {
-    const int held = scale_exponent_of(*scale);
-    if (W == 4) __syncthreads();  // every wave has read the old scale
-    if (e > held) {
-      // codes of the tokens already there, 16 at a time
-      const float f = exp2_int(held - e > -126 ? held - e : -126);
-      const int n16 = g.slot0 * a.D / 16;
-      for (int i = (W == 4 ? threadIdx.x : lane); i < n16; i += 64 * W) {
-        u32x4_t* p = reinterpret_cast<u32x4_t*>(page) + i;
-        u32x4_t c = *p;
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-          const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[d], false);
-          const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[d], true);
-          const float x[4] = {lo[0] * f, lo[1] * f, hi[0] * f, hi[1] * f};
-          c[d] = e4m3x4(x);
-        }
-        *p = c;
-      }
-    } else {
-      e = held;
-    }
-  }
-  if (lane == 0 && (W == 1 || wave == 0)) *scale = exp2_int(e);
-  const float inv = exp2_int(-e);
+  const int e = settle(1, amax);
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     const int r = group + i * groups;
-    if (r < g.n) {
-#pragma unroll
-      for (int d = 0; d < 16; ++d) v[i][d] *= inv;
-      uint8_t* row = page + (int64_t)(g.slot0 + r) * a.D;
-      *reinterpret_cast<u32x2_t*>(row + pl.lo) = u32x2_t{e4m3x4(v[i]), e4m3x4(v[i] + 4)};
-      *reinterpret_cast<u32x2_t*>(row + pl.hi) = u32x2_t{e4m3x4(v[i] + 8), e4m3x4(v[i] + 12)};
+    float v[16];
+    to_float(xv[i], v);
+    if (r < g.n) store_codes(a.codes[1] + (slots + r) * a.D, pv, v, e);
+  }
+}
+
+// Pages with a token or two: a lane group per (page, head, keys or values), its rows one after the other, read again for the
+// codes where there are several.
+template <int DT, bool NORM, bool INTER, bool VEC>
+__global__ void __launch_bounds__(256) kv_append_token_kernel(AppendArgs a, int64_t items, int waves) {
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = linear_block() * 4 + (threadIdx.x >> 6);
+  const int64_t item = unit / waves;
+  if (item >= items) return;
+  Segment g;
+  if (!find_segment(a, item, g)) return;
+  const int width = 1 << a.width_log2, j = lane & (width - 1);
+  const int part = (int)(unit - item * waves) * (64 >> a.width_log2) + (lane >> a.width_log2);
+  const bool live = part < 2 * a.heads;
+  const int kv = live && part >= a.heads, h = !live ? 0 : kv ? part - a.heads : part;
+  const RowPlace pl = row_place<INTER>(j, a.D, a.R);  // (the values' pieces may be the keys')
+  float x[16], amax = 0.0f;
+  auto row = [&](int r) {
+    if (!live) return;
+    Row<DT> w;
+    load_row<DT, VEC>(a, kv, h, g.row0 + r, pl, w);
+    to_float(w, x);
+  };
+  auto key = [&](int r) {
+    if (NORM || a.R > 0) {
+      if (live && !kv) key_row<NORM, INTER>(a, g, r, true, j, pl, x);
     }
+  };
+  row(0);
+  const int64_t id = page_of(a, g);
+  if (id < 0) return;
+  const int64_t entry = id * a.heads + h;
+  const int held = g.slot0 > 0 && live ? scale_exponent_of(a.scale[kv][entry]) : 0;
+  key(0);
+  if (live) amax = row_max(x);
+  for (int r = 1; r < g.n; ++r) {
+    row(r);
+    key(r);
+    if (live) amax = fmaxf(amax, row_max(x));
+  }
+  amax = group_max(amax, width);
+  if (!live) return;
+  uint8_t* page = a.codes[kv] + ((entry << a.page_log2) * a.D);
+  const int e = settle_scale(amax, g.slot0, held, page, a.D, j, width);
+  if (j == 0) a.scale[kv][entry] = exp2_int(e);
+  for (int r = g.n - 1; r >= 0; --r) {  // the last row is still there
+    if (r < g.n - 1) {
+      row(r);
+      key(r);
+    }
+    store_codes(page + (int64_t)(g.slot0 + r) * a.D, pl, x, e);
   }
 }
 
 template <int DT, bool NORM, bool INTER, bool VEC>
 int launch(const AppendArgs& a, hipStream_t st) {
   const int64_t items = (a.tokens >> a.page_log2) + 2 * (int64_t)a.seqs;
-  const int64_t units = items * 2 * a.heads;
+  if (a.tokens <= 2 * (int64_t)a.seqs) {
+    const int parts = 64 >> a.width_log2, waves = (2 * a.heads + parts - 1) / parts;
+    kv_append_token_kernel<DT, NORM, INTER, VEC><<<linear_grid((items * waves + 3) / 4), 256, 0, st>>>(a, items, waves);
+    PDM_CHECK_LAUNCH();
+    return PDM_OK;
+  }
+  const int64_t units = items * a.heads;
   // rows of a page per wave-wide step; more than 4 of them take the four waves of a block
   const int steps = (1 << a.page_log2) * (1 << a.width_log2) / 64;
   const dim3 g1 = linear_grid((units + 3) / 4), g4 = linear_grid(units);
   if (steps <= 1) kv_append_kernel<DT, NORM, INTER, VEC, 1, 1><<<g1, 256, 0, st>>>(a, items);
   else if (steps == 2) kv_append_kernel<DT, NORM, INTER, VEC, 1, 2><<<g1, 256, 0, st>>>(a, items);
-  else if (steps == 4) kv_append_kernel<DT, NORM, INTER, VEC, 1, 4><<<g1, 256, 0, st>>>(a, items);
+  else if (steps == 4) kv_append_kernel<DT, NORM, INTER, VEC, 4, 1><<<g4, 256, 0, st>>>(a, items);
   else if (steps == 8) kv_append_kernel<DT, NORM, INTER, VEC, 4, 2><<<g4, 256, 0, st>>>(a, items);
   else if (steps == 16) kv_append_kernel<DT, NORM, INTER, VEC, 4, 4><<<g4, 256, 0, st>>>(a, items);
   else kv_append_kernel<DT, NORM, INTER, VEC, 4, 8><<<g4, 256, 0, st>>>(a, items);

@@ -34,41 +34,51 @@ __device__ __forceinline__ RowPlace row_place(int j, int D, int R) {
   return p;
 }
 
-// Eight elements of dtype DT (PDM_F32 / PDM_F16 / PDM_BF16) as fp32; VEC: 16-byte aligned.
+// Eight elements of dtype DT (PDM_F32 / PDM_F16 / PDM_BF16) as they are stored, in two (fp32) or one register quads; VEC:
+// 16-byte aligned.
 template <int DT, bool VEC>
-__device__ __forceinline__ void load8(const void* base, int64_t at, float* v) {
+__device__ __forceinline__ void load8_raw(const void* base, int64_t at, u32x4_t* w) {
   if constexpr (DT == PDM_F32) {
-    const float* p = static_cast<const float*>(base) + at;
+    const uint32_t* p = static_cast<const uint32_t*>(base) + at;
     if constexpr (VEC) {
-      const f32x4_t a = *reinterpret_cast<const f32x4_t*>(p), b = *reinterpret_cast<const f32x4_t*>(p + 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = a[i], v[i + 4] = b[i];
+      w[0] = *reinterpret_cast<const u32x4_t*>(p), w[1] = *reinterpret_cast<const u32x4_t*>(p + 4);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = p[i];
+      for (int i = 0; i < 4; ++i) w[0][i] = p[i], w[1][i] = p[4 + i];
     }
   } else {
     const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-    uint32_t w[4];
     if constexpr (VEC) {
-      const u32x4_t a = *reinterpret_cast<const u32x4_t*>(p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = a[i];
+      w[0] = *reinterpret_cast<const u32x4_t*>(p);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = uint32_t(p[2 * i]) | uint32_t(p[2 * i + 1]) << 16;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == PDM_BF16) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      } else {
-        v[2 * i] = f16_bits_to_f32(w[i] & 0xffffu);
-        v[2 * i + 1] = f16_bits_to_f32(w[i] >> 16);
-      }
+      for (int i = 0; i < 4; ++i) w[0][i] = uint32_t(p[2 * i]) | uint32_t(p[2 * i + 1]) << 16;
     }
   }
+}
+
+template <int DT>
+__device__ __forceinline__ void raw_to_float(const u32x4_t* w, float* v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == PDM_F32) {
+      v[i] = __uint_as_float(w[0][i]), v[4 + i] = __uint_as_float(w[1][i]);
+    } else if constexpr (DT == PDM_BF16) {
+      v[2 * i] = __uint_as_float(w[0][i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[0][i] & 0xffff0000u);
+    } else {
+      v[2 * i] = f16_bits_to_f32(w[0][i] & 0xffffu);
+      v[2 * i + 1] = f16_bits_to_f32(w[0][i] >> 16);
+    }
+  }
+}
+
+// The same as fp32.
+template <int DT, bool VEC>
+__device__ __forceinline__ void load8(const void* base, int64_t at, float* v) {
+  u32x4_t w[2];
+  load8_raw<DT, VEC>(base, at, w);
+  raw_to_float<DT>(w, v);
 }
 
 // Eight fp32 values rounded once to dtype DT; the address is 16-byte aligned.
@@ -137,19 +147,16 @@ __device__ __forceinline__ int scale_exponent(float amax) {
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 __device__ __forceinline__ int scale_exponent_of(float scale) { return (int)((__float_as_uint(scale) >> 23) & 0xffu) - 127; }
 
-// Four values (already divided by the scale) to e4m3, nearest even; beyond 448 they saturate, NaN and
-// infinities become the NaN code.
+// Four values (already divided by the scale) to e4m3, nearest even; NaN and infinities become the NaN code, as does what is
+// beyond 448 (after rounding: 464 and more).
 __device__ __forceinline__ uint32_t e4m3x4(const float* v) {
-  uint32_t w = 0;
-  float c[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) c[i] = __builtin_amdgcn_fmed3f(v[i], -kE4m3Max, kE4m3Max);
-  w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], (int)w, false);
-  w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], (int)w, true);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (!(fabsf(v[i]) < __builtin_inff())) w = (w & ~(0xffu << (8 * i))) | 0x7fu << (8 * i);
-  return w;
+  uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], (int)w, true);
+}
+
+// A finite value beyond 448 (under the largest scale alone) saturates.
+__device__ __forceinline__ float e4m3_saturated(float v) {
+  return fabsf(v) < __builtin_inff() ? __builtin_amdgcn_fmed3f(v, -kE4m3Max, kE4m3Max) : v;
 }
 
 // ---- sequences -----------------------------------------------------------------
