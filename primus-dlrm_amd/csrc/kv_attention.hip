@@ -709,10 +709,9 @@ __global__ void __launch_bounds__(256) kv_attn_dealt_join_kernel(AttnArgs a) {
 
 // ---- many rows ---------------------------------------------------------------------
 // 128 rows of a (sequence, key head) against its keys, four waves of 32 rows.  Tiles of KT keys are converted once on
-// their way into LDS: K as rows, two tiles ahead of the values' use, V transposed, one tile ahead, its keys in the order in
-// which the first product leaves P.  The waves meet at one barrier per tile.  A wave computes the scores of tile t + 1
-// beside the exponentials of tile t, and a second workgroup shares the CU: the matrix unit has work while the VALU does
-// a softmax.
+// their way into LDS, one tile ahead of their use, their loads one further: K as rows, V transposed, its keys in the order in
+// which the first product leaves P.  The waves meet at one barrier per tile.  Two workgroups share a CU: one's products run
+// beside the other's softmax.
 constexpr int kManyRows = 128;
 
 template <int D, int KT>
@@ -721,7 +720,7 @@ struct ManyShared {
   static constexpr int VS = 2 * KT + 16;   // bytes of a V^T row
   alignas(16) char k[2][KT * KS];
   alignas(16) char v[2][D * VS];
-  float sc[4][KT / 16];                    // scale2 * scale of 16 keys; NaN where their page does not exist
+  float sc[2][KT / 16];                    // scale2 * scale of 16 keys; NaN where their page does not exist
   int odd[4];                              // a wave's share of V held NaN
 };
 
@@ -803,6 +802,12 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
       }
     }
   }
+  if (a.scale2 < 0.0f) {  // the scale's sign goes into the queries
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[kk][e] ^= 0x80008000u;
+  }
   // keys that every row of this wave sees
   int all_lo = 0, all_hi = sq.hi;
   {
@@ -823,12 +828,11 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
   float kss = 0.0f, vss = 0.0f;
   u32x4_t kr[KP];
   uint32_t vr[4][VD / 4];
-  int v_id = -1;                           // of the V tile that is loaded next
-  float v_sc = 0.0f, v_scale = 0.0f, sc_reg = 0.0f;
+  float v_scale = 0.0f, sc_reg = 0.0f;
   const int kc = (tid % (D / 16)) * 16, kr0 = tid / (D / 16);       // piece and row of K, 4096 / D rows a pass
   const int vm = D == 256 ? wave * 8 + (lane & 7) : (wave & 1) * 8 + (lane & 7);
   const int va = D == 256 ? lane >> 3 : (wave >> 1) * 8 + (lane >> 3);   // four keys of V
-  auto load_k = [&](int t) {
+  auto load = [&](int t) {
     const int key0 = begin + t * KT;
     if (t % PER == 0) {
       const int key = key0 + 16 * lane;
@@ -838,7 +842,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
         if (id >= 0 && id < a.num_pages) {
           ids = id;
           const int64_t entry = (int64_t)id * a.hk + kh;
-          kss = a.k_scale[entry] * a.scale2;
+          // not zero: a hidden score times it stays -inf
+          kss = fmaxf(a.k_scale[entry] * fabsf(a.scale2), 0x1p-126f);
           vss = a.v_scale[entry];
         } else if (a.err) {
           *a.err = 1;
@@ -857,18 +862,15 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
         kr[p] = *reinterpret_cast<const u32x4_t*>(a.k_codes + at * D + (r & 15) * D + kc);
       }
     }
-    v_id = __shfl(ids, g0 + (va >> 2));
-    v_sc = __shfl(vss, g0 + (va >> 2));
+    const int v_id = __shfl(ids, g0 + (va >> 2));
+    v_scale = __shfl(vss, g0 + (va >> 2));
     sc_reg = __shfl(kss, g0 + (lane & (KT / 16 - 1)));
-  };
-  auto load_v = [&](int t) {  // with the page that load_k(t) found
-    v_scale = v_sc;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int e = 0; e < VD / 4; ++e) vr[r][e] = 0;
     if (v_id >= 0) {
-      const int64_t at = (((int64_t)v_id * a.hk + kh) << a.page_log2) + ((begin + t * KT + 16 * (va >> 2)) & mask) + (va & 3) * 4;
+      const int64_t at = (((int64_t)v_id * a.hk + kh) << a.page_log2) + ((key0 + 16 * (va >> 2)) & mask) + (va & 3) * 4;
       const uint8_t* p = a.v_codes + at * D + vm * VD;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -895,7 +897,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
       *reinterpret_cast<u32x4_t*>(dst) = w0;
       *reinterpret_cast<u32x4_t*>(dst + 16) = w1;
     }
-    if (wave == 0 && lane < KT / 16) sh.sc[t & 3][lane] = sc_reg;
+    if (wave == 0 && lane < KT / 16) sh.sc[t & 1][lane] = sc_reg;
   };
   // V^T of tile t; NaN codes become zeros here (0 * NaN would reach rows that do not see the key) and are remembered, or,
   // in MARK, ones where everything else becomes zero.
@@ -938,35 +940,34 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
 
   // ---- products ----
   float m = -kInf, l = 0.0f;
-  f32x16_t o[DD], s[XX], n[XX];
+  f32x16_t o[DD], s[XX];
   constexpr f32x16_t zero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
   for (int d = 0; d < DD; ++d) o[d] = zero16;
   const uint32_t k_at = c * KS + 16 * h, v_at = c * VS + 16 * h;
+  // s = scores of tile t (products alone)
   auto scores = [&](int t) {
     const char* kb = sh.k[t & 1] + k_at;
 #pragma unroll
     for (int x = 0; x < XX; ++x) {
-      n[x] = zero16;
+      s[x] = zero16;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
-        n[x] = mfma32<DT>(*reinterpret_cast<const u32x4_t*>(kb + x * 32 * KS + 32 * kk), q[kk], n[x]);
+        s[x] = mfma32<DT>(*reinterpret_cast<const u32x4_t*>(kb + x * 32 * KS + 32 * kk), q[kk], s[x]);
     }
+    sched_mfma_ds_pipeline<XX * KK, 4>();
   };
-  // s = the new scores in units of log2, hidden ones at -inf; the running maximum
-  auto settle = [&](int t) {
+  // the running maximum, and P from the scores
+  u32x4_t p[2 * XX];
+  auto weights = [&](int t) {
     const int key = begin + t * KT;
-    float sc[2 * XX];
+    float sc[2 * XX];                      // of 16 keys each, not negative
     bool ok = true;
 #pragma unroll
     for (int x = 0; x < 2 * XX; ++x) {
-      sc[x] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sh.sc[t & 3][x])));
+      sc[x] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sh.sc[t & 1][x])));
       ok = ok && sc[x] == sc[x];
     }
-#pragma unroll
-    for (int x = 0; x < XX; ++x)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[x][e] = n[x][e] * sc[2 * x + (e >> 3)];
     if (!(ok && key >= all_lo && key + KT <= all_hi)) {
 #pragma unroll
       for (int x = 0; x < XX; ++x)
@@ -976,12 +977,17 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
           const bool on = sc[2 * x + (e >> 3)] == sc[2 * x + (e >> 3)] && j >= row_lo && j < row_hi;
           s[x][e] = on ? s[x][e] : -kInf;
         }
+#pragma unroll
+      for (int x = 0; x < 2 * XX; ++x) sc[x] = sc[x] == sc[x] ? sc[x] : 1.0f;
     }
-    float top = s[0][0];
+    float top = -kInf;
 #pragma unroll
-    for (int x = 0; x < XX; ++x)
+    for (int x = 0; x < 2 * XX; ++x) {
+      float most = s[x >> 1][8 * (x & 1)];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[x][e]);
+      for (int e = 1; e < 8; ++e) most = fmaxf(most, s[x >> 1][8 * (x & 1) + e]);
+      top = fmaxf(top, most * sc[x]);
+    }
     // the maximum moves only where a weight would pass 2^8: sums and products lose nothing by that
     if (__any(top > m + 8.0f)) {
       top = fmaxf(top, __shfl_xor(top, 32));
@@ -992,15 +998,12 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
 #pragma unroll
       for (int d = 0; d < DD; ++d) o[d] *= f;
     }
-  };
-  u32x4_t p[2 * XX];
-  auto weights = [&]() {
     const float base = m == -kInf ? 0.0f : m;
 #pragma unroll
     for (int x = 0; x < XX; ++x) {
       float v[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = __builtin_amdgcn_exp2f(s[x][e] - base);
+      for (int e = 0; e < 16; ++e) v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], sc[2 * x + (e >> 3)], -base));
 #pragma unroll
       for (int e = 0; e < 16; e += 4) l += (v[e] + v[e + 1]) + (v[e + 2] + v[e + 3]);
 #pragma unroll
@@ -1017,39 +1020,31 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
 #pragma unroll
       for (int d = 0; d < DD; ++d)
         o[d] = mfma32x32x16(*reinterpret_cast<const u32x4_t*>(vb + d * 32 * VS + 32 * y), p[y], o[d]);
+    sched_mfma_ds_pipeline<2 * XX * DD, 4>();
   };
+
   if (tiles > 0) {
     const std::false_type plain;
-    load_k(0);
-    load_v(0);
+    load(0);
     stage_k(0);
     stage_v(0, plain);
-    if (tiles > 1) {
-      load_k(1);
-      load_v(1);
-      stage_k(1);
-    }
-    if (tiles > 2) load_k(2);
-    __syncthreads();
-    scores(0);
-    settle(0);
+    if (tiles > 1) load(1);
 #pragma unroll 1
-    for (int t = 0; t + 1 < tiles; ++t) {
+    for (int t = 0; t < tiles; ++t) {
       __syncthreads();
-      stage_v(t + 1, plain);
-      if (t + 2 < tiles) {
-        load_v(t + 2);
-        stage_k(t + 2);
-        if (t + 3 < tiles) load_k(t + 3);
+      if (t + 1 < tiles) {
+        stage_k(t + 1);
+        stage_v(t + 1, plain);
+        if (t + 2 < tiles) load(t + 2);
       }
-      scores(t + 1);
-      weights();
+      __builtin_amdgcn_sched_barrier(0);
+      scores(t);
+      __builtin_amdgcn_sched_barrier(0);
+      weights(t);
+      __builtin_amdgcn_sched_barrier(0);
       values(t);
-      settle(t + 1);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    __syncthreads();
-    weights();
-    values(tiles - 1);
 
     // NaN among the values of any wave's share: once more over the tiles, with ones for NaN and for keys that are seen
     if (lane == 0) sh.odd[wave] = odd;
@@ -1057,16 +1052,15 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
     if (sh.odd[0] | sh.odd[1] | sh.odd[2] | sh.odd[3]) {
 #pragma unroll 1
       for (int t = 0; t < tiles; ++t) {
-        load_k(t);
-        load_v(t);
+        load(t);
         __syncthreads();  // the tile before is done with
         stage_v(t, std::true_type());
-        if (wave == 0 && lane < KT / 16) sh.sc[t & 3][lane] = sc_reg;
+        if (wave == 0 && lane < KT / 16) sh.sc[t & 1][lane] = sc_reg;
         __syncthreads();
 #pragma unroll 1
         for (int y = 0; y < 2 * XX; ++y) {
           u32x4_t seen;
-          const bool ok = sh.sc[t & 3][y] == sh.sc[t & 3][y];
+          const bool ok = sh.sc[t & 1][y] == sh.sc[t & 1][y];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int j = begin + t * KT + 16 * y + 8 * (e >> 1) + 4 * h + 2 * (e & 1);
