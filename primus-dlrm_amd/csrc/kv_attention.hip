@@ -717,7 +717,10 @@ constexpr int kManyRows = 128;
 template <int D, int KT>
 struct ManyShared {
   static constexpr int KS = 2 * D + 16;    // bytes of a K row: 16 rows of a fragment read fall into different banks
-  static constexpr int VS = 2 * KT + 16;   // bytes of a V^T row
+  static constexpr int VS = 2 * KT;        // bytes of a V^T row, its 16-byte pieces exchanged by turn()
+  // Piece g of row d lies at g ^ turn(d): any 16 rows of a fragment read, and the 8 rows that 8 lanes write at a time
+  // (rows 8 apart), fall into different banks.  (With rows padded to 144 bytes a write took 32 cycles instead of 8.)
+  __device__ static constexpr int turn(int d) { return KT == 64 ? ((d >> 1) ^ (d >> 3)) & 7 : ((d >> 2) ^ (d >> 4)) & 3; }
   alignas(16) char k[2][KT * KS];
   alignas(16) char v[2][D * VS];
   float sc[2][KT / 16];                    // scale2 * scale of 16 keys; NaN where their page does not exist
@@ -905,7 +908,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
   auto stage_v = [&](int t, auto mark) {
     // keys 4 va .. + 3: block va % 4 of their 16; blocks 0, 2 belong to lanes h = 0 of the product, 1, 3 to h = 1
     const int x = va & 3;
-    char* vb = sh.v[t & 1] + 2 * (16 * (va >> 2) + 8 * (x & 1) + 4 * (x >> 1));
+    const uint32_t at = vm * VD * VS + 16 * ((2 * (va >> 2) + (x & 1)) ^ ManyShared<D, KT>::turn(vm * VD)) + 8 * (x >> 1);
     uint32_t nan = 0;
 #pragma unroll
     for (int e = 0; e < VD / 4; ++e)
@@ -933,7 +936,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
       for (int d = 0; d < 4; ++d) {
         const u32x2_t w = d & 1 ? u32x2_t{value_pair_hi(w01[d >> 1], f), value_pair_hi(w23[d >> 1], f)}
                                 : u32x2_t{value_pair_lo(w01[d >> 1], f), value_pair_lo(w23[d >> 1], f)};
-        *reinterpret_cast<u32x2_t*>(vb + (vm * VD + 4 * e + d) * VS) = w;
+        const int r = 4 * e + d;  // turn(row + r) = turn(row) ^ turn(r) for the 4 or 8 rows of a thread
+        *reinterpret_cast<u32x2_t*>(sh.v[t & 1] + (at ^ (16 * ManyShared<D, KT>::turn(r))) + r * VS) = w;
       }
     }
   };
@@ -944,7 +948,12 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
   constexpr f32x16_t zero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
   for (int d = 0; d < DD; ++d) o[d] = zero16;
-  const uint32_t k_at = c * KS + 16 * h, v_at = c * VS + 16 * h;
+  const uint32_t k_at = c * KS + 16 * h;
+  const uint32_t v_at = c * VS + 16 * (h ^ ManyShared<D, KT>::turn(c));
+  // V^T fragment of rows 32 d + c and keys 16 y ..
+  auto v_frag = [&](int t, int d, int y) {
+    return *reinterpret_cast<const u32x4_t*>(sh.v[t & 1] + (v_at ^ (32 * y ^ 16 * ManyShared<D, KT>::turn(32 * d))) + d * 32 * VS);
+  };
   // s = scores of tile t (products alone)
   auto scores = [&](int t) {
     const char* kb = sh.k[t & 1] + k_at;
@@ -1014,12 +1023,10 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
     }
   };
   auto values = [&](int t) {
-    const char* vb = sh.v[t & 1] + v_at;
 #pragma unroll
     for (int y = 0; y < 2 * XX; ++y)
 #pragma unroll
-      for (int d = 0; d < DD; ++d)
-        o[d] = mfma32x32x16(*reinterpret_cast<const u32x4_t*>(vb + d * 32 * VS + 32 * y), p[y], o[d]);
+      for (int d = 0; d < DD; ++d) o[d] = mfma32x32x16(v_frag(t, d, y), p[y], o[d]);
     sched_mfma_ds_pipeline<2 * XX * DD, 4>();
   };
 
@@ -1068,7 +1075,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
           }
 #pragma unroll
           for (int d = 0; d < DD; ++d) {
-            const f32x16_t hits = mfma32x32x16(*reinterpret_cast<const u32x4_t*>(sh.v[t & 1] + v_at + d * 32 * VS + 32 * y), seen, zero16);
+            const f32x16_t hits = mfma32x32x16(v_frag(t, d, y), seen, zero16);
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[d][e] += hits[e] > 0.0f ? __builtin_nanf("") : 0.0f;
           }
