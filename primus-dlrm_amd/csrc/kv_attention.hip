@@ -110,6 +110,8 @@ __device__ __forceinline__ f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c) {
 
 // NaN codes of a dword: bit 7 of each byte that holds one.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// 0xff in the bytes whose bit 7 is set.
+__device__ __forceinline__ uint32_t full_bytes(uint32_t n) { return (n << 1) - (n >> 7); }
 
 template <int DT>
 __device__ __forceinline__ void store4(void* base, int64_t at, float x, float y, float z, float w) {
@@ -489,7 +491,7 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
           for (int e = 0; e < D / 64; ++e) {
             const uint32_t n = nan_bytes(v[x][r][e]);
             any |= n;
-            v[x][r][e] &= ~((n >> 7) * 0xffu);
+            v[x][r][e] &= ~full_bytes(n);
           }
       odd = odd || __any(any != 0);
     }
@@ -760,6 +762,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
   constexpr int KP = KT * D / 16 / 256;    // 16-byte pieces of a K tile per thread
   constexpr int VD = D == 64 ? 4 : 8;      // elements of a thread's 4 keys of V
   constexpr int KS = ManyShared<D, KT>::KS, VS = ManyShared<D, KT>::VS;
+  constexpr int LEAD = 8;                  // fragments read ahead of their products
   __shared__ ManyShared<D, KT> sh;
 
   const int64_t unit = linear_block();
@@ -778,7 +781,11 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
   if (split > 0 && begin >= hi) return;
   const int end = begin + size < hi ? begin + size : hi;
   const int rows = sq.n * a.group;
-  const int tiles = end > begin ? (end - begin + KT - 1) / KT : 0;
+  int tiles = end > begin ? (end - begin + KT - 1) / KT : 0;
+  if (tiles && a.num_pages == 0) {
+    tiles = 0;
+    if (a.err) *a.err = 1;
+  }
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
@@ -858,31 +865,22 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
     for (int p = 0; p < KP; ++p) {
       const int r = kr0 + p * (4096 / D);
       const int grp = __builtin_amdgcn_readfirstlane(r >> 4);
-      const int id = __builtin_amdgcn_readlane(ids, g0 + grp);
-      kr[p] = u32x4_t{0, 0, 0, 0};
-      if (id >= 0) {
-        const int64_t at = (((int64_t)id * a.hk + kh) << a.page_log2) + ((key0 + 16 * grp) & mask);
-        kr[p] = *reinterpret_cast<const u32x4_t*>(a.k_codes + at * D + (r & 15) * D + kc);
-      }
+      const int id = __builtin_amdgcn_readlane(ids, g0 + grp);  // (a page that does not exist: some page, not seen)
+      const int64_t at = (((int64_t)(id < 0 ? 0 : id) * a.hk + kh) << a.page_log2) + ((key0 + 16 * grp) & mask);
+      kr[p] = *reinterpret_cast<const u32x4_t*>(a.k_codes + at * D + ((r & 15) * D + kc));
     }
     const int v_id = __shfl(ids, g0 + (va >> 2));
     v_scale = __shfl(vss, g0 + (va >> 2));
     sc_reg = __shfl(kss, g0 + (lane & (KT / 16 - 1)));
+    const int64_t at = (((int64_t)(v_id < 0 ? 0 : v_id) * a.hk + kh) << a.page_log2) + ((key0 + 16 * (va >> 2)) & mask);
+    const uint8_t* p = a.v_codes + at * D + ((va & 3) * 4 * D + vm * VD);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int e = 0; e < VD / 4; ++e) vr[r][e] = 0;
-    if (v_id >= 0) {
-      const int64_t at = (((int64_t)v_id * a.hk + kh) << a.page_log2) + ((key0 + 16 * (va >> 2)) & mask) + (va & 3) * 4;
-      const uint8_t* p = a.v_codes + at * D + vm * VD;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if constexpr (VD == 4) {
-          vr[r][0] = *reinterpret_cast<const uint32_t*>(p + r * D);
-        } else {
-          const u32x2_t w = *reinterpret_cast<const u32x2_t*>(p + r * D);
-          vr[r][0] = w[0], vr[r][1] = w[1];
-        }
+    for (int r = 0; r < 4; ++r) {
+      if constexpr (VD == 4) {
+        vr[r][0] = *reinterpret_cast<const uint32_t*>(p + r * D);
+      } else {
+        const u32x2_t w = *reinterpret_cast<const u32x2_t*>(p + r * D);
+        vr[r][0] = w[0], vr[r][1] = w[1];
       }
     }
   };
@@ -924,7 +922,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
 #pragma unroll
         for (int e = 0; e < VD / 4; ++e)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) vr[r][e] &= ~((nan_bytes(vr[r][e]) >> 7) * 0xffu);
+          for (int r = 0; r < 4; ++r) vr[r][e] &= ~full_bytes(nan_bytes(vr[r][e]));
       }
     }
     const float f = decltype(mark)::value ? 1.0f : v_scale;
@@ -958,13 +956,13 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
   auto scores = [&](int t) {
     const char* kb = sh.k[t & 1] + k_at;
 #pragma unroll
-    for (int x = 0; x < XX; ++x) {
-      s[x] = zero16;
+    for (int x = 0; x < XX; ++x) s[x] = zero16;
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk)
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int x = 0; x < XX; ++x)
         s[x] = mfma32<DT>(*reinterpret_cast<const u32x4_t*>(kb + x * 32 * KS + 32 * kk), q[kk], s[x]);
-    }
-    sched_mfma_ds_pipeline<XX * KK, 4>();
+    sched_mfma_ds_pipeline<XX * KK, LEAD>();
   };
   // the running maximum, and P from the scores
   u32x4_t p[2 * XX];
@@ -977,17 +975,21 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
       sc[x] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sh.sc[t & 1][x])));
       ok = ok && sc[x] == sc[x];
     }
-    if (!(ok && key >= all_lo && key + KT <= all_hi)) {
+    if (!(key >= all_lo && key + KT <= all_hi)) {
+      const uint32_t from = key + 4 * h - row_lo, span = row_hi > row_lo ? row_hi - row_lo : 0;  // seen: j - row_lo < span
 #pragma unroll
       for (int x = 0; x < XX; ++x)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int j = key + 32 * x + 8 * (e >> 2) + 4 * h + (e & 3);
-          const bool on = sc[2 * x + (e >> 3)] == sc[2 * x + (e >> 3)] && j >= row_lo && j < row_hi;
-          s[x][e] = on ? s[x][e] : -kInf;
-        }
+        for (int e = 0; e < 16; ++e) s[x][e] = from + (32 * x + 8 * (e >> 2) + (e & 3)) < span ? s[x][e] : -kInf;
+    }
+    if (!ok) {
 #pragma unroll
-      for (int x = 0; x < 2 * XX; ++x) sc[x] = sc[x] == sc[x] ? sc[x] : 1.0f;
+      for (int x = 0; x < 2 * XX; ++x)
+        if (sc[x] != sc[x]) {
+          sc[x] = 1.0f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[x >> 1][8 * (x & 1) + e] = -kInf;
+        }
     }
     float top = -kInf;
 #pragma unroll
@@ -1027,7 +1029,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
     for (int y = 0; y < 2 * XX; ++y)
 #pragma unroll
       for (int d = 0; d < DD; ++d) o[d] = mfma32x32x16(v_frag(t, d, y), p[y], o[d]);
-    sched_mfma_ds_pipeline<2 * XX * DD, 4>();
+    sched_mfma_ds_pipeline<2 * XX * DD, LEAD>();
   };
 
   if (tiles > 0) {
