@@ -710,12 +710,12 @@ __global__ void __launch_bounds__(256) kv_attn_dealt_join_kernel(AttnArgs a) {
 }
 
 // ---- many rows ---------------------------------------------------------------------
-// 128 rows of a (sequence, key head) against its keys, four waves of 32 rows.  Tiles of KT keys are converted once on
-// their way into LDS, one tile ahead of their use, their loads one further: K as rows, V transposed, its keys in the order in
-// which the first product leaves P.  The waves meet at one barrier per tile.  Two workgroups share a CU: one's products run
-// beside the other's softmax.
-constexpr int kManyRows = 128;
-
+// 128 NG rows of a (sequence, key head) against its keys, NG groups of four waves of 32 rows.  A wave takes tiles of KT
+// keys in two phases: products (O += V^T P of the tile before, S of this one) and softmax (P from S), with a barrier
+// after each.  With two groups the second is one phase behind the first, so that on every SIMD a wave's products run
+// beside the other's softmax; left to themselves, two waves of a SIMD were found in the same phase and took turns.
+// Tiles are converted once on their way into LDS, in the softmax phase, their loads a tile earlier: K as rows by the
+// first group, V transposed by the second, its keys in the order in which the first product leaves P.
 template <int D, int KT>
 struct ManyShared {
   static constexpr int KS = 2 * D + 16;    // bytes of a K row: 16 rows of a fragment read fall into different banks
@@ -726,24 +726,26 @@ struct ManyShared {
   alignas(16) char k[2][KT * KS];
   alignas(16) char v[2][D * VS];
   float sc[2][KT / 16];                    // scale2 * scale of 16 keys; NaN where their page does not exist
-  int odd[4];                              // a wave's share of V held NaN
+  int odd[8];                              // a wave's share of V held NaN
 };
 
-// Block `item` of the list of (sequence, 128 rows): sequence b's span begins at cu[b] * group / 128 + b.
+// Block `item` of the list of (sequence, M rows): sequence b's span begins at cu[b] * group / M + b.
+template <int M>
 __device__ __forceinline__ bool many_block(const AttnArgs& a, int64_t item, Seq& sq, int& b, int& r0) {
-  b = find_sequence(a.seqs, item, [&](int i) { return (int64_t)a.cu[i] * a.group / kManyRows + i; });
-  const int64_t j = item - ((int64_t)a.cu[b] * a.group / kManyRows + b);
+  b = find_sequence(a.seqs, item, [&](int i) { return (int64_t)a.cu[i] * a.group / M + i; });
+  const int64_t j = item - ((int64_t)a.cu[b] * a.group / M + b);
   if (j < 0 || !seq_of(a, b, sq)) return false;
   const int64_t rows = (int64_t)sq.n * a.group;
-  if (rows <= a.few_rows || j * kManyRows >= rows) return false;
-  r0 = (int)(j * kManyRows);
+  if (rows <= a.few_rows || j * M >= rows) return false;
+  r0 = (int)(j * M);
   return true;
 }
 
-// The keys that rows r0 .. r0 + 127 may see: [lo, hi), lo a multiple of 32.
+// The keys that rows r0 .. r0 + M - 1 may see: [lo, hi), lo a multiple of 32.
+template <int M>
 __device__ __forceinline__ void many_keys(const AttnArgs& a, const Seq& sq, int r0, int& lo, int& hi) {
   const int rows = sq.n * a.group;
-  const int i0 = r0 / a.group, i1 = ((r0 + kManyRows < rows ? r0 + kManyRows : rows) - 1) / a.group;
+  const int i0 = r0 / a.group, i1 = ((r0 + M < rows ? r0 + M : rows) - 1) / a.group;
   const int p0 = sq.len - sq.n + i0, p1 = sq.len - sq.n + i1;
   hi = a.causal && p1 + 1 < sq.hi ? p1 + 1 : sq.hi;
   lo = a.window > 0 && p0 - a.window + 1 > 0 ? (p0 - a.window + 1) & ~31 : 0;
@@ -756,8 +758,9 @@ __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
   else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-template <int DT, int D, int KT>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(AttnArgs a, int64_t items) {
+template <int DT, int D, int KT, int NG>
+__global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kernel(AttnArgs a, int64_t items) {
+  constexpr int M = 128 * NG;
   constexpr int KK = D / 16, DD = D / 32, XX = KT / 32;
   constexpr int KP = KT * D / 16 / 256;    // 16-byte pieces of a K tile per thread
   constexpr int VD = D == 64 ? 4 : 8;      // elements of a thread's 4 keys of V
@@ -773,9 +776,9 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
   if (item < 0) return;
   Seq sq;
   int b, r0;
-  if (!many_block(a, item, sq, b, r0)) return;
+  if (!many_block<M>(a, item, sq, b, r0)) return;
   int lo, hi;
-  many_keys(a, sq, r0, lo, hi);
+  many_keys<M>(a, sq, r0, lo, hi);
   const int size = split_size(hi - lo, a.splits, KT);
   const int begin = lo + split * size;
   if (split > 0 && begin >= hi) return;
@@ -787,13 +790,15 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
     if (a.err) *a.err = 1;
   }
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // of the group
+  const int grp = NG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  const bool k_role = NG == 1 || grp == 0, v_role = NG == 1 || grp == 1;
   const int c = lane & 31, h = lane >> 5;
 
   // this lane's row: its query, and the keys that it sees
   u32x4_t q[KK];
   int row_lo = 0x7fffffff, row_hi = 0;
-  const int row = r0 + wave * 32 + c;
+  const int row = r0 + grp * 128 + wave * 32 + c;
   const int tok = row / a.group, head = kh * a.group + (row - tok * a.group);
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) q[kk] = u32x4_t{0, 0, 0, 0};
@@ -821,7 +826,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
   // keys that every row of this wave sees
   int all_lo = 0, all_hi = sq.hi;
   {
-    const int w0 = r0 + wave * 32;
+    const int w0 = r0 + grp * 128 + wave * 32;
     if (w0 < rows) {
       const int w1 = (w0 + 32 < rows ? w0 + 32 : rows) - 1;
       const int p0 = sq.len - sq.n + w0 / a.group, p1 = sq.len - sq.n + w1 / a.group;
@@ -861,6 +866,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
       }
     }
     const int g0 = (t % PER) * (KT / 16);
+    sc_reg = __shfl(kss, g0 + (lane & (KT / 16 - 1)));
+    if (k_role) {
 #pragma unroll
     for (int p = 0; p < KP; ++p) {
       const int r = kr0 + p * (4096 / D);
@@ -869,9 +876,10 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
       const int64_t at = (((int64_t)(id < 0 ? 0 : id) * a.hk + kh) << a.page_log2) + ((key0 + 16 * grp) & mask);
       kr[p] = *reinterpret_cast<const u32x4_t*>(a.k_codes + at * D + ((r & 15) * D + kc));
     }
+    }
+    if (v_role) {
     const int v_id = __shfl(ids, g0 + (va >> 2));
     v_scale = __shfl(vss, g0 + (va >> 2));
-    sc_reg = __shfl(kss, g0 + (lane & (KT / 16 - 1)));
     const int64_t at = (((int64_t)(v_id < 0 ? 0 : v_id) * a.hk + kh) << a.page_log2) + ((key0 + 16 * (va >> 2)) & mask);
     const uint8_t* p = a.v_codes + at * D + ((va & 3) * 4 * D + vm * VD);
 #pragma unroll
@@ -882,6 +890,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
         const u32x2_t w = *reinterpret_cast<const u32x2_t*>(p + r * D);
         vr[r][0] = w[0], vr[r][1] = w[1];
       }
+    }
     }
   };
   auto stage_k = [&](int t) {
@@ -1033,38 +1042,49 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
   };
 
   if (tiles > 0) {
-    const std::false_type plain;
+    auto stage = [&](int t) {
+      if (k_role) stage_k(t);
+      if (v_role) stage_v(t, std::false_type());
+    };
     load(0);
-    stage_k(0);
-    stage_v(0, plain);
+    stage(0);
     if (tiles > 1) load(1);
+    // Barrier k + 1 begins phase k: the first group has products at even ones, the second at odd ones.  K of tile t + 1 is
+    // written in phase 2 t + 1, where the other group reads that of tile t; V of tile t + 1 in phase 2 t + 2 (or before the
+    // barrier between them, where there is one group): what either overwrites was last read in an earlier phase.
+    if (NG == 2 && grp == 1) __syncthreads();
 #pragma unroll 1
-    for (int t = 0; t < tiles; ++t) {
+    for (int t = 0; t <= tiles; ++t) {
       __syncthreads();
-      if (t + 1 < tiles) {
-        stage_k(t + 1);
-        stage_v(t + 1, plain);
-        if (t + 2 < tiles) load(t + 2);
+      __builtin_amdgcn_sched_barrier(0);
+      if (t > 0) values(t - 1);
+      __builtin_amdgcn_sched_barrier(0);
+      if (t < tiles) scores(t);
+      __builtin_amdgcn_sched_barrier(0);
+      __syncthreads();
+      if (t < tiles) {
+        weights(t);
+        if (t + 1 < tiles) {
+          stage(t + 1);
+          if (t + 2 < tiles) load(t + 2);
+        }
       }
-      __builtin_amdgcn_sched_barrier(0);
-      scores(t);
-      __builtin_amdgcn_sched_barrier(0);
-      weights(t);
-      __builtin_amdgcn_sched_barrier(0);
-      values(t);
-      __builtin_amdgcn_sched_barrier(0);
     }
+    if (NG == 2 && grp == 0) __syncthreads();
 
     // NaN among the values of any wave's share: once more over the tiles, with ones for NaN and for keys that are seen
-    if (lane == 0) sh.odd[wave] = odd;
+    if (lane == 0) sh.odd[grp * 4 + wave] = odd;
     __syncthreads();
-    if (sh.odd[0] | sh.odd[1] | sh.odd[2] | sh.odd[3]) {
+    int any = 0;
+#pragma unroll
+    for (int w = 0; w < 4 * NG; ++w) any |= sh.odd[w];
+    if (any) {
 #pragma unroll 1
       for (int t = 0; t < tiles; ++t) {
         load(t);
         __syncthreads();  // the tile before is done with
-        stage_v(t, std::true_type());
-        if (wave == 0 && lane < KT / 16) sh.sc[t & 1][lane] = sc_reg;
+        if (v_role) stage_v(t, std::true_type());
+        if (v_role && wave == 0 && lane < KT / 16) sh.sc[t & 1][lane] = sc_reg;
         __syncthreads();
 #pragma unroll 1
         for (int y = 0; y < 2 * XX; ++y) {
@@ -1099,7 +1119,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
         store4<DT>(a.out, at * D + 32 * d + 2 * e + 4 * h, o[d][e] * f, o[d][e + 1] * f, o[d][e + 2] * f, o[d][e + 3] * f);
     if (h == 0 && a.lse) a.lse[at] = sum != 0.0f ? (m + __builtin_amdgcn_logf(sum)) * kLn2 : -kInf;
   } else {
-    const int64_t pr = ((item * a.hk + kh) * a.splits + split) * kManyRows + wave * 32 + c;
+    const int64_t pr = ((item * a.hk + kh) * a.splits + split) * M + grp * 128 + wave * 32 + c;
 #pragma unroll
     for (int d = 0; d < DD; ++d)
 #pragma unroll
@@ -1113,25 +1133,25 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attn_many_kernel(Att
 }
 
 // Joins the splits of the many-rows kernel: one wave per row.
-template <int DT, int D, int KT>
+template <int DT, int D, int KT, int M>
 __global__ void __launch_bounds__(256) kv_attn_many_join_kernel(AttnArgs a, int64_t items) {
   const int64_t x = linear_block() * 4 + (threadIdx.x >> 6);
-  const int in = (int)(x % kManyRows);
-  const int64_t ih = x / kManyRows;
+  const int in = (int)(x % M);
+  const int64_t ih = x / M;
   const int kh = (int)(ih % a.hk);
   const int64_t item = ih / a.hk;
   if (item >= items) return;
   Seq sq;
   int b, r0, lo, hi;
-  if (!many_block(a, item, sq, b, r0)) return;
+  if (!many_block<M>(a, item, sq, b, r0)) return;
   const int r = r0 + in;
   if (r >= sq.n * a.group) return;
-  many_keys(a, sq, r0, lo, hi);
+  many_keys<M>(a, sq, r0, lo, hi);
   const int size = split_size(hi - lo, a.splits, KT);
   const int used = hi > lo ? (hi - lo + size - 1) / size : 1;
   if (used == 1) return;
   const int i = r / a.group, h = kh * a.group + (r - i * a.group);
-  join_row<DT, D, 1>(a, used, (sq.row0 + i) * a.hq + h, [&](int x) { return (ih * a.splits + x) * kManyRows + in; });
+  join_row<DT, D, 1>(a, used, (sq.row0 + i) * a.hq + h, [&](int x) { return (ih * a.splits + x) * M + in; });
 }
 
 // ---- host -----------------------------------------------------------------------
@@ -1158,7 +1178,7 @@ struct Plan {
   bool few, many;        // which kernels may have work
   int splits, workers, row_stride;
   int64_t units, part_rows;
-  int many_splits;
+  int groups, many_splits;   // groups of 128 rows of the many-rows kernel
   int64_t items, many_part_rows;
 };
 
@@ -1183,13 +1203,16 @@ Plan plan_of(const pdm_kv_attention_desc* d, const pdm_kv_cache* c, const pdm_kv
   p.row_stride = (int)(rows < 16 * p.mt ? rows : 16 * p.mt);
   p.part_rows = !p.few ? 0 : p.workers ? 2 * p.workers * p.row_stride : p.splits > 1 ? p.units * p.row_stride : 0;
   if (p.many) {
-    p.items = b->tokens * group / kManyRows + b->num_seqs;
+    const int64_t all = b->tokens * group;
+    p.groups = c->head_dim < 256 && all >= 256 * (int64_t)b->num_seqs && all * c->n_kv_heads >= 256 * 256 ? 2 : 1;
+    const int M = 128 * p.groups;
+    p.items = all / M + b->num_seqs;
     const int64_t blocks = p.items * c->n_kv_heads;
     int64_t sp = blocks < 256 ? 512 / blocks : 1;
     const int64_t most_sp = (most + 511) / 512;
     sp = sp < most_sp ? sp : most_sp;
     p.many_splits = (int)(sp > 1 ? sp : 1);
-    p.many_part_rows = p.many_splits > 1 ? blocks * p.many_splits * kManyRows : 0;
+    p.many_part_rows = p.many_splits > 1 ? blocks * p.many_splits * M : 0;
   }
   return p;
 }
@@ -1199,6 +1222,13 @@ int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 // The two kernels run one after the other, each with its join: they share the workspace.
 int64_t part_rows_of(const Plan& p) { return p.part_rows > p.many_part_rows ? p.part_rows : p.many_part_rows; }
 int64_t workspace_of(const Plan& p, int D) { return round256(part_rows_of(p) * D * 4) + round256(part_rows_of(p) * 8) + round256((int64_t)p.workers * 16); }
+
+template <int DT, int D, int KT, int NG>
+void launch_many(const AttnArgs& a, const Plan& p, hipStream_t st) {
+  kv_attn_many_kernel<DT, D, KT, NG><<<linear_grid(p.items * a.hk * a.splits, (int64_t(1) << 23) / NG), 256 * NG, 0, st>>>(a, p.items);
+  if (p.many_part_rows)
+    kv_attn_many_join_kernel<DT, D, KT, 128 * NG><<<linear_grid(p.items * a.hk * 32 * NG), 256, 0, st>>>(a, p.items);
+}
 
 template <int DT, int D>
 void launch(AttnArgs& a, const Plan& p, hipStream_t st) {
@@ -1215,10 +1245,9 @@ void launch(AttnArgs& a, const Plan& p, hipStream_t st) {
   }
   if (!p.many) return;
   a.splits = p.many_splits;
-  constexpr int KT = D == 256 ? 32 : 64;
-  kv_attn_many_kernel<DT, D, KT><<<linear_grid(p.items * a.hk * a.splits), 256, 0, st>>>(a, p.items);
-  if (p.many_part_rows)
-    kv_attn_many_join_kernel<DT, D, KT><<<linear_grid(p.items * a.hk * (kManyRows / 4)), 256, 0, st>>>(a, p.items);
+  if constexpr (D == 256) launch_many<DT, D, 32, 1>(a, p, st);
+  else if (p.groups == 2) launch_many<DT, D, 64, 2>(a, p, st);
+  else launch_many<DT, D, 64, 1>(a, p, st);
 }
 
 template <int DT>
