@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
       ml[wave][1][mt * 16 + c] = l[mt];
     }
   }
-  __syncthreads();
+  lds_barrier();
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     const int r = mt * 16 + c;
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
         sum += ml[w][1][r] * (ml[w][0][r] == -kInf ? 1.0f : __builtin_amdgcn_exp2f(ml[w][0][r] - top));
       ml[kFewWaves][0][r] = top, ml[kFewWaves][1][r] = sum;
     }
-    if (mt) __syncthreads();
+    if (mt) lds_barrier();
     if (r < rows) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -584,7 +584,7 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
           *reinterpret_cast<f32x4_t*>(&red[wave][c][DD * (4 * g + e) + d]) =
               f32x4_t{o[mt][d][e] * f, o[mt][d + 1][e] * f, o[mt][d + 2][e] * f, o[mt][d + 3][e] * f};
     }
-    __syncthreads();
+    lds_barrier();
     const int here = rows - mt * 16 < 16 ? rows - mt * 16 : 16;
     for (int i4 = threadIdx.x; i4 < here * (D / 4); i4 += 256) {
       const int rr = i4 / (D / 4), d = 4 * (i4 - rr * (D / 4)), row = mt * 16 + rr;
@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
     }
   }
   if (!more) return;
-  __syncthreads();
+  lds_barrier();
   }
 }
 
@@ -792,7 +792,6 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
 
   const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // of the group
   const int grp = NG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
-  const bool k_role = NG == 1 || grp == 0, v_role = NG == 1 || grp == 1;
   const int c = lane & 31, h = lane >> 5;
 
   // this lane's row: its query, and the keys that it sees
@@ -843,11 +842,16 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
   float kss = 0.0f, vss = 0.0f;
   u32x4_t kr[KP];
   uint32_t vr[4][VD / 4];
-  float v_scale = 0.0f, sc_reg = 0.0f;
+  float v_scale = 0.0f;
   const int kc = (tid % (D / 16)) * 16, kr0 = tid / (D / 16);       // piece and row of K, 4096 / D rows a pass
   const int vm = D == 256 ? wave * 8 + (lane & 7) : (wave & 1) * 8 + (lane & 7);
   const int va = D == 256 ? lane >> 3 : (wave >> 1) * 8 + (lane >> 3);   // four keys of V
-  auto load = [&](int t) {
+  uint32_t k_off[KP];
+#pragma unroll
+  for (int p = 0; p < KP; ++p) k_off[p] = ((kr0 + p * (4096 / D)) & 15) * D + kc;
+  const uint32_t v_off = (va & 3) * 4 * D + vm * VD;
+  // KV: 1 K, 2 V, 3 both (a type's value)
+  auto load = [&](int t, auto kv) {
     const int key0 = begin + t * KT;
     if (t % PER == 0) {
       const int key = key0 + 16 * lane;
@@ -865,33 +869,42 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
         }
       }
     }
+    // bytes before the 16 keys `grp` of the tile (a page that does not exist: some page, its keys are not seen)
     const int g0 = (t % PER) * (KT / 16);
-    sc_reg = __shfl(kss, g0 + (lane & (KT / 16 - 1)));
-    if (k_role) {
+    auto place = [&](int grp) {
+      const int id = __builtin_amdgcn_readlane(ids, g0 + grp);
+      return ((((int64_t)(id < 0 ? 0 : id) * a.hk + kh) << a.page_log2) + ((key0 + 16 * grp) & mask)) * D;
+    };
+    if constexpr (decltype(kv)::value & 1) {
 #pragma unroll
-    for (int p = 0; p < KP; ++p) {
-      const int r = kr0 + p * (4096 / D);
-      const int grp = __builtin_amdgcn_readfirstlane(r >> 4);
-      const int id = __builtin_amdgcn_readlane(ids, g0 + grp);  // (a page that does not exist: some page, not seen)
-      const int64_t at = (((int64_t)(id < 0 ? 0 : id) * a.hk + kh) << a.page_log2) + ((key0 + 16 * grp) & mask);
-      kr[p] = *reinterpret_cast<const u32x4_t*>(a.k_codes + at * D + ((r & 15) * D + kc));
-    }
-    }
-    if (v_role) {
-    const int v_id = __shfl(ids, g0 + (va >> 2));
-    v_scale = __shfl(vss, g0 + (va >> 2));
-    const int64_t at = (((int64_t)(v_id < 0 ? 0 : v_id) * a.hk + kh) << a.page_log2) + ((key0 + 16 * (va >> 2)) & mask);
-    const uint8_t* p = a.v_codes + at * D + ((va & 3) * 4 * D + vm * VD);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if constexpr (VD == 4) {
-        vr[r][0] = *reinterpret_cast<const uint32_t*>(p + r * D);
-      } else {
-        const u32x2_t w = *reinterpret_cast<const u32x2_t*>(p + r * D);
-        vr[r][0] = w[0], vr[r][1] = w[1];
+      for (int p = 0; p < KP; ++p) {
+        const int grp = __builtin_amdgcn_readfirstlane((kr0 + p * (4096 / D)) >> 4);
+        kr[p] = *reinterpret_cast<const u32x4_t*>(a.k_codes + place(grp) + k_off[p]);
       }
     }
+    if constexpr (decltype(kv)::value & 2) {
+      // lanes 0..31 and 32..63 load keys of two neighbouring 16
+      const int grp = __builtin_amdgcn_readfirstlane(va >> 2);
+      const int64_t p0 = place(grp), p1 = place(grp + 1);
+      const float s0 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vss), g0 + grp));
+      const float s1 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vss), g0 + grp + 1));
+      v_scale = lane < 32 ? s0 : s1;
+      const uint8_t* p = a.v_codes + (lane < 32 ? p0 : p1) + v_off;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (VD == 4) {
+          vr[r][0] = *reinterpret_cast<const uint32_t*>(p + r * D);
+        } else {
+          const u32x2_t w = *reinterpret_cast<const u32x2_t*>(p + r * D);
+          vr[r][0] = w[0], vr[r][1] = w[1];
+        }
+      }
     }
+  };
+  // the K scales of tile t: the lanes that hold them (before the next batch is looked up)
+  auto stage_sc = [&](int t) {
+    const uint32_t x = lane - (t % PER) * (KT / 16);
+    if (wave == 0 && x < KT / 16) sh.sc[t & 1][x] = kss;
   };
   auto stage_k = [&](int t) {
     char* kb = sh.k[t & 1];
@@ -907,7 +920,7 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
       *reinterpret_cast<u32x4_t*>(dst) = w0;
       *reinterpret_cast<u32x4_t*>(dst + 16) = w1;
     }
-    if (wave == 0 && lane < KT / 16) sh.sc[t & 1][lane] = sc_reg;
+    stage_sc(t);
   };
   // V^T of tile t; NaN codes become zeros here (0 * NaN would reach rows that do not see the key) and are remembered, or,
   // in MARK, ones where everything else becomes zero.
@@ -1042,50 +1055,63 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
   };
 
   if (tiles > 0) {
-    auto stage = [&](int t) {
-      if (k_role) stage_k(t);
-      if (v_role) stage_v(t, std::false_type());
-    };
-    load(0);
-    stage(0);
-    if (tiles > 1) load(1);
     // Barrier k + 1 begins phase k: the first group has products at even ones, the second at odd ones.  K of tile t + 1 is
     // written in phase 2 t + 1, where the other group reads that of tile t; V of tile t + 1 in phase 2 t + 2 (or before the
-    // barrier between them, where there is one group): what either overwrites was last read in an earlier phase.
-    if (NG == 2 && grp == 1) __syncthreads();
+    // barrier between them, where there is one group): what either overwrites was last read in an earlier phase.  Behind
+    // the last tile that one is loaded and written again, to no use.
+    auto run = [&](auto kv) {
+      auto stage = [&](int t) {
+        if constexpr (decltype(kv)::value & 1) stage_k(t);
+        if constexpr (decltype(kv)::value & 2) stage_v(t, std::false_type());
+      };
+      const int last = tiles - 1;
+      load(0, kv);
+      stage(0);
+      load(last > 0 ? 1 : 0, kv);
+      if (decltype(kv)::value == 2) lds_barrier();
+      lds_barrier();
+      scores(0);
+      lds_barrier();
+      weights(0);
+      stage(1);
+      load(last < 2 ? last : 2, kv);
 #pragma unroll 1
-    for (int t = 0; t <= tiles; ++t) {
-      __syncthreads();
-      __builtin_amdgcn_sched_barrier(0);
-      if (t > 0) values(t - 1);
-      __builtin_amdgcn_sched_barrier(0);
-      if (t < tiles) scores(t);
-      __builtin_amdgcn_sched_barrier(0);
-      __syncthreads();
-      if (t < tiles) {
+      for (int t = 1; t < tiles; ++t) {
+        lds_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        values(t - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        scores(t);
+        __builtin_amdgcn_sched_barrier(0);
+        lds_barrier();
         weights(t);
-        if (t + 1 < tiles) {
-          stage(t + 1);
-          if (t + 2 < tiles) load(t + 2);
-        }
+        stage(t + 1);
+        load(last < t + 2 ? last : t + 2, kv);
       }
-    }
-    if (NG == 2 && grp == 0) __syncthreads();
+      lds_barrier();
+      values(last);
+      if (decltype(kv)::value == 1) lds_barrier();
+    };
+    if (NG == 1) run(std::integral_constant<int, 3>());
+    else if (grp == 0) run(std::integral_constant<int, 1>());
+    else run(std::integral_constant<int, 2>());
 
     // NaN among the values of any wave's share: once more over the tiles, with ones for NaN and for keys that are seen
     if (lane == 0) sh.odd[grp * 4 + wave] = odd;
-    __syncthreads();
+    lds_barrier();
     int any = 0;
 #pragma unroll
     for (int w = 0; w < 4 * NG; ++w) any |= sh.odd[w];
     if (any) {
 #pragma unroll 1
       for (int t = 0; t < tiles; ++t) {
-        load(t);
-        __syncthreads();  // the tile before is done with
-        if (v_role) stage_v(t, std::true_type());
-        if (v_role && wave == 0 && lane < KT / 16) sh.sc[t & 1][lane] = sc_reg;
-        __syncthreads();
+        load(t, std::integral_constant<int, 2>());
+        lds_barrier();  // the tile before is done with
+        if (grp == NG - 1) {
+          stage_v(t, std::true_type());
+          stage_sc(t);
+        }
+        lds_barrier();
 #pragma unroll 1
         for (int y = 0; y < 2 * XX; ++y) {
           u32x4_t seen;

@@ -127,6 +127,13 @@ __device__ __forceinline__ float group_max(float v, int width) {
   return v;
 }
 
+// A workgroup barrier that orders LDS alone: global loads stay in flight across it (__syncthreads waits for them).
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // ---- positions ---------------------------------------------------------------
 __device__ __forceinline__ int64_t load_position(const void* positions, int bits, int64_t t) {
   return bits == 64 ? static_cast<const int64_t*>(positions)[t] : (int64_t)static_cast<const int32_t*>(positions)[t];
