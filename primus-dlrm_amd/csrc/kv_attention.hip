@@ -108,6 +108,15 @@ __device__ __forceinline__ f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c) {
   else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
+// A lane's value, for the whole wave.
+__device__ __forceinline__ float lane_f(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+
 // NaN codes of a dword: bit 7 of each byte that holds one.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 // 0xff in the bytes whose bit 7 is set.
@@ -296,18 +305,19 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
   int all_lo, all_hi;                     // keys that every row sees (rows that are not there do not count)
   int kh, begin, end, mine;               // of the pair whose tiles are loaded; tiles of this wave
   const int32_t* table;
-  // lane x of a batch of 32 tiles: page and scales of the 16 keys x % 2 of tile x / 2
-  int ids = -1;
-  float kss = 0.0f, vss = 0.0f;
+  // lane x of a batch of 32 tiles: place (in bytes) and scales of the 16 keys x % 2 of tile x / 2
+  uint64_t spot = 0;
+  float kss = 0.0f, vss = 0.0f;           // kss: NaN where the page does not exist
   auto key_of = [&](int i) { return begin + (wave + kFewWaves * i) * kFewKeys; };
   auto look_up = [&](int first) {
     const int key = key_of(first + (lane >> 1)) + (lane & 1) * 16;
-    ids = -1;
+    // (a page that does not exist: some page, its keys are not seen)
+    spot = 0, kss = __builtin_nanf(""), vss = 0.0f;
     if (key < end) {
       const int id = table[key >> a.page_log2];
       if (id >= 0 && id < a.num_pages) {
-        ids = id;
         const int64_t entry = (int64_t)id * a.hk + kh;
+        spot = (uint64_t)((entry << a.page_log2) + (key & ((1 << a.page_log2) - 1))) * D;
         kss = a.k_scale[entry];
         vss = a.v_scale[entry];
       } else if (a.err) {
@@ -315,12 +325,7 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
       }
     }
   };
-  // byte of the first of the 16 keys s of tile i (a page that does not exist: some page, its keys are not seen)
-  auto place = [&](int i, int s) {
-    const int id = __builtin_amdgcn_readlane(ids, (i & 31) * 2 + s);
-    const int slot = (key_of(i) + 16 * s) & ((1 << a.page_log2) - 1);
-    return (((((int64_t)(id < 0 ? 0 : id)) * a.hk + kh) << a.page_log2) + slot) * D;
-  };
+  auto place = [&](int i, int s) { return lane_u64(spot, (i & 31) * 2 + s); };
   u32x4_t k[2][D / 64];                   // 16 bytes of a key row, 64 apart
   uint32_t v[2][4][D / 64];               // rows 4 g + i of 16 keys
   const uint32_t k_off = (uint32_t)(c * D + 16 * g);
@@ -425,9 +430,8 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
 #pragma unroll 1
   for (int i = 0; i < mine; ++i) {
     const int x0 = (i & 31) * 2;
-    auto lane_f = [&](float f, int x) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), x)); };
-    const bool ok[2] = {__builtin_amdgcn_readlane(ids, x0) >= 0, __builtin_amdgcn_readlane(ids, x0 + 1) >= 0};
     const float ks[2] = {a.scale2 * lane_f(kss, x0), a.scale2 * lane_f(kss, x0 + 1)};
+    const bool ok[2] = {ks[0] == ks[0], ks[1] == ks[1]};
     const float vs[2] = {lane_f(vss, x0), lane_f(vss, x0 + 1)};
     f32x4_t s[MT][2];
 #pragma unroll
@@ -509,7 +513,8 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
 #pragma unroll 1
     for (int i = 0; i < mine; ++i) {
       if ((i & 31) == 0) look_up(i);
-      const bool ok[2] = {__builtin_amdgcn_readlane(ids, (i & 31) * 2) >= 0, __builtin_amdgcn_readlane(ids, (i & 31) * 2 + 1) >= 0};
+      const float k0 = lane_f(kss, (i & 31) * 2), k1 = lane_f(kss, (i & 31) * 2 + 1);
+      const bool ok[2] = {k0 == k0, k1 == k1};
       if (whole_tile(i, ok[0] && ok[1])) continue;
       load_v(i);
 #pragma unroll
@@ -714,7 +719,7 @@ __global__ void __launch_bounds__(256) kv_attn_dealt_join_kernel(AttnArgs a) {
 // keys in two phases: products (O += V^T P of the tile before, S of this one) and softmax (P from S), with a barrier
 // after each.  With two groups the second is one phase behind the first, so that on every SIMD a wave's products run
 // beside the other's softmax; left to themselves, two waves of a SIMD were found in the same phase and took turns.
-// Tiles are converted once on their way into LDS, in the softmax phase, their loads a tile earlier: K as rows by the
+// Tiles are converted once on their way into LDS, in the softmax phase, their loads a phase earlier: K as rows by the
 // first group, V transposed by the second, its keys in the order in which the first product leaves P.
 template <int D, int KT>
 struct ManyShared {
@@ -838,7 +843,7 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
   const int32_t* table = a.table + (int64_t)b * a.table_stride;
   const int mask = (1 << a.page_log2) - 1;
   constexpr int PER = 1024 / KT;           // tiles of a batch of 1024 keys
-  int ids = -1;                            // lane i: page and scales of keys 16 i .. of the batch
+  uint64_t spot = 0;                       // lane i: place and scales of keys 16 i .. of the batch
   float kss = 0.0f, vss = 0.0f;
   u32x4_t kr[KP];
   uint32_t vr[4][VD / 4];
@@ -855,12 +860,13 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
     const int key0 = begin + t * KT;
     if (t % PER == 0) {
       const int key = key0 + 16 * lane;
-      ids = -1, kss = __builtin_nanf(""), vss = 0.0f;
+      // (a page that does not exist: some page, its keys are not seen)
+      spot = 0, kss = __builtin_nanf(""), vss = 0.0f;
       if (key < end) {
         const int id = table[key >> a.page_log2];
         if (id >= 0 && id < a.num_pages) {
-          ids = id;
           const int64_t entry = (int64_t)id * a.hk + kh;
+          spot = (uint64_t)((entry << a.page_log2) + (key & mask)) * D;
           // not zero: a hidden score times it stays -inf
           kss = fmaxf(a.k_scale[entry] * fabsf(a.scale2), 0x1p-126f);
           vss = a.v_scale[entry];
@@ -869,12 +875,8 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
         }
       }
     }
-    // bytes before the 16 keys `grp` of the tile (a page that does not exist: some page, its keys are not seen)
     const int g0 = (t % PER) * (KT / 16);
-    auto place = [&](int grp) {
-      const int id = __builtin_amdgcn_readlane(ids, g0 + grp);
-      return ((((int64_t)(id < 0 ? 0 : id) * a.hk + kh) << a.page_log2) + ((key0 + 16 * grp) & mask)) * D;
-    };
+    auto place = [&](int grp) { return lane_u64(spot, g0 + grp); };  // bytes before the 16 keys `grp` of the tile
     if constexpr (decltype(kv)::value & 1) {
 #pragma unroll
       for (int p = 0; p < KP; ++p) {
@@ -885,9 +887,8 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
     if constexpr (decltype(kv)::value & 2) {
       // lanes 0..31 and 32..63 load keys of two neighbouring 16
       const int grp = __builtin_amdgcn_readfirstlane(va >> 2);
-      const int64_t p0 = place(grp), p1 = place(grp + 1);
-      const float s0 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vss), g0 + grp));
-      const float s1 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vss), g0 + grp + 1));
+      const uint64_t p0 = place(grp), p1 = place(grp + 1);
+      const float s0 = lane_f(vss, g0 + grp), s1 = lane_f(vss, g0 + grp + 1);
       v_scale = lane < 32 ? s0 : s1;
       const uint8_t* p = a.v_codes + (lane < 32 ? p0 : p1) + v_off;
 #pragma unroll
@@ -1067,26 +1068,25 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
       const int last = tiles - 1;
       load(0, kv);
       stage(0);
-      load(last > 0 ? 1 : 0, kv);
       if (decltype(kv)::value == 2) lds_barrier();
       lds_barrier();
+      load(last > 0 ? 1 : 0, kv);
       scores(0);
       lds_barrier();
-      weights(0);
       stage(1);
-      load(last < 2 ? last : 2, kv);
+      weights(0);
 #pragma unroll 1
       for (int t = 1; t < tiles; ++t) {
         lds_barrier();
+        load(last < t + 1 ? last : t + 1, kv);
         __builtin_amdgcn_sched_barrier(0);
         values(t - 1);
         __builtin_amdgcn_sched_barrier(0);
         scores(t);
         __builtin_amdgcn_sched_barrier(0);
         lds_barrier();
-        weights(t);
         stage(t + 1);
-        load(last < t + 2 ? last : t + 2, kv);
+        weights(t);
       }
       lds_barrier();
       values(last);
