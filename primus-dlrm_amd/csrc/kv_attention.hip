@@ -1136,7 +1136,7 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
   const float sum = l + __shfl_xor(l, 32);
   if (row >= rows) return;
   const int64_t at = (sq.row0 + tok) * a.hq + head;
-  if (used == 1) {
+  if (NG > 1 || used == 1) {  // (two groups: there are blocks enough, no splits)
     const float f = sum != 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
     for (int d = 0; d < DD; ++d)
@@ -1159,8 +1159,9 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
 }
 
 // Joins the splits of the many-rows kernel: one wave per row.
-template <int DT, int D, int KT, int M>
+template <int DT, int D, int KT>
 __global__ void __launch_bounds__(256) kv_attn_many_join_kernel(AttnArgs a, int64_t items) {
+  constexpr int M = 128;
   const int64_t x = linear_block() * 4 + (threadIdx.x >> 6);
   const int in = (int)(x % M);
   const int64_t ih = x / M;
@@ -1234,7 +1235,7 @@ Plan plan_of(const pdm_kv_attention_desc* d, const pdm_kv_cache* c, const pdm_kv
     const int M = 128 * p.groups;
     p.items = all / M + b->num_seqs;
     const int64_t blocks = p.items * c->n_kv_heads;
-    int64_t sp = blocks < 256 ? 512 / blocks : 1;
+    int64_t sp = blocks < 256 && p.groups == 1 ? 512 / blocks : 1;
     const int64_t most_sp = (most + 511) / 512;
     sp = sp < most_sp ? sp : most_sp;
     p.many_splits = (int)(sp > 1 ? sp : 1);
@@ -1252,8 +1253,8 @@ int64_t workspace_of(const Plan& p, int D) { return round256(part_rows_of(p) * D
 template <int DT, int D, int KT, int NG>
 void launch_many(const AttnArgs& a, const Plan& p, hipStream_t st) {
   kv_attn_many_kernel<DT, D, KT, NG><<<linear_grid(p.items * a.hk * a.splits, (int64_t(1) << 23) / NG), 256 * NG, 0, st>>>(a, p.items);
-  if (p.many_part_rows)
-    kv_attn_many_join_kernel<DT, D, KT, 128 * NG><<<linear_grid(p.items * a.hk * 32 * NG), 256, 0, st>>>(a, p.items);
+  if constexpr (NG == 1)
+    if (p.many_part_rows) kv_attn_many_join_kernel<DT, D, KT><<<linear_grid(p.items * a.hk * 32), 256, 0, st>>>(a, p.items);
 }
 
 template <int DT, int D>

@@ -286,7 +286,119 @@ def test_many_sequences(pdm, dev):
     c.check(c.run(), want)
 
 
-@pytest.mark.parametrize("new,lens", [([1, 1], [900, 30]), ([40, 2, 200], [700, 90, 260])])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new,lens,D,page,hk,group", [
+    ([150, 110], [500, 700], 128, 16, 32, 8), ([260, 0, 1, 600], [260, 9, 130, 901], 64, 64, 16, 5),
+    ([1100, 950], [1100, 1000], 64, 128, 32, 1), ([700], [700], 128, 32, 24, 4), ([33, 400], [33, 64], 128, 64, 32, 8)])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 70), (False, 333)])
+def test_large_batches(pdm, dev, dtype, new, lens, D, page, hk, group, causal, window):
+    """Rows enough that workgroups take 256 of them; blocks that end inside a sequence, a page, a tile."""
+    lens = [max(n, x) for n, x in zip(new, lens)]
+    c = Case(pdm, dev, new, lens, hk * group, hk, D, page, dtype, seed=D + hk)
+    c.check(c.run(causal=causal, window=window), c.want(causal=causal, window=window))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_large_batches_with_bad_places(pdm, dev, D):
+    """The same with a NaN value and a NaN key of one head, seen by some rows only, pages that do not exist, lengths that do
+    not fit, padding; and the same bits from a second run."""
+    new, lens = [500, 300, 600], [800, 350, 600]
+    for which in ("k_codes", "v_codes"):
+        for at in (40, 333, 799):
+            c = Case(pdm, dev, new, lens, 64, 64, D, 32, seed=at)
+            getattr(c.cache, which).view(torch.uint8)[c.table[0][at // 32], 5, at % 32, 7] = 0x7F
+            got = c.run(window=250)
+            c.check(got, c.want(window=250))
+            assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(got, c.run(window=250)))
+    c = Case(pdm, dev, new, lens, 64, 64, D, 32, seed=1)
+    for b, i, bad in ((0, 3, -1), (0, 4, 2 ** 31 - 1), (2, 0, 10_000)):
+        c.table[b][i] = bad
+    want = c.want()
+    q = torch.cat((c.q, torch.full((300, 64, D), math.nan, dtype=c.q.dtype)))
+    out, lse = c.run(q=q)
+    assert c.cache.err_flag.item() == 1 and (out[1400:] == 0).all() and (lse[1400:] == -math.inf).all()
+    c.cache.err_flag.zero_()
+    c.check((out[:1400], lse[:1400]), want)
+    c.lens[1] = 299
+    out, lse = c.run()
+    assert c.cache.err_flag.item() == 1 and (out[500:800] == 0).all() and (lse[500:800] == -math.inf).all()
+    c.cache.err_flag.zero_()
+    keep = torch.cat((torch.arange(500), torch.arange(800, 1400)))
+    c.check((out[keep], lse[keep]), [w[keep] for w in want])
+
+
+def _uneven(seed, n, most, longest):
+    g = torch.Generator().manual_seed(seed)
+    new = torch.randint(0, most + 1, (n,), generator=g).tolist()
+    lens = torch.randint(1, 400, (n,), generator=g).tolist()
+    lens[n // 3], lens[n - 1], lens[0] = longest, 2000, 1
+    return new, [max(a, b) for a, b in zip(new, lens)]
+
+
+@pytest.mark.parametrize("D,page,n,hk,group,most,longest", [
+    (64, 16, 40, 8, 4, 2, 5000), (128, 32, 33, 8, 1, 8, 9000), (256, 64, 64, 4, 2, 2, 3500), (128, 128, 256, 4, 3, 1, 6001),
+    (64, 64, 255, 2, 5, 1, 20000), (128, 16, 9, 40, 8, 1, 2500)])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 150), (False, 1000)])
+def test_many_uneven_contexts(pdm, dev, D, page, n, hk, group, most, longest, causal, window):
+    """Batches whose keys are dealt to the workgroups: parts of a (sequence, head), several in a workgroup, one over many
+    workgroups; sequences without new tokens."""
+    new, lens = _uneven(D + n, n, most, longest)
+    c = Case(pdm, dev, new, lens, hk * group, hk, D, page, torch.float16 if n == 64 else torch.bfloat16, seed=n, extra=1)
+    kw = dict(causal=causal, window=window)
+    want = c.want(**kw)
+    c.check(c.run(max_q_len=most, **kw), want)
+    c.check(c.run(max_q_len=8 // group, **kw), want)
+
+
+def test_many_uneven_contexts_with_bad_places(pdm, dev):
+    """NaN keys and values, infinite queries, pages that do not exist, sequences that do not fit, padding, in turn."""
+    new, lens = _uneven(3, 40, 2, 4000)
+    new[13], new[20] = 2, 1
+    for which in ("k_codes", "v_codes"):
+        c = Case(pdm, dev, new, lens, 16, 8, 128, 32, seed=1)
+        for at in (0, 1500, lens[13] - 1):
+            getattr(c.cache, which).view(torch.uint8)[c.table[13][at // 32], 3, at % 32, 64] = 0x7F
+            for window in (0, 300):
+                c.check(c.run(max_q_len=2, window=window), c.want(window=window))
+    c = Case(pdm, dev, new, lens, 16, 8, 128, 32, seed=2)
+    base = c.run(max_q_len=2)
+    r = c.cu[13]
+    c.q[r, 5] = math.inf
+    got = c.run(max_q_len=2)
+    keep = torch.ones(c.q.shape[:2], dtype=torch.bool)
+    keep[r, 5] = False
+    assert torch.equal(got[0].cpu()[keep], base[0].cpu()[keep]) and got[0][r, 5].isnan().all()
+    c = Case(pdm, dev, new, lens, 16, 8, 128, 32, seed=2)
+    for i in (0, 30, 31, 90):
+        c.table[13][i] = -1
+    c.table[20] = [-1] * len(c.table[20])
+    want = c.want()
+    q = torch.cat((c.q, torch.full((5, 16, 128), math.nan, dtype=c.q.dtype)))
+    T = len(c.q)
+    out, lse = c.run(q=q, max_q_len=2)
+    assert c.cache.err_flag.item() == 1 and (out[T:] == 0).all() and (lse[T:] == -math.inf).all()
+    c.cache.err_flag.zero_()
+    c.check((out[:T], lse[:T]), want)
+    fit = list(c.lens)
+    c.lens[13] = 1  # below its two new tokens
+    out, lse = c.run(max_q_len=2)
+    assert c.cache.err_flag.item() == 1 and (out[r:r + 2] == 0).all() and (lse[r:r + 2] == -math.inf).all()
+    c.cache.err_flag.zero_()
+    keep = torch.tensor([t for t in range(T) if not r <= t < r + 2])
+    c.check((out[keep], lse[keep]), [w[keep] for w in want])
+    c.lens = fit
+    out, lse = c.run(max_q_len=1)  # more new tokens than promised
+    assert c.cache.err_flag.item() == 1
+    c.cache.err_flag.zero_()
+    one = torch.tensor([t for b in range(40) for t in range(c.cu[b], c.cu[b + 1]) if new[b] == 1])
+    assert (out[r:r + 2] == 0).all() and (lse[r:r + 2] == -math.inf).all()
+    c.check((out[one], lse[one]), [w[one] for w in want])
+
+
+UNEVEN = _uneven(5, 140, 1, 2500)
+
+
+@pytest.mark.parametrize("new,lens", [([1, 1], [900, 30]), ([40, 2, 200], [700, 90, 260]), UNEVEN, ([9000, 7400], [9000, 7400])])
 def test_repeats_streams_and_graphs(pdm, dev, new, lens):
     """The same bits every time; two captured graphs and eager calls in turn, with lengths that change in place."""
     cs = [Case(pdm, dev, new, lens, 4, 2, 128, 32, seed=s, extra=2) for s in (0, 1)]
@@ -296,7 +408,8 @@ def test_repeats_streams_and_graphs(pdm, dev, new, lens):
 
     def step(i):
         k = cs[i].cache
-        return pdm.kv_attention(dq[i], k.k_codes, k.v_codes, k.k_scale, k.v_scale, cu, table[i], ln, return_lse=True)
+        return pdm.kv_attention(dq[i], k.k_codes, k.v_codes, k.k_scale, k.v_scale, cu, table[i], ln, max_q_len=max(new),
+                                return_lse=True)
 
     first = [step(0), step(1)]
     side = torch.cuda.Stream()
