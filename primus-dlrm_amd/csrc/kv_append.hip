@@ -95,6 +95,16 @@ __device__ __forceinline__ void to_float(const Row<DT>& x, float* v) {
   raw_to_float<DT>(x.w + (DT == PDM_F32 ? 2 : 1), v + 8);
 }
 
+// x in fp32, rounded to odd: what is cut off leaves the last bit set, so that the code's rounding sees on which side of a tie
+// x lies.  (On the words of the double: 4 integer operations, where a comparison with the rounded number cost 1 us of 15.)
+__device__ __forceinline__ float to_odd(double x) {
+  constexpr uint32_t cut = 0x1fffffffu;  // the 29 bits that fp32 does not have
+  const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)bits;
+  const uint64_t odd = (bits >> 32) << 32 | ((lo | ((lo & cut) + cut)) & ~cut);
+  return (float)__builtin_bit_cast(double, odd);
+}
+
 // A key row normed and rotated, in 64 bits (as fast as 32 here): its code is the nearest to the key itself, whatever the
 // order of the sum.  Called by the row's whole group; `ok`: this row exists.
 template <bool NORM, bool INTER>
@@ -136,8 +146,8 @@ __device__ __forceinline__ void key_row(const AppendArgs& a, const Segment& g, i
       y = y * (double)c[i] + x * (double)s[i];
       x = t;
     }
-    v[ia] = zero ? 0.0f : (float)x;
-    v[ib] = zero ? 0.0f : (float)y;
+    v[ia] = zero ? 0.0f : to_odd(x);
+    v[ib] = zero ? 0.0f : to_odd(y);
   }
 }
 
