@@ -730,8 +730,8 @@ struct ManyShared {
   static constexpr int KS = 2 * D + 16;    // bytes of a K row: 16 rows of a fragment read fall into different banks
   static constexpr int VS = 2 * KT;        // bytes of a V^T row, its 16-byte pieces exchanged by turn()
   // Piece g of row d lies at g ^ turn(d): any 16 rows of a fragment read, and the 8 rows that 8 lanes write at a time
-  // (rows 8 apart), fall into different banks.  (With rows padded to 144 bytes a write took 32 cycles instead of 8.)
-  __device__ static constexpr int turn(int d) { return KT == 64 ? ((d >> 1) ^ (d >> 3)) & 7 : ((d >> 2) ^ (d >> 4)) & 3; }
+  // (rows 16 apart), fall into different banks.  (With rows padded to 144 bytes a write took 32 cycles instead of 8.)
+  __device__ static constexpr int turn(int d) { return KT == 64 ? ((d >> 1) ^ (d >> 4)) & 7 : ((d >> 2) ^ (d >> 4)) & 3; }
   alignas(16) char k[2][KT * KS];
   alignas(16) char v[2][D * VS];
   float sc[2][KT / 16];                    // scale2 * scale of 16 keys; NaN where their page does not exist
@@ -850,15 +850,19 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
   uint64_t spot = 0;                       // lane i: place and scales of keys 16 i .. of the batch
   float kss = 0.0f, vss = 0.0f;
   u32x4_t kr[KP];
-  uint32_t vr[4][VD / 4];
+  u32x4_t vw[D == 64 ? 1 : 2];             // 16 elements of a key, or of two keys
+  uint32_t vr[4][VD / 4];                  // VD elements of four keys, exchanged
   float v_scale = 0.0f;
   const int kc = (tid % (D / 16)) * 16, kr0 = tid / (D / 16);       // piece and row of K, 4096 / D rows a pass
-  const int vm = D == 256 ? wave * 8 + (lane & 7) : (wave & 1) * 8 + (lane & 7);
-  const int va = D == 256 ? lane >> 3 : (wave >> 1) * 8 + (lane >> 3);   // four keys of V
+  // V: lanes 0 .. 31 and 32 .. 63 (D = 64: a row of 16 lanes each) load keys of the same four, 16 elements of each, and
+  // then exchange them for VD elements of all four: piece vm, four keys va
+  constexpr int VC = D / 16;               // 16-byte pieces of a row
+  const int va = D == 256 ? wave * 2 + (lane >> 4 & 1) : wave * 4 + (D == 64 ? lane >> 2 & 3 : lane >> 3 & 3);
+  const int vm = D == 64 ? 4 * (lane & 3) + (lane >> 4) : 2 * (lane & (VC - 1)) + (lane >> 5);
   uint32_t k_off[KP];
 #pragma unroll
   for (int p = 0; p < KP; ++p) k_off[p] = ((kr0 + p * (4096 / D)) & 15) * D + kc;
-  const uint32_t v_off = (va & 3) * 4 * D + vm * VD;
+  const uint32_t v_off = ((va & 3) * 4 + (D == 64 ? lane >> 4 : 2 * (lane >> 5))) * D + 16 * (lane & (VC - 1));
   // KV: 1 K, 2 V, 3 both (a type's value)
   auto load = [&](int t, auto kv) {
     const int key0 = begin + t * KT;
@@ -889,21 +893,28 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
       }
     }
     if constexpr (decltype(kv)::value & 2) {
-      // lanes 0..31 and 32..63 load keys of two neighbouring 16
-      const int grp = __builtin_amdgcn_readfirstlane(va >> 2);
-      const uint64_t p0 = place(grp), p1 = place(grp + 1);
-      const float s0 = lane_f(vss, g0 + grp), s1 = lane_f(vss, g0 + grp + 1);
-      v_scale = lane < 32 ? s0 : s1;
-      const uint8_t* p = a.v_codes + (lane < 32 ? p0 : p1) + v_off;
+      const int grp = D == 256 ? wave >> 1 : wave;
+      v_scale = lane_f(vss, g0 + grp);
+      const uint8_t* p = a.v_codes + place(grp) + v_off;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if constexpr (VD == 4) {
-          vr[r][0] = *reinterpret_cast<const uint32_t*>(p + r * D);
-        } else {
-          const u32x2_t w = *reinterpret_cast<const u32x2_t*>(p + r * D);
-          vr[r][0] = w[0], vr[r][1] = w[1];
+      for (int r = 0; r < (D == 64 ? 1 : 2); ++r) vw[r] = *reinterpret_cast<const u32x4_t*>(p + r * D);
+    }
+  };
+  auto exchange = [&]() {
+    if constexpr (D == 64) {
+      const u32x2_t x = __builtin_amdgcn_permlane32_swap(vw[0][0], vw[0][2], false, false);
+      const u32x2_t y = __builtin_amdgcn_permlane32_swap(vw[0][1], vw[0][3], false, false);
+      const u32x2_t lo = __builtin_amdgcn_permlane16_swap(x[0], y[0], false, false);
+      const u32x2_t hi = __builtin_amdgcn_permlane16_swap(x[1], y[1], false, false);
+      vr[0][0] = lo[0], vr[1][0] = lo[1], vr[2][0] = hi[0], vr[3][0] = hi[1];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const u32x2_t x = __builtin_amdgcn_permlane32_swap(vw[r][e], vw[r][2 + e], false, false);
+          vr[r][e] = x[0], vr[2 + r][e] = x[1];
         }
-      }
     }
   };
   // the K scales of tile t: the lanes that hold them (before the next batch is looked up)
@@ -934,6 +945,7 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
     // keys 4 va .. + 3: block va % 4 of their 16; blocks 0, 2 belong to lanes h = 0 of the product, 1, 3 to h = 1
     const int x = va & 3;
     const uint32_t at = vm * VD * VS + 16 * ((2 * (va >> 2) + (x & 1)) ^ ManyShared<D, KT>::turn(vm * VD)) + 8 * (x >> 1);
+    exchange();
     uint32_t nan = 0;
 #pragma unroll
     for (int e = 0; e < VD / 4; ++e)
