@@ -198,18 +198,18 @@ __device__ __forceinline__ void store_codes(uint8_t* row, const RowPlace& pl, fl
   *reinterpret_cast<u32x2_t*>(row + pl.hi) = u32x2_t{e4m3x4(v + 8), e4m3x4(v + 12)};
 }
 
-// Pages with many new tokens: a page and head, its keys and then its values, per W waves; a lane group takes NI rows.  The loads
-// of both are in flight together, and the values stay in registers between the maximum and the codes.
+// Pages with several new tokens (`least` or more): a page and head, its keys and then its values, per W waves; a lane group takes
+// NI rows.  The loads of both are in flight together, and the values stay in registers between the maximum and the codes.
 template <int DT, bool NORM, bool INTER, bool VEC, int W, int NI>
-__global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a, int64_t items) {
+__device__ __forceinline__ void append_page(const AppendArgs& a, int64_t items, int64_t block, int least) {
   __shared__ float red[2][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t unit = (linear_block() * 4 + wave) / W;
+  const int64_t unit = (block * 4 + wave) / W;
   const int64_t item = unit / a.heads;
   if (item >= items) return;  // W == 4: the same for the whole block
   const int h = (int)(unit - item * a.heads);
   Segment g;
-  if (!find_segment(a, item, g)) return;
+  if (!find_segment(a, item, g) || g.n < least) return;
 
   const int width = 1 << a.width_log2;
   const int j = lane & (width - 1);
@@ -275,16 +275,23 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a, int64_t it
   }
 }
 
+template <int DT, bool NORM, bool INTER, bool VEC, int W, int NI>
+__global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a, int64_t items) {
+  append_page<DT, NORM, INTER, VEC, W, NI>(a, items, linear_block(), 1);
+}
+
 // Pages with a token or two: a lane group per (page, head, keys or values), its rows one after the other, read again for the
-// codes where there are several.
+// codes where there are two.
+constexpr int kFewTokens = 2;
+
 template <int DT, bool NORM, bool INTER, bool VEC>
-__global__ void __launch_bounds__(256) kv_append_token_kernel(AppendArgs a, int64_t items, int waves) {
+__device__ __forceinline__ void append_tokens(const AppendArgs& a, int64_t items, int waves, int64_t block) {
   const int lane = threadIdx.x & 63;
-  const int64_t unit = linear_block() * 4 + (threadIdx.x >> 6);
+  const int64_t unit = block * 4 + (threadIdx.x >> 6);
   const int64_t item = unit / waves;
   if (item >= items) return;
   Segment g;
-  if (!find_segment(a, item, g)) return;
+  if (!find_segment(a, item, g) || g.n > kFewTokens) return;
   const int width = 1 << a.width_log2, j = lane & (width - 1);
   const int part = (int)(unit - item * waves) * (64 >> a.width_log2) + (lane >> a.width_log2);
   const bool live = part < 2 * a.heads;
@@ -328,25 +335,39 @@ __global__ void __launch_bounds__(256) kv_append_token_kernel(AppendArgs a, int6
   }
 }
 
+// A batch of single tokens, as a rule; a sequence with more has its pages in the workgroups behind the first `few`.
+template <int DT, bool NORM, bool INTER, bool VEC, int W, int NI>
+__global__ void __launch_bounds__(256) kv_append_token_kernel(AppendArgs a, int64_t items, int waves, int64_t few) {
+  const int64_t block = linear_block();
+  if (block < few) append_tokens<DT, NORM, INTER, VEC>(a, items, waves, block);
+  else append_page<DT, NORM, INTER, VEC, W, NI>(a, items, block - few, kFewTokens + 1);
+}
+
+template <int DT, bool NORM, bool INTER, bool VEC, int W, int NI>
+void launch_kernel(const AppendArgs& a, int64_t items, hipStream_t st) {
+  const int64_t blocks = (items * a.heads * W + 3) / 4;
+  // 64 sequences, 8 heads of 128, pages of 64: one token each 5.5 us in the first kernel, 8.0 in the second; two each 8.2 and
+  // 7.7; 64 tokens of one sequence 7.7 (151 where lane groups take them row by row)
+  if (a.tokens <= a.seqs) {
+    const int parts = 64 >> a.width_log2, waves = (2 * a.heads + parts - 1) / parts;
+    const int64_t few = (items * waves + 3) / 4;
+    kv_append_token_kernel<DT, NORM, INTER, VEC, W, NI><<<linear_grid(few + blocks), 256, 0, st>>>(a, items, waves, few);
+  } else {
+    kv_append_kernel<DT, NORM, INTER, VEC, W, NI><<<linear_grid(blocks), 256, 0, st>>>(a, items);
+  }
+}
+
 template <int DT, bool NORM, bool INTER, bool VEC>
 int launch(const AppendArgs& a, hipStream_t st) {
   const int64_t items = (a.tokens >> a.page_log2) + 2 * (int64_t)a.seqs;
-  if (a.tokens <= 2 * (int64_t)a.seqs) {
-    const int parts = 64 >> a.width_log2, waves = (2 * a.heads + parts - 1) / parts;
-    kv_append_token_kernel<DT, NORM, INTER, VEC><<<linear_grid((items * waves + 3) / 4), 256, 0, st>>>(a, items, waves);
-    PDM_CHECK_LAUNCH();
-    return PDM_OK;
-  }
-  const int64_t units = items * a.heads;
   // rows of a page per wave-wide step; more than 4 of them take the four waves of a block
   const int steps = (1 << a.page_log2) * (1 << a.width_log2) / 64;
-  const dim3 g1 = linear_grid((units + 3) / 4), g4 = linear_grid(units);
-  if (steps <= 1) kv_append_kernel<DT, NORM, INTER, VEC, 1, 1><<<g1, 256, 0, st>>>(a, items);
-  else if (steps == 2) kv_append_kernel<DT, NORM, INTER, VEC, 1, 2><<<g1, 256, 0, st>>>(a, items);
-  else if (steps == 4) kv_append_kernel<DT, NORM, INTER, VEC, 4, 1><<<g4, 256, 0, st>>>(a, items);
-  else if (steps == 8) kv_append_kernel<DT, NORM, INTER, VEC, 4, 2><<<g4, 256, 0, st>>>(a, items);
-  else if (steps == 16) kv_append_kernel<DT, NORM, INTER, VEC, 4, 4><<<g4, 256, 0, st>>>(a, items);
-  else kv_append_kernel<DT, NORM, INTER, VEC, 4, 8><<<g4, 256, 0, st>>>(a, items);
+  if (steps <= 1) launch_kernel<DT, NORM, INTER, VEC, 1, 1>(a, items, st);
+  else if (steps == 2) launch_kernel<DT, NORM, INTER, VEC, 1, 2>(a, items, st);
+  else if (steps == 4) launch_kernel<DT, NORM, INTER, VEC, 4, 1>(a, items, st);
+  else if (steps == 8) launch_kernel<DT, NORM, INTER, VEC, 4, 2>(a, items, st);
+  else if (steps == 16) launch_kernel<DT, NORM, INTER, VEC, 4, 4>(a, items, st);
+  else launch_kernel<DT, NORM, INTER, VEC, 4, 8>(a, items, st);
   PDM_CHECK_LAUNCH();
   return PDM_OK;
 }

@@ -250,6 +250,32 @@ def test_bad_positions_and_rows_behind_the_last_sequence(pdm, dev):
     pool.check()
 
 
+@pytest.mark.parametrize("D,page", [(64, 128), (128, 16), (256, 64)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_one_busy_sequence_among_idle_ones(pdm, dev, D, page, dtype):
+    """No more new tokens than sequences, but most of them one sequence's: several rows for each lane group."""
+    hk, R = 3, D // 2
+    g = torch.Generator().manual_seed(D)
+    ang = torch.rand(400, R // 2, generator=g, dtype=torch.float64) * 50
+    cos, sin = ang.cos().float(), ang.sin().float()
+    w = 1 + 0.3 * torch.randn(D, generator=g)
+    lens = [0] * 160
+    final = [3] * 160
+    final[7], final[100] = 300, 40
+    pages = sum(-(-n // page) for n in final) + 2
+    table = _deal(final, page, pages, 2)
+    pool = Pool(pdm, dev, pages, page, hk, D)
+    for step, some in enumerate(({7: 150, 100: 5}, {7: 1, 100: 2, 8: 1, 159: 3}, {7: 149, 100: 6}, {100: 27, 0: 3})):
+        more = [some.get(i, 0) for i in range(160)]
+        start, lens = lens, [a + b for a, b in zip(lens, more)]
+        k, v = _rows(sum(more), hk, D, dtype, step)
+        pos = torch.cat([torch.arange(s, s + m) for s, m in zip(start, more)])
+        pool.append(k, v, _cu(more), table, lens, ref.norm_rope(k, w, pos, cos, sin, 1e-6, False), v.double(),
+                    cos=cos.to(dev), sin=sin.to(dev), k_weight=w.to(dev))
+        pool.check()
+    pool.cache.check()
+
+
 def test_many_sequences(pdm, dev):
     """More sequences than two rounds of the search over 64 entries hold, empty ones among them."""
     D, page, hk = 64, 16, 1
