@@ -617,7 +617,8 @@ typedef struct {
  * page_table[b * table_stride + i / page_size].  Everything is read on the
  * device: nothing here makes the host wait.  What does not fit (spans outside
  * [0, tokens], more new tokens than seq_lens, a page outside [0, num_pages), a
- * length beyond table_width pages) is left out and sets err_flag. */
+ * length beyond table_width pages) is left out and sets err_flag.
+ * tokens < 2^31, num_seqs <= 2^24, table_width * page_size <= 2^30. */
 typedef struct {
   const int32_t* cu_seqlens; /* device [num_seqs + 1] */
   const int32_t* seq_lens;   /* device [num_seqs] */

@@ -10,6 +10,9 @@
 // page's scale is a factor of the scores in fp32, values are converted with their power-of-two scale, which bf16
 // holds exactly.  Weights are rounded to bf16 (half a step is 2^-8 of a weight, against 2^-4 of an 8-bit value);
 // the running sum takes them before that.
+//
+// The simplest kernel, a wave for each (row, head), took 289 us for one sequence of 1,000 tokens, 4,764 for 64 of 128 to 8,192
+// and 110,493 for two prompts of 4,000 tokens behind 4,000 (32 query heads, 8 key heads of 128); these take 9.4, 63 and 780.
 #include <type_traits>
 
 #include "kv_common.h"
@@ -170,7 +173,11 @@ __device__ __forceinline__ void clear_rows(const AttnArgs& a, int64_t first) {
 // ---- few rows ---------------------------------------------------------------------
 // Up to 16 MT rows against a split of the keys.  Four waves take tiles of 32 keys in turn, each with its own
 // maximum, sum and O, and join in LDS; splits join in kv_attn_join_kernel.  Bound by the bytes of the codes: a wave
-// has the next tile's loads (8 KB at D = 128) in flight while it works on one.
+// has the next tile's loads (8 KB at D = 128) in flight while it works on one; the operands come from registers, since no
+// two waves share a key.  One token for 4 sequences of 60,000 to 120,000 tokens (32 query heads, 8 key heads of 128) 137 us,
+// 5.2 TB/s, as fast as a copy; for 64 sequences of 128 to 8,192 63 us, 4.1 TB/s (57 and 5.5 for the join: what is missing is
+// the first tile of each of 512 pairs and the run-out); 16 tokens for 256 sequences of 300 to 1,500 (6 heads of 64) 40 us,
+// 3.9 TB/s; one token for one sequence of 1,000 9.4 us, two launches' latency.
 constexpr int kFewKeys = 32, kFewWaves = 4, kFewStep = kFewKeys * kFewWaves;
 constexpr int kDealt = 256;   // sequences of a call that is dealt
 
@@ -187,15 +194,19 @@ __device__ __forceinline__ int steps_of(const Seq& s) { return s.hi > s.lo ? (s.
 // Dealt: the steps of 128 keys of all (sequence, key head) pairs, in order, are dealt to `workers` workgroups in equal
 // runs, so that a batch of long and short sequences keeps every CU busy to the end.  A run ends some pairs and begins
 // one: a workgroup leaves at most two partial results, that of a pair which it did not begin (slot 2 w) and that of one which
-// it did not end (2 w + 1).  Every workgroup computes the plan itself, a sequence per thread.
+// it did not end (2 w + 1).  Every workgroup computes the plan itself, a sequence per thread.  Against equal splits, 64
+// sequences with 8 key heads of 128: of 128 to 8,192 tokens 63 us instead of 91, of 1,000 to 3,200 60 and 59.
 struct FewDeal {
   int64_t first[kDealt + 1];  // steps before a sequence, of all its heads
   int64_t sums[4];
+  int most[4], some[4];       // steps of a wave's longest pair; its sequences that have any
   int row0[kDealt], n[kDealt], len[kDealt];
   int found;
 };
 
-__device__ __forceinline__ int64_t few_deal(const AttnArgs& a, FewDeal& sh) {  // steps of a run
+// Where no pair has more than 1.25 times the average, every pair has workgroups of its own instead (`even`, equal parts of
+// it): 64 sequences of 2,000 tokens 55 us instead of 61, of 1,700 to 2,300 56 instead of 61, 40 of 1,300 to 2,700 44 and 43.
+__device__ __forceinline__ int64_t few_deal(const AttnArgs& a, FewDeal& sh, bool& even) {  // steps of a run
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   Seq s;
   int64_t steps = 0;
@@ -208,13 +219,19 @@ __device__ __forceinline__ int64_t few_deal(const AttnArgs& a, FewDeal& sh) {  /
     const int64_t v = __shfl_up(upto, o);
     upto += lane >= o ? v : 0;
   }
-  if (lane == 63) sh.sums[wave] = upto;
+  const int most = (int)group_max((float)(steps / a.hk), 64);  // at most 2^23: exact
+  const int some = __builtin_popcountll(__ballot(steps > 0));
+  if (lane == 63) sh.sums[wave] = upto, sh.most[wave] = most, sh.some[wave] = some;
   __syncthreads();
   for (int w = 0; w < wave; ++w) upto += sh.sums[w];
+  int top = 0, n = 0;
+  for (int w = 0; w < 4; ++w) top = sh.most[w] > top ? sh.most[w] : top, n += sh.some[w];
   sh.first[tid] = upto - steps;
   if (tid == kDealt - 1) sh.first[kDealt] = upto;
   __syncthreads();
-  return (sh.first[kDealt] + a.workers - 1) / a.workers;
+  const int64_t all = sh.first[kDealt];
+  even = a.seqs * a.hk <= a.workers && (int64_t)top * n * a.hk * 4 <= all * 5;
+  return (all + a.workers - 1) / a.workers;
 }
 
 // The part of run [x, to) that belongs to the pair at x; returns the steps taken.  FIRST: the run's first pair (a barrier);
@@ -275,12 +292,32 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
   int64_t x = 0, from = 0, to = 0;
   FewUnit fu;
   if (a.workers) {
-    const int64_t per = few_deal(a, deal);
-    from = x = unit * per;
-    to = x + per < deal.first[kDealt] ? x + per : deal.first[kDealt];
+    bool even;
+    const int64_t per = few_deal(a, deal, even);
+    int pair_parts = 0, pair_b = 0, pair_kh = 0;
+    if (even) {
+      const int shares = a.workers / (a.seqs * a.hk), i = (int)(unit % shares), pair = (int)(unit / shares);
+      if (pair < a.seqs * a.hk) {
+        pair_b = pair / a.hk, pair_kh = pair - pair_b * a.hk;
+        const int steps = (int)((deal.first[pair_b + 1] - deal.first[pair_b]) / a.hk), size = (steps + shares - 1) / shares;
+        const int64_t begin = deal.first[pair_b] + (int64_t)pair_kh * steps;
+        if (i * size < steps) {
+          from = begin + i * size;
+          to = from + size < begin + steps ? from + size : begin + steps;
+          pair_parts = i == 0 && size < steps ? (steps + size - 1) / size : 0;
+        }
+      }
+    } else {
+      from = unit * per;
+      to = from + per < deal.first[kDealt] ? from + per : deal.first[kDealt];
+    }
+    x = from;
     if (threadIdx.x == 0) {
       int parts = 0;
-      if (x < to && to < deal.first[kDealt]) {  // the pair of the last step, and where it ends
+      if (even) {
+        parts = pair_parts;
+        a.joins[4 * unit] = pair_b, a.joins[4 * unit + 1] = pair_kh;
+      } else if (x < to && to < deal.first[kDealt]) {  // the pair of the last step, and where it ends
         int b = 0, n = kDealt;
         while (n > 1) {
           const int half = n >> 1;
@@ -725,6 +762,11 @@ __global__ void __launch_bounds__(256) kv_attn_dealt_join_kernel(AttnArgs a) {
 // beside the other's softmax; left to themselves, two waves of a SIMD were found in the same phase and took turns.
 // Tiles are converted once on their way into LDS, in the softmax phase, their loads a phase earlier: K as rows by the
 // first group, V transposed by the second, its keys in the order in which the first product leaves P.
+// Bound by the softmax phase: two prompts of 3,500 to 4,500 tokens behind 3,000 to 5,000 (32 query heads, 8 key heads of 128)
+// 752 to 795 us by the card, 0.97 to 1.03 PFLOP/s, where a bf16 product of 8,192^3 reaches 1.37.  The matrix units are busy
+// 45 % of the time and the vector units as long; a tile's products take 1,024 cycles of a wave at best, its softmax about 1,400
+// (512 of them exponentials) and staging 500.  Tried on it: loads in the softmax phase (854 us against 796), staging between
+// the products (857 against 834), priority for either phase (no change or 3 % slower).
 template <int D, int KT>
 struct ManyShared {
   static constexpr int KS = 2 * D + 16;    // bytes of a K row: 16 rows of a fragment read fall into different banks
@@ -1251,8 +1293,11 @@ Plan plan_of(const pdm_kv_attention_desc* d, const pdm_kv_cache* c, const pdm_kv
   const int64_t pairs = (int64_t)(b->num_seqs > 0 ? b->num_seqs : 1) * c->n_kv_heads;
   const int64_t cap = (most + kFewStep - 1) / kFewStep;  // steps of a pair
   const int resident = 256 * (c->head_dim * p.mt <= 64 ? 4 : c->head_dim * p.mt <= 128 ? 3 : 2);
+  // Dealt where there are pairs enough that an uneven batch leaves CUs idle, and rows so few that partial results stay small;
+  // with 2,048 pairs and more the hardware's own order does as well, and longer rows would write more than they save.
   p.workers = p.few && b->num_seqs > 1 && b->num_seqs <= kDealt && pairs >= 256 && pairs < 2048 && rows <= 8 && pairs * cap > resident
                   ? resident : 0;
+  // else equal splits, as many as fill the CUs once: a second round of workgroups would only add joins
   int64_t splits = p.workers || pairs >= 1024 ? 1 : resident / pairs;
   splits = splits < cap ? splits : cap;
   p.splits = (int)(splits > 1 ? splits : 1);
@@ -1261,6 +1306,8 @@ Plan plan_of(const pdm_kv_attention_desc* d, const pdm_kv_cache* c, const pdm_kv
   p.part_rows = !p.few ? 0 : p.workers ? 2 * p.workers * p.row_stride : p.splits > 1 ? p.units * p.row_stride : 0;
   if (p.many) {
     const int64_t all = b->tokens * group;
+    // 256 rows a workgroup where they fill most of its blocks (256 rows a sequence on average) and there is one for each CU;
+    // fewer rows would leave CUs idle.  Heads of 256 need the registers of two such waves for one.
     p.groups = c->head_dim < 256 && all >= 256 * (int64_t)b->num_seqs && all * c->n_kv_heads >= 256 * 256 ? 2 : 1;
     const int M = 128 * p.groups;
     p.items = all / M + b->num_seqs;

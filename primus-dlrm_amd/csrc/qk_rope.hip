@@ -5,7 +5,10 @@
 //   y_a = n_a cos - n_b sin,  y_b = n_b cos + n_a sin                      (elements behind R: y = n)
 // Backward, from dy: g = dy turned back, h = g w,
 //   dx = r (h - x r mean(h x r)),   dw = sum over tokens and heads of g x r
-// in fp32, rounded once.  Both are bound by HBM: 2 and 3 times the tensors' bytes.
+// in fp32, rounded once.  Both are bound by HBM: 2 and 3 times the tensors' bytes.  Lane groups of D / 16 lanes take rows, a
+// row's 16 elements a lane in registers from its one load to its one store: 8,192 tokens of 32 + 8 heads of 128 in bf16 36 us
+// (4.7 TB/s; a copy reaches 5.2), 16 tokens 3.2 us.  With the backward pass, 24,259 tokens of 6 + 6 heads of 64 18.6 + 32.9 +
+// 3.9 us (4.0 and 3.4 TB/s, sums of dw), 16,384 tokens of 24 + 6 heads of 128 in fp16 52.3 + 81.2 + 4.0 us (4.8 and 4.6 TB/s).
 #include "kv_common.h"
 
 namespace pdm {
@@ -91,7 +94,8 @@ __global__ void __launch_bounds__(256) rope_fwd_kernel(RopeArgs q, RopeArgs k, u
   }
 }
 
-// A block walks rows block, block + blocks, ... of its part and leaves one partial sum of dw.
+// A block walks rows block, block + blocks, ... of its part and leaves one partial sum of dw: no atomics, so that the same
+// inputs give the same bits.
 template <int DT, bool NORM, bool INTER, bool VEC>
 __global__ void __launch_bounds__(256) rope_bwd_kernel(RopeArgs q, RopeArgs k, uint32_t q_blocks, RopeShared s) {
   __shared__ float red[256 * 16];

@@ -350,6 +350,23 @@ def test_many_uneven_contexts(pdm, dev, D, page, n, hk, group, most, longest, ca
     c.check(c.run(max_q_len=8 // group, **kw), want)
 
 
+@pytest.mark.parametrize("D,page,n,hk,group,most", [
+    (64, 16, 32, 8, 4, 2), (128, 32, 33, 8, 1, 8), (128, 64, 90, 8, 2, 4), (256, 128, 64, 8, 3, 1), (64, 128, 255, 2, 8, 1)])
+@pytest.mark.parametrize("lo,hi", [(700, 840), (150, 250), (130, 1000)])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 140)])
+def test_many_even_contexts(pdm, dev, D, page, n, hk, group, most, lo, hi, causal, window):
+    """About equal contexts (the last range is not): parts of their own for each (sequence, head), one to four of them, some
+    of which come out empty; sequences without new tokens among them."""
+    g = torch.Generator().manual_seed(n)
+    new = torch.randint(0, most + 1, (n,), generator=g).tolist()
+    lens = torch.randint(lo, hi, (n,), generator=g).tolist()
+    c = Case(pdm, dev, new, lens, hk * group, hk, D, page, torch.float16 if n == 64 else torch.bfloat16, seed=n, extra=9)
+    kw = dict(causal=causal, window=window)
+    got = c.run(max_q_len=most, **kw)
+    c.check(got, c.want(**kw))
+    assert all(torch.equal(a, b) for a, b in zip(got, c.run(max_q_len=most, **kw)))
+
+
 def test_many_uneven_contexts_with_bad_places(pdm, dev):
     """NaN keys and values, infinite queries, pages that do not exist, sequences that do not fit, padding, in turn."""
     new, lens = _uneven(3, 40, 2, 4000)
