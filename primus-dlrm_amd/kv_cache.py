@@ -183,7 +183,10 @@ class QKNormRope(nn.Module):
     """The norms (``q_norm.weight``, ``k_norm.weight``) and the rotation of a layer's queries and keys.
 
     ``forward(q, k, positions)`` is :func:`qk_norm_rope`; k may be None, where :meth:`PagedKVCache.append` norms and
-    rotates the keys on their way into the cache.  The cos / sin tables stay fp32 when the module is cast."""
+    rotates the keys on their way into the cache.  The cos / sin tables stay fp32 when the module is cast.
+
+    Before a backward pass is captured into a HIP graph, let go of eager outputs of the same parameters: torch
+    accumulates their gradients on the stream that those were made on, which a capture does not survive."""
 
     def __init__(self, head_dim: int, max_positions: int, rotary_dim: Optional[int] = None, theta: float = 10000.0,
                  eps: float = 1e-6, interleaved: bool = False, norm: bool = True, device=None):
