@@ -38,14 +38,11 @@ struct Segment {
   int slot0, n;          // first slot and number of tokens
 };
 
-// Item i of the list of (sequence, touched page): sequence b's span begins at cu[b] / page + 2 b and is never
-// shorter than the pages it touches, (n_b - 2) / page + 2 at most, so the list needs no prefix sum.
-__device__ __forceinline__ bool find_segment(const AppendArgs& a, int64_t item, Segment& g) {
+// The j-th page that sequence b's new tokens touch.
+__device__ __forceinline__ bool segment_of(const AppendArgs& a, int b, int64_t c0, int64_t j, Segment& g) {
   const int lg = a.page_log2;
-  const int b = find_sequence(a.seqs, item, [&](int i) { return ((int64_t)a.cu[i] >> lg) + 2 * (int64_t)i; });
-  const int64_t c0 = a.cu[b], c1 = a.cu[b + 1], len = a.lens[b];
+  const int64_t c1 = a.cu[b + 1], len = a.lens[b];
   const int64_t n = c1 - c0;
-  const int64_t j = item - ((c0 >> lg) + 2 * (int64_t)b);
   if (j < 0 || n <= 0) {
     if (n < 0 && a.err) *a.err = 1;
     return false;
@@ -69,6 +66,15 @@ __device__ __forceinline__ bool find_segment(const AppendArgs& a, int64_t item, 
   g.slot0 = (int)(lo - (page << lg));
   g.n = (int)(hi - lo);
   return true;
+}
+
+// Item i of the list of (sequence, touched page): sequence b's span begins at cu[b] / page + 2 b and is never
+// shorter than the pages it touches, (n_b - 2) / page + 2 at most, so the list needs no prefix sum.
+__device__ __forceinline__ bool find_segment(const AppendArgs& a, int64_t item, Segment& g) {
+  const int lg = a.page_log2;
+  const int b = find_sequence(a.seqs, item, [&](int i) { return ((int64_t)a.cu[i] >> lg) + 2 * (int64_t)i; });
+  const int64_t c0 = a.cu[b];
+  return segment_of(a, b, c0, item - ((c0 >> lg) + 2 * (int64_t)b), g);
 }
 
 // The segment's page, -1 where it does not exist.  (Looked up after the rows' loads have been issued.)
@@ -201,19 +207,12 @@ __device__ __forceinline__ void store_codes(uint8_t* row, const RowPlace& pl, fl
   *reinterpret_cast<u32x2_t*>(row + pl.hi) = u32x2_t{e4m3x4(v + 8), e4m3x4(v + 12)};
 }
 
-// Pages with several new tokens (`least` or more): a page and head, its keys and then its values, per W waves; a lane group takes
-// NI rows.  The loads of both are in flight together, and the values stay in registers between the maximum and the codes.
+// Pages with several new tokens: a page and head, its keys and then its values, per W waves; a lane group takes NI rows.  The
+// loads of both are in flight together, and the values stay in registers between the maximum and the codes.
 template <int DT, bool NORM, bool INTER, bool VEC, int W, int NI>
-__device__ __forceinline__ void append_page(const AppendArgs& a, int64_t items, int64_t block, int least) {
+__device__ __forceinline__ void append_page(const AppendArgs& a, const Segment& g, int h) {
   __shared__ float red[2][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t unit = (block * 4 + wave) / W;
-  const int64_t item = unit / a.heads;
-  if (item >= items) return;  // W == 4: the same for the whole block
-  const int h = (int)(unit - item * a.heads);
-  Segment g;
-  if (!find_segment(a, item, g) || g.n < least) return;
-
   const int width = 1 << a.width_log2;
   const int j = lane & (width - 1);
   const int per_wave = 64 >> a.width_log2;
@@ -280,7 +279,11 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int64_t items, 
 
 template <int DT, bool NORM, bool INTER, bool VEC, int W, int NI>
 __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a, int64_t items) {
-  append_page<DT, NORM, INTER, VEC, W, NI>(a, items, linear_block(), 1);
+  const int64_t unit = (linear_block() * 4 + (threadIdx.x >> 6)) / W;
+  const int64_t item = unit / a.heads;
+  if (item >= items) return;  // W == 4: the same for the whole block
+  Segment g;
+  if (find_segment(a, item, g)) append_page<DT, NORM, INTER, VEC, W, NI>(a, g, (int)(unit - item * a.heads));
 }
 
 // Pages with a token or two: a lane group per (page, head, keys or values), its rows one after the other, read again for the
@@ -338,25 +341,56 @@ __device__ __forceinline__ void append_tokens(const AppendArgs& a, int64_t items
   }
 }
 
+// The pages with more tokens of 256 sequences, by kParts workgroups: they look at the sequences, not at each page and head, so
+// that a batch without any pays little (single tokens of 4,096 sequences 26 us; 95 with a workgroup for every page and head).
+constexpr int kParts = 64;
+
+template <int DT, bool NORM, bool INTER, bool VEC, int W, int NI>
+__device__ __forceinline__ void append_busy(const AppendArgs& a, int64_t block) {
+  __shared__ uint64_t busy[4];
+  const int64_t first = block / kParts * 256;
+  const int part = (int)(block % kParts);
+  const int64_t mine = first + threadIdx.x;
+  const bool more = mine < a.seqs && (int64_t)a.cu[mine + 1] - a.cu[mine] > kFewTokens;
+  const uint64_t found = __ballot(more);
+  if ((threadIdx.x & 63) == 0) busy[threadIdx.x >> 6] = found;
+  if (!__syncthreads_or(more)) return;
+  uint64_t left = 0;
+  for (int w = -1;;) {
+    while (left == 0 && ++w < 4) left = busy[w];
+    if (left == 0) return;
+    const int b = (int)first + 64 * w + __builtin_ctzll(left);
+    left &= left - 1;
+    const int64_t c0 = a.cu[b], c1 = a.cu[b + 1], n = c1 - c0;
+    if (c0 < 0 || c1 > a.tokens || n > a.lens[b]) continue;  // (the other workgroups set the flag)
+    const int64_t units = ((n - 2 >> a.page_log2) + 2) * a.heads;  // pages that n tokens may touch
+    // (W == 4: the same for the whole block, and what a turn leaves in LDS is read before the next one's first barrier)
+    for (int64_t u = part * (4 / W) + (W == 4 ? 0 : threadIdx.x >> 6); u < units; u += kParts * (4 / W)) {
+      const int64_t j = u / a.heads;
+      Segment g;
+      if (segment_of(a, b, c0, j, g) && g.n > kFewTokens) append_page<DT, NORM, INTER, VEC, W, NI>(a, g, (int)(u - j * a.heads));
+    }
+  }
+}
+
 // A batch of single tokens, as a rule; a sequence with more has its pages in the workgroups behind the first `few`.
 template <int DT, bool NORM, bool INTER, bool VEC, int W, int NI>
-__global__ void __launch_bounds__(256) kv_append_token_kernel(AppendArgs a, int64_t items, int waves, int64_t few) {
+__global__ void __launch_bounds__(256) kv_append_token_kernel(AppendArgs a, int64_t items, int waves, int64_t few, int64_t all) {
   const int64_t block = linear_block();
   if (block < few) append_tokens<DT, NORM, INTER, VEC>(a, items, waves, block);
-  else append_page<DT, NORM, INTER, VEC, W, NI>(a, items, block - few, kFewTokens + 1);
+  else if (block < all) append_busy<DT, NORM, INTER, VEC, W, NI>(a, block - few);
 }
 
 template <int DT, bool NORM, bool INTER, bool VEC, int W, int NI>
 void launch_kernel(const AppendArgs& a, int64_t items, hipStream_t st) {
-  const int64_t blocks = (items * a.heads * W + 3) / 4;
   // 64 sequences, 8 heads of 128, pages of 64: one token each 5.5 us in the first kernel, 8.0 in the second; two each 8.2 and
-  // 7.7; 64 tokens of one sequence 7.7 (151 where lane groups take them row by row)
+  // 7.7; 64 tokens of one sequence 8.6 (151 where lane groups take them row by row); single tokens of 4,096 sequences 26
   if (a.tokens <= a.seqs) {
     const int parts = 64 >> a.width_log2, waves = (2 * a.heads + parts - 1) / parts;
-    const int64_t few = (items * waves + 3) / 4;
-    kv_append_token_kernel<DT, NORM, INTER, VEC, W, NI><<<linear_grid(few + blocks), 256, 0, st>>>(a, items, waves, few);
+    const int64_t few = (items * waves + 3) / 4, all = few + ((int64_t)a.seqs + 255) / 256 * kParts;
+    kv_append_token_kernel<DT, NORM, INTER, VEC, W, NI><<<linear_grid(all), 256, 0, st>>>(a, items, waves, few, all);
   } else {
-    kv_append_kernel<DT, NORM, INTER, VEC, W, NI><<<linear_grid(blocks), 256, 0, st>>>(a, items);
+    kv_append_kernel<DT, NORM, INTER, VEC, W, NI><<<linear_grid((items * a.heads * W + 3) / 4), 256, 0, st>>>(a, items);
   }
 }
 

@@ -276,6 +276,44 @@ def test_one_busy_sequence_among_idle_ones(pdm, dev, D, page, dtype):
     pool.cache.check()
 
 
+@pytest.mark.parametrize("page,D", [(16, 64), (64, 128)])
+def test_busy_sequences_among_many(pdm, dev, page, D):
+    """The same over more than 256 sequences, several of them busy, single tokens beside them; a busy one that holds fewer
+    tokens than it brings, and one with a page that does not exist, are left out."""
+    hk, B = 2, 700
+    some = {0: 40, 7: 1, 255: 130, 256: 3, 300: 90, 301: 2, 302: 33, 650: 1, 699: 70}
+    more = [some.get(i, 0) for i in range(B)]
+    past = [i % 23 for i in range(B)]
+    lens = [n + p for n, p in zip(more, past)]
+    pages = sum(-(-n // page) for n in lens) + 2
+    table = _deal(lens, page, pages, 3)
+    pool = Pool(pdm, dev, pages, page, hk, D)
+    k, v = _rows(B, hk, D, torch.bfloat16, 1)  # rows behind the last sequence too
+    pool.append(k, v, _cu(more), table, lens, k.double(), v.double())
+    pool.check()
+    assert pool.cache.err_flag.item() == 0
+    pool = Pool(pdm, dev, pages, page, hk, D)
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    short = list(lens)
+    short[255] = 129
+    holed = [list(r) for r in table]
+    holed[300][(past[300] + 60) // page] = pages
+    c = pool.cache
+    pdm.kv_append(k.to(dev), v.to(dev), c.k_codes, c.v_codes, c.k_scale, c.v_scale, t(_cu(more)), t(holed), t(short),
+                  err_flag=c.err_flag)
+    assert c.err_flag.item() == 1
+    # the reference, on the host, for what is left: whole sequences but 255, and 300 without its lost page
+    cu = _cu(more)
+    for x, codes, scale in ((k.double(), pool.codes[0], pool.scale[0]), (v.double(), pool.codes[1], pool.scale[1])):
+        lost = table[300][(past[300] + 60) // page]
+        keep = codes[lost].clone(), scale[lost].clone()
+        for b in some:
+            if b != 255:
+                ref.append(x[cu[b]:cu[b + 1]], codes, scale, [0, more[b]], [table[b]], [lens[b]])
+        codes[lost], scale[lost] = keep
+    pool.check()
+
+
 def test_many_sequences(pdm, dev):
     """More sequences than two rounds of the search over 64 entries hold, empty ones among them."""
     D, page, hk = 64, 16, 1
