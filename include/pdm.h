@@ -679,6 +679,7 @@ typedef struct {
  * codes are exact in both; weights are rounded to bf16).  A row that sees no
  * key, a row left out and a row behind the last sequence is zeros, lse -inf.
  * Keys that a row does not see do not reach it, whatever they hold.
+ * Pages that no row of a sequence sees are not looked at, nor flagged.
  * out: device, contiguous [tokens, n_q_heads, D] of dtype, 16-byte aligned;
  * lse: optional device fp32 [tokens, n_q_heads].  workspace: 256-byte aligned,
  * the size below (it depends on sizes alone), no initialisation needed; calls

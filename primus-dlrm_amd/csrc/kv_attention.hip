@@ -1217,7 +1217,7 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
         store4<DT>(a.out, at * D + 32 * d + 2 * e + 4 * h, o[d][e] * f, o[d][e + 1] * f, o[d][e + 2] * f, o[d][e + 3] * f);
     if (h == 0 && a.lse) a.lse[at] = sum != 0.0f ? (m + __builtin_amdgcn_logf(sum)) * kLn2 : -kInf;
   } else {
-    const int64_t pr = ((item * a.hk + kh) * a.splits + split) * M + grp * 128 + wave * 32 + c;
+    const int64_t pr = at * a.splits + split;
 #pragma unroll
     for (int d = 0; d < DD; ++d)
 #pragma unroll
@@ -1230,27 +1230,23 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
   }
 }
 
-// Joins the splits of the many-rows kernel: one wave per row.
+// Joins the splits of the many-rows kernel: one wave per row of the batch.
 template <int DT, int D, int KT>
-__global__ void __launch_bounds__(256) kv_attn_many_join_kernel(AttnArgs a, int64_t items) {
+__global__ void __launch_bounds__(256) kv_attn_many_join_kernel(AttnArgs a, int64_t units) {
   constexpr int M = 128;
-  const int64_t x = linear_block() * 4 + (threadIdx.x >> 6);
-  const int in = (int)(x % M);
-  const int64_t ih = x / M;
-  const int kh = (int)(ih % a.hk);
-  const int64_t item = ih / a.hk;
-  if (item >= items) return;
+  const int64_t at = linear_block() * 4 + (threadIdx.x >> 6);
+  if (at >= units) return;
+  const int64_t t = at / a.hq;
+  const int head = (int)(at - t * a.hq);
+  const int b = find_sequence(a.seqs, t, [&](int i) { return (int64_t)a.cu[i]; });
   Seq sq;
-  int b, r0, lo, hi;
-  if (!many_block<M>(a, item, sq, b, r0)) return;
-  const int r = r0 + in;
-  if (r >= sq.n * a.group) return;
-  many_keys<M>(a, sq, r0, lo, hi);
+  if (!seq_of(a, b, sq) || t < sq.row0 || t >= sq.row0 + sq.n || (int64_t)sq.n * a.group <= a.few_rows) return;
+  const int r = (int)(t - sq.row0) * a.group + head % a.group;
+  int lo, hi;
+  many_keys<M>(a, sq, r / M * M, lo, hi);
   const int size = split_size(hi - lo, a.splits, KT);
   const int used = hi > lo ? (hi - lo + size - 1) / size : 1;
-  if (used == 1) return;
-  const int i = r / a.group, h = kh * a.group + (r - i * a.group);
-  join_row<DT, D, 1>(a, used, (sq.row0 + i) * a.hq + h, [&](int x) { return (ih * a.splits + x) * M + in; });
+  if (used > 1) join_row<DT, D, 1>(a, used, at, [&](int x) { return at * a.splits + x; });
 }
 
 // ---- host -----------------------------------------------------------------------
@@ -1311,12 +1307,15 @@ Plan plan_of(const pdm_kv_attention_desc* d, const pdm_kv_cache* c, const pdm_kv
     p.groups = c->head_dim < 256 && all >= 256 * (int64_t)b->num_seqs && all * c->n_kv_heads >= 256 * 256 ? 2 : 1;
     const int M = 128 * p.groups;
     p.items = all / M + b->num_seqs;
-    const int64_t blocks = p.items * c->n_kv_heads;
+    // Blocks that are likely to have rows, where one sequence in five has many: too few for the CUs are split.  Behind 4,096
+    // tokens, heads as above: 40 tokens of one of 64 sequences, single ones of the others 202 us unsplit, 146 split; 16 tokens of
+    // 32 153 and 102.  (One in eight instead of five would split 10 tokens of 64 sequences, 38 -> 56 us behind 700 tokens.)
+    const int64_t blocks = (all / M + 1 + b->num_seqs / 5) * c->n_kv_heads;
     int64_t sp = blocks < 256 && p.groups == 1 ? 512 / blocks : 1;
     const int64_t most_sp = (most + 511) / 512;
     sp = sp < most_sp ? sp : most_sp;
     p.many_splits = (int)(sp > 1 ? sp : 1);
-    p.many_part_rows = p.many_splits > 1 ? blocks * p.many_splits * M : 0;
+    p.many_part_rows = p.many_splits > 1 ? b->tokens * d->n_q_heads * p.many_splits : 0;
   }
   return p;
 }
@@ -1331,7 +1330,10 @@ template <int DT, int D, int KT, int NG>
 void launch_many(const AttnArgs& a, const Plan& p, hipStream_t st) {
   kv_attn_many_kernel<DT, D, KT, NG><<<linear_grid(p.items * a.hk * a.splits, (int64_t(1) << 23) / NG), 256 * NG, 0, st>>>(a, p.items);
   if constexpr (NG == 1)
-    if (p.many_part_rows) kv_attn_many_join_kernel<DT, D, KT><<<linear_grid(p.items * a.hk * 32), 256, 0, st>>>(a, p.items);
+    if (p.many_part_rows) {
+      const int64_t rows = a.tokens * a.hq;
+      kv_attn_many_join_kernel<DT, D, KT><<<linear_grid((rows + 3) / 4), 256, 0, st>>>(a, rows);
+    }
 }
 
 template <int DT, int D>

@@ -327,6 +327,31 @@ def test_large_batches_with_bad_places(pdm, dev, D):
     c.check((out[keep], lse[keep]), [w[keep] for w in want])
 
 
+@pytest.mark.parametrize("dtype,D,page", [(torch.bfloat16, 128, 32), (torch.float16, 64, 16), (torch.bfloat16, 256, 64)])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 700)])
+def test_prompts_among_single_tokens(pdm, dev, dtype, D, page, causal, window):
+    """Keys of the sequences with many rows are split, those of the others too; some have no new tokens, one a page that does
+    not exist in one of its splits, one a NaN value that some of its rows see; rows behind the last sequence."""
+    new = [1, 60, 0, 1, 150, 2, 1, 0, 1, 33]
+    lens = [900, 2500, 70, 5, 1800, 640, 3000, 40, 1, 33]
+    c = Case(pdm, dev, new, lens, 8, 2, D, page, dtype, seed=D, extra=3)
+    c.cache.v_codes.view(torch.uint8)[c.table[4][1700 // page], 1, 1700 % page, 9] = 0x7F
+    c.table[1][1200 // page] = -1
+    kw = dict(causal=causal, window=window)
+    want = c.want(**kw)
+    q = torch.cat((c.q, torch.full((7, 8, D), math.nan, dtype=dtype)))
+    T = len(c.q)
+    first = None
+    for _ in range(2):
+        out, lse = c.run(q=q, max_q_len=150, **kw)
+        # (pages that no row's window reaches are not looked at: the lost one ends 1,200 tokens before the first row)
+        assert c.cache.err_flag.item() == (window == 0) and (out[T:] == 0).all() and (lse[T:] == -math.inf).all()
+        c.cache.err_flag.zero_()
+        c.check((out[:T], lse[:T]), want)
+        assert first is None or torch.equal(out.view(torch.int16), first.view(torch.int16))
+        first = out
+
+
 def _uneven(seed, n, most, longest):
     g = torch.Generator().manual_seed(seed)
     new = torch.randint(0, most + 1, (n,), generator=g).tolist()
