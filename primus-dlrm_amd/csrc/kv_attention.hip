@@ -1283,10 +1283,12 @@ Plan plan_of(const pdm_kv_attention_desc* d, const pdm_kv_cache* c, const pdm_kv
   const int64_t max_q = d->max_q_len < b->tokens ? d->max_q_len : b->tokens;
   const int64_t rows = max_q * group;
   p.mt = c->head_dim == 256 || (group <= 16 && (rows <= 16 || rows > 32)) ? 1 : 2;
+  p.splits = 1;
+  if (b->num_seqs == 0) return p;  // padding alone: the few-rows kernel's blocks behind its units clear it
   p.few = group <= 16 * p.mt;
   p.many = rows > 16 * p.mt;
   const int64_t most = (int64_t)b->table_width * c->page_size;
-  const int64_t pairs = (int64_t)(b->num_seqs > 0 ? b->num_seqs : 1) * c->n_kv_heads;
+  const int64_t pairs = (int64_t)b->num_seqs * c->n_kv_heads;
   const int64_t cap = (most + kFewStep - 1) / kFewStep;  // steps of a pair
   const int resident = 256 * (c->head_dim * p.mt <= 64 ? 4 : c->head_dim * p.mt <= 128 ? 3 : 2);
   // Dealt where there are pairs enough that an uneven batch leaves CUs idle, and rows so few that partial results stay small;
@@ -1338,7 +1340,7 @@ void launch_many(const AttnArgs& a, const Plan& p, hipStream_t st) {
 
 template <int DT, int D>
 void launch(AttnArgs& a, const Plan& p, hipStream_t st) {
-  const int64_t units = p.few && a.seqs ? p.units : 0, guards = (a.tokens + 255) / 256;
+  const int64_t units = p.few ? p.units : 0, guards = (a.tokens + 255) / 256;
   const dim3 grid = linear_grid(units + guards);
   if (p.mt == 1) kv_attn_few_kernel<DT, D, 1><<<grid, 256, 0, st>>>(a, units, guards);
   else if constexpr (D < 256) kv_attn_few_kernel<DT, D, 2><<<grid, 256, 0, st>>>(a, units, guards);  // more rows of 256 spill

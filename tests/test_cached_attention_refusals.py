@@ -176,3 +176,36 @@ def test_reference_quantizer_matches_the_cast():
     x = torch.cat((x, -x))
     assert torch.equal(ref.round_e4m3(x), x.float().to(torch.float8_e4m3fn).double())
     assert [ref.scale_exponent(v) for v in (448.0, 448.0000001, 224.0, 1.75, 1.76, 0.0)] == [0, 1, -1, -8, -7, -117]
+
+
+NO_SEQUENCES = """
+import ctypes, sys
+sys.path.insert(0, {root!r})
+import __graft_entry__
+L = __graft_entry__.pdm_import()._lib
+lib, by = L.lib(), ctypes.byref
+cache = L.KvCacheDesc(16, 16, 16, 16, 4, 2, 64, 64, 0)
+for group, tokens, width, most in {cases!r}:
+    batch = L.KvBatchDesc(16, 16, 16, width, tokens, 0, width)
+    att = L.KvAttentionDesc(L.PDM_BF16, 2 * group, 1, 0, 0.1, min(most, tokens), 2 * group * 64, 64)
+    size = lib.pdm_kv_attention_workspace_size(by(att), by(cache), by(batch))
+    lib.pdm_kv_attention_fwd(by(att), by(cache), by(batch), 256, 256, None, 256, 1 << 40, None, None)
+    print(size, flush=True)
+"""
+
+
+def test_attention_without_sequences(pdm):
+    """A batch of padding alone is laid out without keys: no split, no join, no workspace, whatever the width of its table and
+    the number of its rows.  The process has no GPU: it may not launch anything, and has to come back."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    cases = [(2, 5, 1, 5), (2, 5, 10, 5), (2, 40, 1, 40), (2, 40, 10, 40), (2, 300, 1, 300), (2, 300, 64, 1), (24, 3, 10, 3),
+             (40, 300, 10, 300)]
+    env = {**os.environ, "HIP_VISIBLE_DEVICES": "-1", "ROCR_VISIBLE_DEVICES": "-1", "CUDA_VISIBLE_DEVICES": "-1"}
+    r = subprocess.run([sys.executable, "-c", NO_SEQUENCES.format(root=root, cases=cases)], env=env, capture_output=True,
+                       text=True)
+    assert r.returncode == 0, (r.returncode, r.stdout, r.stderr[-500:])
+    assert r.stdout.split() == ["0"] * len(cases)

@@ -562,3 +562,17 @@ def test_a_layer_as_it_is_served(pdm, dev):
         c = Case.__new__(Case)
         c.q, c.cache = qr.cpu(), cache
         c.check((out, lse), want)
+
+
+@pytest.mark.parametrize("T", [5, 40, 300])
+@pytest.mark.parametrize("width", [0, 1, 64])
+@pytest.mark.parametrize("D,hq,hk", [(64, 4, 2), (128, 40, 1), (256, 8, 8)])
+def test_no_sequences(pdm, dev, T, width, D, hq, hk):
+    """A batch of padding rows alone, few and many of them, with tables of any width: zeros."""
+    cache = pdm.PagedKVCache(3, 16, hk, D, dev)
+    q = torch.full((T, hq, D), math.nan, dtype=torch.bfloat16, device=dev)
+    for most in (None, 1):
+        out, lse = cache.attend(q, _t([0], dev), torch.zeros(0, width, dtype=torch.int32, device=dev), _t([], dev),
+                                max_q_len=most, return_lse=True)
+        assert (out == 0).all() and (lse == -math.inf).all()
+    cache.check()
