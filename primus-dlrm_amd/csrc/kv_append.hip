@@ -135,12 +135,12 @@ __device__ __forceinline__ void key_row(const AppendArgs& a, const Segment& g, i
     load8f(a.w + pl.hi, w + 8);
   }
   bool zero = false;
-  if (pl.turned) {
+  if (a.R > 0) {  // (also behind the rotated part: outside the tables the whole key is zero)
     const int64_t p = a.positions ? load_position(a.positions, a.bits, g.row0 + r) : g.index0 + r;
     zero = p < 0 || p >= a.table_rows;
     if (zero) {
       if (a.err) *a.err = 1;
-    } else {
+    } else if (pl.turned) {
       load8f(a.cos + p * (a.R / 2) + 8 * j, c);
       load8f(a.sin + p * (a.R / 2) + 8 * j, s);
     }

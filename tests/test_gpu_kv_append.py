@@ -386,3 +386,40 @@ def test_pages_beyond_32_bit_offsets(pdm, dev):
         ref.append(x.double(), want, ws, [0, 140], [[1, 0]], [140])
         assert torch.equal(codes[-2:].cpu().double(), want) and torch.equal(scale[-2:].cpu().double(), ws)
         assert not codes[:4].view(torch.uint8).any()
+
+
+@pytest.mark.parametrize("D,R,inter", [(64, 16, False), (128, 64, True), (256, 128, False), (128, 128, False)])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("bits", [None, torch.int32, torch.int64])
+def test_positions_outside_the_tables_of_partly_rotated_keys(pdm, dev, D, R, inter, norm, bits):
+    """A key whose position the tables do not hold is zero in all of its elements, the ones behind the rotated part too, and
+    counts as zero for its page's scale; by prompts and by single tokens, positions given or not."""
+    hk, page, rows = 2, 16, 24
+    g = torch.Generator().manual_seed(D + R)
+    ang = torch.rand(rows, R // 2, generator=g, dtype=torch.float64) * 50
+    cos, sin = ang.cos().float(), ang.sin().float()
+    w = 1 + 0.3 * torch.randn(D, generator=g)
+    kw = dict(cos=cos.to(dev), sin=sin.to(dev), interleaved=inter)
+    if norm:
+        kw["k_weight"] = w.to(dev)
+    final = [45, 20, 27, 1]
+    table = _deal(final, page, 12, 2)
+    pool = Pool(pdm, dev, 12, page, hk, D)
+    lens = [0] * 4
+    for step, more in enumerate(([40, 19, 25, 0], [1, 0, 1, 1], [1, 1, 1, 0], [3, 0, 0, 0])):
+        start, lens = lens, [a + b for a, b in zip(lens, more)]
+        k, v = _rows(sum(more), hk, D, torch.bfloat16, step)
+        pos = torch.cat([torch.arange(s, s + m) for s, m in zip(start, more)])
+        if bits is not None:
+            pos = torch.randint(-rows, 2 * rows, pos.shape, generator=g).to(bits)
+            if bits == torch.int64:
+                pos[0] = 2 ** 40
+            kw["positions"] = pos.to(dev)
+        # (one sequence's largest keys lie outside)
+        outside = (pos < 0) | (pos >= rows)
+        k[outside] *= 64
+        pool.cache.err_flag.zero_()
+        pool.append(k, v, _cu(more), table, lens, ref.norm_rope(k, w if norm else None, pos, cos, sin, 1e-6, inter),
+                    v.double(), **kw)
+        pool.check()
+        assert pool.cache.err_flag.item() == int(outside.any())
