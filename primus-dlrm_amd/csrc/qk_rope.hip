@@ -348,7 +348,7 @@ extern "C" int pdm_qk_norm_rope_bwd(const pdm_qk_rope_desc* d, const void* q, co
   clear_error();
   if (int e = check(__func__, d)) return e;
   const uint32_t rq = (uint32_t)(d->tokens * d->n_q_heads), rk = (uint32_t)(d->tokens * d->n_k_heads);
-  const bool norm = (rq ? q_weight : k_weight) != nullptr;
+  const bool norm = (rq ? q_weight : rk ? k_weight : q_weight ? q_weight : k_weight) != nullptr;  // (no rows: zero sums)
   PDM_CHECK_ARG((!rq || (grad_q_out && grad_q && (!norm || q))) && (!rk || (grad_k_out && grad_k && (!norm || k))),
                 "null q / k or gradients");
   PDM_CHECK_ARG(!d->tokens || positions, "null positions");

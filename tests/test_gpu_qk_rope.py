@@ -293,3 +293,20 @@ def test_rows_beyond_32_bit_offsets(pdm, dev):
     got, _ = pdm.qk_norm_rope(q, None, *args[2:5], args[5])
     want, _ = pdm.qk_norm_rope(args[0], None, *args[2:5], args[5])
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+def test_weight_gradients_without_tokens(pdm, dev, dtype, D):
+    """No tokens, with and without k: the weights' gradients are zeros, not what their memory held."""
+    w = [torch.ones(D, device=dev, requires_grad=True) for _ in range(2)]
+    cos, sin = torch.ones(4, D // 2, device=dev), torch.zeros(4, D // 2, device=dev)
+    pos = torch.zeros(0, dtype=torch.int64, device=dev)
+    x = torch.zeros(0, 2, D, dtype=dtype, device=dev, requires_grad=True)
+    for k, kw in ((None, None), (x, w[1])):
+        # the gradients' memory is of this size
+        held = [torch.full((D,), float("nan"), device=dev) for _ in range(8)]
+        del held
+        y = pdm.qk_norm_rope(x, k, pos, cos, sin, w[0], kw)
+        grads = torch.autograd.grad(sum(t.sum() for t in y if t is not None), [w[0]] if kw is None else w)
+        assert all((g == 0).all() for g in grads)
