@@ -277,9 +277,21 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, const Segment& 
   }
 }
 
+// Sets the flag for spans of 256 sequences that do not fit.  The list above need not lead to them: a first span may lie behind
+// the batch, one that runs backwards may be passed over.
+__device__ __forceinline__ void check_spans(const AppendArgs& a, int64_t first) {
+  const int64_t b = first + threadIdx.x;
+  if (!a.err || b >= a.seqs) return;
+  const int64_t c0 = a.cu[b], c1 = a.cu[b + 1];
+  if (c1 != c0 && (c0 < 0 || c1 < c0 || c1 > a.tokens || c1 - c0 > a.lens[b])) *a.err = 1;
+}
+
+// (behind the first `blocks` workgroups those that check the spans)
 template <int DT, bool NORM, bool INTER, bool VEC, int W, int NI>
-__global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a, int64_t items) {
-  const int64_t unit = (linear_block() * 4 + (threadIdx.x >> 6)) / W;
+__global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a, int64_t items, int64_t blocks) {
+  const int64_t block = linear_block();
+  if (block >= blocks) return check_spans(a, (block - blocks) * 256);
+  const int64_t unit = (block * 4 + (threadIdx.x >> 6)) / W;
   const int64_t item = unit / a.heads;
   if (item >= items) return;  // W == 4: the same for the whole block
   Segment g;
@@ -351,6 +363,7 @@ __device__ __forceinline__ void append_busy(const AppendArgs& a, int64_t block) 
   const int64_t first = block / kParts * 256;
   const int part = (int)(block % kParts);
   const int64_t mine = first + threadIdx.x;
+  if (part == 0) check_spans(a, first);
   const bool more = mine < a.seqs && (int64_t)a.cu[mine + 1] - a.cu[mine] > kFewTokens;
   const uint64_t found = __ballot(more);
   if ((threadIdx.x & 63) == 0) busy[threadIdx.x >> 6] = found;
@@ -362,7 +375,7 @@ __device__ __forceinline__ void append_busy(const AppendArgs& a, int64_t block) 
     const int b = (int)first + 64 * w + __builtin_ctzll(left);
     left &= left - 1;
     const int64_t c0 = a.cu[b], c1 = a.cu[b + 1], n = c1 - c0;
-    if (c0 < 0 || c1 > a.tokens || n > a.lens[b]) continue;  // (the other workgroups set the flag)
+    if (c0 < 0 || c1 > a.tokens || n > a.lens[b]) continue;
     const int64_t units = ((n - 2 >> a.page_log2) + 2) * a.heads;  // pages that n tokens may touch
     // (W == 4: the same for the whole block, and what a turn leaves in LDS is read before the next one's first barrier)
     for (int64_t u = part * (4 / W) + (W == 4 ? 0 : threadIdx.x >> 6); u < units; u += kParts * (4 / W)) {
@@ -390,7 +403,8 @@ void launch_kernel(const AppendArgs& a, int64_t items, hipStream_t st) {
     const int64_t few = (items * waves + 3) / 4, all = few + ((int64_t)a.seqs + 255) / 256 * kParts;
     kv_append_token_kernel<DT, NORM, INTER, VEC, W, NI><<<linear_grid(all), 256, 0, st>>>(a, items, waves, few, all);
   } else {
-    kv_append_kernel<DT, NORM, INTER, VEC, W, NI><<<linear_grid((items * a.heads * W + 3) / 4), 256, 0, st>>>(a, items);
+    const int64_t blocks = (items * a.heads * W + 3) / 4, all = blocks + ((int64_t)a.seqs + 255) / 256;
+    kv_append_kernel<DT, NORM, INTER, VEC, W, NI><<<linear_grid(all), 256, 0, st>>>(a, items, blocks);
   }
 }
 

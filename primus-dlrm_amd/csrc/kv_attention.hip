@@ -286,7 +286,11 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
   __shared__ FewDeal deal;
   const int64_t unit = linear_block();
   if (unit >= units) {
-    if (unit < units + guards) clear_rows<D>(a, (unit - units) * 256);
+    if (unit >= units + guards) return;
+    const int64_t first = (unit - units) * 256;
+    Seq s;
+    if (units == 0 && first + threadIdx.x < a.seqs) seq_of(a, (int)first + threadIdx.x, s);  // sets the flag where it does not fit
+    clear_rows<D>(a, first);
     return;
   }
   int64_t x = 0, from = 0, to = 0;
@@ -1340,7 +1344,8 @@ void launch_many(const AttnArgs& a, const Plan& p, hipStream_t st) {
 
 template <int DT, int D>
 void launch(AttnArgs& a, const Plan& p, hipStream_t st) {
-  const int64_t units = p.few ? p.units : 0, guards = (a.tokens + 255) / 256;
+  // `guards`: blocks that look for rows to clear and, where no unit looks at each sequence, at those, 256 of either
+  const int64_t units = p.few ? p.units : 0, guards = ((units || a.tokens > a.seqs ? a.tokens : (int64_t)a.seqs) + 255) / 256;
   const dim3 grid = linear_grid(units + guards);
   if (p.mt == 1) kv_attn_few_kernel<DT, D, 1><<<grid, 256, 0, st>>>(a, units, guards);
   else if constexpr (D < 256) kv_attn_few_kernel<DT, D, 2><<<grid, 256, 0, st>>>(a, units, guards);  // more rows of 256 spill

@@ -423,3 +423,26 @@ def test_positions_outside_the_tables_of_partly_rotated_keys(pdm, dev, D, R, int
                     v.double(), **kw)
         pool.check()
         assert pool.cache.err_flag.item() == int(outside.any())
+
+
+@pytest.mark.parametrize("cu,lens", [
+    ([1000, 1003], [3]), ([1000, 1003, 1003, 1003, 1003, 1003, 1003], [3] * 6), ([2 ** 31 - 4, 2 ** 31 - 1], [3]),
+    ([0, 4, 0, 4], [4, 9, 4]), ([0, 4, 0, 4, 4, 4], [4, 9, 4, 0, 0]), ([-3, 0], [3]), ([-1000, 0] + [0] * 5, [1000] * 6)])
+def test_spans_outside_the_batch_set_the_flag(pdm, dev, cu, lens):
+    """Also where no row or page of the batch leads to them: a first span behind the batch, one that runs backwards; in batches
+    of more and of no more tokens than sequences.  Nothing of them is written."""
+    D, page, hk, T = 64, 16, 2, 5
+    k, v = _rows(T, hk, D, torch.bfloat16, 9)
+    B = len(lens)
+    pool = Pool(pdm, dev, 2 * B, page, hk, D)
+    c = pool.cache
+    table = [[2 * b, 2 * b + 1] for b in range(B)]
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    c.append(k.to(dev), v.to(dev), t(cu), t(table), t(lens))
+    assert c.err_flag.item() == 1
+    for b in range(B):
+        if 0 <= cu[b] < cu[b + 1] <= T:
+            for x, codes, scale in ((k, pool.codes[0], pool.scale[0]), (v, pool.codes[1], pool.scale[1])):
+                n = cu[b + 1] - cu[b]
+                ref.append(x[cu[b]:cu[b + 1]].double(), codes, scale, [0, n], [table[b]], [lens[b]])
+    pool.check()

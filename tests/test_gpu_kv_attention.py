@@ -576,3 +576,18 @@ def test_no_sequences(pdm, dev, T, width, D, hq, hk):
                                 max_q_len=most, return_lse=True)
         assert (out == 0).all() and (lse == -math.inf).all()
     cache.check()
+
+
+@pytest.mark.parametrize("group", [2, 24, 40])
+@pytest.mark.parametrize("cu", [[1000, 1003], [2 ** 31 - 4, 2 ** 31 - 1], [1000, 1003, 1003, 1003], [-3, 0], [6, 5]])
+def test_spans_outside_the_batch_set_the_flag(pdm, dev, group, cu):
+    """Also where no row of the batch leads to them, by either kernel."""
+    cache = pdm.PagedKVCache(3, 16, 1, 64, dev)
+    B = len(cu) - 1
+    for most in (None, 3):
+        out, lse = cache.attend(torch.ones(5, group, 64, dtype=torch.bfloat16, device=dev), _t(cu, dev),
+                                torch.zeros(B, 1, dtype=torch.int32, device=dev), _t([9] * B, dev), max_q_len=most,
+                                return_lse=True)
+        assert (out == 0).all() and (lse == -math.inf).all()
+        assert cache.err_flag.item() == 1
+        cache.err_flag.zero_()
