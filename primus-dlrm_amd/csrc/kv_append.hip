@@ -354,35 +354,45 @@ __device__ __forceinline__ void append_tokens(const AppendArgs& a, int64_t items
 }
 
 // The pages with more tokens of 256 sequences, by kParts workgroups: they look at the sequences, not at each page and head, so
-// that a batch without any pays little (single tokens of 4,096 sequences 26 us; 95 with a workgroup for every page and head).
-constexpr int kParts = 64;
+// that a batch without any pays little (single tokens of 4,096 sequences 28 us; 95 with a workgroup for every page and head).
+// The pages and heads of all busy sequences are dealt to them in turn: 3 tokens of each of 85 sequences, nothing of 171, 51 us
+// (382 where each sequence's pages began with the first workgroup, 99 with 64 of them), 6 heads of 64 12 us (360, 17).
+constexpr int kParts = 128;
 
 template <int DT, bool NORM, bool INTER, bool VEC, int W, int NI>
 __device__ __forceinline__ void append_busy(const AppendArgs& a, int64_t block) {
-  __shared__ uint64_t busy[4];
+  __shared__ int before[256], sums[4];  // pages before a sequence's, and of a wave's sequences
   const int64_t first = block / kParts * 256;
-  const int part = (int)(block % kParts);
+  const int part = (int)(block % kParts), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t mine = first + threadIdx.x;
   if (part == 0) check_spans(a, first);
-  const bool more = mine < a.seqs && (int64_t)a.cu[mine + 1] - a.cu[mine] > kFewTokens;
-  const uint64_t found = __ballot(more);
-  if ((threadIdx.x & 63) == 0) busy[threadIdx.x >> 6] = found;
-  if (!__syncthreads_or(more)) return;
-  uint64_t left = 0;
-  for (int w = -1;;) {
-    while (left == 0 && ++w < 4) left = busy[w];
-    if (left == 0) return;
-    const int b = (int)first + 64 * w + __builtin_ctzll(left);
-    left &= left - 1;
-    const int64_t c0 = a.cu[b], c1 = a.cu[b + 1], n = c1 - c0;
-    if (c0 < 0 || c1 > a.tokens || n > a.lens[b]) continue;
-    const int64_t units = ((n - 2 >> a.page_log2) + 2) * a.heads;  // pages that n tokens may touch
-    // (W == 4: the same for the whole block, and what a turn leaves in LDS is read before the next one's first barrier)
-    for (int64_t u = part * (4 / W) + (W == 4 ? 0 : threadIdx.x >> 6); u < units; u += kParts * (4 / W)) {
-      const int64_t j = u / a.heads;
-      Segment g;
-      if (segment_of(a, b, c0, j, g) && g.n > kFewTokens) append_page<DT, NORM, INTER, VEC, W, NI>(a, g, (int)(u - j * a.heads));
-    }
+  int pages = 0;  // that the sequence's tokens may touch
+  if (mine < a.seqs) {
+    const int64_t c0 = a.cu[mine], c1 = a.cu[mine + 1], n = c1 - c0;
+    if (n > kFewTokens && c0 >= 0 && c1 <= a.tokens && n <= a.lens[mine]) pages = (int)(n - 2 >> a.page_log2) + 2;
+  }
+  if (!__syncthreads_or(pages)) return;
+  int upto = pages;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int v = __shfl_up(upto, o);
+    upto += lane >= o ? v : 0;
+  }
+  if (lane == 63) sums[wave] = upto;
+  __syncthreads();
+  int all = 0;
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) upto += sums[w];
+    all += sums[w];
+  }
+  before[threadIdx.x] = upto - pages;
+  __syncthreads();
+  // (W == 4: the same for the whole block, and what a turn leaves in LDS is read before the next one's first barrier)
+  for (int64_t u = part * (4 / W) + (W == 4 ? 0 : wave); u < (int64_t)all * a.heads; u += kParts * (4 / W)) {
+    const int page = (int)(u / a.heads), i = find_sequence(256, page, [&](int x) { return before[x]; });
+    const int b = (int)first + i;
+    Segment g;
+    if (segment_of(a, b, a.cu[b], page - before[i], g) && g.n > kFewTokens)
+      append_page<DT, NORM, INTER, VEC, W, NI>(a, g, (int)(u - (int64_t)page * a.heads));
   }
 }
 
@@ -396,8 +406,8 @@ __global__ void __launch_bounds__(256) kv_append_token_kernel(AppendArgs a, int6
 
 template <int DT, bool NORM, bool INTER, bool VEC, int W, int NI>
 void launch_kernel(const AppendArgs& a, int64_t items, hipStream_t st) {
-  // 64 sequences, 8 heads of 128, pages of 64: one token each 5.5 us in the first kernel, 8.0 in the second; two each 8.2 and
-  // 7.7; 64 tokens of one sequence 8.6 (151 where lane groups take them row by row); single tokens of 4,096 sequences 26
+  // 64 sequences, 8 heads of 128, pages of 64: one token each 5.7 us in the first kernel, 8.0 in the second; two each 8.2 and
+  // 7.7; 64 tokens of one sequence 8.9 (151 where lane groups take them row by row); single tokens of 4,096 sequences 28
   if (a.tokens <= a.seqs) {
     const int parts = 64 >> a.width_log2, waves = (2 * a.heads + parts - 1) / parts;
     const int64_t few = (items * waves + 3) / 4, all = few + ((int64_t)a.seqs + 255) / 256 * kParts;

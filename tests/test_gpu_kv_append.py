@@ -446,3 +446,26 @@ def test_spans_outside_the_batch_set_the_flag(pdm, dev, cu, lens):
                 n = cu[b + 1] - cu[b]
                 ref.append(x[cu[b]:cu[b + 1]].double(), codes, scale, [0, n], [table[b]], [lens[b]])
     pool.check()
+
+
+@pytest.mark.parametrize("D,page,hk", [(128, 64, 3), (64, 16, 1), (128, 16, 2), (256, 128, 1)])
+def test_a_third_of_the_sequences_busy(pdm, dev, D, page, hk):
+    """Many sequences with a few tokens each beside many with none, more of them than workgroups that share them out; pages
+    begun in earlier calls, tokens that pass on to another page, a single token and a longer run between them."""
+    B = 600
+    final = [100 if i % 3 == 0 else 5 for i in range(B)]
+    pages = sum(-(-n // page) for n in final) + 2
+    table = _deal(final, page, pages, 4)
+    pool = Pool(pdm, dev, pages, page, hk, D)
+    lens = [0] * B
+    for step in range(3):
+        more = [(3 if i < 500 else 0) if i % 3 == 0 else 0 for i in range(B)]
+        more[1], more[300] = 1, 3 + 17 * step
+        if step == 1:
+            more[0], more[597] = 0, 29
+        start, lens = lens, [a + b for a, b in zip(lens, more)]
+        assert sum(more) <= B
+        k, v = _rows(sum(more), hk, D, torch.bfloat16, step)
+        pool.append(k, v, _cu(more), table, lens, k.double(), v.double())
+        pool.check()
+    assert pool.cache.err_flag.item() == 0
