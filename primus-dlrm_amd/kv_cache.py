@@ -47,7 +47,11 @@ def _heads(t: torch.Tensor) -> torch.Tensor:
 
 
 def _traced(t: torch.Tensor) -> bool:
-    return torch.compiler.is_compiling() or isinstance(t, torch.fx.Proxy)
+    """True where a call has to be seen by the dispatcher: in compiled and traced graphs, under a dispatch mode, and for tensors
+    without memory (fake, meta) or with a dispatch of their own."""
+    return (torch.compiler.is_compiling() or isinstance(t, torch.fx.Proxy)
+            or type(t).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__ or t.is_meta
+            or torch._C._len_torch_dispatch_stack() > 0 or torch._C._get_tracing_state() is not None)
 
 
 def _fp32(w: Optional[torch.Tensor]) -> Optional[torch.Tensor]:

@@ -209,3 +209,30 @@ def test_attention_without_sequences(pdm):
                        text=True)
     assert r.returncode == 0, (r.returncode, r.stdout, r.stderr[-500:])
     assert r.stdout.split() == ["0"] * len(cases)
+
+
+@pytest.mark.parametrize("how", ["fake", "meta"])
+def test_tensors_without_memory(pdm, how):
+    """Shapes and dtypes come out where no kernel can run, as from the framework's other operators; the cache is left alone."""
+    import contextlib
+
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    where = "meta" if how == "meta" else "cpu"
+    with FakeTensorMode() if how == "fake" else contextlib.nullcontext():
+        e = lambda *s, dtype=torch.bfloat16: torch.empty(*s, dtype=dtype, device=where)  # noqa: E731
+        i = lambda *s: torch.empty(*s, dtype=torch.int32, device=where)  # noqa: E731
+        q, k = e(3, 4, 64), e(3, 2, 64)
+        f32 = lambda *s: e(*s, dtype=torch.float32)  # noqa: E731
+        yq, yk = pdm.qk_norm_rope(q, k, e(3, dtype=torch.int64), f32(8, 32), f32(8, 32), f32(64), f32(64))
+        assert yq.shape == q.shape and yk.shape == k.shape and yq.dtype == q.dtype
+        yq, none = pdm.qk_norm_rope(q.view(1, 3, 4, 64), None, e(1, 3, dtype=torch.int64), None, None)
+        assert yq.shape == (1, 3, 4, 64) and none is None
+        cache = [e(5, 2, 16, 64, dtype=torch.float8_e4m3fn) for _ in range(2)] + [f32(5, 2) for _ in range(2)]
+        batch = (i(2), i(1, 4), i(1))
+        assert pdm.kv_append(k, k, *cache, *batch, err_flag=i(1)) is None
+        out = pdm.kv_attention(q, *cache, *batch)
+        assert out.shape == q.shape and out.dtype == q.dtype
+        out, lse = pdm.kv_attention(q, *cache, *batch, return_lse=True)
+        assert lse.shape == (3, 4) and lse.dtype == torch.float32
+        assert all(t.device.type == where for t in (yq, out, lse))

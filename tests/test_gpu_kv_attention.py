@@ -591,3 +591,26 @@ def test_spans_outside_the_batch_set_the_flag(pdm, dev, group, cu):
         assert (out == 0).all() and (lse == -math.inf).all()
         assert cache.err_flag.item() == 1
         cache.err_flag.zero_()
+
+
+def test_traced(pdm, dev):
+    """torch.jit.trace keeps the three operators: a traced step gives new results for new inputs."""
+    c = Case(pdm, dev, [3, 1], [40, 9], 4, 2, 64, 16, seed=2)
+    k, other = c.cache, Case(pdm, dev, [3, 1], [40, 9], 4, 2, 64, 16, seed=3)
+    batch = (_t(c.cu, dev), _t(c.table, dev), _t(c.lens, dev))
+    cos, sin = pdm.rotary_tables(50, 64, device=dev)
+    pos = torch.tensor([37, 38, 39, 8], device=dev)
+    held = (k.k_codes.view(torch.uint8), k.v_codes.view(torch.uint8), k.k_scale, k.v_scale)
+
+    def f(q, kv):
+        yq, yk = pdm.qk_norm_rope(q, kv, pos, cos, sin)
+        codes = [t.clone() for t in held]
+        pdm.kv_append(yk, kv, *codes, *batch)
+        return pdm.kv_attention(yq, *codes, *batch, return_lse=True)
+
+    kv = [torch.randn(4, 2, 64, device=dev).to(torch.bfloat16) for _ in range(2)]
+    q = [x.q.to(dev) for x in (c, other)]
+    traced = torch.jit.trace(f, (q[0], kv[0]), check_trace=False)
+    for i in (0, 1):
+        want, got = f(q[i], kv[i]), traced(q[i], kv[i])
+        assert all(torch.equal(a, b) for a, b in zip(want, got)), i
