@@ -20,6 +20,7 @@ from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import ops
 from .onetrans import RMSNorm
@@ -52,6 +53,14 @@ def _traced(t: torch.Tensor) -> bool:
     return (torch.compiler.is_compiling() or isinstance(t, torch.fx.Proxy)
             or type(t).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__ or t.is_meta
             or torch._C._len_torch_dispatch_stack() > 0 or torch._C._get_tracing_state() is not None)
+
+
+def _no_tangent(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    if torch.compiler.is_compiling() or forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative: give it the primals of its inputs")
 
 
 def _fp32(w: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -92,6 +101,7 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     2i + 1) instead of (i, i + rotary_dim / 2).  q_weight, k_weight: [D], fp32 or q's dtype; None: no norm."""
     if (cos is not None and cos.requires_grad) or (sin is not None and sin.requires_grad):
         raise ValueError("cos and sin take no gradient")
+    _no_tangent("qk_norm_rope", q, k, cos, sin, q_weight, k_weight)
     lead = q.shape[:-2]
     if positions.shape != lead:
         raise ValueError(f"positions must be {tuple(lead)}, one for each token, got {tuple(positions.shape)}")
@@ -119,6 +129,7 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
 
 
 def _no_grad(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    _no_tangent(name, *tensors)
     for t in tensors:
         if t is None or not t.requires_grad or not torch.is_grad_enabled():
             continue
@@ -143,7 +154,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: 
     the page holds already are brought to it (exactly, but for the smallest).  NaN and infinities become NaN.  A page that
     is written belongs to one sequence of the call.  ``err_flag`` (int32) is set where spans, lengths, pages or positions
     do not fit; such tokens are left out."""
-    _no_grad("kv_append", k, v, k_weight)
+    _no_grad("kv_append", k, v, k_codes, v_codes, k_scale, v_scale, cos, sin, k_weight)
     kw = k_weight
     if kw is not None:
         if kw.dtype not in (torch.float32, k.dtype):
@@ -169,7 +180,7 @@ def kv_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, 
     ``max_q_len``: the most new tokens that any sequence has, where the program knows it (1 when decoding); a sequence
     with more is left out and sets ``err_flag``.  Slice ``page_table`` to the columns that the longest sequence needs: its
     width bounds the lengths the work is laid out for."""
-    _no_grad("kv_attention", q)
+    _no_grad("kv_attention", q, k_codes, v_codes, k_scale, v_scale, out)
     q = _heads(q)
     if _traced(q):
         if out is not None:

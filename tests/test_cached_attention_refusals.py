@@ -236,3 +236,41 @@ def test_tensors_without_memory(pdm, how):
         out, lse = pdm.kv_attention(q, *cache, *batch, return_lse=True)
         assert lse.shape == (3, 4) and lse.dtype == torch.float32
         assert all(t.device.type == where for t in (yq, out, lse))
+
+
+@pytest.mark.parametrize("which", ["q", "k", "q_weight", "k_weight", "cos"])
+def test_forward_mode_is_refused_by_qk_norm_rope(pdm, which):
+    from torch.autograd import forward_ad
+
+    a = _rope()
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="GPU only"):
+            pdm.qk_norm_rope(**a)
+        a[which] = forward_ad.make_dual(a[which], torch.ones_like(a[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            pdm.qk_norm_rope(**a)
+
+
+@pytest.mark.parametrize("how", ["tangent", "gradient"])
+@pytest.mark.parametrize("which", ["k", "v", "q", "k_codes", "v_codes", "k_scale", "v_scale", "k_weight", "cos", "sin", "out"])
+def test_derivatives_of_the_cache_are_refused(pdm, how, which):
+    """A derivative that nothing would carry on is refused, by whichever input it comes."""
+    from torch.autograd import forward_ad
+
+    app = dict(k=torch.zeros(3, 2, 64), v=torch.zeros(3, 2, 64), k_weight=torch.ones(64), cos=torch.zeros(8, 32),
+               sin=torch.zeros(8, 32), **_cache(), **_batch())
+    att = dict(q=torch.zeros(3, 4, 64, dtype=torch.bfloat16), out=torch.zeros(3, 4, 64, dtype=torch.bfloat16), **_cache(),
+               **_batch())
+    for f, a in ((pdm.kv_append, app), (pdm.kv_attention, att)):
+        if which not in a:
+            continue
+        with forward_ad.dual_level():
+            if how == "tangent":
+                a[which] = forward_ad.make_dual(a[which], torch.ones_like(a[which]))
+            else:
+                a[which] = a[which].requires_grad_(True)
+            with pytest.raises(RuntimeError, match="forward-mode" if how == "tangent" else "no backward"):
+                f(**a)
+            if how == "gradient":
+                with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
+                    f(**a)
