@@ -870,6 +870,11 @@ def _on_device(index: int):
     return _SAME_DEVICE if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
+def _written(*tensors: Optional[torch.Tensor]) -> None:
+    """Tells autograd of tensors that a launch outside the dispatcher writes: a backward pass that saved one raises."""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+
+
 def _gpu_index(*tensors: Optional[torch.Tensor]) -> int:
     """Index of the one GPU that the given tensors are on; raises as ``_require_cuda`` does."""
     index = -1
@@ -976,6 +981,8 @@ def qk_norm_rope_raw(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
             ctypes.byref(desc), q.data_ptr(), _ptr(k), positions.data_ptr(), _ptr(cos), _ptr(sin), _ptr(q_weight),
             _ptr(k_weight), q_out.data_ptr(), _ptr(k_out), _ptr(err_flag), L.raw_stream(index)),
             "pdm_qk_norm_rope_fwd")
+    if err_flag is not None:
+        _written(err_flag)
     return q_out, k_out
 
 
@@ -1141,6 +1148,7 @@ def kv_append_raw(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_cod
         L.check(L.lib().pdm_kv_append(
             ctypes.byref(desc), ctypes.byref(cache), ctypes.byref(batch), k.data_ptr(), v.data_ptr(), _ptr(positions),
             _ptr(cos), _ptr(sin), _ptr(k_weight), _ptr(err_flag), L.raw_stream(index)), "pdm_kv_append")
+    _written(k_codes, v_codes, k_scale, v_scale, err_flag)
 
 
 @torch.library.custom_op("pdm::kv_append", mutates_args=("k_codes", "v_codes", "k_scale", "v_scale", "err_flag"))
@@ -1188,6 +1196,7 @@ def kv_attention_raw(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tens
         raise ValueError("out must be contiguous and of q's shape and dtype")
     _check_err_flag(err_flag)
     index = _gpu_index(q, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, out, err_flag)
+    given = out
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
@@ -1203,6 +1212,8 @@ def kv_attention_raw(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tens
         L.check(lib.pdm_kv_attention_fwd(
             ctypes.byref(desc), ctypes.byref(cache), ctypes.byref(batch), q.data_ptr(), out.data_ptr(), _ptr(lse),
             _ptr(ws), ws_bytes, _ptr(err_flag), L.raw_stream(index)), "pdm_kv_attention_fwd")
+    if given is not None or err_flag is not None:
+        _written(given, err_flag)
     return out, lse
 
 

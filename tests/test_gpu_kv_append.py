@@ -469,3 +469,41 @@ def test_a_third_of_the_sequences_busy(pdm, dev, D, page, hk):
         pool.append(k, v, _cu(more), table, lens, k.double(), v.double())
         pool.check()
     assert pool.cache.err_flag.item() == 0
+
+
+def test_autograd_notices_what_is_written(pdm, dev):
+    """A backward pass that saved a scale, codes, the flag or a given output before a call wrote it raises; inference tensors,
+    which have no versions, are written all the same."""
+    D, page, hk = 64, 16, 2
+    k, v = (t.to(dev) for t in _rows(5, hk, D, torch.bfloat16, 0))
+    cu, table, lens = (torch.tensor(x, dtype=torch.int32, device=dev) for x in ([0, 5], [[1]], [9]))
+    c = pdm.PagedKVCache(2, page, hk, D, dev)
+    a = torch.ones((), device=dev, requires_grad=True)
+    for name in ("k_scale", "v_scale"):
+        y = (a * getattr(c, name)).sum()
+        c.append(k, v, cu, table, lens)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            y.backward()
+    tensors = (c.k_codes, c.v_codes, c.k_scale, c.v_scale, c.err_flag)
+    held = [t._version for t in tensors]
+    c.append(k, v, cu, table, lens)
+    assert all(t._version > x for t, x in zip(tensors, held))
+    q, out = torch.ones(5, 4, D, dtype=torch.bfloat16, device=dev), torch.zeros(5, 4, D, dtype=torch.bfloat16, device=dev)
+    y = (a * out).sum()
+    held = c.err_flag._version
+    pdm.kv_attention(q, *tensors[:4], cu, table, lens, out=out, err_flag=c.err_flag)
+    assert c.err_flag._version > held
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+    held = c.err_flag._version
+    pdm.qk_norm_rope(q, None, torch.arange(5, device=dev), None, None, err_flag=c.err_flag)
+    assert c.err_flag._version > held
+    with torch.inference_mode():
+        d = pdm.PagedKVCache(2, page, hk, D, dev)
+        d.append(k, v, cu, table, lens)
+        d.attend(q, cu, table, lens)
+    e = pdm.PagedKVCache(2, page, hk, D, dev)
+    e.append(k, v, cu, table, lens)
+    assert torch.equal(d.k_codes.view(torch.uint8), e.k_codes.view(torch.uint8)) and torch.equal(d.v_scale, e.v_scale)
+    d.append(k, v, cu, table, lens)  # inference tensors outside the mode
+    d.check()
