@@ -50,13 +50,14 @@ def _heads(t: torch.Tensor) -> torch.Tensor:
 def _traced(t: torch.Tensor) -> bool:
     """True where a call has to be seen by the dispatcher: in compiled and traced graphs, under a dispatch mode, and for tensors
     without memory (fake, meta) or with a dispatch of their own."""
-    return (torch.compiler.is_compiling() or isinstance(t, torch.fx.Proxy)
-            or type(t).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__ or t.is_meta
-            or torch._C._len_torch_dispatch_stack() > 0 or torch._C._get_tracing_state() is not None)
+    if torch.compiler.is_compiling() or isinstance(t, torch.fx.Proxy):
+        return True
+    return (t.is_meta or type(t).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__
+            or torch._C._len_torch_dispatch_stack() > 0 or torch._C._is_tracing())
 
 
 def _no_tangent(name: str, *tensors: Optional[torch.Tensor]) -> None:
-    if torch.compiler.is_compiling() or forward_ad._current_level < 0:
+    if forward_ad._current_level < 0 or torch.compiler.is_compiling():
         return
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
@@ -130,10 +131,10 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
 
 def _no_grad(name: str, *tensors: Optional[torch.Tensor]) -> None:
     _no_tangent(name, *tensors)
-    for t in tensors:
-        if t is None or not t.requires_grad or not torch.is_grad_enabled():
-            continue
-        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or detach its inputs")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or detach its inputs")
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor,
