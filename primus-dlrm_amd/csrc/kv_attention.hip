@@ -46,6 +46,23 @@ struct AttnArgs {
 constexpr float kInf = __builtin_inff();
 constexpr float kLn2 = 0.69314718055994531f;
 
+// Weights are exp2 of scores less a reference, which moves only where a weight would pass 2^8: sums and products lose nothing
+// by that while the values are below 2^89, whatever the number of keys.  Where a page's scale is above kHugeScale (so that its
+// values may reach 448 * 2^119), the reference lies 40 above the largest score from then on, and weights stay below 2^-32: 2^30
+// keys of the largest value do not overflow, and only weights 2^-86 of the row's largest are lost.
+constexpr float kHugeScale = 0x1p80f;
+struct Reference {
+  float room = 8.0f, lift = 0.0f;
+  __device__ __forceinline__ void raise(bool huge) {  // the same for the whole wave
+    if (huge) room = -32.0f, lift = 40.0f;
+  }
+};
+
+// log sum_j exp(s_j) of a row whose weights 2^(s_j - m) have this sum.
+__device__ __forceinline__ float row_lse(float m, float sum) {
+  return ((m + (float)__builtin_amdgcn_frexp_expf(sum)) + __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(sum))) * kLn2;
+}
+
 // What a sequence's rows see.
 struct Seq {
   int64_t row0;   // its first row of the batch
@@ -353,6 +370,7 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
   // lane x of a batch of 32 tiles: place (in bytes) and scales of the 16 keys x % 2 of tile x / 2
   uint64_t spot = 0;
   float kss = 0.0f, vss = 0.0f;           // kss: NaN where the page does not exist
+  Reference ref;
   auto key_of = [&](int i) { return begin + (wave + kFewWaves * i) * kFewKeys; };
   auto look_up = [&](int first) {
     const int key = key_of(first + (lane >> 1)) + (lane & 1) * 16;
@@ -369,6 +387,7 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
         *a.err = 1;
       }
     }
+    ref.raise(__any(vss > kHugeScale));
   };
   auto place = [&](int i, int s) { return lane_u64(spot, (i & 31) * 2 + s); };
   u32x4_t k[2][D / 64];                   // 16 bytes of a key row, 64 apart
@@ -423,6 +442,7 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
       if (a.err) *a.err = 1;
     }
     mine = tiles > wave ? (tiles - wave + kFewWaves - 1) / kFewWaves : 0;
+    ref = Reference();
     if (mine > 0) look_up(0);
     all_lo = 0, all_hi = sq.hi;
     const int p0 = sq.len - sq.n, p1 = sq.len - 1;
@@ -513,11 +533,10 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
       float top = w[0];
 #pragma unroll
       for (int e = 1; e < 8; ++e) top = fmaxf(top, w[e]);
-      // the maximum moves only where a weight would pass 2^8: sums and products lose nothing by that
-      if (__any(top > m[mt] + 8.0f)) {
+      if (__any(top > m[mt] + ref.room)) {
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float now = top > m[mt] + 8.0f ? top : m[mt];  // by row: other rows change nothing
+        const float now = top > m[mt] + ref.room ? top + ref.lift : m[mt];  // by row: other rows change nothing
         const float f = now == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m[mt] - now);
         m[mt] = now;
         l[mt] *= f;
@@ -647,7 +666,7 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
         const int64_t at = (cur.sq.row0 + i) * a.hq + h;
         const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
         store4<DT>(a.out, at * D + d, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
-        if (d == 0 && a.lse) a.lse[at] = sum != 0.0f ? (top_r + __builtin_amdgcn_logf(sum)) * kLn2 : -kInf;
+        if (d == 0 && a.lse) a.lse[at] = sum != 0.0f ? row_lse(top_r, sum) : -kInf;
       } else {
         const int64_t at = cur.slot * a.row_stride + row;
         *reinterpret_cast<f32x4_t*>(a.part_o + at * D + d) = acc;
@@ -722,7 +741,7 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, int used, int64_t ou
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) store_out(a, DT, out * D + lane * E + e, sum != 0.0f ? acc[e] / sum : 0.0f);
-  if (lane == 0 && a.lse) a.lse[out] = sum != 0.0f ? (top + __builtin_amdgcn_logf(sum)) * kLn2 : -kInf;
+  if (lane == 0 && a.lse) a.lse[out] = sum != 0.0f ? row_lse(top, sum) : -kInf;
 }
 
 // Joins the equal parts of the few-rows kernel's pairs: W waves per row.
@@ -895,6 +914,7 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
   constexpr int PER = 1024 / KT;           // tiles of a batch of 1024 keys
   uint64_t spot = 0;                       // lane i: place and scales of keys 16 i .. of the batch
   float kss = 0.0f, vss = 0.0f;
+  Reference ref;
   u32x4_t kr[KP];
   u32x4_t vw[D == 64 ? 1 : 2];             // 16 elements of a key, or of two keys
   uint32_t vr[4][VD / 4];                  // VD elements of four keys, exchanged
@@ -928,6 +948,7 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
           *a.err = 1;
         }
       }
+      ref.raise(__any(vss > kHugeScale));
     }
     const int g0 = (t % PER) * (KT / 16);
     auto place = [&](int grp) { return lane_u64(spot, g0 + grp); };  // bytes before the 16 keys `grp` of the tile
@@ -1088,10 +1109,9 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
       for (int e = 1; e < 8; ++e) most = fmaxf(most, s[x >> 1][8 * (x & 1) + e]);
       top = fmaxf(top, most * sc[x]);
     }
-    // the maximum moves only where a weight would pass 2^8: sums and products lose nothing by that
-    if (__any(top > m + 8.0f)) {
+    if (__any(top > m + ref.room)) {
       top = fmaxf(top, __shfl_xor(top, 32));
-      const float now = top > m + 8.0f ? top : m;  // by row: other rows change nothing
+      const float now = top > m + ref.room ? top + ref.lift : m;  // by row: other rows change nothing
       const float f = now == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - now);
       m = now;
       l *= f;
@@ -1219,7 +1239,7 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
 #pragma unroll
       for (int e = 0; e < 16; e += 4)
         store4<DT>(a.out, at * D + 32 * d + 2 * e + 4 * h, o[d][e] * f, o[d][e + 1] * f, o[d][e + 2] * f, o[d][e + 3] * f);
-    if (h == 0 && a.lse) a.lse[at] = sum != 0.0f ? (m + __builtin_amdgcn_logf(sum)) * kLn2 : -kInf;
+    if (h == 0 && a.lse) a.lse[at] = sum != 0.0f ? row_lse(m, sum) : -kInf;
   } else {
     const int64_t pr = at * a.splits + split;
 #pragma unroll

@@ -614,3 +614,44 @@ def test_traced(pdm, dev):
     for i in (0, 1):
         want, got = f(q[i], kv[i]), traced(q[i], kv[i])
         assert all(torch.equal(a, b) for a, b in zip(want, got)), i
+
+
+HUGE = {  # new tokens, lengths, query heads per key head, key heads, max_q_len
+    "alone": ([1], [100], 2, 2, 1), "split": ([3, 1], [2500, 700], 2, 1, 3), "two tiles of rows": ([7], [900], 4, 1, 7),
+    "dealt": ([1] * 40, [130 + 40 * i for i in range(40)], 2, 8, 1), "even": ([1] * 40, [500] * 40, 2, 8, 1),
+    "many": ([150, 40], [470, 900], 2, 2, 150), "many, split": ([60, 1], [2500, 30], 4, 1, 60),
+    "two groups": ([500, 300, 600], [800, 350, 600], 1, 64, 600),
+}
+
+
+@pytest.mark.parametrize("which", HUGE)
+@pytest.mark.parametrize("D,e", [(64, 81), (64, 119), (128, 113), (128, 119), (256, 119)])
+def test_values_near_the_top_of_the_range(pdm, dev, which, D, e):
+    """Values of up to 448 * 2^119, one step below what bf16 holds, behind scores that grow by 7.5 (a weight of 2^7.5 before the
+    maximum moves) or move it with every tile: every output is a mean of the values, so it is finite, whatever sums it comes
+    from.  The other places of the cache hold values of ordinary size."""
+    new, lens, group, hk, most = HUGE[which]
+    if len(new) == 3 and D == 256:
+        hk = 8
+    c = Case(pdm, dev, new, lens, group * hk, hk, D, 32, seed=e + D)
+    c.q.zero_()
+    c.q[..., 0] = 1.0
+    for grow in (lambda j: torch.where(j < 40, 0.0, 7.5), lambda j: 6.5 * (j // 32).clamp(max=60), lambda j: 0.0 * j):
+        k = torch.zeros(c.cache.k_codes.shape)
+        for row, n in zip(c.table, lens):
+            for i, p in enumerate(row):
+                if p >= 0:
+                    k[p, :, :, 0] = grow(torch.arange(32) + 32 * i)
+        c.cache.k_codes.copy_(k.to(torch.float8_e4m3fn))
+        c.cache.k_scale.fill_(1.0)
+        v = c.cache.v_codes.float()
+        v[:, 0] = 448.0
+        if grow(torch.tensor([41])) == 0:  # with equal scores, the first pages of ordinary size
+            c.cache.v_scale.fill_(2.0 ** e)
+            c.cache.v_scale[[row[0] for row in c.table]] = 2.0 ** -6
+        else:
+            c.cache.v_scale.fill_(2.0 ** e)
+        c.cache.v_codes.copy_(v.to(torch.float8_e4m3fn))
+        got, want = c.run(scale=math.log(2), max_q_len=most), c.want(scale=math.log(2))
+        assert torch.isfinite(got[0]).all()
+        c.check(got, want)
