@@ -676,8 +676,11 @@ typedef struct {
  * and j > p - window (window > 0):
  *   out = sum_j softmax_j(scale * q . k_j) v_j,  lse = log sum_j exp(scale * q . k_j)
  * Scores, softmax and sums are fp32 (the products take bf16 or f16 operands:
- * codes are exact in both; weights are rounded to bf16).  A row that sees no
- * key, a row left out and a row behind the last sequence is zeros, lse -inf.
+ * codes are exact in both; a weight is a bf16 number and its bf16 remainder,
+ * 2^-16 of it left, but for bf16 sequences of more than 16 or 32 rows per key
+ * head, whose weights are rounded to bf16 as their outputs are).  A row that
+ * sees no key, a row left out and a row behind the last sequence is zeros, lse
+ * -inf.
  * Keys that a row does not see do not reach it, whatever they hold.
  * Pages that no row of a sequence sees are not looked at, nor flagged.
  * out: device, contiguous [tokens, n_q_heads, D] of dtype, 16-byte aligned;

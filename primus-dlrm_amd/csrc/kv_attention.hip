@@ -8,8 +8,12 @@
 //
 // Codes become operands by conversion alone: e4m3 is a subset of bf16 and of f16, keys are converted bare and their
 // page's scale is a factor of the scores in fp32, values are converted with their power-of-two scale, which bf16
-// holds exactly.  Weights are rounded to bf16 (half a step is 2^-8 of a weight, against 2^-4 of an 8-bit value);
-// the running sum takes them before that.
+// holds exactly.  f16 would not hold the values, so weights are bf16 as well, which leaves 2^-8 of a weight, half a step of a bf16
+// output and eight of an fp16 one.  So a weight goes in as a bf16 number and the bf16 remainder, 2^-16 of it left, by a second
+// product with the same values: few rows, whose matrix units wait for the keys (62.6 -> 64.1 us for 64 sequences of 128 to
+// 8,192 tokens), and many rows of fp16 (794 -> 1,061 us for the prompts below).  Many rows of bf16 do without it: the error of
+// their outputs goes from 1.7e-3, of the output's own rounding, to 2.4e-3, at 794 us instead of 1,048.  The running sum takes
+// weights before any rounding.
 //
 // The simplest kernel, a wave for each (row, head), took 289 us for one sequence of 1,000 tokens, 4,764 for 64 of 128 to 8,192
 // and 110,493 for two prompts of 4,000 tokens behind 4,000 (32 query heads, 8 key heads of 128); these take 9.4, 63 and 780.
@@ -126,6 +130,11 @@ template <int DT>
 __device__ __forceinline__ f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c) {
   if constexpr (DT == PDM_BF16) return mfma16x16x32(a, b, c);
   else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// What rounding a pair of weights to the bf16 numbers `hi` left, as bf16 numbers.
+__device__ __forceinline__ uint32_t remainder_pair(float x, float y, uint32_t hi) {
+  return pack_bf16x2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
 }
 
 // A lane's value, for the whole wave.
@@ -517,7 +526,7 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
     }
     const int key = key_of(i);
     const bool whole = whole_tile(i, ok[0] && ok[1]);
-    u32x4_t p[MT];
+    u32x4_t p[MT], rest[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       float w[8];
@@ -547,7 +556,11 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(w[e] - base);
       l[mt] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-      p[mt] = u32x4_t{pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]), pack_bf16x2(w[4], w[5]), pack_bf16x2(w[6], w[7])};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        p[mt][e] = pack_bf16x2(w[2 * e], w[2 * e + 1]);
+        rest[mt][e] = remainder_pair(w[2 * e], w[2 * e + 1], p[mt][e]);
+      }
     }
     if (!whole) {
       uint32_t any = 0;
@@ -569,7 +582,7 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
       for (int x = 0; x < 4; ++x) {
         const u32x4_t vf = value_tile(h, x, vs[0], vs[1]);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) o[mt][4 * h + x] = mfma16x16x32(vf, p[mt], o[mt][4 * h + x]);
+        for (int mt = 0; mt < MT; ++mt) o[mt][4 * h + x] = mfma16x16x32(vf, p[mt], mfma16x16x32(vf, rest[mt], o[mt][4 * h + x]));
       }
     if (i + 1 < mine) load_v(i + 1);
   }
@@ -840,6 +853,7 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
   constexpr int VD = D == 64 ? 4 : 8;      // elements of a thread's 4 keys of V
   constexpr int KS = ManyShared<D, KT>::KS, VS = ManyShared<D, KT>::VS;
   constexpr int LEAD = 8;                  // fragments read ahead of their products
+  constexpr bool FINE = DT == PDM_F16;     // weights as two bf16 numbers (see the head of the file)
   __shared__ ManyShared<D, KT> sh;
 
   const int64_t unit = linear_block();
@@ -1074,8 +1088,8 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
     sched_mfma_ds_pipeline<XX * KK, LEAD>();
   };
   // the running maximum, and P from the scores
-  u32x4_t p[2 * XX];
-  auto weights = [&](int t) {
+  u32x4_t p[2 * XX], rest[2 * XX];
+  auto weights = [&](int t) __attribute__((always_inline)) {
     const int key = begin + t * KT;
     float sc[2 * XX];                      // of 16 keys each, not negative
     bool ok = true;
@@ -1130,15 +1144,28 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
       for (int e = 0; e < 4; ++e) {
         p[2 * x][e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
         p[2 * x + 1][e] = pack_bf16x2(v[8 + 2 * e], v[8 + 2 * e + 1]);
+        if constexpr (FINE) {
+          rest[2 * x][e] = remainder_pair(v[2 * e], v[2 * e + 1], p[2 * x][e]);
+          rest[2 * x + 1][e] = remainder_pair(v[8 + 2 * e], v[8 + 2 * e + 1], p[2 * x + 1][e]);
+        }
       }
     }
   };
-  auto values = [&](int t) {
+  auto values = [&](int t) __attribute__((always_inline)) {  // (not inlined, it would have O in memory)
 #pragma unroll
-    for (int y = 0; y < 2 * XX; ++y)
+    for (int y = 0; y < 2 * XX; ++y) {
+      u32x4_t vf[DD];
 #pragma unroll
-      for (int d = 0; d < DD; ++d) o[d] = mfma32x32x16(v_frag(t, d, y), p[y], o[d]);
-    sched_mfma_ds_pipeline<2 * XX * DD, LEAD>();
+      for (int d = 0; d < DD; ++d) {
+        vf[d] = v_frag(t, d, y);
+        o[d] = mfma32x32x16(vf[d], p[y], o[d]);
+      }
+      if constexpr (FINE) {
+#pragma unroll
+        for (int d = 0; d < DD; ++d) o[d] = mfma32x32x16(vf[d], rest[y], o[d]);
+      }
+    }
+    sched_mfma_ds_pipeline<2 * XX * DD, LEAD, FINE ? 2 : 1>();
   };
 
   if (tiles > 0) {

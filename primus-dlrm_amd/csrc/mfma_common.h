@@ -27,18 +27,18 @@ __device__ __forceinline__ f32x4_t mfma16x16x32(u32x4_t a, u32x4_t b, f32x4_t c)
                                                  c, 0, 0, 0);
 }
 
-// Pins the instruction order of a fully unrolled loop of N MFMAs, each fed by
-// one LDS read: the first LEAD reads are issued up front, then one MFMA and
-// the next read alternate, so every read has LEAD MFMAs of latency slack.
-template <int N, int LEAD>
+// Pins the instruction order of a fully unrolled loop of N x EACH MFMAs, EACH of
+// them fed by one LDS read: the first LEAD reads are issued up front, then EACH MFMAs
+// and the next read alternate, so every read has LEAD x EACH MFMAs of latency slack.
+template <int N, int LEAD, int EACH = 1>
 __device__ __forceinline__ void sched_mfma_ds_pipeline() {
   __builtin_amdgcn_sched_group_barrier(0x100, LEAD, 0);  // DS reads
 #pragma unroll
   for (int i = 0; i < N - LEAD; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
-    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // DS read
+    __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);  // MFMA
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);     // DS read
   }
-  __builtin_amdgcn_sched_group_barrier(0x008, LEAD, 0);
+  __builtin_amdgcn_sched_group_barrier(0x008, LEAD * EACH, 0);
 }
 
 // bf16 rounding of the block kernels: the hardware conversion (v_cvt_pk_bf16_f32,

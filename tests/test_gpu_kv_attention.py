@@ -655,3 +655,21 @@ def test_values_near_the_top_of_the_range(pdm, dev, which, D, e):
         got, want = c.run(scale=math.log(2), max_q_len=most), c.want(scale=math.log(2))
         assert torch.isfinite(got[0]).all()
         c.check(got, want)
+
+
+@pytest.mark.parametrize("dtype,which", [(t, n) for n in HUGE for t in STEP if t == torch.float16 or HUGE[n][4] <= 16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_weights_are_finer_than_the_output(pdm, dev, dtype, which, D):
+    """Weights reach the second product as a bf16 number and the bf16 remainder (all but many rows of bf16 outputs, whose own
+    half step is a weight's): each rounding leaves 2^-8 of what it rounds, so a weight is off by 2^-16 of itself.  Sums of N
+    products, N weights and up to N / 32 changes of the maximum are within (3 N + 16) u of their terms' sizes."""
+    new, lens, group, hk, most = HUGE[which]
+    if len(new) == 3 and D == 256:
+        hk = 8
+    c = Case(pdm, dev, new, lens, group * hk, hk, D, 32, dtype, seed=D)
+    (out, lse), want = c.run(max_q_len=most), c.want()
+    c.check((out, lse), want)
+    w_out, _, mag, sabs = want
+    slack = (2.0 ** -16 + 2 * (D + 8) * U * sabs[..., None] + 2.0 ** -20 + (3 * max(lens) + 16) * U) * mag
+    bad = (out.cpu().double() - w_out).abs() - slack - STEP[dtype] * (w_out.abs() + slack) - 2.0 ** -25
+    assert bad.max().item() <= 0, f"over by {bad.max().item():.3e}"
