@@ -243,7 +243,7 @@ int check(const char* fn, const pdm_qk_rope_desc* d) {
   if (d->table_rows < 0) return bad("negative table_rows");
   if (!(d->eps >= 0)) return bad("eps must not be negative");
   const int64_t heads = d->n_q_heads > d->n_k_heads ? d->n_q_heads : d->n_k_heads;
-  if (d->tokens * heads >= (int64_t(1) << 31) || heads > (1 << 20) || d->tokens > (int64_t(1) << 31))
+  if (heads > (1 << 20) || d->tokens > (int64_t(1) << 31) || d->tokens * heads >= (int64_t(1) << 31))
     return bad("tokens * heads must be below 2^31");
   return PDM_OK;
 }

@@ -274,3 +274,11 @@ def test_derivatives_of_the_cache_are_refused(pdm, how, which):
             if how == "gradient":
                 with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
                     f(**a)
+
+
+def test_sizes_whose_product_passes_64_bits(pdm):
+    """(Where the product overflows, the sanitized build stops.)"""
+    L = pdm._lib
+    d = L.QkRopeDesc(1 << 62, 4, 1, 64, 64, L.PDM_BF16, 64, 0, 1e-6, 8, 128, 64, 64, 64)
+    assert L.lib().pdm_qk_norm_rope_fwd(ctypes.byref(d), *[None] * 11) == L.PDM_ERR_INVALID and "2^31" in L.last_error()
+    assert L.lib().pdm_qk_norm_rope_bwd_workspace_size(ctypes.byref(d)) == L.PDM_ERR_INVALID
