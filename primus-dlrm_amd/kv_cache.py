@@ -219,8 +219,9 @@ class QKNormRope(nn.Module):
         self.register_buffer("sin", sin, persistent=False)
 
     def _apply(self, fn, *args, **kwargs):
+        empty = self.cos is not None and self.cos.is_meta
         super()._apply(fn, *args, **kwargs)
-        if self.cos is not None and self.cos.dtype != torch.float32:
+        if self.cos is not None and (self.cos.dtype != torch.float32 or (empty and not self.cos.is_meta)):
             self.cos, self.sin = rotary_tables(self.max_positions, self.rotary_dim, self.theta, self.cos.device)
         return self
 

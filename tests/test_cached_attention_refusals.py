@@ -282,3 +282,15 @@ def test_sizes_whose_product_passes_64_bits(pdm):
     d = L.QkRopeDesc(1 << 62, 4, 1, 64, 64, L.PDM_BF16, 64, 0, 1e-6, 8, 128, 64, 64, 64)
     assert L.lib().pdm_qk_norm_rope_fwd(ctypes.byref(d), *[None] * 11) == L.PDM_ERR_INVALID and "2^31" in L.last_error()
     assert L.lib().pdm_qk_norm_rope_bwd_workspace_size(ctypes.byref(d)) == L.PDM_ERR_INVALID
+
+
+def test_module_that_was_made_without_memory(pdm):
+    """The tables are in no state dict: they are there once the module has memory, whatever that held."""
+    want = pdm.rotary_tables(10, 32)
+    for dtype in (torch.float32, torch.bfloat16):
+        with torch.device("meta"):
+            m = pdm.QKNormRope(64, 10, rotary_dim=32)
+        m = m.to(dtype).to_empty(device="cpu")
+        assert m.cos.device.type == "cpu" and torch.equal(m.cos, want[0]) and torch.equal(m.sin, want[1])
+        m.load_state_dict(pdm.QKNormRope(64, 10, rotary_dim=32).state_dict())
+        assert m.q_norm.weight.dtype == dtype and torch.equal(m.to(torch.float64).cos, want[0])
