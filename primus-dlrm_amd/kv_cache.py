@@ -47,13 +47,14 @@ def _heads(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
-def _traced(t: torch.Tensor) -> bool:
-    """True where a call has to be seen by the dispatcher: in compiled and traced graphs, under a dispatch mode, and for tensors
-    without memory (fake, meta) or with a dispatch of their own."""
+def _traced(t: torch.Tensor, direct: bool = False) -> bool:
+    """True where a call has to be seen by the dispatcher: in compiled and traced graphs, for tensors without memory (fake, meta)
+    or with a dispatch of their own, and under a dispatch mode unless ``direct`` (the call has an argument that the registered
+    operator has not)."""
     if torch.compiler.is_compiling() or isinstance(t, torch.fx.Proxy):
         return True
-    return (t.is_meta or type(t).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__
-            or torch._C._len_torch_dispatch_stack() > 0 or torch._C._is_tracing())
+    return (t.is_meta or type(t).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__ or torch._C._is_tracing()
+            or (torch._C._len_torch_dispatch_stack() > 0 and not direct))
 
 
 def _no_tangent(name: str, *tensors: Optional[torch.Tensor]) -> None:
@@ -114,9 +115,9 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     q3, k3 = _heads(q), None if k is None else _heads(k)
     pos = positions if len(lead) == 1 and positions.is_contiguous() else positions.reshape(-1).contiguous()
     qw, kw = _fp32(q_weight), _fp32(k_weight)
-    if _traced(q):
+    if _traced(q, direct=err_flag is not None):
         if err_flag is not None:
-            raise ValueError("err_flag is not available in a compiled graph")
+            raise ValueError("err_flag is not available in a compiled or traced graph")
         q_out, k_out = torch.ops.pdm.qk_norm_rope(q3, k3, pos, cos, sin, qw, kw, eps, interleaved)
         k_out = None if k is None else k_out
     elif torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q3, k3, qw, kw)):
@@ -183,9 +184,9 @@ def kv_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, 
     width bounds the lengths the work is laid out for."""
     _no_grad("kv_attention", q, k_codes, v_codes, k_scale, v_scale, out)
     q = _heads(q)
-    if _traced(q):
+    if _traced(q, direct=out is not None):
         if out is not None:
-            raise ValueError("out is not available in a compiled graph")
+            raise ValueError("out is not available in a compiled or traced graph")
         out, lse = torch.ops.pdm.kv_attention(q, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens,
                                               q.shape[-1] ** -0.5 if scale is None else scale, causal, window,
                                               q.shape[0] if max_q_len is None else max_q_len, return_lse, err_flag)

@@ -673,3 +673,31 @@ def test_weights_are_finer_than_the_output(pdm, dev, dtype, which, D):
     slack = (2.0 ** -16 + 2 * (D + 8) * U * sabs[..., None] + 2.0 ** -20 + (3 * max(lens) + 16) * U) * mag
     bad = (out.cpu().double() - w_out).abs() - slack - STEP[dtype] * (w_out.abs() + slack) - 2.0 ** -25
     assert bad.max().item() <= 0, f"over by {bad.max().item():.3e}"
+
+
+def test_under_a_dispatch_mode(pdm, dev):
+    """A mode that watches operators sees the calls that are registered operators and leaves the others (a flag of
+    qk_norm_rope, a given output) as they are."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    seen = []
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    c = Case(pdm, dev, [3, 1], [40, 9], 4, 2, 64, 16, seed=2)
+    k = c.cache
+    args = (k.k_codes, k.v_codes, k.k_scale, k.v_scale, _t(c.cu, dev), _t(c.table, dev), _t(c.lens, dev))
+    q, pos, err = c.q.to(dev), torch.arange(4, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    cos, sin = pdm.rotary_tables(50, 64, device=dev)
+    want = pdm.kv_attention(q, *args), pdm.qk_norm_rope(q, None, pos, cos, sin)[0]
+    given = torch.empty_like(q)
+    with Watch():
+        got = pdm.kv_attention(q, *args), pdm.qk_norm_rope(q, None, pos, cos, sin)[0]
+        flagged = pdm.qk_norm_rope(q, None, pos, cos, sin, err_flag=err)[0]
+        pdm.kv_attention(q, *args, out=given)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(flagged, want[1]) and torch.equal(given, want[0])
+    assert [s for s in seen if s.startswith("pdm.")] == ["pdm.kv_attention.default", "pdm.qk_norm_rope.default"]
