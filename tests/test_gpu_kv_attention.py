@@ -701,3 +701,26 @@ def test_under_a_dispatch_mode(pdm, dev):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert torch.equal(flagged, want[1]) and torch.equal(given, want[0])
     assert [s for s in seen if s.startswith("pdm.")] == ["pdm.kv_attention.default", "pdm.qk_norm_rope.default"]
+
+
+def test_registered_operators(pdm, dev):
+    """Schemas, shapes without memory, autograd registration and dispatch of the three operators."""
+    c = Case(pdm, dev, [3, 1], [40, 9], 4, 2, 64, 16, seed=2)
+    k = c.cache
+    held = [k.k_codes.view(torch.uint8).clone(), k.v_codes.view(torch.uint8).clone(), k.k_scale.clone(), k.v_scale.clone()]
+    batch = (_t(c.cu, dev), _t(c.table, dev), _t(c.lens, dev))
+    cos, sin = pdm.rotary_tables(50, 64, device=dev)
+    pos, err = torch.arange(4, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    q, kv = c.q.to(dev), torch.randn(4, 2, 64, device=dev).to(torch.bfloat16)
+    w = [torch.ones(64, device=dev) for _ in range(2)]
+    grad = lambda t: t.detach().clone().requires_grad_(True)  # noqa: E731
+    check = torch.library.opcheck
+    ops = torch.ops.pdm
+    check(ops.qk_norm_rope.default, (grad(q), grad(kv), pos, cos, sin, grad(w[0]), grad(w[1]), 1e-6, False))
+    check(ops.qk_norm_rope.default, (grad(q), None, pos, cos, sin, grad(w[0]), None, 1e-6, True))
+    check(ops.qk_norm_rope.default, (q, None, pos, None, None, None, None, 1e-6, False))
+    check(ops.qk_norm_rope_backward.default, (q, kv, pos, cos, sin, *w, q, kv, 1e-6, False))
+    for flag in (err, None):
+        check(ops.kv_append.default, (kv, kv, *held, *batch, None, cos, sin, w[0], 1e-6, False, flag))
+        for lse in (True, False):
+            check(ops.kv_attention.default, (q, *held, *batch, 0.125, True, 0, 3, lse, flag))
