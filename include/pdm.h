@@ -645,7 +645,8 @@ typedef struct {
  * (k_weight not NULL) and rotated (rotary_dim > 0) first as in
  * pdm_qk_norm_rope_fwd, by positions[row] or, when positions is NULL, by the
  * token's index in its sequence (a position outside the tables: a zero key,
- * and err_flag).
+ * all of its elements, and err_flag; without rotation positions are not looked
+ * at).
  * Of the new values x on a page (keys and values apart, each head by itself),
  * e is the smallest exponent with max |x| <= 448 * 2^e; where the page already
  * holds tokens of the sequence, e is not below the page's own, and their codes

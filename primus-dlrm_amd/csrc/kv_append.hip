@@ -10,7 +10,7 @@
 // Bound by HBM (2 bytes read and 1 written per bf16 element) for prompts, by latency for single tokens.  A page's share of
 // the batch stays in registers from its load to its codes, so that the maximum costs no second read: 17,800 tokens of 5 prompts,
 // 8 heads of 128, 33 us (3.3 TB/s; 49 with keys in one pass and values in another), 1 to 60 tokens of 512 sequences, 6 heads of
-// 64, 15.5 us, 64 single tokens 5.0 us.
+// 64, 15.8 us, 64 single tokens behind 100 to 2,000 5.2 us.
 #include "kv_common.h"
 
 namespace pdm {
@@ -114,8 +114,9 @@ __device__ __forceinline__ float to_odd(double x) {
   return (float)__builtin_bit_cast(double, odd);
 }
 
-// A key row normed and rotated, in 64 bits (as fast as 32 here): its code is the nearest to the key itself, whatever the
-// order of the sum.  Called by the row's whole group; `ok`: this row exists.
+// A key row normed and rotated, in 64 bits: its code is the nearest to the key itself, whatever the order of the sum.
+// (Against 32 bits, in a kernel that took keys and values in two passes, the prompts above went from 35 to 49 us.)  Called by
+// the row's whole group; `ok`: this row exists.
 template <bool NORM, bool INTER>
 __device__ __forceinline__ void key_row(const AppendArgs& a, const Segment& g, int r, bool ok, int j, const RowPlace& pl, float* v) {
   double rs = 1.0;
@@ -406,8 +407,9 @@ __global__ void __launch_bounds__(256) kv_append_token_kernel(AppendArgs a, int6
 
 template <int DT, bool NORM, bool INTER, bool VEC, int W, int NI>
 void launch_kernel(const AppendArgs& a, int64_t items, hipStream_t st) {
-  // 64 sequences, 8 heads of 128, pages of 64: one token each 5.7 us in the first kernel, 8.0 in the second; two each 8.2 and
-  // 7.7; 64 tokens of one sequence 8.9 (151 where lane groups take them row by row); single tokens of 4,096 sequences 28
+  // 64 sequences behind 100 tokens each, 8 heads of 128, pages of 64: one token each 5.7 us in the first kernel, 8.0 in the
+  // second; two each 8.2 and 7.7; 64 tokens of one sequence 8.9 (151 where lane groups take them row by row); single tokens of
+  // 4,096 sequences 28
   if (a.tokens <= a.seqs) {
     const int parts = 64 >> a.width_log2, waves = (2 * a.heads + parts - 1) / parts;
     const int64_t few = (items * waves + 3) / 4, all = few + ((int64_t)a.seqs + 255) / 256 * kParts;

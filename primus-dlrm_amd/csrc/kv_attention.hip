@@ -8,15 +8,15 @@
 //
 // Codes become operands by conversion alone: e4m3 is a subset of bf16 and of f16, keys are converted bare and their
 // page's scale is a factor of the scores in fp32, values are converted with their power-of-two scale, which bf16
-// holds exactly.  f16 would not hold the values, so weights are bf16 as well, which leaves 2^-8 of a weight, half a step of a bf16
-// output and eight of an fp16 one.  So a weight goes in as a bf16 number and the bf16 remainder, 2^-16 of it left, by a second
-// product with the same values: few rows, whose matrix units wait for the keys (62.6 -> 64.1 us for 64 sequences of 128 to
-// 8,192 tokens), and many rows of fp16 (794 -> 1,061 us for the prompts below).  Many rows of bf16 do without it: the error of
-// their outputs goes from 1.7e-3, of the output's own rounding, to 2.4e-3, at 794 us instead of 1,048.  The running sum takes
-// weights before any rounding.
+// holds exactly.  f16 would not hold the values, so weights are bf16 as well, which leaves 2^-8 of a weight, half a step of a
+// bf16 output and eight of an fp16 one.  So a weight goes in as a bf16 number and the bf16 remainder, 2^-16 of it left, by a
+// second product with the same values: few rows, whose matrix units wait for the keys (63.4 -> 64.1 us for 64 sequences of 128
+// to 8,192 tokens), and many rows of fp16 (794 -> 1,061 us for the prompts below).  Many rows of bf16 do without it: the error
+// of their outputs goes from 1.7e-3, of the output's own rounding, to 2.1e-3, at 794 us instead of 1,048.  The running sum
+// takes weights before any rounding.
 //
 // The simplest kernel, a wave for each (row, head), took 289 us for one sequence of 1,000 tokens, 4,764 for 64 of 128 to 8,192
-// and 110,493 for two prompts of 4,000 tokens behind 4,000 (32 query heads, 8 key heads of 128); these take 9.4, 63 and 780.
+// and 110,493 for two prompts of 4,000 tokens behind 4,000 (32 query heads, 8 key heads of 128); these take 9.6, 65 and 786.
 #include <type_traits>
 
 #include "kv_common.h"
@@ -201,9 +201,9 @@ __device__ __forceinline__ void clear_rows(const AttnArgs& a, int64_t first) {
 // maximum, sum and O, and join in LDS; splits join in kv_attn_join_kernel.  Bound by the bytes of the codes: a wave
 // has the next tile's loads (8 KB at D = 128) in flight while it works on one; the operands come from registers, since no
 // two waves share a key.  One token for 4 sequences of 60,000 to 120,000 tokens (32 query heads, 8 key heads of 128) 137 us,
-// 5.2 TB/s, as fast as a copy; for 64 sequences of 128 to 8,192 63 us, 4.1 TB/s (57 and 5.5 for the join: what is missing is
-// the first tile of each of 512 pairs and the run-out); 16 tokens for 256 sequences of 300 to 1,500 (6 heads of 64) 40 us,
-// 3.9 TB/s; one token for one sequence of 1,000 9.4 us, two launches' latency.
+// 5.2 TB/s, as fast as a copy; for 64 sequences of 128 to 8,192 65 us, 3.9 TB/s (59 and 5.4 for the join: what is missing is
+// the first tile of each of 512 pairs and the run-out); 16 tokens for 256 sequences of 300 to 1,500 (6 heads of 64) 41 us,
+// 3.8 TB/s; one token for one sequence of 1,000 9.6 us, two launches' latency.
 constexpr int kFewKeys = 32, kFewWaves = 4, kFewStep = kFewKeys * kFewWaves;
 constexpr int kDealt = 256;   // sequences of a call that is dealt
 
@@ -221,7 +221,8 @@ __device__ __forceinline__ int steps_of(const Seq& s) { return s.hi > s.lo ? (s.
 // runs, so that a batch of long and short sequences keeps every CU busy to the end.  A run ends some pairs and begins
 // one: a workgroup leaves at most two partial results, that of a pair which it did not begin (slot 2 w) and that of one which
 // it did not end (2 w + 1).  Every workgroup computes the plan itself, a sequence per thread.  Against equal splits, 64
-// sequences with 8 key heads of 128: of 128 to 8,192 tokens 63 us instead of 91, of 1,000 to 3,200 60 and 59.
+// sequences with 8 key heads of 128: of 128 to 8,192 tokens 63 us instead of 91, of 1,000 to 3,200 60 and 59 (these and those
+// below before the weights' remainder, which costs all of them 1 to 2 %).
 struct FewDeal {
   int64_t first[kDealt + 1];  // steps before a sequence, of all its heads
   int64_t sums[4];
@@ -315,7 +316,8 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
     if (unit >= units + guards) return;
     const int64_t first = (unit - units) * 256;
     Seq s;
-    if (units == 0 && first + threadIdx.x < a.seqs) seq_of(a, (int)first + threadIdx.x, s);  // sets the flag where it does not fit
+    // (sets the flag for a sequence that does not fit)
+    if (units == 0 && first + threadIdx.x < a.seqs) seq_of(a, (int)first + threadIdx.x, s);
     clear_rows<D>(a, first);
     return;
   }
@@ -799,8 +801,8 @@ __global__ void __launch_bounds__(256) kv_attn_dealt_join_kernel(AttnArgs a) {
 // Tiles are converted once on their way into LDS, in the softmax phase, their loads a phase earlier: K as rows by the
 // first group, V transposed by the second, its keys in the order in which the first product leaves P.
 // Bound by the softmax phase: two prompts of 3,500 to 4,500 tokens behind 3,000 to 5,000 (32 query heads, 8 key heads of 128)
-// 752 to 795 us by the card, 0.97 to 1.03 PFLOP/s, where a bf16 product of 8,192^3 reaches 1.37.  The matrix units are busy
-// 45 % of the time and the vector units as long; a tile's products take 1,024 cycles of a wave at best, its softmax about 1,400
+// 786 to 809 us by the card, 0.96 to 0.98 PFLOP/s, where a bf16 product of 8,192^3 reaches 1.37.  The matrix units are busy
+// 44 % of the time and the vector units as long; a tile's products take 1,024 cycles of a wave at best, its softmax about 1,400
 // (512 of them exponentials) and staging 500.  Tried on it: loads in the softmax phase (854 us against 796), staging between
 // the products (857 against 834), priority for either phase (no change or 3 % slower).
 template <int D, int KT>
@@ -1342,8 +1344,9 @@ Plan plan_of(const pdm_kv_attention_desc* d, const pdm_kv_cache* c, const pdm_kv
   const int64_t pairs = (int64_t)b->num_seqs * c->n_kv_heads;
   const int64_t cap = (most + kFewStep - 1) / kFewStep;  // steps of a pair
   const int resident = 256 * (c->head_dim * p.mt <= 64 ? 4 : c->head_dim * p.mt <= 128 ? 3 : 2);
-  // Dealt where there are pairs enough that an uneven batch leaves CUs idle, and rows so few that partial results stay small;
-  // with 2,048 pairs and more the hardware's own order does as well, and longer rows would write more than they save.
+  // Dealt between the limits that it was made for and measured within (see few_deal): a sequence per thread, a pair for each CU
+  // and more, up to eight times that, and partial results of 8 rows, two of each workgroup.  Outside them a batch gets equal
+  // splits, or none from 1,024 pairs on, whatever its contexts; how much an uneven one loses by that has not been measured.
   p.workers = p.few && b->num_seqs > 1 && b->num_seqs <= kDealt && pairs >= 256 && pairs < 2048 && rows <= 8 && pairs * cap > resident
                   ? resident : 0;
   // else equal splits, as many as fill the CUs once: a second round of workgroups would only add joins

@@ -180,7 +180,8 @@ def kv_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, 
     sum of exponentials [T, Hq].  Rows that see no key and rows behind the last sequence are zeros, with lse -inf.
 
     ``max_q_len``: the most new tokens that any sequence has, where the program knows it (1 when decoding); a sequence
-    with more is left out and sets ``err_flag``.  Slice ``page_table`` to the columns that the longest sequence needs: its
+    with more is left out and sets ``err_flag``.  Without it the work is laid out for any share of the rows, and a decoding
+    batch takes up to half as long again.  Slice ``page_table`` to the columns that the longest sequence needs: its
     width bounds the lengths the work is laid out for."""
     _no_grad("kv_attention", q, k_codes, v_codes, k_scale, v_scale, out)
     q = _heads(q)

@@ -1173,7 +1173,9 @@ def kv_attention_raw(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tens
                      max_q_len: Optional[int] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None,
                      err_flag: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Launches pdm_kv_attention_fwd on q [T, Hq, D]; returns (out, lse or None).  ``max_q_len``: no sequence has more
-    new tokens (default: T, which costs a second launch and idle blocks)."""
+    new tokens.  Default: T, as if one sequence might have them all; a batch of single tokens then gets equal splits of the
+    keys instead of dealt ones (83 us instead of 54 for 64 ragged contexts of 128 to 8,192, 8 key heads of 128) and a launch
+    for many rows that finds none."""
     cache = _kv_cache_desc(k_codes, v_codes, k_scale, v_scale)
     T, hq, D, q_st, q_sh, code = _check_heads("q", q)
     if code == L.PDM_F32:
