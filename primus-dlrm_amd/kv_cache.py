@@ -21,6 +21,7 @@ from typing import Optional, Tuple
 import torch
 import torch.nn as nn
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import ops
 from .onetrans import RMSNorm
@@ -49,12 +50,13 @@ def _heads(t: torch.Tensor) -> torch.Tensor:
 
 def _traced(t: torch.Tensor, direct: bool = False) -> bool:
     """True where a call has to be seen by the dispatcher: in compiled and traced graphs, for tensors without memory (fake, meta)
-    or with a dispatch of their own, and under a dispatch mode unless ``direct`` (the call has an argument that the registered
-    operator has not)."""
+    or with a dispatch of their own, and under a dispatch mode.  ``direct``: the call has an argument that the registered
+    operator has not; a mode that records no graph then does without it."""
     if torch.compiler.is_compiling() or isinstance(t, torch.fx.Proxy):
         return True
-    return (t.is_meta or type(t).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__ or torch._C._is_tracing()
-            or (torch._C._len_torch_dispatch_stack() > 0 and not direct))
+    if t.is_meta or type(t).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__ or torch._C._is_tracing():
+        return True
+    return torch._C._len_torch_dispatch_stack() > 0 and not (direct and get_proxy_mode() is None)
 
 
 def _no_tangent(name: str, *tensors: Optional[torch.Tensor]) -> None:

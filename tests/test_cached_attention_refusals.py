@@ -294,3 +294,25 @@ def test_module_that_was_made_without_memory(pdm):
         assert m.cos.device.type == "cpu" and torch.equal(m.cos, want[0]) and torch.equal(m.sin, want[1])
         m.load_state_dict(pdm.QKNormRope(64, 10, rotary_dim=32).state_dict())
         assert m.q_norm.weight.dtype == dtype and torch.equal(m.to(torch.float64).cos, want[0])
+
+
+@pytest.mark.parametrize("mode", ["real", "fake"])
+def test_arguments_that_a_recorded_graph_would_lose(pdm, mode):
+    """A given output and the flag of qk_norm_rope are not arguments of the registered operators: a graph that is being recorded
+    refuses them, where it would come out without the call."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    a = dict(q=torch.zeros(3, 4, 64, dtype=torch.bfloat16), **_cache(), **_batch())
+    out, r = torch.zeros(3, 4, 64, dtype=torch.bfloat16), _rope()
+    flag = torch.zeros(1, dtype=torch.int32)
+
+    def attend(q, out):
+        return pdm.kv_attention(**{**a, "q": q}, out=out)
+
+    def turn(q, flag):
+        return pdm.qk_norm_rope(**{**r, "q": q}, err_flag=flag)
+
+    with pytest.raises(ValueError, match="traced graph"):
+        make_fx(attend, tracing_mode=mode)(a["q"], out)
+    with pytest.raises(ValueError, match="traced graph"):
+        make_fx(turn, tracing_mode=mode)(r["q"], flag)
