@@ -698,6 +698,89 @@ int pdm_kv_attention_fwd(const pdm_kv_attention_desc* desc,
                          int64_t workspace_bytes, int32_t* err_flag,
                          pdm_stream_t stream);
 
+/* Attention of a ragged batch whose keys and values are tensors beside it (as in
+ * training), forward and backward.  Sequence b's queries are rows cu_q[b] ..
+ * cu_q[b + 1] of q, its keys and values rows cu_k[b] .. cu_k[b + 1] of k and v;
+ * query i of n_q stands at position p = n_k - n_q + i of its n_k keys.  It sees
+ * the keys j with j <= p (causal) and, with window > 0, j > p - window or
+ * j < sinks.  Its score of key j is
+ *   scale * q . k_j + bias[h][c],  c = p - j - bias_start held within [0, bias_span)
+ * Tokens < 2^30, tokens * heads < 2^31, num_seqs <= 2^24. */
+typedef struct {
+  int32_t dtype;      /* PDM_F16 | PDM_BF16: q, k, v, out and their gradients */
+  int32_t n_q_heads;  /* a multiple of n_kv_heads, at most 65535 */
+  int32_t n_kv_heads;
+  int32_t head_dim;   /* 64 or 128 */
+  int32_t num_seqs;
+  int32_t causal;
+  int32_t window;     /* 0: none */
+  int32_t sinks;
+  int32_t bias_start; /* distance of the first column */
+  int32_t bias_span;  /* columns; 0: no bias */
+  float scale;
+  int32_t reserved;
+  int64_t q_tokens, k_tokens;     /* rows of q; of k and v */
+  int64_t q_stride_t, q_stride_h; /* element (t, h, d) of q at q[t * q_stride_t + h * q_stride_h + d] */
+  int64_t k_stride_t, k_stride_h;
+  int64_t v_stride_t, v_stride_h;
+} pdm_jagged_attention_desc;
+
+/* out: contiguous [q_tokens, n_q_heads, head_dim], 16-byte aligned.
+ * bias: fp32 [n_q_heads, bias_span].
+ * lse: optional fp32 [q_tokens, n_q_heads], log of the sum of exponentials.
+ * For the backward pass: stats, fp32 [q_tokens, n_q_heads, 2], and, where the
+ * bias's gradient is wanted, out_rest (as out: what its rounding left).
+ * A row that sees no key, and a row that no sequence covers, is zeros with lse
+ * -inf; so is one whose scores are all -inf.  Keys and values that a query does
+ * not see do not reach it, whatever they hold.  Spans that decrease or leave
+ * the batch set err_flag (optional device int32); outputs then hold nothing of
+ * use.  Scores, softmax and sums are fp32; weights are rounded to dtype for
+ * their product (not with out_rest, where their remainders follow).
+ * workspace: 256-byte aligned, no initialisation needed. */
+int64_t pdm_jagged_attention_workspace_size(const pdm_jagged_attention_desc* desc);
+
+int pdm_jagged_attention_fwd(const pdm_jagged_attention_desc* desc,
+                             const void* q, const void* k, const void* v,
+                             const int32_t* cu_q, const int32_t* cu_k,
+                             const float* bias, void* out, void* out_rest,
+                             float* lse, float* stats, void* workspace,
+                             int64_t workspace_bytes, int32_t* err_flag,
+                             pdm_stream_t stream);
+
+/* Gradients of q, k, v (contiguous, 16-byte aligned, rows that nothing reaches
+ * are zeros) and, where grad_bias is not NULL, of the bias (fp32, summed over
+ * sequences and pairs).  out, out_rest (with grad_bias), stats: of the forward
+ * pass; grad_out: contiguous, 16-byte aligned; grad_lse: optional, of lse.  Sums
+ * run in one fixed order: the same inputs give the same bits.
+ * |bias_start| < 2^30. */
+int64_t pdm_jagged_attention_bwd_workspace_size(const pdm_jagged_attention_desc* desc, int32_t with_grad_bias);
+
+int pdm_jagged_attention_bwd(const pdm_jagged_attention_desc* desc,
+                             const void* q, const void* k, const void* v,
+                             const int32_t* cu_q, const int32_t* cu_k,
+                             const float* bias, const void* out,
+                             const void* out_rest, const float* stats,
+                             const void* grad_out, const float* grad_lse,
+                             void* grad_q, void* grad_k, void* grad_v,
+                             float* grad_bias, void* workspace,
+                             int64_t workspace_bytes, pdm_stream_t stream);
+
+/* A table of buckets spread over distances: out[h][c] = table[buckets[c]][h]
+ * (fp32; 0 where the bucket lies outside [0, num_buckets)), and its gradient
+ * grad_table[b][h] = sum over c with buckets[c] = b of grad_out[h][c], summed in
+ * one fixed order and rounded once to dtype (PDM_F32 | PDM_F16 | PDM_BF16).
+ * table: contiguous [num_buckets, heads]; buckets: int32 [span];
+ * num_buckets <= 8192, heads <= 65535, span <= 2^24. */
+int pdm_bucket_bias_fwd(const void* table, int32_t dtype, int32_t num_buckets,
+                        int32_t heads, const int32_t* buckets, int32_t span,
+                        float* out, pdm_stream_t stream);
+
+/* workspace: 8 * num_buckets bytes, 4-byte aligned, no initialisation needed. */
+int pdm_bucket_bias_bwd(const float* grad_out, const int32_t* buckets,
+                        int32_t span, int32_t num_buckets, int32_t heads,
+                        int32_t dtype, void* grad_table, void* workspace,
+                        int64_t workspace_bytes, pdm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

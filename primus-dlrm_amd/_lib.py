@@ -70,6 +70,12 @@ EXPORTED_SYMBOLS = (
     "pdm_kv_append",
     "pdm_kv_attention_workspace_size",
     "pdm_kv_attention_fwd",
+    "pdm_jagged_attention_workspace_size",
+    "pdm_jagged_attention_fwd",
+    "pdm_jagged_attention_bwd_workspace_size",
+    "pdm_jagged_attention_bwd",
+    "pdm_bucket_bias_fwd",
+    "pdm_bucket_bias_bwd",
 )
 
 
@@ -257,6 +263,31 @@ class KvAttentionDesc(ctypes.Structure):
     ]
 
 
+class JaggedAttentionDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("n_q_heads", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("num_seqs", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+        ("bias_start", ctypes.c_int32),
+        ("bias_span", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("q_tokens", ctypes.c_int64),
+        ("k_tokens", ctypes.c_int64),
+        ("q_stride_t", ctypes.c_int64),
+        ("q_stride_h", ctypes.c_int64),
+        ("k_stride_t", ctypes.c_int64),
+        ("k_stride_h", ctypes.c_int64),
+        ("v_stride_t", ctypes.c_int64),
+        ("v_stride_h", ctypes.c_int64),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -345,6 +376,18 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.pdm_kv_attention_fwd.restype = ctypes.c_int
     lib.pdm_kv_attention_fwd.argtypes = [ctypes.POINTER(KvAttentionDesc), ctypes.POINTER(KvCacheDesc),
                                          ctypes.POINTER(KvBatchDesc), vp, vp, vp, vp, i64, vp, vp]
+    lib.pdm_jagged_attention_workspace_size.restype = i64
+    lib.pdm_jagged_attention_workspace_size.argtypes = [ctypes.POINTER(JaggedAttentionDesc)]
+    lib.pdm_jagged_attention_fwd.restype = ctypes.c_int
+    lib.pdm_jagged_attention_fwd.argtypes = [ctypes.POINTER(JaggedAttentionDesc)] + [vp] * 11 + [i64, vp, vp]
+    lib.pdm_jagged_attention_bwd_workspace_size.restype = i64
+    lib.pdm_jagged_attention_bwd_workspace_size.argtypes = [ctypes.POINTER(JaggedAttentionDesc), i32]
+    lib.pdm_jagged_attention_bwd.restype = ctypes.c_int
+    lib.pdm_jagged_attention_bwd.argtypes = [ctypes.POINTER(JaggedAttentionDesc)] + [vp] * 16 + [i64, vp]
+    lib.pdm_bucket_bias_fwd.restype = ctypes.c_int
+    lib.pdm_bucket_bias_fwd.argtypes = [vp, i32, i32, i32, vp, i32, vp, vp]
+    lib.pdm_bucket_bias_bwd.restype = ctypes.c_int
+    lib.pdm_bucket_bias_bwd.argtypes = [vp, vp, i32, i32, i32, i32, vp, vp, i64, vp]
     lib.pdm_cross_hash_fwd.restype = ctypes.c_int
     lib.pdm_cross_hash_fwd.argtypes = [ctypes.POINTER(vp), ctypes.POINTER(i64), i32, i64, ctypes.c_uint64,
                                        ctypes.c_uint64, vp, vp]

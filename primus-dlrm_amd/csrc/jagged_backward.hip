@@ -1,0 +1,527 @@
+// Attention of ragged batches, backward, without atomics on memory: the same inputs give the same bits.
+//
+// With P the weights, dP = dO V^T and delta = rowsum(dO O) = rowsum(P dP):
+//   dS = P (dP - delta),  dV = P^T dO,  dQ = scale dS K,  dK = scale dS^T Q,  dbias[c] = sum of dS over the pairs of column c.
+// Two kernels compute S and dP again, one by blocks of queries (dQ, delta, the bias's gradient), one by blocks of keys (dK, dV):
+// 7 products where one kernel would need 5 and sums of dQ over its workgroups.  In both a lane holds scores of one column (a
+// query, a key) and passes them on to the next product as the first leaves them.
+//
+// P and dS are rounded to the type of the operands for their products; the bias's gradient takes dS in 32 bits.  fp16 would
+// lose small dS (below 2^-14): its dS are multiplied by a power of two that brings dO to 2^-6, of each query for dQ, and of
+// 32 queries for dK, whose sums so far are brought to it.  (What is not finite does not count.)
+#include <type_traits>
+
+#include "jagged_common.h"
+
+namespace pdm {
+
+int jag_args(const char* fn, const pdm_jagged_attention_desc* d, JagArgs& a);
+int jag_inputs(const char* fn, JagArgs& a, const pdm_jagged_attention_desc* d, const void* q, const void* k, const void* v,
+               const int32_t* cu_q, const int32_t* cu_k, const float* bias);
+
+namespace {
+
+constexpr int M = 128, KT = 64;
+constexpr int kOut = -5;     // |dO| below 2^kOut after its power of two
+constexpr int kNone = -100;  // exponent of rows of zeros
+
+__device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
+
+// ---- by queries -----------------------------------------------------------------------
+// Gradients of the bias: a wave adds its dS of a tile to a window of 95 distances in LDS, the two halves of the wave to one
+// each, so that no two lanes of an instruction meet.  Distances fall from tile to tile, and a thread sums those that are its
+// number modulo 256 and writes each once, when the tiles have passed it.
+template <int DT, int D, bool BIAS, bool GB>
+__global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units) {
+  constexpr int KK = D / 16, DD = D / 32;
+  __shared__ alignas(1024) char sk[2][KT * Tile<D>::RS];
+  __shared__ alignas(1024) char sv[2][KT * Tile<D>::RS];
+  __shared__ float sb[2][BIAS ? M + KT : 1];
+  __shared__ float win[2][GB ? 4 : 1][2][GB ? 96 : 1];
+  __shared__ float ends[GB ? 8 : 1];
+
+  const int64_t unit = linear_block();
+  if (unit >= units) {
+    const int64_t first = (unit - units) * 256;
+    if (first >= a.q_tokens && first >= a.seqs) return;
+    jag_guard(a, a.cu_q, a.q_tokens, first, [&](int64_t t) { clear_row(a.dq, t * a.hq * D, a.hq * D); });
+    return;
+  }
+  const int hx = (int)(unit % a.hq), kh = hx % a.hk, head = kh * a.group + hx / a.hk;
+  const int64_t item = a.items - 1 - unit / a.hq;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  JagSeq s;
+  int b, r0;
+  if (!jag_block<M>(a, a.cu_q, item, s, b, r0)) {
+    if (GB && hx == 0 && tid == 0) a.part_range[2 * item] = 1, a.part_range[2 * item + 1] = 0;
+    return;
+  }
+  const int c = lane & 31, h = lane >> 5;
+  const int off = s.nk - s.nq;
+  const JagKeys keys = jag_keys<KT>(a, s, r0, (r0 + M < s.nq ? r0 + M : s.nq) - 1);
+
+  const int row = r0 + wave * 32 + c, pos = off + row;
+  const bool there = row < s.nq;
+  const int64_t at = (s.q0 + row) * a.hq + head;
+  int row_lo = 0, row_n = 0, row_first = 0;
+  u32x4_t q[KK], g[KK];
+  float delta = 0.0f, most = 0.0f, m = 0.0f, inv = 0.0f;
+  {
+    const uint16_t* x = static_cast<const uint16_t*>(a.q) + (s.q0 + row) * a.q_st + head * a.q_sh + 8 * h;
+    const uint16_t *y = static_cast<const uint16_t*>(a.dout) + at * D + 8 * h, *z = static_cast<const uint16_t*>(a.out) + at * D + 8 * h;
+    const uint16_t* r = static_cast<const uint16_t*>(a.rest) + at * D + 8 * h;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      q[kk] = load16(x + 16 * kk, there);
+      g[kk] = load16(y + 16 * kk, there);
+      const u32x4_t o = load16(z + 16 * kk, there);
+      u32x4_t o2 = {0, 0, 0, 0};
+      if (GB) o2 = load16(r + 16 * kk, there);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float lo = lo_of<DT>(g[kk][e]), hi = hi_of<DT>(g[kk][e]);
+        delta = __builtin_fmaf(lo, lo_of<DT>(o[e]), delta);
+        delta = __builtin_fmaf(hi, hi_of<DT>(o[e]), delta);
+        if (GB) {
+          delta = __builtin_fmaf(lo, lo_of<DT>(o2[e]), delta);
+          delta = __builtin_fmaf(hi, hi_of<DT>(o2[e]), delta);
+        }
+        if (DT == PDM_F16) most = fmaxf(most, fmaxf(fabsf(lo) < kInf ? fabsf(lo) : 0.0f, fabsf(hi) < kInf ? fabsf(hi) : 0.0f));
+      }
+    }
+    delta += __shfl_xor(delta, 32);
+  }
+  float back = a.scale, ahead = 1.0f;  // fp16: the row's power of two
+  if (DT == PDM_F16) {
+    most = fmaxf(most, __shfl_xor(most, 32));
+    const int e = most > 0.0f ? __builtin_amdgcn_frexp_expf(most) : kNone;
+    const int of = (int)group_max((float)e, 64);
+    if (lane == 0 && r0 + wave * 32 < s.nq) a.expo[(item * 4 + wave) * a.hq + head] = of;
+    if (e != kNone) ahead = pow2(kOut - e), back = a.scale * pow2(e - kOut);
+  }
+  if (there) {
+    const int hi = a.causal && pos + 1 < s.nk ? (pos + 1 > 0 ? pos + 1 : 0) : s.nk;
+    row_lo = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
+    row_n = hi > row_lo ? hi - row_lo : 0;
+    row_first = a.sinks < hi ? a.sinks : hi;
+    m = a.stats[2 * at], inv = a.stats[2 * at + 1];
+    if (a.dlse) delta -= a.dlse[at];  // d lse / d s = P
+    if (h == 0) a.delta[at] = delta;
+  }
+  const int w0 = r0 + wave * 32, p_first = off + w0, p_last = off + (w0 + 31 < s.nq ? w0 + 31 : s.nq - 1);
+
+  const uint16_t* kp = static_cast<const uint16_t*>(a.k) + s.k0 * a.k_st + kh * a.k_sh;
+  const uint16_t* vp = static_cast<const uint16_t*>(a.v) + s.k0 * a.v_st + kh * a.v_sh;
+  const float* brow = BIAS ? a.bias + (int64_t)head * (a.bias_last + 1) : nullptr;
+  Bring<D, KT> bring_k, bring_v;
+  bring_k.init(a.k_st, lane, wave);
+  bring_v.init(a.v_st, lane, wave);
+  float bias_next = 0.0f;
+  auto load = [&](int t) {
+    const int key = jag_key<KT>(keys, t);
+    bring_k.load(kp, a.k_st, key, s.nk, sk[t & 1], wave);
+    bring_v.load(vp, a.v_st, key, s.nk, sv[t & 1], wave);
+    if (BIAS && tid < M + KT) bias_next = bias2(a, brow, (int64_t)off + r0 + tid - (KT - 1) - key);
+  };
+
+  // the bias's gradient: columns 0 .. cols - 1 of the partial result, then what lies behind them and before them
+  const int cols = (int)a.part_stride - 2;
+  float* part = GB ? a.part + (item * a.hq + head) * a.part_stride : nullptr;
+  float far = 0.0f, near = 0.0f, sum = 0.0f;
+  int mine = 0;  // the distance that this thread sums
+  auto put = [&](int d, float v) {
+    const int x = d - a.bias_start;
+    if (x >= 0 && x < cols) part[x] = v;
+  };
+  auto gather = [&](int t) {  // the windows of tile t
+    const int base = off + r0 - jag_key<KT>(keys, t) - (KT - 1), rel = (tid - base) & 255;
+    if (t == 0) {
+      mine = base + rel;
+    } else if (mine != base + rel) {
+      put(mine, sum);
+      for (mine -= 256; mine > base + rel; mine -= 256) put(mine, 0.0f);
+      sum = 0.0f;
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int x = rel - 32 * w;
+      if (x >= 0 && x < 95) {
+        sum += win[t & 1][w][0][x] + win[t & 1][w][1][x];
+        win[t & 1][w][0][x] = 0.0f, win[t & 1][w][1][x] = 0.0f;
+      }
+    }
+  };
+  if (GB) {
+    float* w = &win[0][0][0][0];
+    for (int i = tid; i < 2 * 4 * 2 * 96; i += 256) w[i] = 0.0f;
+    if (hx == 0 && tid == 0) {
+      a.part_range[2 * item] = keys.tiles ? off + r0 - jag_key<KT>(keys, keys.tiles - 1) - (KT - 1) : 1;
+      a.part_range[2 * item + 1] = keys.tiles ? off + r0 - jag_key<KT>(keys, 0) + M - 1 : 0;
+    }
+  }
+
+  constexpr f32x16_t zero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+  f32x16_t dq[DD];
+#pragma unroll
+  for (int d = 0; d < DD; ++d) dq[d] = zero16;
+  const uint32_t row_at = Tile<D>::row_at(lane), col_at = Tile<D>::col_at(lane);
+
+  if (keys.tiles > 0) load(0);
+#pragma unroll 1
+  for (int t = 0; t < keys.tiles; ++t) {
+    const int key = jag_key<KT>(keys, t);
+    if (BIAS && tid < M + KT) sb[t & 1][tid] = bias_next;
+    brought();
+    lds_barrier();  // the tile is there, and the one before it is done with
+    if (t + 1 < keys.tiles) load(t + 1);
+    if (GB && t > 0) gather(t - 1);
+    if (w0 >= s.nq || (a.causal && key > p_last) || (a.window > 0 && key + KT - 1 <= p_first - a.window && key >= a.sinks)) continue;
+    const char *tk = sk[t & 1], *tv = sv[t & 1];
+    const bool whole = key + KT <= s.nk && (!a.causal || key + KT - 1 <= p_first) &&
+                       (a.window == 0 || key > p_last - a.window || key + KT <= a.sinks);
+    auto sees = [&](int j) { return (uint32_t)(key + j - row_lo) < (uint32_t)row_n || key + j < row_first; };
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      f32x16_t sc = zero16, dp = zero16;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) sc = mfma32<DT>(Tile<D>::rows(tk, row_at, 32 * x, kk), q[kk], sc);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) dp = mfma32<DT>(Tile<D>::rows(tv, row_at, 32 * x, kk), g[kk], dp);
+      float ds[16];
+      const int local = c - 32 * x - 4 * h + KT - 1;  // of the window of a wave, less 8 (e / 4) + e % 4
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int j = 8 * (e >> 2) + (e & 3);
+        const float w = BIAS ? __builtin_fmaf(sc[e], a.scale2, sb[t & 1][wave * 32 + local - j]) : sc[e] * a.scale2;
+        const float p = __builtin_amdgcn_exp2f(w - m) * inv;
+        ds[e] = p * (dp[e] - delta);
+      }
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) ds[e] = sees(32 * x + 4 * h + 8 * (e >> 2) + (e & 3)) ? ds[e] : 0.0f;
+      }
+      if (GB) {
+        const int first = p_first - key - 32 * x - 31 - a.bias_start, last = first + 62;  // columns of the wave's pairs
+        const int col = pos - key - 32 * x - 4 * h - a.bias_start;
+        float* wp = &win[t & 1][wave][h][0];
+        if (first >= a.bias_last) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) far += ds[e];
+        } else if (last < 0) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) near += ds[e];
+        } else if (first >= 0 && last < a.bias_last) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            __hip_atomic_fetch_add(wp + local - 8 * (e >> 2) - (e & 3), ds[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int j = 8 * (e >> 2) + (e & 3), x = col - j;
+            if (x >= a.bias_last) far += ds[e];
+            else if (x < 0) near += ds[e];
+            else __hip_atomic_fetch_add(wp + local - j, ds[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          }
+        }
+      }
+      u32x4_t w[2];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e >> 2][e & 3] = DT == PDM_F16 ? pack2<DT>(ds[2 * e] * ahead, ds[2 * e + 1] * ahead) : pack2<DT>(ds[2 * e], ds[2 * e + 1]);
+      if (!whole && odd_rows<DT, D, 2>(tk, col_at, 32 * x)) add_cols_odd<DT, D, 2, false>(dq, tk, col_at, 32 * x, w, sees);
+      else add_cols<DT, D, 2>(dq, tk, col_at, 32 * x, w);
+    }
+  }
+  if (GB) {
+    __syncthreads();
+    if (keys.tiles > 0) {
+      gather(keys.tiles - 1);
+      put(mine, sum);
+    }
+    far = group_sum(far, 64), near = group_sum(near, 64);
+    if (lane == 0) ends[wave] = far, ends[4 + wave] = near;
+    __syncthreads();
+    if (tid < 2) part[cols + tid] = (ends[4 * tid] + ends[4 * tid + 1]) + (ends[4 * tid + 2] + ends[4 * tid + 3]);
+  }
+  if (!there) return;
+#pragma unroll
+  for (int d = 0; d < DD; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4)
+      *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.dq) + at * D + 32 * d + 2 * e + 4 * h) =
+          u32x2_t{pack2<DT>(dq[d][e] * back, dq[d][e + 1] * back), pack2<DT>(dq[d][e + 2] * back, dq[d][e + 3] * back)};
+}
+
+// Sums the partial gradients of a column over the blocks of queries, in 64 bits: a lane per column, the blocks dealt to 16 waves.
+__global__ void __launch_bounds__(1024) jag_dbias_kernel(JagArgs a) {
+  __shared__ double part[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cols = (int)a.part_stride - 2;
+  const int head = blockIdx.y, col = blockIdx.x * 64 + lane;
+  double sum = 0.0;
+  for (int64_t i = wave; i < a.items; i += 16) {
+    const int lo = a.part_range[2 * i], hi = a.part_range[2 * i + 1];
+    if (lo > hi) continue;
+    const float* p = a.part + (i * a.hq + head) * a.part_stride;
+    const int64_t d = (int64_t)col + a.bias_start;
+    if (col < cols && col < a.bias_last && d >= lo && d <= hi) sum += p[col];
+    if (col == a.bias_last) sum += p[cols];
+    if (col == 0) sum += p[cols + 1];
+  }
+  part[wave][lane] = sum;
+  __syncthreads();
+  if (wave || col > a.bias_last) return;
+  for (int w = 1; w < 16; ++w) sum += part[w][lane];
+  a.dbias[(int64_t)head * (a.bias_last + 1) + col] = (float)sum;
+}
+
+// ---- by keys ----------------------------------------------------------------------------
+template <int DT, int D, bool BIAS>
+__global__ void __launch_bounds__(256, D == 64 ? 2 : 1) jag_dkv_kernel(JagArgs a, int64_t items, int64_t units) {
+  constexpr int KK = D / 16, DD = D / 32, QT = 64;
+  __shared__ alignas(1024) char sq[2][QT * Tile<D>::RS];
+  __shared__ alignas(1024) char sg[2][QT * Tile<D>::RS];
+  __shared__ float sb[2][BIAS ? M + QT : 1];
+  __shared__ float ss[2][3][QT];
+
+  const int64_t unit = linear_block();
+  if (unit >= units) {
+    const int64_t first = (unit - units) * 256;
+    if (first >= a.k_tokens && first >= a.seqs) return;
+    jag_guard(a, a.cu_k, a.k_tokens, first, [&](int64_t t) {
+      clear_row(a.dk, t * a.hk * D, a.hk * D);
+      clear_row(a.dv, t * a.hk * D, a.hk * D);
+    });
+    return;
+  }
+  const int kh = (int)(unit % a.hk);
+  JagSeq s;
+  int b, j0;
+  if (!jag_block<M>(a, a.cu_k, unit / a.hk, s, b, j0)) return;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, h = lane >> 5;
+  const int off = s.nk - s.nq;
+  // queries that see a key of the block
+  const int j1 = (j0 + M < s.nk ? j0 + M : s.nk) - 1;
+  int i_lo = a.causal && j0 - off > 0 ? (j0 - off) & ~(QT - 1) : 0, i_hi = s.nq;
+  if (a.window > 0 && j0 >= a.sinks && j1 + a.window - off < i_hi) i_hi = j1 + a.window - off;
+  const int tiles = i_hi > i_lo ? (i_hi - i_lo + QT - 1) / QT : 0, all = tiles * a.group;
+
+  // this lane's key and the queries that see it: [see_lo, see_lo + see_n)
+  const int key = j0 + wave * 32 + c;
+  const bool there = key < s.nk;
+  int see_lo = 0, see_n = 0;
+  if (there) {
+    see_lo = a.causal && key - off > 0 ? key - off : 0;
+    const int hi = a.window > 0 && key >= a.sinks && key + a.window - off < s.nq ? key + a.window - off : s.nq;
+    see_n = hi > see_lo ? hi - see_lo : 0;
+  }
+  u32x4_t kf[KK], vf[KK];
+  {
+    const uint16_t* x = static_cast<const uint16_t*>(a.k) + (s.k0 + key) * a.k_st + kh * a.k_sh + 8 * h;
+    const uint16_t* y = static_cast<const uint16_t*>(a.v) + (s.k0 + key) * a.v_st + kh * a.v_sh + 8 * h;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) kf[kk] = load16(x + 16 * kk, there), vf[kk] = load16(y + 16 * kk, there);
+  }
+  const int jw = j0 + wave * 32;
+
+  Bring<D, QT> bring_q, bring_g;
+  const int64_t g_st = (int64_t)a.hq * D;
+  bring_q.init(a.q_st, lane, wave);
+  bring_g.init(g_st, lane, wave);
+  float bias_next = 0.0f, stat_next = 0.0f;
+  int head_next = 0, tile_next = 0;
+  auto load = [&](int n) {  // the head and tile at which the next load stands
+    const int head = kh * a.group + head_next, i = i_lo + tile_next * QT;
+    bring_q.load(static_cast<const uint16_t*>(a.q) + s.q0 * a.q_st + head * a.q_sh, a.q_st, i, s.nq, sq[n & 1], wave);
+    bring_g.load(static_cast<const uint16_t*>(a.dout) + s.q0 * g_st + head * D, g_st, i, s.nq, sg[n & 1], wave);
+    if (BIAS && tid < M + QT) bias_next = bias2(a, a.bias + (int64_t)head * (a.bias_last + 1), (int64_t)off + i + tid - (M - 1) - j0);
+    stat_next = 0.0f;
+    const int r = i + (tid & (QT - 1));
+    if (tid < 3 * QT && r < s.nq) {
+      const int64_t at = (s.q0 + r) * a.hq + head;
+      stat_next = tid < QT ? a.stats[2 * at] : tid < 2 * QT ? a.stats[2 * at + 1] : a.delta[at];
+    }
+    if (++tile_next == tiles) tile_next = 0, ++head_next;
+  };
+
+  constexpr f32x16_t zero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+  f32x16_t dk[DD], dv[DD];
+#pragma unroll
+  for (int d = 0; d < DD; ++d) dk[d] = zero16, dv[d] = zero16;
+  const uint32_t row_at = Tile<D>::row_at(lane), col_at = Tile<D>::col_at(lane);
+  int power = 100;  // fp16: dk holds sums times 2^power
+  const int64_t item0 = (int64_t)a.cu_q[b] / M + b;
+
+  if (all > 0) load(0);
+  int hh = 0, tt = 0;
+#pragma unroll 1
+  for (int n = 0; n < all; ++n) {
+    const int i0 = i_lo + tt * QT, head = kh * a.group + hh;
+    if (++tt == tiles) tt = 0, ++hh;
+    if (BIAS && tid < M + QT) sb[n & 1][tid] = bias_next;
+    if (tid < 3 * QT) ss[n & 1][tid / QT][tid & (QT - 1)] = stat_next;
+    brought();
+    lds_barrier();  // the tile is there, and the one before it is done with
+    if (n + 1 < all) load(n + 1);
+    const char *tq = sq[n & 1], *tg = sg[n & 1];
+#pragma unroll
+    for (int x = 0; x < QT / 32; ++x) {
+      const int i = i0 + 32 * x, p0 = off + i;
+      if (i >= s.nq || jw >= s.nk || (a.causal && p0 + 31 < jw) || (a.window > 0 && p0 >= jw + 31 + a.window && jw >= a.sinks)) continue;
+      const bool whole = i + 32 <= s.nq && jw + 32 <= s.nk && (!a.causal || p0 >= jw + 31) &&
+                         (a.window == 0 || p0 + 31 < jw + a.window || jw + 32 <= a.sinks);
+      auto sees = [&](int r) { return (uint32_t)(i0 + r - see_lo) < (uint32_t)see_n; };
+      f32x16_t sc = zero16, dp = zero16;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) sc = mfma32<DT>(Tile<D>::rows(tq, row_at, 32 * x, kk), kf[kk], sc);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) dp = mfma32<DT>(Tile<D>::rows(tg, row_at, 32 * x, kk), vf[kk], dp);
+      float ahead = 1.0f;
+      if (DT == PDM_F16) {
+        const int want = kOut - a.expo[((item0 + (i >> 7)) * 4 + (i >> 5 & 3)) * a.hq + head];
+        if (want < power) {  // larger gradients than any before
+          const float f = pow2(want - power);
+          power = want;
+#pragma unroll
+          for (int d = 0; d < DD; ++d) dk[d] *= f;
+        }
+        ahead = pow2(power);
+      }
+      float p[16], ds[16];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int r = 32 * x + 8 * y + 4 * h;
+        const f32x4_t m = *reinterpret_cast<const f32x4_t*>(&ss[n & 1][0][r]), inv = *reinterpret_cast<const f32x4_t*>(&ss[n & 1][1][r]);
+        const f32x4_t delta = *reinterpret_cast<const f32x4_t*>(&ss[n & 1][2][r]);
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const int e = 4 * y + z;
+          const float w = BIAS ? __builtin_fmaf(sc[e], a.scale2, sb[n & 1][r + z - wave * 32 - c + M - 1]) : sc[e] * a.scale2;
+          p[e] = __builtin_amdgcn_exp2f(w - m[z]) * inv[z];
+          ds[e] = p[e] * (dp[e] - delta[z]);
+        }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const bool ok = sees(32 * x + 4 * h + 8 * (e >> 2) + (e & 3));
+          p[e] = ok ? p[e] : 0.0f, ds[e] = ok ? ds[e] : 0.0f;
+        }
+      }
+      u32x4_t pw[2], dw[2];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        pw[e >> 2][e & 3] = pack2<DT>(p[2 * e], p[2 * e + 1]);
+        dw[e >> 2][e & 3] = DT == PDM_F16 ? pack2<DT>(ds[2 * e] * ahead, ds[2 * e + 1] * ahead) : pack2<DT>(ds[2 * e], ds[2 * e + 1]);
+      }
+      if (!whole && odd_rows<DT, D, 2>(tg, col_at, 32 * x)) add_cols_odd<DT, D, 2, false>(dv, tg, col_at, 32 * x, pw, sees);
+      else add_cols<DT, D, 2>(dv, tg, col_at, 32 * x, pw);
+      if (!whole && odd_rows<DT, D, 2>(tq, col_at, 32 * x)) add_cols_odd<DT, D, 2, false>(dk, tq, col_at, 32 * x, dw, sees);
+      else add_cols<DT, D, 2>(dk, tq, col_at, 32 * x, dw);
+    }
+  }
+  if (!there) return;
+  const float back = DT == PDM_F16 ? a.scale * pow2(-power) : a.scale;
+  const int64_t at = ((s.k0 + key) * a.hk + kh) * D;
+#pragma unroll
+  for (int d = 0; d < DD; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int64_t x = at + 32 * d + 2 * e + 4 * h;
+      *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.dv) + x) = u32x2_t{pack2<DT>(dv[d][e], dv[d][e + 1]), pack2<DT>(dv[d][e + 2], dv[d][e + 3])};
+      *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.dk) + x) =
+          u32x2_t{pack2<DT>(dk[d][e] * back, dk[d][e + 1] * back), pack2<DT>(dk[d][e + 2] * back, dk[d][e + 3] * back)};
+    }
+}
+
+// ---- host -------------------------------------------------------------------------------
+int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
+
+// Columns of a partial gradient of the bias: those that a distance of the batch may reach, but for the last.
+int64_t part_cols(const JagArgs& a) {
+  const int64_t reach = a.k_tokens - a.bias_start;
+  return reach < 0 ? 0 : reach < a.bias_last ? reach : a.bias_last;
+}
+
+struct Space {
+  int64_t delta, expo, range, part, total;
+};
+Space space_of(const JagArgs& a, int dtype, bool gb) {
+  Space s{};
+  s.expo = round256(a.q_tokens * a.hq * 4);
+  s.range = s.expo + round256(dtype == PDM_F16 ? a.items * 16 * a.hq : 0);
+  s.part = s.range + round256(gb ? a.items * 8 : 0);
+  s.total = s.part + round256(gb ? a.items * a.hq * (part_cols(a) + 2) * 4 : 0);
+  return s;
+}
+
+template <int DT, int D, bool BIAS>
+void launch(const JagArgs& a, hipStream_t st) {
+  if (a.q_tokens > 0) {
+    const int64_t units = a.items * a.hq, most = a.q_tokens > a.seqs ? a.q_tokens : a.seqs;
+    const dim3 grid = linear_grid(units + (most + 255) / 256);
+    if constexpr (BIAS) {
+      if (a.dbias) jag_dq_kernel<DT, D, true, true><<<grid, 256, 0, st>>>(a, units);
+      else jag_dq_kernel<DT, D, true, false><<<grid, 256, 0, st>>>(a, units);
+    } else {
+      jag_dq_kernel<DT, D, false, false><<<grid, 256, 0, st>>>(a, units);
+    }
+  }
+  if (a.dbias) jag_dbias_kernel<<<dim3(a.bias_last / 64 + 1, a.hq), 1024, 0, st>>>(a);
+  if (a.k_tokens > 0) {
+    const int64_t items = a.seqs ? a.k_tokens / M + a.seqs : 0, units = items * a.hk, most = a.k_tokens > a.seqs ? a.k_tokens : a.seqs;
+    jag_dkv_kernel<DT, D, BIAS><<<linear_grid(units + (most + 255) / 256), 256, 0, st>>>(a, items, units);
+  }
+}
+
+}  // namespace
+}  // namespace pdm
+
+using namespace pdm;
+
+extern "C" int64_t pdm_jagged_attention_bwd_workspace_size(const pdm_jagged_attention_desc* desc, int32_t with_grad_bias) {
+  clear_error();
+  JagArgs a{};
+  if (int e = jag_args(__func__, desc, a)) return e;
+  PDM_CHECK_ARG(!with_grad_bias || desc->bias_span > 0, "grad_bias without a bias");
+  return space_of(a, desc->dtype, with_grad_bias != 0).total;
+}
+
+extern "C" int pdm_jagged_attention_bwd(const pdm_jagged_attention_desc* desc, const void* q, const void* k, const void* v,
+                                        const int32_t* cu_q, const int32_t* cu_k, const float* bias, const void* out,
+                                        const void* out_rest, const float* stats, const void* grad_out, const float* grad_lse, void* grad_q,
+                                        void* grad_k, void* grad_v, float* grad_bias, void* workspace, int64_t workspace_bytes,
+                                        pdm_stream_t stream) {
+  clear_error();
+  JagArgs a{};
+  if (int e = jag_args(__func__, desc, a)) return e;
+  if (int e = jag_inputs(__func__, a, desc, q, k, v, cu_q, cu_k, bias)) return e;
+  PDM_CHECK_ARG(a.q_tokens == 0 || (out && stats && grad_out && grad_q), "null out / stats / grad_out / grad_q");
+  PDM_CHECK_ARG(a.k_tokens == 0 || (grad_k && grad_v), "null grad_k / grad_v");
+  PDM_CHECK_ARG(!grad_bias || (bias && (a.q_tokens == 0 || out_rest)), "grad_bias without bias or out_rest");
+  for (const void* p : {out, out_rest, grad_out, (const void*)grad_q, (const void*)grad_k, (const void*)grad_v})
+    PDM_CHECK_ARG((reinterpret_cast<uintptr_t>(p) & 15) == 0, "outputs and their gradients must be 16-byte aligned");
+  const Space sp = space_of(a, desc->dtype, grad_bias != nullptr);
+  if (sp.total && (!workspace || workspace_bytes < sp.total)) {
+    set_error(std::string(__func__) + ": workspace of " + std::to_string(sp.total) + " bytes needed");
+    return PDM_ERR_WORKSPACE;
+  }
+  PDM_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "workspace must be 256-byte aligned");
+  char* ws = static_cast<char*>(workspace);
+  a.out = const_cast<void*>(out), a.rest = const_cast<void*>(out_rest), a.stats = const_cast<float*>(stats);
+  a.dout = grad_out, a.dlse = grad_lse, a.dq = grad_q, a.dk = grad_k, a.dv = grad_v, a.dbias = grad_bias;
+  a.delta = reinterpret_cast<float*>(ws), a.expo = reinterpret_cast<int32_t*>(ws + sp.expo);
+  a.part_range = reinterpret_cast<int32_t*>(ws + sp.range), a.part = reinterpret_cast<float*>(ws + sp.part);
+  a.part_stride = grad_bias ? part_cols(a) + 2 : 0;
+  if (a.q_tokens == 0 && grad_bias) a.items = 0;  // nothing was written that could be summed
+  const bool bf16 = desc->dtype == PDM_BF16, biased = bias != nullptr;
+  auto run = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    if (bf16) biased ? launch<PDM_BF16, D, true>(a, stream) : launch<PDM_BF16, D, false>(a, stream);
+    else biased ? launch<PDM_F16, D, true>(a, stream) : launch<PDM_F16, D, false>(a, stream);
+  };
+  if (desc->head_dim == 64) run(std::integral_constant<int, 64>());
+  else run(std::integral_constant<int, 128>());
+  PDM_CHECK_LAUNCH();
+  return PDM_OK;
+}

@@ -1,0 +1,299 @@
+// Device helpers of the attention of ragged batches (jagged_attention.hip, jagged_backward.hip): sequences and the keys
+// that their queries see, tiles in LDS and their fragments, the bias by distance.
+#pragma once
+
+#include "kv_common.h"
+
+namespace pdm {
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+
+struct JagArgs {
+  const void *q, *k, *v;
+  const int32_t *cu_q, *cu_k;
+  const float* bias;                 // [hq, bias_last + 1] or null
+  int32_t* err;
+  void *out, *rest;                  // forward; rest: what rounding out left (may be null)
+  float *lse, *stats;                // stats: a row's reference (log2) and 1 / the sum of its weights
+  const void* dout;                  // backward
+  const float* dlse;
+  void *dq, *dk, *dv;
+  float* dbias;
+  float* delta;                      // sum_d dout out - dlse, [q_tokens, hq]
+  int32_t* expo;                     // fp16: exponent of the largest |dout| of 32 rows, [items of 128 rows, 4, hq]
+  float* part;                       // partial gradients of the bias, [items of 128 rows, hq, part_stride]
+  int32_t* part_range;               // [items, 2]: the distances that a partial gradient holds
+  int64_t part_stride;
+  int64_t q_tokens, k_tokens, items;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
+  int32_t seqs, hq, hk, group, causal, window, sinks, bias_start, bias_last;
+  float scale, scale2;               // scale2 = scale * log2(e)
+};
+
+constexpr float kInf = __builtin_inff();
+constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.44269504088896341f;
+
+// ---- sequences -------------------------------------------------------------------
+struct JagSeq {
+  int64_t q0, k0;  // its first rows
+  int nq, nk;
+};
+
+// False where the spans do not fit the batch.
+__device__ __forceinline__ bool jag_seq(const JagArgs& a, int b, JagSeq& s) {
+  const int64_t c0 = a.cu_q[b], c1 = a.cu_q[b + 1], k0 = a.cu_k[b], k1 = a.cu_k[b + 1];
+  s.q0 = c0, s.k0 = k0, s.nq = (int)(c1 - c0), s.nk = (int)(k1 - k0);
+  return c0 >= 0 && c0 <= c1 && c1 <= a.q_tokens && k0 >= 0 && k0 <= k1 && k1 <= a.k_tokens;
+}
+
+// Block `item` of the list of (sequence, M rows of the spans `cu`): sequence b's part of it begins at cu[b] / M + b.
+// False for an item without rows.
+template <int M>
+__device__ __forceinline__ bool jag_block(const JagArgs& a, const int32_t* cu, int64_t item, JagSeq& s, int& b, int& r0) {
+  b = find_sequence(a.seqs, item, [&](int i) { return (int64_t)cu[i] / M + i; });
+  const int64_t j = item - ((int64_t)cu[b] / M + b);
+  if (j < 0 || !jag_seq(a, b, s) || j * M >= (cu == a.cu_q ? s.nq : s.nk)) return false;
+  r0 = (int)(j * M);
+  return true;
+}
+
+// Rows [first, first + 256) of the batch that no sequence which fits covers are given to clear(row), one after the other, by
+// the whole block of 256 threads; sequences [first, first + 256) that do not fit set the flag.
+template <typename F>
+__device__ __forceinline__ void jag_guard(const JagArgs& a, const int32_t* cu, int64_t tokens, int64_t first, F clear) {
+  __shared__ int bad[256];
+  const int64_t t = first + threadIdx.x;
+  JagSeq s;
+  if (t < a.seqs && !jag_seq(a, (int)t, s) && a.err) *a.err = 1;
+  bool covered = false;
+  if (t < tokens && a.seqs > 0) {
+    int lo = 0, hi = a.seqs;  // last b with cu[b] <= t
+    while (hi - lo > 1) {
+      const int mid = lo + (hi - lo) / 2;
+      if (cu[mid] <= t) lo = mid;
+      else hi = mid;
+    }
+    covered = cu[lo] <= t && t < cu[lo + 1] && jag_seq(a, lo, s);
+  }
+  const bool open = t < tokens && !covered;
+  bad[threadIdx.x] = open;
+  if (!__syncthreads_or(open)) return;
+  for (int r = 0; r < 256 && first + r < tokens; ++r)
+    if (bad[r]) clear(first + r);
+}
+
+__device__ __forceinline__ void clear_row(void* base, int64_t at, int elements) {  // of 16 bits; 16-byte aligned, all of a block
+  u32x4_t* p = reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(base) + at);
+  for (int i = threadIdx.x; i < elements / 8; i += 256) p[i] = u32x4_t{0, 0, 0, 0};
+}
+
+// ---- what a block of queries sees ------------------------------------------------------
+// Tiles of KT keys: those of the first tokens that stay visible, then [lo, hi), lo a multiple of KT.
+struct JagKeys {
+  int lo, hi, first, tiles;  // first: tiles before lo
+};
+template <int KT>
+__device__ __forceinline__ JagKeys jag_keys(const JagArgs& a, const JagSeq& s, int i0, int i1) {  // queries i0 .. i1
+  const int p0 = s.nk - s.nq + i0, p1 = s.nk - s.nq + i1;
+  JagKeys k;
+  k.hi = a.causal && p1 + 1 < s.nk ? p1 + 1 : s.nk;
+  if (k.hi < 0) k.hi = 0;
+  k.lo = a.window > 0 && p0 - a.window + 1 > 0 ? (p0 - a.window + 1) & ~(KT - 1) : 0;
+  if (k.lo > k.hi) k.lo = (k.hi + KT - 1) & ~(KT - 1);
+  const int sinks = a.sinks < k.hi ? a.sinks : k.hi;
+  k.first = (sinks + KT - 1) / KT;
+  if (k.first * KT >= k.lo) k.first = 0, k.lo = sinks > 0 ? 0 : k.lo;
+  k.tiles = k.first + (k.hi > k.lo ? (k.hi - k.lo + KT - 1) / KT : 0);
+  return k;
+}
+template <int KT>
+__device__ __forceinline__ int jag_key(const JagKeys& k, int t) { return t < k.first ? t * KT : k.lo + (t - k.first) * KT; }
+
+// ---- types -----------------------------------------------------------------------------
+template <int DT>
+__device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+  if constexpr (DT == PDM_BF16) return mfma32x32x16(a, b, c);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {  // nearest even
+  if constexpr (DT == PDM_BF16) return pack_bf16x2(lo, hi);
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{lo, hi}, f16x2_t));
+}
+template <int DT>
+__device__ __forceinline__ float lo_of(uint32_t w) {
+  return DT == PDM_BF16 ? __uint_as_float(w << 16) : f16_bits_to_f32(w & 0xffffu);
+}
+template <int DT>
+__device__ __forceinline__ float hi_of(uint32_t w) {
+  return DT == PDM_BF16 ? __uint_as_float(w & 0xffff0000u) : f16_bits_to_f32(w >> 16);
+}
+template <int DT>
+__device__ __forceinline__ uint32_t left2(float lo, float hi, uint32_t w) {  // what rounding the pair to w left
+  return pack2<DT>(lo - lo_of<DT>(w), hi - hi_of<DT>(w));
+}
+// Bits 15 and 31: the element there is infinite or NaN.
+template <int DT>
+__device__ __forceinline__ uint32_t odd2(uint32_t w) {
+  constexpr uint32_t E = DT == PDM_BF16 ? 0x7f807f80u : 0x7c007c00u, U = DT == PDM_BF16 ? 0x00800080u : 0x04000400u;
+  return ((w & E) + U) & 0x80008000u;
+}
+
+// ---- tiles in LDS -----------------------------------------------------------------------
+// Rows of D elements in pieces of 16 bytes; piece g of row r lies at place g ^ turn(r).  The rows of a fragment read then begin
+// in different banks, and so do the 4 rows of 4 pieces that half a wave takes by a transposing read.
+template <int D>
+struct Tile {
+  static constexpr int RS = 2 * D;
+  __device__ static constexpr int turn(int r) {
+    return D == 64 ? (r >> 1 & 1) << 2 | (r & 1) << 1 | (r >> 2 & 1) : (r & 3) << 2 | (r >> 2 & 3);
+  }
+  // A fragment's element i of lane l: row l % 32, column 16 kk + 8 (l / 32) + i.
+  static __device__ __forceinline__ uint32_t row_at(int lane) { return (lane & 31) * RS + 16 * (lane >> 5 ^ turn(lane & 31)); }
+  static __device__ __forceinline__ u32x4_t rows(const char* t, uint32_t at, int row, int kk) {
+    return *reinterpret_cast<const u32x4_t*>(t + (at ^ (32 * kk)) + row * RS);
+  }
+  // Transposed: lane l has column 32 d + l % 32 of the 8 rows y + 4 (l / 32) + {0 .. 3, 8 .. 11}, which is the order in
+  // which a 32x32 product leaves its rows.  A read of 16 lanes transposes 4 rows of 16 elements.
+  static __device__ __forceinline__ uint32_t col_at(int lane) {
+    const int r = 4 * (lane >> 5) + ((lane & 15) >> 2);
+    return r * RS + 16 * ((2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ turn(r)) + 8 * (lane & 1);
+  }
+  static __device__ __forceinline__ u32x4_t cols(const char* t, uint32_t at, int y, int d) {
+    typedef __attribute__((address_space(3))) s16x4_t* lds_t;
+    char* p = const_cast<char*>(t) + y * RS;
+    const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(p + (at ^ (64 * d)))));
+    const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(p + (at ^ (64 * d ^ 16 * turn(8))) + 8 * RS)));
+    return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+  }
+};
+
+// Eight elements, zeros where !there.
+__device__ __forceinline__ u32x4_t load16(const uint16_t* p, bool there) {
+  return there ? *reinterpret_cast<const u32x4_t*>(p) : u32x4_t{0, 0, 0, 0};
+}
+
+// A workgroup of 4 waves brings ROWS rows of a head into a tile without registers in between: buffer loads into LDS, whose lanes
+// land 16 bytes apart, so that a lane takes the piece that belongs at its place.  Rows behind the n that are there come as zeros.
+// Counted by vmcnt.
+template <int D, int ROWS>
+struct Bring {
+  static constexpr int N = ROWS * D / 8 / 256;  // loads of a wave
+  static constexpr int R = 64 / (D / 8);        // rows of a load
+  uint32_t off[D == 64 ? 1 : N];                // of this lane's pieces, but for the rows of a load of D = 64
+  uint32_t step;
+  __device__ __forceinline__ void init(int64_t stride, int lane, int wave) {
+    step = (uint32_t)stride * 2;
+#pragma unroll
+    for (int i = 0; i < (D == 64 ? 1 : N); ++i) {
+      const int r = (wave * N + i) * R + lane / (D / 8);
+      off[i] = r * step + 16 * ((lane % (D / 8)) ^ Tile<D>::turn(r));
+    }
+  }
+  __device__ __forceinline__ void load(const uint16_t* head, int64_t stride, int row0, int n, const char* tile, int wave) const {
+    const int rows = n - row0 < ROWS ? n - row0 : ROWS;
+    const uint64_t base = reinterpret_cast<uint64_t>(head + row0 * stride);
+    typedef uint32_t u32x4s __attribute__((ext_vector_type(4)));
+    const u32x4s rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32) & 0xffffu),
+                         (uint32_t)__builtin_amdgcn_readfirstlane((rows - 1) * step + 2 * D), 0x00027000u};
+    const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>(
+        (__attribute__((address_space(3))) const char*)tile) + wave * N * 1024);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t v = D == 64 ? off[0] + i * R * step : off[D == 64 ? 0 : i];
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                   :: "v"(v), "s"(rsrc), "s"(lds + i * 1024) : "memory", "m0");
+    }
+  }
+};
+// This wave's loads into LDS have landed.
+__device__ __forceinline__ void brought() { __builtin_amdgcn_s_waitcnt(kWaitVmcnt0); }
+
+// ---- products with a tile's columns ------------------------------------------------------
+// acc[d] += columns of rows [y0, y0 + 16 Y) of the tile, times w (the weights of these rows, as a 32x32 product left them);
+// TWICE: and times rest.
+template <int DT, int D, int Y, bool TWICE = false>
+__device__ __forceinline__ void add_cols(f32x16_t* acc, const char* t, uint32_t at, int y0, const u32x4_t* w, const u32x4_t* rest = nullptr) {
+#pragma unroll
+  for (int y = 0; y < Y; ++y)
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) {
+      const u32x4_t f = Tile<D>::cols(t, at, y0 + 16 * y, d);
+      acc[d] = mfma32<DT>(f, w[y], acc[d]);
+      if constexpr (TWICE) acc[d] = mfma32<DT>(f, rest[y], acc[d]);
+    }
+}
+
+// True where the tile's rows [y0, y0 + 16 Y) hold infinities or NaN (for the whole wave).
+template <int DT, int D, int Y>
+__device__ __forceinline__ bool odd_rows(const char* t, uint32_t at, int y0) {
+  uint32_t odd = 0;
+#pragma unroll 1
+  for (int y = 0; y < Y; ++y)
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) {
+      const u32x4_t f = Tile<D>::cols(t, at, y0 + 16 * y, d);
+      odd |= (odd2<DT>(f[0]) | odd2<DT>(f[1])) | (odd2<DT>(f[2]) | odd2<DT>(f[3]));
+    }
+  return __any(odd != 0);
+}
+
+// add_cols where some weights belong to pairs that are not seen: they are zeros, and what they meet must not matter, though 0
+// times an infinity or NaN would.  Such elements are left out here, and brought to the pairs that are seen by products of ones:
+// +-infinity, and NaN as both.  sees(r): whether this lane's column sees row r of the tile.  Rare: a loop of little code.
+template <int DT, int D, int Y, bool TWICE, typename F>
+__device__ __forceinline__ void add_cols_odd(f32x16_t* acc, const char* t, uint32_t at, int y0, const u32x4_t* w, F sees, const u32x4_t* rest = nullptr) {
+  constexpr uint32_t one = DT == PDM_BF16 ? 0x3f80u : 0x3c00u, pos = DT == PDM_BF16 ? 0x7f80u : 0x7c00u, neg = pos | 0x8000u;
+  const int h4 = 4 * (threadIdx.x >> 5 & 1);
+#pragma unroll 1
+  for (int y = 0; y < Y; ++y) {
+    u32x4_t seen, wy = w[0], ry = {0, 0, 0, 0};
+    if constexpr (TWICE) ry = rest[0];
+#pragma unroll
+    for (int i = 1; i < Y; ++i) {
+      wy = y == i ? w[i] : wy;
+      if constexpr (TWICE) ry = y == i ? rest[i] : ry;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = y0 + 16 * y + h4 + 8 * (e >> 1) + 2 * (e & 1);
+      seen[e] = (sees(r) ? one : 0u) | (sees(r + 1) ? one << 16 : 0u);
+    }
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) {
+      u32x4_t f = Tile<D>::cols(t, at, y0 + 16 * y, d), fp, fn;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t full = (odd2<DT>(f[e]) >> 15) * 0xffffu, x = f[e] & 0xffffu, z = f[e] >> 16;
+        const uint32_t ones = full & (one | one << 16);
+        fp[e] = ones & ((x == neg ? 0u : 0xffffu) | (z == neg ? 0u : 0xffff0000u));
+        fn[e] = ones & ((x == pos ? 0u : 0xffffu) | (z == pos ? 0u : 0xffff0000u));
+        f[e] &= ~full;
+      }
+      acc[d] = mfma32<DT>(f, wy, acc[d]);
+      if constexpr (TWICE) acc[d] = mfma32<DT>(f, ry, acc[d]);
+      constexpr f32x16_t zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+      __builtin_amdgcn_sched_barrier(0);
+      const f32x16_t up = mfma32<DT>(fp, seen, zero);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[d][e] += up[e] > 0.0f ? kInf : 0.0f;
+      __builtin_amdgcn_sched_barrier(0);
+      const f32x16_t down = mfma32<DT>(fn, seen, zero);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[d][e] -= down[e] > 0.0f ? kInf : 0.0f;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+// ---- the bias by distance -----------------------------------------------------------------
+// Of distance d in units of log2, finite where the bias is.
+__device__ __forceinline__ float bias2(const JagArgs& a, const float* row, int64_t d) {
+  const int64_t c = d - a.bias_start;
+  const float b = row[c < 0 ? 0 : c > a.bias_last ? a.bias_last : c], v = b * kLog2e;
+  return fabsf(b) < kInf ? __builtin_amdgcn_fmed3f(v, -3.402823466e38f, 3.402823466e38f) : v;
+}
+
+}  // namespace pdm

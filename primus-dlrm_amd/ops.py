@@ -1235,3 +1235,269 @@ def _(q, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, s
       return_lse, err_flag):
     return (q.new_empty(q.shape),
             q.new_empty(q.shape[:2] if return_lse else (0,), dtype=torch.float32))
+
+
+# ---------------------------------------------------------------------------
+# Attention of ragged batches with its backward pass; the bias by distance
+# ---------------------------------------------------------------------------
+
+def _even_heads(t: torch.Tensor) -> torch.Tensor:
+    """t [tokens, heads, D] as the kernels read it: 16-byte aligned, strides multiples of 8.  A copy where it is not."""
+    st, sh, _ = t.stride()
+    if t.data_ptr() % 16 or (t.shape[0] > 1 and (st % 8 or st >= 1 << 24)) or (t.shape[1] > 1 and sh % 8):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _even(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """Contiguous and 16-byte aligned."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16 else t
+
+
+def _check_spans(name: str, cu: torch.Tensor) -> int:
+    if cu.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32, got {cu.dtype}")
+    if cu.dim() != 1 or cu.shape[0] < 1 or not cu.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous [sequences + 1] tensor, got {tuple(cu.shape)}")
+    return cu.shape[0] - 1
+
+
+def _check_bias(bias: Optional[torch.Tensor], heads: int, bias_start: int) -> int:
+    """Columns of the bias; 0 without one."""
+    if not -2 ** 30 < bias_start < 2 ** 30:
+        raise ValueError(f"bias_start must lie in (-2^30, 2^30), got {bias_start}")
+    if bias is None:
+        return 0
+    if bias.dtype != torch.float32 or bias.dim() != 2 or bias.shape[0] != heads or not bias.is_contiguous():
+        raise ValueError(f"bias must be a contiguous float32 [{heads}, distances] tensor, got {bias.dtype} {tuple(bias.shape)}")
+    if not 1 <= bias.shape[1] <= 2 ** 30:
+        raise ValueError("bias must have 1 to 2^30 columns")
+    return bias.shape[1]
+
+
+def _jagged_desc(q, k, v, cu_seqlens, cu_seqlens_k, bias, scale, causal, window, sinks, bias_start) -> "L.JaggedAttentionDesc":
+    T, hq, D, q_st, q_sh, code = _check_heads("q", q)
+    kT, hk, kD, k_st, k_sh, k_code = _check_heads("k", k)
+    _, _, _, v_st, v_sh, v_code = _check_heads("v", v)
+    if code == L.PDM_F32:
+        raise TypeError("q, k and v must be float16 or bfloat16")
+    if k_code != code or v_code != code:
+        raise TypeError(f"q, k and v must be of one dtype, got {q.dtype}, {k.dtype} and {v.dtype}")
+    if v.shape != k.shape:
+        raise ValueError(f"v must be {tuple(k.shape)} as k is, got {tuple(v.shape)}")
+    if D not in (64, 128) or kD != D:
+        raise ValueError(f"head_dim must be 64 or 128, the same for q, k and v, got {D} and {kD}")
+    if hk == 0 or hq == 0 or hq % hk:
+        raise ValueError(f"the query heads ({hq}) must be a multiple of the key heads ({hk})")
+    seqs = _check_spans("cu_seqlens", cu_seqlens)
+    if _check_spans("cu_seqlens_k", cu_seqlens_k) != seqs:
+        raise ValueError(f"cu_seqlens_k must have as many entries as cu_seqlens, got {cu_seqlens_k.shape[0]} and {seqs + 1}")
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    for n, x in (("window", window), ("sinks", sinks)):
+        if not 0 <= x < 2 ** 31:
+            raise ValueError(f"{n} must lie in [0, 2^31), got {x}")
+    span = _check_bias(bias, hq, bias_start)
+    # (a dimension of one entry may have any stride)
+    return L.JaggedAttentionDesc(code, hq, hk, D, seqs, int(causal), window, sinks, bias_start, span, scale, 0, T, kT,
+                                 q_st if T > 1 else 0, q_sh if hq > 1 else 0, k_st if kT > 1 else 0, k_sh if hk > 1 else 0,
+                                 v_st if kT > 1 else 0, v_sh if hk > 1 else 0)
+
+
+def jagged_attention_raw(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                         cu_seqlens_k: torch.Tensor, bias: Optional[torch.Tensor], scale: float, causal: bool = True,
+                         window: int = 0, sinks: int = 0, bias_start: int = 0, return_lse: bool = False, keep: int = 0,
+                         err_flag: Optional[torch.Tensor] = None):
+    """Launches pdm_jagged_attention_fwd on q [T, Hq, D], k and v [S, Hk, D]: (out, lse, stats, rest), None where not wanted.
+    ``keep``: what a backward pass needs, 1 the rows' statistics, 2 what the rounding of out left too (for the bias's gradient)."""
+    _check_err_flag(err_flag)
+    index = _gpu_index(q, k, v, cu_seqlens, cu_seqlens_k, bias, err_flag)
+    q, k, v = _even_heads(q), _even_heads(k), _even_heads(v)
+    desc = _jagged_desc(q, k, v, cu_seqlens, cu_seqlens_k, bias, scale, causal, window, sinks, bias_start)
+    T, hq = q.shape[:2]
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty((T, hq), dtype=torch.float32, device=q.device) if return_lse else None
+    stats = torch.empty((T, hq, 2), dtype=torch.float32, device=q.device) if keep else None
+    rest = torch.empty_like(out) if keep > 1 and bias is not None else None
+    lib = L.lib()
+    ws_bytes = int(lib.pdm_jagged_attention_workspace_size(ctypes.byref(desc)))
+    if ws_bytes < 0:
+        raise L.PdmError(ws_bytes, "pdm_jagged_attention_workspace_size", L.last_error())
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    with _on_device(index):
+        L.check(lib.pdm_jagged_attention_fwd(
+            ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(),
+            _ptr(bias), out.data_ptr(), _ptr(rest), _ptr(lse), _ptr(stats), _ptr(ws), ws_bytes, _ptr(err_flag),
+            L.raw_stream(index)), "pdm_jagged_attention_fwd")
+    if err_flag is not None:
+        _written(err_flag)
+    return out, lse, stats, rest
+
+
+def jagged_attention_backward_raw(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                                  cu_seqlens_k: torch.Tensor, bias: Optional[torch.Tensor], out: torch.Tensor,
+                                  stats: torch.Tensor, rest: Optional[torch.Tensor], grad_out: torch.Tensor,
+                                  grad_lse: Optional[torch.Tensor], scale: float, causal: bool, window: int, sinks: int,
+                                  bias_start: int):
+    """Launches pdm_jagged_attention_bwd: gradients of q, k, v and, with ``rest``, of the bias (else None)."""
+    index = _gpu_index(q, k, v, cu_seqlens, cu_seqlens_k, bias, out, stats, rest, grad_out, grad_lse)
+    if grad_out.shape != q.shape or grad_out.dtype != q.dtype:
+        raise ValueError(f"grad_out must be {q.dtype} {tuple(q.shape)}, got {grad_out.dtype} {tuple(grad_out.shape)}")
+    if grad_lse is not None and (grad_lse.shape != q.shape[:2] or grad_lse.dtype != torch.float32):
+        raise ValueError(f"grad_lse must be float32 {tuple(q.shape[:2])}, got {grad_lse.dtype} {tuple(grad_lse.shape)}")
+    q, k, v, grad_out, grad_lse = _even_heads(q), _even_heads(k), _even_heads(v), _even(grad_out), _even(grad_lse)
+    desc = _jagged_desc(q, k, v, cu_seqlens, cu_seqlens_k, bias, scale, causal, window, sinks, bias_start)
+    gq, gk, gv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
+    gb = torch.empty_like(bias) if rest is not None else None
+    lib = L.lib()
+    ws_bytes = int(lib.pdm_jagged_attention_bwd_workspace_size(ctypes.byref(desc), int(gb is not None)))
+    if ws_bytes < 0:
+        raise L.PdmError(ws_bytes, "pdm_jagged_attention_bwd_workspace_size", L.last_error())
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    with _on_device(index):
+        L.check(lib.pdm_jagged_attention_bwd(
+            ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(),
+            _ptr(bias), out.data_ptr(), _ptr(rest), stats.data_ptr(), grad_out.data_ptr(), _ptr(grad_lse), gq.data_ptr(),
+            gk.data_ptr(), gv.data_ptr(), _ptr(gb), _ptr(ws), ws_bytes, L.raw_stream(index)), "pdm_jagged_attention_bwd")
+    return gq, gk, gv, gb
+
+
+@torch.library.custom_op("pdm::jagged_attention", mutates_args=())
+def jagged_attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                        cu_seqlens_k: torch.Tensor, bias: Optional[torch.Tensor], scale: float, causal: bool, window: int,
+                        sinks: int, bias_start: int, keep: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """out, lse, and what ``keep`` asks for (else empty)."""
+    out, lse, stats, rest = jagged_attention_raw(q, k, v, cu_seqlens, cu_seqlens_k, bias, scale, causal, window, sinks,
+                                                 bias_start, True, keep)
+    return (out, lse, q.new_empty(0, dtype=torch.float32) if stats is None else stats,
+            q.new_empty(0) if rest is None else rest)
+
+
+@jagged_attention_op.register_fake
+def _(q, k, v, cu_seqlens, cu_seqlens_k, bias, scale, causal, window, sinks, bias_start, keep):
+    T, hq, _ = q.shape
+    return (q.new_empty(q.shape), q.new_empty((T, hq), dtype=torch.float32),
+            q.new_empty((T, hq, 2) if keep else (0,), dtype=torch.float32),
+            q.new_empty(q.shape if keep > 1 and bias is not None else (0,)))
+
+
+@torch.library.custom_op("pdm::jagged_attention_backward", mutates_args=())
+def jagged_attention_backward_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                                 cu_seqlens_k: torch.Tensor, bias: Optional[torch.Tensor], out: torch.Tensor,
+                                 stats: torch.Tensor, rest: Optional[torch.Tensor], grad_out: torch.Tensor,
+                                 grad_lse: Optional[torch.Tensor], scale: float, causal: bool, window: int, sinks: int,
+                                 bias_start: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients of q, k, v and the bias (empty without ``rest``)."""
+    gq, gk, gv, gb = jagged_attention_backward_raw(q, k, v, cu_seqlens, cu_seqlens_k, bias, out, stats, rest, grad_out,
+                                                   grad_lse, scale, causal, window, sinks, bias_start)
+    return gq, gk, gv, q.new_empty(0, dtype=torch.float32) if gb is None else gb
+
+
+@jagged_attention_backward_op.register_fake
+def _(q, k, v, cu_seqlens, cu_seqlens_k, bias, out, stats, rest, grad_out, grad_lse, scale, causal, window, sinks, bias_start):
+    return (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape),
+            q.new_empty(bias.shape if rest is not None else (0,), dtype=torch.float32))
+
+
+def _jagged_attention_setup(ctx, inputs, output):
+    q, k, v, cu_seqlens, cu_seqlens_k, bias, *ctx.rest_args, keep = inputs
+    out, _, stats, rest = output
+    if not keep:
+        raise RuntimeError("pdm::jagged_attention needs keep = 1 or 2 for its backward pass")
+    ctx.has_rest = keep > 1 and bias is not None
+    ctx.save_for_backward(q, k, v, cu_seqlens, cu_seqlens_k, bias, out, stats, rest)
+
+
+def _jagged_attention_backward(ctx, grad_out, grad_lse, grad_stats, grad_rest):
+    q, k, v, cu_seqlens, cu_seqlens_k, bias, out, stats, rest = ctx.saved_tensors
+    if grad_out is None:
+        grad_out = torch.zeros_like(out)
+    gq, gk, gv, gb = torch.ops.pdm.jagged_attention_backward(q, k, v, cu_seqlens, cu_seqlens_k, bias, out, stats,
+                                                             rest if ctx.has_rest else None, grad_out, grad_lse,
+                                                             *ctx.rest_args)
+    need = ctx.needs_input_grad
+    return (gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, None, None,
+            gb if ctx.has_rest and need[5] else None, None, None, None, None, None, None)
+
+
+jagged_attention_op.register_autograd(_jagged_attention_backward, setup_context=_jagged_attention_setup)
+
+
+def _check_buckets(table_shape, dtype, buckets: torch.Tensor) -> Tuple[int, int, int, int]:
+    """(buckets, heads, columns, dtype code)."""
+    code = TORCH_TO_PDM.get(dtype)
+    if code is None:
+        raise TypeError(f"table must be float32, float16 or bfloat16, got {dtype}")
+    if len(table_shape) != 2 or not 1 <= table_shape[0] <= 8192 or not 1 <= table_shape[1] <= 65535:
+        raise ValueError(f"table must be [1 .. 8192 buckets, 1 .. 65535 heads], got {tuple(table_shape)}")
+    if buckets.dtype != torch.int32:
+        raise TypeError(f"buckets must be int32, got {buckets.dtype}")
+    if buckets.dim() != 1 or not 1 <= buckets.shape[0] <= 2 ** 24 or not buckets.is_contiguous():
+        raise ValueError(f"buckets must be a contiguous tensor of 1 to 2^24 entries, got {tuple(buckets.shape)}")
+    return table_shape[0], table_shape[1], buckets.shape[0], code
+
+
+def bucket_bias_raw(table: torch.Tensor, buckets: torch.Tensor) -> torch.Tensor:
+    """Launches pdm_bucket_bias_fwd: table [buckets, heads] spread to fp32 [heads, distances]."""
+    n, heads, span, code = _check_buckets(table.shape, table.dtype, buckets)
+    index = _gpu_index(table, buckets)
+    table = table.contiguous()
+    out = torch.empty((heads, span), dtype=torch.float32, device=table.device)
+    with _on_device(index):
+        L.check(L.lib().pdm_bucket_bias_fwd(table.data_ptr(), code, n, heads, buckets.data_ptr(), span, out.data_ptr(),
+                                            L.raw_stream(index)), "pdm_bucket_bias_fwd")
+    return out
+
+
+def bucket_bias_backward_raw(grad_out: torch.Tensor, buckets: torch.Tensor, num_buckets: int, dtype: torch.dtype) -> torch.Tensor:
+    """Launches pdm_bucket_bias_bwd: the gradient of the table."""
+    if grad_out.dim() != 2 or grad_out.dtype != torch.float32 or grad_out.shape[1:] != buckets.shape:
+        raise ValueError(f"grad_out must be float32 [heads, {tuple(buckets.shape)}], got {grad_out.dtype} {tuple(grad_out.shape)}")
+    n, heads, span, code = _check_buckets((num_buckets, grad_out.shape[0]), dtype, buckets)
+    index = _gpu_index(grad_out, buckets)
+    grad_out = grad_out.contiguous()
+    grad = torch.empty((n, heads), dtype=dtype, device=grad_out.device)
+    ws = torch.empty(2 * n, dtype=torch.int32, device=grad_out.device)
+    with _on_device(index):
+        L.check(L.lib().pdm_bucket_bias_bwd(grad_out.data_ptr(), buckets.data_ptr(), span, n, heads, code, grad.data_ptr(),
+                                            ws.data_ptr(), 8 * n, L.raw_stream(index)), "pdm_bucket_bias_bwd")
+    return grad
+
+
+@torch.library.custom_op("pdm::bucket_bias", mutates_args=())
+def bucket_bias_op(table: torch.Tensor, buckets: torch.Tensor) -> torch.Tensor:
+    return bucket_bias_raw(table, buckets)
+
+
+@bucket_bias_op.register_fake
+def _(table, buckets):
+    return table.new_empty((table.shape[1], buckets.shape[0]), dtype=torch.float32)
+
+
+@torch.library.custom_op("pdm::bucket_bias_backward", mutates_args=())
+def bucket_bias_backward_op(grad_out: torch.Tensor, buckets: torch.Tensor, num_buckets: int, dtype: torch.dtype) -> torch.Tensor:
+    return bucket_bias_backward_raw(grad_out, buckets, num_buckets, dtype)
+
+
+@bucket_bias_backward_op.register_fake
+def _(grad_out, buckets, num_buckets, dtype):
+    return grad_out.new_empty((num_buckets, grad_out.shape[0]), dtype=dtype)
+
+
+def _bucket_bias_setup(ctx, inputs, output):
+    table, buckets = inputs
+    ctx.save_for_backward(buckets)
+    ctx.shape, ctx.dtype = table.shape, table.dtype
+
+
+def _bucket_bias_backward(ctx, grad_out):
+    (buckets,) = ctx.saved_tensors
+    return torch.ops.pdm.bucket_bias_backward(grad_out, buckets, ctx.shape[0], ctx.dtype), None
+
+
+bucket_bias_op.register_autograd(_bucket_bias_backward, setup_context=_bucket_bias_setup)
