@@ -698,6 +698,28 @@ int pdm_kv_attention_fwd(const pdm_kv_attention_desc* desc,
                          int64_t workspace_bytes, int32_t* err_flag,
                          pdm_stream_t stream);
 
+/* What pdm_kv_attention_fwd has not: first tokens that stay visible under a
+ * window, and a bias by distance.  With window > 0 a query sees the keys j <
+ * sinks too (up to its own token where causal); its score of key j has
+ * bias[h][c] added, c = p - j - bias_start held within [0, bias_span).  Pages
+ * that hold none of the keys that a sequence's queries see need not be there. */
+typedef struct {
+  const float* bias;  /* device fp32 [n_q_heads, bias_span], or NULL */
+  int32_t bias_start; /* distance of the first column, |bias_start| < 2^30 */
+  int32_t bias_span;  /* 0 without a bias, at most 2^30 */
+  int32_t sinks;
+  int32_t reserved;
+} pdm_kv_attention_bias;
+
+/* pdm_kv_attention_fwd with these (extra may be NULL); the same workspace. */
+int pdm_kv_attention_biased_fwd(const pdm_kv_attention_desc* desc,
+                                const pdm_kv_attention_bias* extra,
+                                const pdm_kv_cache* cache,
+                                const pdm_kv_batch* batch, const void* q,
+                                void* out, float* lse, void* workspace,
+                                int64_t workspace_bytes, int32_t* err_flag,
+                                pdm_stream_t stream);
+
 /* Attention of a ragged batch whose keys and values are tensors beside it (as in
  * training), forward and backward.  Sequence b's queries are rows cu_q[b] ..
  * cu_q[b + 1] of q, its keys and values rows cu_k[b] .. cu_k[b + 1] of k and v;

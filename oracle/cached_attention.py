@@ -75,7 +75,7 @@ def append(x, codes, scale, cu, table, lens):
                 codes[p, h, slot:slot + m] = round_e4m3(v * 2.0 ** -e)
 
 
-def attention(q, k_val, v_val, cu, table, lens, scale, causal, window):
+def attention(q, k_val, v_val, cu, table, lens, scale, causal, window, sinks=0, bias=None, start=0):
     """q [T, Hq, D]; k_val, v_val [pages, Hk, page, D] (the values that the codes stand for).  Returns out, lse, and for
     tolerances mag = sum_j p_j |v_j| and serr = the largest scale * sum_d |q_d k_jd| of a row."""
     T, hq, D = q.shape
@@ -100,12 +100,13 @@ def attention(q, k_val, v_val, cu, table, lens, scale, causal, window):
         if causal:
             seen &= j[None] <= p
         if window:
-            seen &= j[None] > p - window
+            seen &= (j[None] > p - window) | (j[None] < sinks)
         for h in range(hk):
             k, v = k_val[at, h, slot].double(), v_val[at, h, slot].double()
             for g in range(h * (hq // hk), (h + 1) * (hq // hk)):
                 qr = q[cu[b]:cu[b + 1], g]
-                s = torch.where(seen, qr @ k.T * scale, torch.full((), -math.inf, dtype=torch.float64))
+                add = 0.0 if bias is None else bias[g].double()[(p - j[None] - start).clamp(0, bias.shape[1] - 1)]
+                s = torch.where(seen, qr @ k.T * scale + add, torch.full((), -math.inf, dtype=torch.float64))
                 m = s.amax(-1, keepdim=True)
                 m = torch.where(torch.isinf(m), torch.zeros_like(m), m)
                 w = torch.where(seen, torch.exp(s - m), torch.zeros_like(s))
@@ -121,6 +122,6 @@ def attention(q, k_val, v_val, cu, table, lens, scale, causal, window):
                 out[cu[b]:cu[b + 1], g] = o
                 mag[cu[b]:cu[b + 1], g] = w.nan_to_num() @ v.nan_to_num().abs()
                 lse[cu[b]:cu[b + 1], g] = torch.where(some, m + total.log(), -math.inf)[:, 0]
-                sa = torch.where(seen, qr.abs() @ k.nan_to_num().abs().T * abs(scale), 0.0)
+                sa = torch.where(seen, qr.abs() @ k.nan_to_num().abs().T * abs(scale) + (0.0 if bias is None else add.abs()), 0.0)
                 serr[cu[b]:cu[b + 1], g] = sa.amax(-1)
     return out, lse, mag, serr

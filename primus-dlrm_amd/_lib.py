@@ -70,6 +70,7 @@ EXPORTED_SYMBOLS = (
     "pdm_kv_append",
     "pdm_kv_attention_workspace_size",
     "pdm_kv_attention_fwd",
+    "pdm_kv_attention_biased_fwd",
     "pdm_jagged_attention_workspace_size",
     "pdm_jagged_attention_fwd",
     "pdm_jagged_attention_bwd_workspace_size",
@@ -263,6 +264,16 @@ class KvAttentionDesc(ctypes.Structure):
     ]
 
 
+class KvAttentionBias(ctypes.Structure):
+    _fields_ = [
+        ("bias", ctypes.c_void_p),
+        ("bias_start", ctypes.c_int32),
+        ("bias_span", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 class JaggedAttentionDesc(ctypes.Structure):
     _fields_ = [
         ("dtype", ctypes.c_int32),
@@ -376,6 +387,10 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.pdm_kv_attention_fwd.restype = ctypes.c_int
     lib.pdm_kv_attention_fwd.argtypes = [ctypes.POINTER(KvAttentionDesc), ctypes.POINTER(KvCacheDesc),
                                          ctypes.POINTER(KvBatchDesc), vp, vp, vp, vp, i64, vp, vp]
+    lib.pdm_kv_attention_biased_fwd.restype = ctypes.c_int
+    lib.pdm_kv_attention_biased_fwd.argtypes = [ctypes.POINTER(KvAttentionDesc), ctypes.POINTER(KvAttentionBias),
+                                                ctypes.POINTER(KvCacheDesc), ctypes.POINTER(KvBatchDesc), vp, vp, vp, vp, i64,
+                                                vp, vp]
     lib.pdm_jagged_attention_workspace_size.restype = i64
     lib.pdm_jagged_attention_workspace_size.argtypes = [ctypes.POINTER(JaggedAttentionDesc)]
     lib.pdm_jagged_attention_fwd.restype = ctypes.c_int

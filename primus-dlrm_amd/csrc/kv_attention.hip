@@ -45,10 +45,12 @@ struct AttnArgs {
   int32_t few_rows;          // sequences of at most so many rows are kv_attn_few_kernel's
   int32_t vec;               // q takes 16-byte loads
   float scale2;              // scale * log2(e)
+  const float* bias;         // by distance, [hq, bias_last + 1], or null
+  int32_t bias_start, bias_last, sinks;
 };
 
 constexpr float kInf = __builtin_inff();
-constexpr float kLn2 = 0.69314718055994531f;
+constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.44269504088896341f;
 
 // Weights are exp2 of scores less a reference, which moves only where a weight would pass 2^8: sums and products lose nothing
 // by that while the values are below 2^89, whatever the number of keys.  Where a page's scale is above kHugeScale (so that its
@@ -72,17 +74,34 @@ struct Seq {
   int64_t row0;   // its first row of the batch
   int n, len;     // new tokens, length
   int lo, hi;     // keys that any of its rows may see, lo a multiple of 32
+  // With sinks before a window the kernels count keys without the gap between them: [lo, end), of which those from `first` on
+  // lie `gap` further on.  Keys below `see` that are no sinks are seen by no row.
+  int end, first, gap, see;
 };
 
 __device__ __forceinline__ bool seq_fits(const AttnArgs& a, int64_t c0, int64_t c1, int64_t len) {
   return c0 >= 0 && c1 <= a.tokens && c1 - c0 <= a.max_q && c1 - c0 <= len;
 }
 
+// Takes the gap between the sinks, in whole units of keys, and lo out of the count.
+__device__ __forceinline__ void skip_gap(const AttnArgs& a, Seq& s, int unit) {
+  s.end = s.hi, s.first = 0, s.gap = 0;
+  if (a.sinks == 0 || s.lo == 0) return;
+  const int sinks = a.sinks < s.hi ? a.sinks : s.hi, first = (sinks + unit - 1) / unit * unit;
+  if (s.lo > first) {
+    s.first = first, s.gap = s.lo - first;
+    s.end = s.hi > s.lo ? s.hi - s.gap : sinks;
+  }
+  s.lo = 0;
+}
+
 __device__ __forceinline__ void seq_keys(const AttnArgs& a, Seq& s) {
   const int64_t most = (int64_t)a.table_width << a.page_log2;
   s.hi = s.len < most ? s.len : (int)most;
   const int64_t first = (int64_t)s.len - s.n - a.window + 1;
-  s.lo = a.window > 0 && first > 0 ? (int)first & ~31 : 0;
+  s.see = a.window > 0 && first > 0 ? (int)first : 0;
+  s.lo = s.see & ~31;
+  skip_gap(a, s, 32);
 }
 
 // False for a sequence without rows, and for one that does not fit (which sets the flag).
@@ -136,6 +155,14 @@ __device__ __forceinline__ f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c) {
 __device__ __forceinline__ uint32_t remainder_pair(float x, float y, uint32_t hi) {
   return pack_bf16x2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
 }
+
+// The bias of distance d for the head whose row this is, in units of log2, finite where the bias is.
+__device__ __forceinline__ float bias_in_log2(float b) {
+  const float v = b * kLog2e;
+  return fabsf(b) < kInf ? __builtin_amdgcn_fmed3f(v, -3.402823466e38f, 3.402823466e38f) : v;
+}
+__device__ __forceinline__ int bias_column(const AttnArgs& a, int c) { return c < 0 ? 0 : c > a.bias_last ? a.bias_last : c; }
+typedef float f32x4u_t __attribute__((ext_vector_type(4), aligned(4)));
 
 // A lane's value, for the whole wave.
 __device__ __forceinline__ float lane_f(float v, int lane) {
@@ -215,7 +242,7 @@ struct FewUnit {
   int64_t slot;     // else the place of the partial result
 };
 
-__device__ __forceinline__ int steps_of(const Seq& s) { return s.hi > s.lo ? (s.hi - s.lo + kFewStep - 1) / kFewStep : 1; }
+__device__ __forceinline__ int steps_of(const Seq& s) { return s.end > s.lo ? (s.end - s.lo + kFewStep - 1) / kFewStep : 1; }
 
 // Dealt: the steps of 128 keys of all (sequence, key head) pairs, in order, are dealt to `workers` workgroups in equal
 // runs, so that a batch of long and short sequences keeps every CU busy to the end.  A run ends some pairs and begins
@@ -283,7 +310,7 @@ __device__ __forceinline__ int64_t few_next(const AttnArgs& a, FewDeal& sh, int6
   const int s0 = (int)(local - (int64_t)u.kh * steps);
   const int n = to - x < steps - s0 ? (int)(to - x) : steps - s0;
   u.begin = u.sq.lo + s0 * kFewStep;
-  u.end = s0 + n < steps ? u.begin + n * kFewStep : u.sq.hi;
+  u.end = s0 + n < steps ? u.begin + n * kFewStep : u.sq.end;
   u.alone = n == steps;
   u.slot = 2 * worker + (x - s0 < from ? 0 : 1);
   return n;
@@ -295,16 +322,17 @@ __device__ __forceinline__ bool few_split(const AttnArgs& a, int64_t unit, FewUn
   const int64_t bh = unit / a.splits;
   u.kh = (int)(bh % a.hk), u.b = (int)(bh / a.hk);
   if (!seq_of(a, u.b, u.sq) || (int64_t)u.sq.n * a.group > a.few_rows) return false;
-  const int size = split_size(u.sq.hi - u.sq.lo, a.splits, kFewStep);
+  const int size = split_size(u.sq.end - u.sq.lo, a.splits, kFewStep);
   u.begin = u.sq.lo + split * size;
-  if (split > 0 && u.begin >= u.sq.hi) return false;
-  u.end = u.begin + size < u.sq.hi ? u.begin + size : u.sq.hi;
-  u.alone = u.sq.hi - u.sq.lo <= size;
+  if (split > 0 && u.begin >= u.sq.end) return false;
+  u.end = u.begin + size < u.sq.end ? u.begin + size : u.sq.end;
+  u.alone = u.sq.end - u.sq.lo <= size;
   u.slot = unit;
   return true;
 }
 
-template <int DT, int D, int MT>
+// EXT: sinks or a bias, whose loads and selects the plain form does without.
+template <int DT, int D, int MT, bool EXT>
 __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D * MT <= 256 ? 2 : 1) kv_attn_few_kernel(AttnArgs a, int64_t units, int64_t guards) {
   constexpr int KK = D / 32;              // steps of the first product
   constexpr int DD = D / 16;              // tiles of the second: O^T row m of tile dd is element DD m + dd
@@ -382,12 +410,17 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
   uint64_t spot = 0;
   float kss = 0.0f, vss = 0.0f;           // kss: NaN where the page does not exist
   Reference ref;
-  auto key_of = [&](int i) { return begin + (wave + kFewWaves * i) * kFewKeys; };
+  int gap_at = 0, gap = 0, see = 0;       // see Seq
+  const float* brow[EXT ? MT : 1];        // EXT: the rows' heads of the bias, and their column of key 0
+  int bcol[EXT ? MT : 1], pos0 = 0, pos1 = 0;
+  auto real = [&](int key) { return EXT && key >= gap_at ? key + gap : key; };
+  auto count_of = [&](int i) { return begin + (wave + kFewWaves * i) * kFewKeys; };
+  auto key_of = [&](int i) { return real(count_of(i)); };
   auto look_up = [&](int first) {
-    const int key = key_of(first + (lane >> 1)) + (lane & 1) * 16;
+    const int count = count_of(first + (lane >> 1)) + (lane & 1) * 16, key = real(count);
     // (a page that does not exist: some page, its keys are not seen)
     spot = 0, kss = __builtin_nanf(""), vss = 0.0f;
-    if (key < end) {
+    if (count < end && (key + 16 > see || (EXT && key < a.sinks))) {
       const int id = table[key >> a.page_log2];
       if (id >= 0 && id < a.num_pages) {
         const int64_t entry = (int64_t)id * a.hk + kh;
@@ -401,6 +434,7 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
     ref.raise(__any(vss > kHugeScale));
   };
   auto place = [&](int i, int s) { return lane_u64(spot, (i & 31) * 2 + s); };
+  auto seen_by = [&](int mt, int j) { return (j >= row_lo[mt] || (EXT && j < a.sinks)) && j < row_hi[mt]; };
   u32x4_t k[2][D / 64];                   // 16 bytes of a key row, 64 apart
   uint32_t v[2][4][D / 64];               // rows 4 g + i of 16 keys
   const uint32_t k_off = (uint32_t)(c * D + 16 * g);
@@ -440,12 +474,16 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
     return x & 1 ? u32x4_t{value_pair_hi(w[0], s0), value_pair_hi(w[1], s0), value_pair_hi(w[2], s1), value_pair_hi(w[3], s1)}
                  : u32x4_t{value_pair_lo(w[0], s0), value_pair_lo(w[1], s0), value_pair_lo(w[2], s1), value_pair_lo(w[3], s1)};
   };
-  auto whole_tile = [&](int i, bool ok) { return ok && key_of(i) >= all_lo && key_of(i) + kFewKeys <= all_hi; };
+  auto whole_tile = [&](int i, bool ok) {
+    const int key = key_of(i);
+    return ok && (key >= all_lo || (EXT && key + kFewKeys <= a.sinks)) && key + kFewKeys <= all_hi;
+  };
   // What comes before a unit's first tile, and that tile's loads.
   auto start = [&]() {
     const Seq& sq = fu.sq;
     const int rows = sq.n * a.group;
     kh = fu.kh, begin = fu.begin, end = fu.end;
+    gap_at = sq.first, gap = sq.gap, see = sq.see;
     table = a.table + (int64_t)fu.b * a.table_stride;
     int tiles = end > begin ? (end - begin + kFewKeys - 1) / kFewKeys : 0;
     if (tiles && a.num_pages == 0) {
@@ -459,10 +497,15 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
     const int p0 = sq.len - sq.n, p1 = sq.len - 1;
     if (a.causal && p0 + 1 < all_hi) all_hi = p0 + 1;
     if (a.window > 0 && p1 - a.window + 1 > 0) all_lo = p1 - a.window + 1;
+    pos0 = p0, pos1 = p1;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const int r = mt * 16 + c;
       const int i = r / a.group, h = kh * a.group + (r - i * a.group);
+      if (EXT) {  // (rows that are not there: the first one's)
+        brow[mt] = a.bias + (int64_t)(r < rows ? h : kh * a.group) * (a.bias_last + 1);
+        bcol[mt] = p0 + (r < rows ? i : 0) - a.bias_start;
+      }
       row_lo[mt] = 0x7fffffff, row_hi[mt] = 0;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) q[mt][kk] = u32x4_t{0, 0, 0, 0};
@@ -506,6 +549,31 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
 #pragma unroll 1
   for (int i = 0; i < mine; ++i) {
     const int x0 = (i & 31) * 2;
+    f32x4_t bias[EXT ? MT : 1][2];
+    if constexpr (EXT) {
+      if (a.bias) {
+        const int key = key_of(i);  // columns of the rows and keys of the tile: [lo, hi]
+        const int64_t lo = (int64_t)pos0 - key - (kFewKeys - 1) - a.bias_start, hi = (int64_t)pos1 - key - a.bias_start;
+        const bool inside = lo >= 0 && hi <= a.bias_last, alike = lo >= a.bias_last || hi <= 0;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const float one = alike ? brow[mt][lo >= a.bias_last ? a.bias_last : 0] : 0.0f;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int c3 = bcol[mt] - key - 16 * x - 4 * g - 3;
+            if (alike) {
+              bias[mt][x] = f32x4_t{one, one, one, one};
+            } else if (inside) {
+              const f32x4u_t v = *reinterpret_cast<const f32x4u_t*>(brow[mt] + c3);
+              bias[mt][x] = f32x4_t{v[3], v[2], v[1], v[0]};
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) bias[mt][x][e] = brow[mt][bias_column(a, c3 + 3 - e)];
+            }
+          }
+        }
+      }
+    }
     const float ks[2] = {a.scale2 * lane_f(kss, x0), a.scale2 * lane_f(kss, x0 + 1)};
     const bool ok[2] = {ks[0] == ks[0], ks[1] == ks[1]};
     const float vs[2] = {lane_f(vss, x0), lane_f(vss, x0 + 1)};
@@ -534,11 +602,15 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
       float w[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e] = s[mt][e >> 2][e & 3] * ks[e >> 2];
+      if (EXT && a.bias) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] += bias_in_log2(bias[mt][e >> 2][e & 3]);
+      }
       if (!whole) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int j = key + 16 * (e >> 2) + 4 * g + (e & 3);
-          w[e] = ok[e >> 2] && j >= row_lo[mt] && j < row_hi[mt] ? w[e] : -kInf;
+          w[e] = ok[e >> 2] && seen_by(mt, j) ? w[e] : -kInf;
         }
       }
       float top = w[0];
@@ -608,8 +680,7 @@ __global__ void __launch_bounds__(256, D * MT <= 64 ? 4 : D * MT <= 128 ? 3 : D 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int j = key_of(i) + 16 * (e >> 1) + 4 * g + 2 * (e & 1);
-          seen[mt][e] = (ok[e >> 1] && j >= row_lo[mt] && j < row_hi[mt] ? 0x3f80u : 0u) |
-                        (ok[e >> 1] && j + 1 >= row_lo[mt] && j + 1 < row_hi[mt] ? 0x3f800000u : 0u);
+          seen[mt][e] = (ok[e >> 1] && seen_by(mt, j) ? 0x3f80u : 0u) | (ok[e >> 1] && seen_by(mt, j + 1) ? 0x3f800000u : 0u);
         }
 #pragma unroll
       for (int h = 0; h < D / 64; ++h)
@@ -771,8 +842,8 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(AttnArgs a, int64_t u
   if (!seq_of(a, b, sq)) return;
   const int64_t rows = (int64_t)sq.n * a.group;
   if (rows > a.few_rows || row >= rows) return;
-  const int size = split_size(sq.hi - sq.lo, a.splits, kFewStep);
-  const int used = sq.hi > sq.lo ? (sq.hi - sq.lo + size - 1) / size : 1;
+  const int size = split_size(sq.end - sq.lo, a.splits, kFewStep);
+  const int used = sq.end > sq.lo ? (sq.end - sq.lo + size - 1) / size : 1;
   if (used == 1) return;
   const int i = row / a.group, h = kh * a.group + (row - i * a.group);
   join_row<DT, D, W>(a, used, (sq.row0 + i) * a.hq + h, [&](int s) { return (bh * a.splits + s) * a.row_stride + row; });
@@ -830,15 +901,19 @@ __device__ __forceinline__ bool many_block(const AttnArgs& a, int64_t item, Seq&
   return true;
 }
 
-// The keys that rows r0 .. r0 + M - 1 may see: [lo, hi), lo a multiple of 32.
-template <int M>
-__device__ __forceinline__ void many_keys(const AttnArgs& a, const Seq& sq, int r0, int& lo, int& hi) {
+// The keys that rows r0 .. r0 + M - 1 may see (as those of a sequence): [lo, end), lo a multiple of 32.
+template <int M, int KT>
+__device__ __forceinline__ Seq many_keys(const AttnArgs& a, const Seq& sq, int r0) {
+  Seq k = sq;
   const int rows = sq.n * a.group;
   const int i0 = r0 / a.group, i1 = ((r0 + M < rows ? r0 + M : rows) - 1) / a.group;
   const int p0 = sq.len - sq.n + i0, p1 = sq.len - sq.n + i1;
-  hi = a.causal && p1 + 1 < sq.hi ? p1 + 1 : sq.hi;
-  lo = a.window > 0 && p0 - a.window + 1 > 0 ? (p0 - a.window + 1) & ~31 : 0;
-  if (lo > hi) lo = hi & ~31;
+  k.hi = a.causal && p1 + 1 < sq.hi ? p1 + 1 : sq.hi;
+  k.see = a.window > 0 && p0 - a.window + 1 > 0 ? p0 - a.window + 1 : 0;
+  k.lo = k.see & ~31;
+  if (k.lo > k.hi) k.lo = k.hi & ~31;
+  skip_gap(a, k, KT);
+  return k;
 }
 
 template <int DT>
@@ -847,7 +922,7 @@ __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
   else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-template <int DT, int D, int KT, int NG>
+template <int DT, int D, int KT, int NG, bool EXT>
 __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kernel(AttnArgs a, int64_t items) {
   constexpr int M = 128 * NG;
   constexpr int KK = D / 16, DD = D / 32, XX = KT / 32;
@@ -867,12 +942,13 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
   Seq sq;
   int b, r0;
   if (!many_block<M>(a, item, sq, b, r0)) return;
-  int lo, hi;
-  many_keys<M>(a, sq, r0, lo, hi);
+  const Seq keys_of = many_keys<M, KT>(a, sq, r0);
+  const int lo = keys_of.lo, hi = keys_of.end;
   const int size = split_size(hi - lo, a.splits, KT);
   const int begin = lo + split * size;
   if (split > 0 && begin >= hi) return;
   const int end = begin + size < hi ? begin + size : hi;
+  auto real = [&](int key) { return EXT && key >= keys_of.first ? key + keys_of.gap : key; };
   const int rows = sq.n * a.group;
   int tiles = end > begin ? (end - begin + KT - 1) / KT : 0;
   if (tiles && a.num_pages == 0) {
@@ -912,6 +988,11 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
 #pragma unroll
       for (int e = 0; e < 4; ++e) q[kk][e] ^= 0x80008000u;
   }
+  // EXT: the row's head of the bias and its column of key 0 (rows that are not there: the first one's)
+  const int tok0 = r0 / a.group;
+  const float* brow = EXT ? a.bias + (int64_t)(row < rows ? head : kh * a.group) * (a.bias_last + 1) : nullptr;
+  const int bcol = sq.len - sq.n + (row < rows ? tok : tok0) - a.bias_start;
+  const int pos0 = sq.len - sq.n + tok0, pos1 = sq.len - sq.n + (r0 + M < rows ? r0 + M - 1 : rows - 1) / a.group;
   // keys that every row of this wave sees
   int all_lo = 0, all_hi = sq.hi;
   {
@@ -949,10 +1030,10 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
   auto load = [&](int t, auto kv) {
     const int key0 = begin + t * KT;
     if (t % PER == 0) {
-      const int key = key0 + 16 * lane;
+      const int count = key0 + 16 * lane, key = real(count);
       // (a page that does not exist: some page, its keys are not seen)
       spot = 0, kss = __builtin_nanf(""), vss = 0.0f;
-      if (key < end) {
+      if (count < end && (key + 16 > keys_of.see || (EXT && key < a.sinks))) {
         const int id = table[key >> a.page_log2];
         if (id >= 0 && id < a.num_pages) {
           const int64_t entry = (int64_t)id * a.hk + kh;
@@ -1092,7 +1173,7 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
   // the running maximum, and P from the scores
   u32x4_t p[2 * XX], rest[2 * XX];
   auto weights = [&](int t) __attribute__((always_inline)) {
-    const int key = begin + t * KT;
+    const int key = real(begin + t * KT);
     float sc[2 * XX];                      // of 16 keys each, not negative
     bool ok = true;
 #pragma unroll
@@ -1100,13 +1181,43 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
       sc[x] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sh.sc[t & 1][x])));
       ok = ok && sc[x] == sc[x];
     }
-    if (!(key >= all_lo && key + KT <= all_hi)) {
+    if constexpr (EXT) {
+      if (a.bias) {  // scores with their scale and bias
+        const int64_t low = (int64_t)pos0 - key - (KT - 1) - a.bias_start, high = (int64_t)pos1 - key - a.bias_start;
+        const bool inside = low >= 0 && high <= a.bias_last, alike = low >= a.bias_last || high <= 0;
+        const float one = alike ? bias_in_log2(brow[low >= a.bias_last ? a.bias_last : 0]) : 0.0f;
+#pragma unroll
+        for (int x = 0; x < XX; ++x)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int c3 = bcol - key - 32 * x - 8 * y - 4 * h - 3;
+            f32x4_t v = {one, one, one, one};
+            if (inside) {
+              const f32x4u_t u = *reinterpret_cast<const f32x4u_t*>(brow + c3);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = bias_in_log2(u[3 - e]);
+            } else if (!alike) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = bias_in_log2(brow[bias_column(a, c3 + 3 - e)]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[x][4 * y + e] = __builtin_fmaf(s[x][4 * y + e], sc[2 * x + (y >> 1)], v[e]);
+          }
+#pragma unroll
+        for (int x = 0; x < 2 * XX; ++x) sc[x] = sc[x] == sc[x] ? 1.0f : sc[x];
+      }
+    }
+    if (!((key >= all_lo || (EXT && key + KT <= a.sinks)) && key + KT <= all_hi)) {
       uint32_t from = key + 4 * h - row_lo, span = row_hi > row_lo ? row_hi - row_lo : 0;  // seen: j - row_lo < span
       only_here(from);
+      const int first = EXT ? (a.sinks < row_hi ? a.sinks : row_hi) - key - 4 * h : 0;     // or: a sink
 #pragma unroll
       for (int x = 0; x < XX; ++x)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[x][e] = from + (32 * x + 8 * (e >> 2) + (e & 3)) < span ? s[x][e] : -kInf;
+        for (int e = 0; e < 16; ++e) {
+          const int j = 32 * x + 8 * (e >> 2) + (e & 3);
+          s[x][e] = from + j < span || (EXT && j < first) ? s[x][e] : -kInf;
+        }
     }
     if (!ok) {
 #pragma unroll
@@ -1243,8 +1354,9 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
           const bool ok = sh.sc[t & 1][y] == sh.sc[t & 1][y];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int j = begin + t * KT + 16 * y + 8 * (e >> 1) + 4 * h + 2 * (e & 1);
-            seen[e] = (ok && j >= row_lo && j < row_hi ? 0x3f80u : 0u) | (ok && j + 1 >= row_lo && j + 1 < row_hi ? 0x3f800000u : 0u);
+            const int j = real(begin + t * KT) + 16 * y + 8 * (e >> 1) + 4 * h + 2 * (e & 1);
+            auto sees = [&](int x) { return ok && (x >= row_lo || (EXT && x < a.sinks)) && x < row_hi; };
+            seen[e] = (sees(j) ? 0x3f80u : 0u) | (sees(j + 1) ? 0x3f800000u : 0u);
           }
 #pragma unroll
           for (int d = 0; d < DD; ++d) {
@@ -1295,8 +1407,8 @@ __global__ void __launch_bounds__(256) kv_attn_many_join_kernel(AttnArgs a, int6
   Seq sq;
   if (!seq_of(a, b, sq) || t < sq.row0 || t >= sq.row0 + sq.n || (int64_t)sq.n * a.group <= a.few_rows) return;
   const int r = (int)(t - sq.row0) * a.group + head % a.group;
-  int lo, hi;
-  many_keys<M>(a, sq, r / M * M, lo, hi);
+  const Seq keys_of = many_keys<M, KT>(a, sq, r / M * M);
+  const int lo = keys_of.lo, hi = keys_of.end;
   const int size = split_size(hi - lo, a.splits, KT);
   const int used = hi > lo ? (hi - lo + size - 1) / size : 1;
   if (used > 1) join_row<DT, D, 1>(a, used, at, [&](int x) { return at * a.splits + x; });
@@ -1382,9 +1494,9 @@ int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 int64_t part_rows_of(const Plan& p) { return p.part_rows > p.many_part_rows ? p.part_rows : p.many_part_rows; }
 int64_t workspace_of(const Plan& p, int D) { return round256(part_rows_of(p) * D * 4) + round256(part_rows_of(p) * 8) + round256((int64_t)p.workers * 16); }
 
-template <int DT, int D, int KT, int NG>
+template <int DT, int D, int KT, int NG, bool EXT>
 void launch_many(const AttnArgs& a, const Plan& p, hipStream_t st) {
-  kv_attn_many_kernel<DT, D, KT, NG><<<linear_grid(p.items * a.hk * a.splits, (int64_t(1) << 23) / NG), 256 * NG, 0, st>>>(a, p.items);
+  kv_attn_many_kernel<DT, D, KT, NG, EXT><<<linear_grid(p.items * a.hk * a.splits, (int64_t(1) << 23) / NG), 256 * NG, 0, st>>>(a, p.items);
   if constexpr (NG == 1)
     if (p.many_part_rows) {
       const int64_t rows = a.tokens * a.hq;
@@ -1392,13 +1504,13 @@ void launch_many(const AttnArgs& a, const Plan& p, hipStream_t st) {
     }
 }
 
-template <int DT, int D>
+template <int DT, int D, bool EXT>
 void launch(AttnArgs& a, const Plan& p, hipStream_t st) {
   // `guards`: blocks that look for rows to clear and, where no unit looks at each sequence, at those, 256 of either
   const int64_t units = p.few ? p.units : 0, guards = ((units || a.tokens > a.seqs ? a.tokens : (int64_t)a.seqs) + 255) / 256;
   const dim3 grid = linear_grid(units + guards);
-  if (p.mt == 1) kv_attn_few_kernel<DT, D, 1><<<grid, 256, 0, st>>>(a, units, guards);
-  else if constexpr (D < 256) kv_attn_few_kernel<DT, D, 2><<<grid, 256, 0, st>>>(a, units, guards);  // more rows of 256 spill
+  if (p.mt == 1) kv_attn_few_kernel<DT, D, 1, EXT><<<grid, 256, 0, st>>>(a, units, guards);
+  else if constexpr (D < 256) kv_attn_few_kernel<DT, D, 2, EXT><<<grid, 256, 0, st>>>(a, units, guards);  // more rows of 256 spill
   if (p.workers) {
     kv_attn_dealt_join_kernel<DT, D><<<(unsigned)p.workers, 256, 0, st>>>(a);
   } else if (p.part_rows) {
@@ -1408,16 +1520,16 @@ void launch(AttnArgs& a, const Plan& p, hipStream_t st) {
   }
   if (!p.many) return;
   a.splits = p.many_splits;
-  if constexpr (D == 256) launch_many<DT, D, 32, 1>(a, p, st);
-  else if (p.groups == 2) launch_many<DT, D, 64, 2>(a, p, st);
-  else launch_many<DT, D, 64, 1>(a, p, st);
+  if constexpr (D == 256) launch_many<DT, D, 32, 1, EXT>(a, p, st);
+  else if (p.groups == 2) launch_many<DT, D, 64, 2, EXT>(a, p, st);
+  else launch_many<DT, D, 64, 1, EXT>(a, p, st);
 }
 
-template <int DT>
+template <int DT, bool EXT>
 void launch_dt(AttnArgs& a, int D, const Plan& p, hipStream_t st) {
-  if (D == 64) launch<DT, 64>(a, p, st);
-  else if (D == 128) launch<DT, 128>(a, p, st);
-  else launch<DT, 256>(a, p, st);
+  if (D == 64) launch<DT, 64, EXT>(a, p, st);
+  else if (D == 128) launch<DT, 128, EXT>(a, p, st);
+  else launch<DT, 256, EXT>(a, p, st);
 }
 
 }  // namespace
@@ -1435,8 +1547,19 @@ extern "C" int64_t pdm_kv_attention_workspace_size(const pdm_kv_attention_desc* 
 extern "C" int pdm_kv_attention_fwd(const pdm_kv_attention_desc* d, const pdm_kv_cache* c, const pdm_kv_batch* b,
                                     const void* q, void* out, float* lse, void* workspace, int64_t workspace_bytes,
                                     int32_t* err_flag, pdm_stream_t stream) {
+  return pdm_kv_attention_biased_fwd(d, nullptr, c, b, q, out, lse, workspace, workspace_bytes, err_flag, stream);
+}
+
+extern "C" int pdm_kv_attention_biased_fwd(const pdm_kv_attention_desc* d, const pdm_kv_attention_bias* x, const pdm_kv_cache* c,
+                                           const pdm_kv_batch* b, const void* q, void* out, float* lse, void* workspace,
+                                           int64_t workspace_bytes, int32_t* err_flag, pdm_stream_t stream) {
   clear_error();
   if (int e = check(__func__, d, c, b)) return e;
+  if (x) {
+    PDM_CHECK_ARG(x->sinks >= 0, "sinks must not be negative");
+    PDM_CHECK_ARG((x->bias != nullptr) == (x->bias_span > 0) && x->bias_span <= (1 << 30), "bias and bias_span (up to 2^30) are given together");
+    PDM_CHECK_ARG(x->bias_start > -(1 << 30) && x->bias_start < (1 << 30), "bias_start must lie in (-2^30, 2^30)");
+  }
   if (b->tokens == 0) return PDM_OK;
   PDM_CHECK_ARG(q && out, "null q / out");
   PDM_CHECK_ARG((reinterpret_cast<uintptr_t>(out) & 15) == 0, "out must be 16-byte aligned");
@@ -1463,8 +1586,10 @@ extern "C" int pdm_kv_attention_fwd(const pdm_kv_attention_desc* d, const pdm_kv
   a.splits = p.splits, a.workers = p.workers, a.row_stride = p.row_stride, a.few_rows = p.few ? 16 * p.mt : 0;
   a.vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && d->q_stride_t % 8 == 0 && d->q_stride_h % 8 == 0;
   a.scale2 = d->scale * 1.44269504088896341f;
-  if (d->dtype == PDM_BF16) launch_dt<PDM_BF16>(a, c->head_dim, p, stream);
-  else launch_dt<PDM_F16>(a, c->head_dim, p, stream);
+  if (x) a.bias = x->bias, a.bias_start = x->bias_start, a.bias_last = x->bias_span - 1, a.sinks = d->window > 0 ? x->sinks : 0;
+  const bool bf16 = d->dtype == PDM_BF16;
+  if (a.bias || a.sinks) bf16 ? launch_dt<PDM_BF16, true>(a, c->head_dim, p, stream) : launch_dt<PDM_F16, true>(a, c->head_dim, p, stream);
+  else bf16 ? launch_dt<PDM_BF16, false>(a, c->head_dim, p, stream) : launch_dt<PDM_F16, false>(a, c->head_dim, p, stream);
   PDM_CHECK_LAUNCH();
   return PDM_OK;
 }

@@ -174,28 +174,38 @@ def kv_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, 
                  v_scale: torch.Tensor, cu_seqlens: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, *,
                  scale: Optional[float] = None, causal: bool = True, window: int = 0,
                  max_q_len: Optional[int] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None,
-                 err_flag: Optional[torch.Tensor] = None):
+                 err_flag: Optional[torch.Tensor] = None, sinks: int = 0, bias: Optional[torch.Tensor] = None,
+                 bias_start: int = 0):
     """Attention of the new tokens q [T, Hq, D] (bf16 or fp16) over the cache, their own keys and values included (call
     :func:`kv_append` first).  Sequences and cache as there; query head h reads key head ``h // (Hq / Hk)``.  A query at
     index p of its sequence sees the keys up to p (``causal``) and none of ``window`` or more tokens before it (``window``
     > 0); ``scale`` defaults to D^-1/2.  Returns out [T, Hq, D], and with ``return_lse`` the fp32 logarithm of each row's
     sum of exponentials [T, Hq].  Rows that see no key and rows behind the last sequence are zeros, with lse -inf.
 
+    ``sinks``: under a window, the first so many tokens stay visible.  ``bias`` [Hq, distances] (fp32 or q's dtype) is added to
+    the scores: ``bias[h, p - j - bias_start]`` for the key j, the column held within the bias (:class:`RelativeBias` makes one;
+    spread it once).  Pages that hold no key that a query sees need not be there: a window's may be given back behind the sinks.
+
     ``max_q_len``: the most new tokens that any sequence has, where the program knows it (1 when decoding); a sequence
     with more is left out and sets ``err_flag``.  Without it the work is laid out for any share of the rows, and a decoding
     batch takes up to half as long again.  Slice ``page_table`` to the columns that the longest sequence needs: its
     width bounds the lengths the work is laid out for."""
-    _no_grad("kv_attention", q, k_codes, v_codes, k_scale, v_scale, out)
+    _no_grad("kv_attention", q, k_codes, v_codes, k_scale, v_scale, out, bias)
     q = _heads(q)
+    if bias is not None:
+        if bias.dtype not in (torch.float32, q.dtype):
+            raise TypeError(f"bias must be float32 or {q.dtype}, got {bias.dtype}")
+        bias = _fp32(bias)
     if _traced(q, direct=out is not None):
         if out is not None:
             raise ValueError("out is not available in a compiled or traced graph")
         out, lse = torch.ops.pdm.kv_attention(q, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens,
                                               q.shape[-1] ** -0.5 if scale is None else scale, causal, window,
-                                              q.shape[0] if max_q_len is None else max_q_len, return_lse, err_flag)
+                                              q.shape[0] if max_q_len is None else max_q_len, return_lse, err_flag, sinks,
+                                              bias, bias_start)
     else:
         out, lse = ops.kv_attention_raw(q, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, scale,
-                                        causal, window, max_q_len, return_lse, out, err_flag)
+                                        causal, window, max_q_len, return_lse, out, err_flag, sinks, bias, bias_start)
     return (out, lse) if return_lse else out
 
 
@@ -267,11 +277,11 @@ class PagedKVCache:
 
     def attend(self, q: torch.Tensor, cu_seqlens: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, *,
                scale: Optional[float] = None, causal: bool = True, window: int = 0, max_q_len: Optional[int] = None,
-               return_lse: bool = False):
+               return_lse: bool = False, sinks: int = 0, bias: Optional[torch.Tensor] = None, bias_start: int = 0):
         """:func:`kv_attention` over this cache."""
         return kv_attention(q, self.k_codes, self.v_codes, self.k_scale, self.v_scale, cu_seqlens, page_table, seq_lens,
                             scale=scale, causal=causal, window=window, max_q_len=max_q_len, return_lse=return_lse,
-                            err_flag=self.err_flag)
+                            err_flag=self.err_flag, sinks=sinks, bias=bias, bias_start=bias_start)
 
     def values(self) -> Tuple[torch.Tensor, torch.Tensor]:
         """The keys and values that the codes stand for, bf16 (exact) [num_pages, n_kv_heads, page_size, head_dim]."""

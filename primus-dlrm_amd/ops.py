@@ -1171,8 +1171,9 @@ def kv_attention_raw(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tens
                      v_scale: torch.Tensor, cu_seqlens: torch.Tensor, page_table: torch.Tensor,
                      seq_lens: torch.Tensor, scale: Optional[float] = None, causal: bool = True, window: int = 0,
                      max_q_len: Optional[int] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None,
-                     err_flag: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """Launches pdm_kv_attention_fwd on q [T, Hq, D]; returns (out, lse or None).  ``max_q_len``: no sequence has more
+                     err_flag: Optional[torch.Tensor] = None, sinks: int = 0, bias: Optional[torch.Tensor] = None,
+                     bias_start: int = 0) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Launches pdm_kv_attention_biased_fwd on q [T, Hq, D]; returns (out, lse or None).  ``max_q_len``: no sequence has more
     new tokens.  Default: T, as if one sequence might have them all; a batch of single tokens then gets equal splits of the
     keys instead of dealt ones (83 us instead of 54 for 64 ragged contexts of 128 to 8,192, 8 key heads of 128) and a launch
     for many rows that finds none."""
@@ -1190,6 +1191,12 @@ def kv_attention_raw(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tens
         raise ValueError("scale must be finite")
     if not 0 <= window < 2 ** 31:
         raise ValueError(f"window must lie in [0, 2^31), got {window}")
+    extra = None
+    if sinks or bias is not None:
+        if not 0 <= sinks < 2 ** 31:
+            raise ValueError(f"sinks must lie in [0, 2^31), got {sinks}")
+        span = _check_bias(bias, hq, bias_start)
+        extra = ctypes.byref(L.KvAttentionBias(_ptr(bias), bias_start, span, sinks, 0))
     if max_q_len is None:
         max_q_len = T
     elif max_q_len < 0:
@@ -1197,7 +1204,7 @@ def kv_attention_raw(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tens
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
         raise ValueError("out must be contiguous and of q's shape and dtype")
     _check_err_flag(err_flag)
-    index = _gpu_index(q, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, out, err_flag)
+    index = _gpu_index(q, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, out, err_flag, bias)
     given = out
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -1211,9 +1218,9 @@ def kv_attention_raw(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tens
         raise L.PdmError(ws_bytes, "pdm_kv_attention_workspace_size", L.last_error())
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     with _on_device(index):
-        L.check(lib.pdm_kv_attention_fwd(
-            ctypes.byref(desc), ctypes.byref(cache), ctypes.byref(batch), q.data_ptr(), out.data_ptr(), _ptr(lse),
-            _ptr(ws), ws_bytes, _ptr(err_flag), L.raw_stream(index)), "pdm_kv_attention_fwd")
+        L.check(lib.pdm_kv_attention_biased_fwd(
+            ctypes.byref(desc), extra, ctypes.byref(cache), ctypes.byref(batch), q.data_ptr(), out.data_ptr(), _ptr(lse),
+            _ptr(ws), ws_bytes, _ptr(err_flag), L.raw_stream(index)), "pdm_kv_attention_biased_fwd")
     if given is not None or err_flag is not None:
         _written(given, err_flag)
     return out, lse
@@ -1223,16 +1230,17 @@ def kv_attention_raw(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tens
 def kv_attention_op(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor,
                     v_scale: torch.Tensor, cu_seqlens: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
                     scale: float, causal: bool, window: int, max_q_len: int, return_lse: bool,
-                    err_flag: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+                    err_flag: Optional[torch.Tensor], sinks: int = 0, bias: Optional[torch.Tensor] = None,
+                    bias_start: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
     """Without ``return_lse`` the second output is empty."""
     out, lse = kv_attention_raw(q, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, scale, causal,
-                                window, max_q_len, return_lse, None, err_flag)
+                                window, max_q_len, return_lse, None, err_flag, sinks, bias, bias_start)
     return out, q.new_empty(0, dtype=torch.float32) if lse is None else lse
 
 
 @kv_attention_op.register_fake
 def _(q, k_codes, v_codes, k_scale, v_scale, cu_seqlens, page_table, seq_lens, scale, causal, window, max_q_len,
-      return_lse, err_flag):
+      return_lse, err_flag, sinks=0, bias=None, bias_start=0):
     return (q.new_empty(q.shape),
             q.new_empty(q.shape[:2] if return_lse else (0,), dtype=torch.float32))
 
