@@ -21,23 +21,26 @@ int jag_inputs(const char* fn, JagArgs& a, const pdm_jagged_attention_desc* d, c
 
 namespace {
 
-constexpr int M = 128, KT = 64;
+constexpr int M = 128;
 constexpr int kOut = -5;     // |dO| below 2^kOut after its power of two
 constexpr int kNone = -100;  // exponent of rows of zeros
 
 __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
 
 // ---- by queries -----------------------------------------------------------------------
-// Gradients of the bias: a wave adds its dS of a tile to a window of 95 distances in LDS, the two halves of the wave to one
-// each, so that no two lanes of an instruction meet.  Distances fall from tile to tile, and a thread sums those that are its
-// number modulo 256 and writes each once, when the tiles have passed it.
+// Gradients of the bias: sums along the diagonals of dS.  A wave writes 32 x 32 of them to LDS, row r shifted by 31 - r places in
+// a line of 64 (the places that no row has stay zero), reads the lines back, a lane the sum of its place, and leaves its 63
+// distances in a window.  (Atomic adds to LDS instead took 1,172 us for the sequences of 1,001 to 2,777 tokens below.)
+// Distances fall from tile to tile; a thread sums those that are its number modulo 256 over the windows of the waves and writes
+// each once, when the tiles have passed it.
 template <int DT, int D, bool BIAS, bool GB>
 __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units) {
-  constexpr int KK = D / 16, DD = D / 32;
+  constexpr int KK = D / 16, DD = D / 32, KT = D == 64 ? 64 : 32, XX = KT / 32;  // (LDS for two workgroups on a CU)
   __shared__ alignas(1024) char sk[2][KT * Tile<D>::RS];
   __shared__ alignas(1024) char sv[2][KT * Tile<D>::RS];
   __shared__ float sb[2][BIAS ? M + KT : 1];
-  __shared__ float win[2][GB ? 4 : 1][2][GB ? 96 : 1];
+  __shared__ float win[2][GB ? 4 : 1][XX][GB ? 64 : 1];
+  __shared__ float skew[GB ? 4 : 1][GB ? 32 : 1][64];
   __shared__ float ends[GB ? 8 : 1];
 
   const int64_t unit = linear_block();
@@ -144,16 +147,16 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
     }
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const int x = rel - 32 * w;
-      if (x >= 0 && x < 95) {
-        sum += win[t & 1][w][0][x] + win[t & 1][w][1][x];
-        win[t & 1][w][0][x] = 0.0f, win[t & 1][w][1][x] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < XX; ++x) {
+        const int place = rel - 32 * w - 32 * (XX - 1 - x);
+        if (place >= 0 && place < 63) sum += win[t & 1][w][x][place];
       }
     }
   };
   if (GB) {
-    float* w = &win[0][0][0][0];
-    for (int i = tid; i < 2 * 4 * 2 * 96; i += 256) w[i] = 0.0f;
+    float* w = &skew[0][0][0];
+    for (int i = tid; i < 4 * 32 * 64; i += 256) w[i] = 0.0f;
     if (hx == 0 && tid == 0) {
       a.part_range[2 * item] = keys.tiles ? off + r0 - jag_key<KT>(keys, keys.tiles - 1) - (KT - 1) : 1;
       a.part_range[2 * item + 1] = keys.tiles ? off + r0 - jag_key<KT>(keys, 0) + M - 1 : 0;
@@ -175,20 +178,25 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
     lds_barrier();  // the tile is there, and the one before it is done with
     if (t + 1 < keys.tiles) load(t + 1);
     if (GB && t > 0) gather(t - 1);
-    if (w0 >= s.nq || (a.causal && key > p_last) || (a.window > 0 && key + KT - 1 <= p_first - a.window && key >= a.sinks)) continue;
+    if (w0 >= s.nq || (a.causal && key > p_last) || (a.window > 0 && key + KT - 1 <= p_first - a.window && key >= a.sinks)) {
+#pragma unroll
+      for (int x = 0; x < XX; ++x)
+        if (GB) win[t & 1][wave][x][lane] = 0.0f;
+      continue;
+    }
     const char *tk = sk[t & 1], *tv = sv[t & 1];
     const bool whole = key + KT <= s.nk && (!a.causal || key + KT - 1 <= p_first) &&
                        (a.window == 0 || key > p_last - a.window || key + KT <= a.sinks);
     auto sees = [&](int j) { return (uint32_t)(key + j - row_lo) < (uint32_t)row_n || key + j < row_first; };
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < XX; ++x) {
       f32x16_t sc = zero16, dp = zero16;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) sc = mfma32<DT>(Tile<D>::rows(tk, row_at, 32 * x, kk), q[kk], sc);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) dp = mfma32<DT>(Tile<D>::rows(tv, row_at, 32 * x, kk), g[kk], dp);
       float ds[16];
-      const int local = c - 32 * x - 4 * h + KT - 1;  // of the window of a wave, less 8 (e / 4) + e % 4
+      const int local = c - 32 * x - 4 * h + KT - 1;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int j = 8 * (e >> 2) + (e & 3);
@@ -203,26 +211,38 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
       if (GB) {
         const int first = p_first - key - 32 * x - 31 - a.bias_start, last = first + 62;  // columns of the wave's pairs
         const int col = pos - key - 32 * x - 4 * h - a.bias_start;
-        float* wp = &win[t & 1][wave][h][0];
+        float along = 0.0f;
         if (first >= a.bias_last) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) far += ds[e];
         } else if (last < 0) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) near += ds[e];
-        } else if (first >= 0 && last < a.bias_last) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            __hip_atomic_fetch_add(wp + local - 8 * (e >> 2) - (e & 3), ds[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         } else {
+          float* line = &skew[wave][4 * h][c + 31 - 4 * h];
+          if (first >= 0 && last < a.bias_last) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int j = 8 * (e >> 2) + (e & 3), x = col - j;
-            if (x >= a.bias_last) far += ds[e];
-            else if (x < 0) near += ds[e];
-            else __hip_atomic_fetch_add(wp + local - j, ds[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            for (int e = 0; e < 16; ++e) line[(8 * (e >> 2) + (e & 3)) * 63] = ds[e];
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int j = 8 * (e >> 2) + (e & 3), y = col - j;
+              far += y >= a.bias_last ? ds[e] : 0.0f;
+              near += y < 0 ? ds[e] : 0.0f;
+              line[j * 63] = y >= 0 && y < a.bias_last ? ds[e] : 0.0f;
+            }
           }
+          __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+          __builtin_amdgcn_wave_barrier();
+          __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+#pragma unroll
+          for (int r = 0; r < 32; r += 4)
+            along += (skew[wave][r][lane] + skew[wave][r + 1][lane]) + (skew[wave][r + 2][lane] + skew[wave][r + 3][lane]);
+          __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+          __builtin_amdgcn_wave_barrier();
+          __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
         }
+        win[t & 1][wave][x][lane] = along;
       }
       u32x4_t w[2];
 #pragma unroll
@@ -274,72 +294,108 @@ __global__ void __launch_bounds__(1024) jag_dbias_kernel(JagArgs a) {
 }
 
 // ---- by keys ----------------------------------------------------------------------------
-template <int DT, int D, bool BIAS>
-__global__ void __launch_bounds__(256, D == 64 ? 2 : 1) jag_dkv_kernel(JagArgs a, int64_t items, int64_t units) {
-  constexpr int KK = D / 16, DD = D / 32, QT = 64;
+// A workgroup takes 128 keys of a key head, 32 a wave, and walks the queries that see them under the window, head by head of the
+// group.  Sums of 128 elements take half of the registers of two waves, so there K is read from LDS for every product.
+//
+// First tokens that stay visible (SINK) have many more queries than other keys: those beyond the window are a kernel of their
+// own, a workgroup per 32 such keys and a share of these queries, which its waves take in turn.  Both leave sums in fp32, which
+// jag_sinks_kernel joins and rounds.
+__device__ __forceinline__ int64_t sink_slots(const JagArgs& a, int b, int block, int kh) {
+  return (((int64_t)b * a.sink_blocks + block) * a.hk + kh) * (a.sink_shares + 1);
+}
+
+template <int DT, int D, bool BIAS, bool SINK>
+__global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, int64_t units) {
+  constexpr int KK = D / 16, DD = D / 32;
+  constexpr int QT = SINK ? 128 : D == 64 ? 64 : 32, KEYS = SINK ? 32 : M;
+  constexpr bool KL = D == 128 && !SINK;   // K in LDS
   __shared__ alignas(1024) char sq[2][QT * Tile<D>::RS];
   __shared__ alignas(1024) char sg[2][QT * Tile<D>::RS];
-  __shared__ float sb[2][BIAS ? M + QT : 1];
+  __shared__ alignas(1024) char sk[KL ? KEYS * Tile<D>::RS : 16];
+  __shared__ float sb[2][BIAS ? KEYS + QT : 1];
   __shared__ float ss[2][3][QT];
 
   const int64_t unit = linear_block();
-  if (unit >= units) {
-    const int64_t first = (unit - units) * 256;
-    if (first >= a.k_tokens && first >= a.seqs) return;
-    jag_guard(a, a.cu_k, a.k_tokens, first, [&](int64_t t) {
-      clear_row(a.dk, t * a.hk * D, a.hk * D);
-      clear_row(a.dv, t * a.hk * D, a.hk * D);
-    });
-    return;
-  }
-  const int kh = (int)(unit % a.hk);
-  JagSeq s;
-  int b, j0;
-  if (!jag_block<M>(a, a.cu_k, unit / a.hk, s, b, j0)) return;
-
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
-  const int off = s.nk - s.nq;
+  JagSeq s;
+  int b, j0, kh, share = 0;
+  if constexpr (SINK) {
+    if (unit >= units) return;
+    share = (int)(unit % a.sink_shares);
+    int64_t x = unit / a.sink_shares;
+    kh = (int)(x % a.hk), x /= a.hk;
+    j0 = (int)(x % a.sink_blocks) * KEYS, b = (int)(x / a.sink_blocks);
+    if (!jag_seq(a, b, s) || j0 >= s.nk) return;
+  } else {
+    if (unit >= units) {
+      const int64_t first = (unit - units) * 256;
+      if (first >= a.k_tokens && first >= a.seqs) return;
+      jag_guard(a, a.cu_k, a.k_tokens, first, [&](int64_t t) {
+        clear_row(a.dk, t * a.hk * D, a.hk * D);
+        clear_row(a.dv, t * a.hk * D, a.hk * D);
+      });
+      return;
+    }
+    kh = (int)(unit % a.hk);
+    if (!jag_block<M>(a, a.cu_k, unit / a.hk, s, b, j0)) return;
+  }
+  const int off = s.nk - s.nq, jw = SINK ? j0 : j0 + wave * 32;
   // queries that see a key of the block
-  const int j1 = (j0 + M < s.nk ? j0 + M : s.nk) - 1;
-  int i_lo = a.causal && j0 - off > 0 ? (j0 - off) & ~(QT - 1) : 0, i_hi = s.nq;
-  if (a.window > 0 && j0 >= a.sinks && j1 + a.window - off < i_hi) i_hi = j1 + a.window - off;
-  const int tiles = i_hi > i_lo ? (i_hi - i_lo + QT - 1) / QT : 0, all = tiles * a.group;
+  const int j1 = (j0 + KEYS < s.nk ? j0 + KEYS : s.nk) - 1;
+  int i_lo = a.causal && j0 - off > 0 ? j0 - off : 0, i_hi = s.nq;
+  if (SINK) i_lo = j0 + a.window - off > 0 ? j0 + a.window - off : 0;
+  else if (a.window > 0 && j1 + a.window - off < i_hi) i_hi = j1 + a.window - off;
+  i_lo &= ~(QT - 1);
+  const int tiles = i_hi > i_lo ? (i_hi - i_lo + QT - 1) / QT : 0;
+  const int64_t all = (int64_t)tiles * a.group;
+  const int n0 = SINK ? (int)(all * share / a.sink_shares) : 0, n1 = SINK ? (int)(all * (share + 1) / a.sink_shares) : (int)all;
 
-  // this lane's key and the queries that see it: [see_lo, see_lo + see_n)
-  const int key = j0 + wave * 32 + c;
+  // this lane's key and the queries that see it here: [see_lo, see_lo + see_n)
+  const int key = jw + c;
   const bool there = key < s.nk;
   int see_lo = 0, see_n = 0;
-  if (there) {
-    see_lo = a.causal && key - off > 0 ? key - off : 0;
-    const int hi = a.window > 0 && key >= a.sinks && key + a.window - off < s.nq ? key + a.window - off : s.nq;
+  if (there && !(SINK && key >= a.sinks)) {
+    const int edge = key + a.window - off;
+    see_lo = SINK ? (edge > 0 ? edge : 0) : a.causal && key - off > 0 ? key - off : 0;
+    const int hi = !SINK && a.window > 0 && edge < s.nq ? edge : s.nq;
     see_n = hi > see_lo ? hi - see_lo : 0;
   }
-  u32x4_t kf[KK], vf[KK];
+  u32x4_t kf[KL ? 1 : KK], vf[KK];
   {
     const uint16_t* x = static_cast<const uint16_t*>(a.k) + (s.k0 + key) * a.k_st + kh * a.k_sh + 8 * h;
     const uint16_t* y = static_cast<const uint16_t*>(a.v) + (s.k0 + key) * a.v_st + kh * a.v_sh + 8 * h;
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) kf[kk] = load16(x + 16 * kk, there), vf[kk] = load16(y + 16 * kk, there);
+    for (int kk = 0; kk < KK; ++kk) {
+      if constexpr (!KL) kf[kk] = load16(x + 16 * kk, there);
+      vf[kk] = load16(y + 16 * kk, there);
+    }
   }
-  const int jw = j0 + wave * 32;
+  if constexpr (KL) {
+    Bring<D, KEYS> bring_k;
+    bring_k.init(a.k_st, lane, wave);
+    bring_k.load(static_cast<const uint16_t*>(a.k) + s.k0 * a.k_st + kh * a.k_sh, a.k_st, j0, s.nk, sk, wave);
+  }
 
   Bring<D, QT> bring_q, bring_g;
   const int64_t g_st = (int64_t)a.hq * D;
   bring_q.init(a.q_st, lane, wave);
   bring_g.init(g_st, lane, wave);
-  float bias_next = 0.0f, stat_next = 0.0f;
-  int head_next = 0, tile_next = 0;
+  float bias_next = 0.0f, stat_next[QT == 128 ? 2 : 1];
+  int head_next = tiles ? n0 / tiles : 0, tile_next = tiles ? n0 % tiles : 0;
   auto load = [&](int n) {  // the head and tile at which the next load stands
     const int head = kh * a.group + head_next, i = i_lo + tile_next * QT;
     bring_q.load(static_cast<const uint16_t*>(a.q) + s.q0 * a.q_st + head * a.q_sh, a.q_st, i, s.nq, sq[n & 1], wave);
     bring_g.load(static_cast<const uint16_t*>(a.dout) + s.q0 * g_st + head * D, g_st, i, s.nq, sg[n & 1], wave);
-    if (BIAS && tid < M + QT) bias_next = bias2(a, a.bias + (int64_t)head * (a.bias_last + 1), (int64_t)off + i + tid - (M - 1) - j0);
-    stat_next = 0.0f;
-    const int r = i + (tid & (QT - 1));
-    if (tid < 3 * QT && r < s.nq) {
-      const int64_t at = (s.q0 + r) * a.hq + head;
-      stat_next = tid < QT ? a.stats[2 * at] : tid < 2 * QT ? a.stats[2 * at + 1] : a.delta[at];
+    if (BIAS && tid < KEYS + QT) bias_next = bias2(a, a.bias + (int64_t)head * (a.bias_last + 1), (int64_t)off + i + tid - (KEYS - 1) - j0);
+#pragma unroll
+    for (int u = 0; u < (QT == 128 ? 2 : 1); ++u) {
+      const int x = tid + 256 * u, r = i + (x & (QT - 1));
+      stat_next[u] = 0.0f;
+      if (x < 3 * QT && r < s.nq) {
+        const int64_t at = (s.q0 + r) * a.hq + head;
+        stat_next[u] = x < QT ? a.stats[2 * at] : x < 2 * QT ? a.stats[2 * at + 1] : a.delta[at];
+      }
     }
     if (++tile_next == tiles) tile_next = 0, ++head_next;
   };
@@ -352,28 +408,36 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) jag_dkv_kernel(JagArgs a
   int power = 100;  // fp16: dk holds sums times 2^power
   const int64_t item0 = (int64_t)a.cu_q[b] / M + b;
 
-  if (all > 0) load(0);
-  int hh = 0, tt = 0;
+  int hh = head_next, tt = tile_next;
+  if (n1 > n0) load(n0);
 #pragma unroll 1
-  for (int n = 0; n < all; ++n) {
+  for (int n = n0; n < n1; ++n) {
     const int i0 = i_lo + tt * QT, head = kh * a.group + hh;
     if (++tt == tiles) tt = 0, ++hh;
-    if (BIAS && tid < M + QT) sb[n & 1][tid] = bias_next;
-    if (tid < 3 * QT) ss[n & 1][tid / QT][tid & (QT - 1)] = stat_next;
+    if (BIAS && tid < KEYS + QT) sb[n & 1][tid] = bias_next;
+#pragma unroll
+    for (int u = 0; u < (QT == 128 ? 2 : 1); ++u)
+      if (tid + 256 * u < 3 * QT) (&ss[n & 1][0][0])[tid + 256 * u] = stat_next[u];
     brought();
     lds_barrier();  // the tile is there, and the one before it is done with
-    if (n + 1 < all) load(n + 1);
+    if (n + 1 < n1) load(n + 1);
     const char *tq = sq[n & 1], *tg = sg[n & 1];
 #pragma unroll
-    for (int x = 0; x < QT / 32; ++x) {
-      const int i = i0 + 32 * x, p0 = off + i;
-      if (i >= s.nq || jw >= s.nk || (a.causal && p0 + 31 < jw) || (a.window > 0 && p0 >= jw + 31 + a.window && jw >= a.sinks)) continue;
-      const bool whole = i + 32 <= s.nq && jw + 32 <= s.nk && (!a.causal || p0 >= jw + 31) &&
-                         (a.window == 0 || p0 + 31 < jw + a.window || jw + 32 <= a.sinks);
+    for (int y0 = 0; y0 < (SINK ? 1 : QT / 32); ++y0) {
+      const int x = SINK ? wave : y0, i = i0 + 32 * x, p0 = off + i;
+      if (i >= s.nq || jw >= s.nk) continue;
+      if (SINK ? p0 + 31 < jw + a.window : (a.causal && p0 + 31 < jw) || (a.window > 0 && p0 >= jw + 31 + a.window)) continue;
+      const bool whole = i + 32 <= s.nq && jw + 32 <= (SINK ? a.sinks : s.nk) &&
+                         (SINK ? p0 >= jw + 31 + a.window : (!a.causal || p0 >= jw + 31) && (a.window == 0 || p0 + 31 < jw + a.window));
       auto sees = [&](int r) { return (uint32_t)(i0 + r - see_lo) < (uint32_t)see_n; };
       f32x16_t sc = zero16, dp = zero16;
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) sc = mfma32<DT>(Tile<D>::rows(tq, row_at, 32 * x, kk), kf[kk], sc);
+      for (int kk = 0; kk < KK; ++kk) {
+        u32x4_t f;
+        if constexpr (KL) f = Tile<D>::rows(sk, row_at, 32 * wave, kk);
+        else f = kf[kk];
+        sc = mfma32<DT>(Tile<D>::rows(tq, row_at, 32 * x, kk), f, sc);
+      }
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) dp = mfma32<DT>(Tile<D>::rows(tg, row_at, 32 * x, kk), vf[kk], dp);
       float ahead = 1.0f;
@@ -396,7 +460,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) jag_dkv_kernel(JagArgs a
 #pragma unroll
         for (int z = 0; z < 4; ++z) {
           const int e = 4 * y + z;
-          const float w = BIAS ? __builtin_fmaf(sc[e], a.scale2, sb[n & 1][r + z - wave * 32 - c + M - 1]) : sc[e] * a.scale2;
+          const float w = BIAS ? __builtin_fmaf(sc[e], a.scale2, sb[n & 1][r + z - (jw - j0) - c + KEYS - 1]) : sc[e] * a.scale2;
           p[e] = __builtin_amdgcn_exp2f(w - m[z]) * inv[z];
           ds[e] = p[e] * (dp[e] - delta[z]);
         }
@@ -420,8 +484,39 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) jag_dkv_kernel(JagArgs a
       else add_cols<DT, D, 2>(dk, tq, col_at, 32 * x, dw);
     }
   }
+  const float back = DT == PDM_F16 ? pow2(-power) : 1.0f;
+  // sums of a sink's block in fp32: [dk, dv][d][32 keys]
+  auto sums_of = [&](int block, int slot) { return a.sink_part + (sink_slots(a, b, block, kh) + slot) * (2 * D * 32); };
+  if constexpr (SINK) {
+    float* to = sums_of(j0 / 32, share);
+    float* mine = reinterpret_cast<float*>(wave < 2 ? sq[wave & 1] : sg[wave & 1]);  // QT rows of a tile: D x 32 floats and more
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      __syncthreads();  // the tiles, or the sums before, are done with
+#pragma unroll
+      for (int d = 0; d < DD; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mine[(32 * d + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + c] = z ? dv[d][e] : dk[d][e] * back;
+      __syncthreads();
+      for (int x = tid; x < D * 32; x += 256)
+        to[z * D * 32 + x] = (reinterpret_cast<const float*>(sq[0])[x] + reinterpret_cast<const float*>(sq[1])[x]) +
+                             (reinterpret_cast<const float*>(sg[0])[x] + reinterpret_cast<const float*>(sg[1])[x]);
+    }
+    return;
+  }
+  if (a.sink_blocks > jw / 32 && jw < s.nk) {
+    float* to = sums_of(jw / 32, a.sink_shares);
+#pragma unroll
+    for (int d = 0; d < DD; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int x = (32 * d + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + c;
+        to[x] = dk[d][e] * back, to[D * 32 + x] = dv[d][e];
+      }
+    return;
+  }
   if (!there) return;
-  const float back = DT == PDM_F16 ? a.scale * pow2(-power) : a.scale;
+  const float f = a.scale * back;
   const int64_t at = ((s.k0 + key) * a.hk + kh) * D;
 #pragma unroll
   for (int d = 0; d < DD; ++d)
@@ -430,8 +525,28 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) jag_dkv_kernel(JagArgs a
       const int64_t x = at + 32 * d + 2 * e + 4 * h;
       *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.dv) + x) = u32x2_t{pack2<DT>(dv[d][e], dv[d][e + 1]), pack2<DT>(dv[d][e + 2], dv[d][e + 3])};
       *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.dk) + x) =
-          u32x2_t{pack2<DT>(dk[d][e] * back, dk[d][e + 1] * back), pack2<DT>(dk[d][e + 2] * back, dk[d][e + 3] * back)};
+          u32x2_t{pack2<DT>(dk[d][e] * f, dk[d][e + 1] * f), pack2<DT>(dk[d][e + 2] * f, dk[d][e + 3] * f)};
     }
+}
+
+// Gradients of 32 sinks of a key head: their sums under the window and beyond it.
+template <int DT, int D>
+__global__ void __launch_bounds__(256) jag_sinks_kernel(JagArgs a, int64_t units) {
+  const int64_t unit = linear_block();
+  if (unit >= units) return;
+  const int kh = (int)(unit % a.hk);
+  const int64_t x = unit / a.hk;
+  const int j0 = (int)(x % a.sink_blocks) * 32, b = (int)(x / a.sink_blocks);
+  JagSeq s;
+  if (!jag_seq(a, b, s)) return;
+  const float* from = a.sink_part + sink_slots(a, b, j0 / 32, kh) * (2 * D * 32);
+  for (int i = threadIdx.x; i < 2 * D * 32; i += 256) {
+    const int z = i / (D * 32), key = j0 + i % 32, d = i / 32 % D;
+    if (key >= s.nk) continue;
+    float sum = 0.0f;
+    for (int n = 0; n <= a.sink_shares; ++n) sum += from[(int64_t)n * (2 * D * 32) + i];
+    static_cast<uint16_t*>(z ? a.dv : a.dk)[((s.k0 + key) * a.hk + kh) * D + d] = (uint16_t)pack2<DT>(z ? sum : sum * a.scale, 0.0f);
+  }
 }
 
 // ---- host -------------------------------------------------------------------------------
@@ -443,15 +558,28 @@ int64_t part_cols(const JagArgs& a) {
   return reach < 0 ? 0 : reach < a.bias_last ? reach : a.bias_last;
 }
 
+// Blocks of 32 sinks of a sequence, and the shares that the queries beyond the window are dealt to: about 1,024 workgroups, each
+// of 8 tiles and more on average.
+void sinks_of(JagArgs& a) {
+  a.sink_blocks = a.seqs && a.q_tokens ? (a.sinks + 31) / 32 : 0;
+  if (!a.sink_blocks) return;
+  const int64_t units = (int64_t)a.seqs * a.sink_blocks * a.hk, most = a.group * (a.q_tokens / a.seqs) / (8 * 128);
+  int64_t shares = 1024 / units;
+  shares = shares < most ? shares : most;
+  a.sink_shares = (int32_t)(shares > 1 ? shares : 1);
+}
+
 struct Space {
-  int64_t delta, expo, range, part, total;
+  int64_t delta, expo, range, part, sinks, total;
 };
-Space space_of(const JagArgs& a, int dtype, bool gb) {
+Space space_of(JagArgs& a, int dtype, int head_dim, bool gb) {
+  sinks_of(a);
   Space s{};
   s.expo = round256(a.q_tokens * a.hq * 4);
   s.range = s.expo + round256(dtype == PDM_F16 ? a.items * 16 * a.hq : 0);
   s.part = s.range + round256(gb ? a.items * 8 : 0);
-  s.total = s.part + round256(gb ? a.items * a.hq * (part_cols(a) + 2) * 4 : 0);
+  s.sinks = s.part + round256(gb ? a.items * a.hq * (part_cols(a) + 2) * 4 : 0);
+  s.total = s.sinks + (int64_t)a.seqs * a.sink_blocks * a.hk * (a.sink_shares + 1) * 2 * head_dim * 32 * 4;
   return s;
 }
 
@@ -470,7 +598,12 @@ void launch(const JagArgs& a, hipStream_t st) {
   if (a.dbias) jag_dbias_kernel<<<dim3(a.bias_last / 64 + 1, a.hq), 1024, 0, st>>>(a);
   if (a.k_tokens > 0) {
     const int64_t items = a.seqs ? a.k_tokens / M + a.seqs : 0, units = items * a.hk, most = a.k_tokens > a.seqs ? a.k_tokens : a.seqs;
-    jag_dkv_kernel<DT, D, BIAS><<<linear_grid(units + (most + 255) / 256), 256, 0, st>>>(a, items, units);
+    jag_dkv_kernel<DT, D, BIAS, false><<<linear_grid(units + (most + 255) / 256), 256, 0, st>>>(a, units);
+    if (a.sink_blocks) {
+      const int64_t blocks = (int64_t)a.seqs * a.sink_blocks * a.hk;
+      jag_dkv_kernel<DT, D, BIAS, true><<<linear_grid(blocks * a.sink_shares), 256, 0, st>>>(a, blocks * a.sink_shares);
+      jag_sinks_kernel<DT, D><<<linear_grid(blocks), 256, 0, st>>>(a, blocks);
+    }
   }
 }
 
@@ -484,7 +617,7 @@ extern "C" int64_t pdm_jagged_attention_bwd_workspace_size(const pdm_jagged_atte
   JagArgs a{};
   if (int e = jag_args(__func__, desc, a)) return e;
   PDM_CHECK_ARG(!with_grad_bias || desc->bias_span > 0, "grad_bias without a bias");
-  return space_of(a, desc->dtype, with_grad_bias != 0).total;
+  return space_of(a, desc->dtype, desc->head_dim, with_grad_bias != 0).total;
 }
 
 extern "C" int pdm_jagged_attention_bwd(const pdm_jagged_attention_desc* desc, const void* q, const void* k, const void* v,
@@ -501,7 +634,7 @@ extern "C" int pdm_jagged_attention_bwd(const pdm_jagged_attention_desc* desc, c
   PDM_CHECK_ARG(!grad_bias || (bias && (a.q_tokens == 0 || out_rest)), "grad_bias without bias or out_rest");
   for (const void* p : {out, out_rest, grad_out, (const void*)grad_q, (const void*)grad_k, (const void*)grad_v})
     PDM_CHECK_ARG((reinterpret_cast<uintptr_t>(p) & 15) == 0, "outputs and their gradients must be 16-byte aligned");
-  const Space sp = space_of(a, desc->dtype, grad_bias != nullptr);
+  const Space sp = space_of(a, desc->dtype, desc->head_dim, grad_bias != nullptr);
   if (sp.total && (!workspace || workspace_bytes < sp.total)) {
     set_error(std::string(__func__) + ": workspace of " + std::to_string(sp.total) + " bytes needed");
     return PDM_ERR_WORKSPACE;
@@ -512,6 +645,7 @@ extern "C" int pdm_jagged_attention_bwd(const pdm_jagged_attention_desc* desc, c
   a.dout = grad_out, a.dlse = grad_lse, a.dq = grad_q, a.dk = grad_k, a.dv = grad_v, a.dbias = grad_bias;
   a.delta = reinterpret_cast<float*>(ws), a.expo = reinterpret_cast<int32_t*>(ws + sp.expo);
   a.part_range = reinterpret_cast<int32_t*>(ws + sp.range), a.part = reinterpret_cast<float*>(ws + sp.part);
+  a.sink_part = reinterpret_cast<float*>(ws + sp.sinks);
   a.part_stride = grad_bias ? part_cols(a) + 2 : 0;
   if (a.q_tokens == 0 && grad_bias) a.items = 0;  // nothing was written that could be summed
   const bool bf16 = desc->dtype == PDM_BF16, biased = bias != nullptr;
