@@ -95,6 +95,15 @@ __global__ void __launch_bounds__(256, 2) jag_fwd_kernel(JagArgs a, int64_t unit
   for (int d = 0; d < DD; ++d) o[d] = zero16;
   const uint32_t row_at = Tile<D>::row_at(lane), col_at = Tile<D>::col_at(lane);
 
+  // of a tile: no query of this wave sees a key; every one sees all keys; of a key: this lane's query sees it
+  auto unseen = [&](int key) {
+    return w0 >= s.nq || (a.causal && key > p_last) || (a.window > 0 && key + KT - 1 <= p_first - a.window && key >= a.sinks);
+  };
+  auto all_seen = [&](int key) {
+    return key + KT <= s.nk && (!a.causal || key + KT - 1 <= p_first) && (a.window == 0 || key > p_last - a.window || key + KT <= a.sinks);
+  };
+  auto sees = [&](int j) { return (uint32_t)(j - row_lo) < (uint32_t)row_n || j < row_first; };
+  bool odd = false;
   if (keys.tiles > 0) load(0);
 #pragma unroll 1
   for (int t = 0; t < keys.tiles; ++t) {
@@ -104,9 +113,8 @@ __global__ void __launch_bounds__(256, 2) jag_fwd_kernel(JagArgs a, int64_t unit
     lds_barrier();  // the tile is there, and the one before it is done with
     if (t + 1 < keys.tiles) load(t + 1);
     const char *tk = sk[t & 1], *tv = sv[t & 1];
-    if (w0 >= s.nq || (a.causal && key > p_last) || (a.window > 0 && key + KT - 1 <= p_first - a.window && key >= a.sinks)) continue;
-    const bool whole = key + KT <= s.nk && (!a.causal || key + KT - 1 <= p_first) &&
-                       (a.window == 0 || key > p_last - a.window || key + KT <= a.sinks);
+    if (unseen(key)) continue;
+    const bool whole = all_seen(key);
     f32x16_t sc[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -121,10 +129,9 @@ __global__ void __launch_bounds__(256, 2) jag_fwd_kernel(JagArgs a, int64_t unit
       const int j = 32 * (e >> 4) + 8 * ((e >> 2) & 3) + (e & 3);  // and 4 h: the element's key
       w[e] = BIAS ? __builtin_fmaf(sc[e >> 4][e & 15], a.scale2, sb[t & 1][bias_at - j]) : sc[e >> 4][e & 15] * a.scale2;
     }
-    auto sees = [&](int j) { return (uint32_t)(key + j - row_lo) < (uint32_t)row_n || key + j < row_first; };
     if (!whole) {
 #pragma unroll
-      for (int e = 0; e < 32; ++e) w[e] = sees(4 * h + 32 * (e >> 4) + 8 * ((e >> 2) & 3) + (e & 3)) ? w[e] : -kInf;
+      for (int e = 0; e < 32; ++e) w[e] = sees(key + 4 * h + 32 * (e >> 4) + 8 * ((e >> 2) & 3) + (e & 3)) ? w[e] : -kInf;
     }
     float top = w[0];
 #pragma unroll
@@ -149,8 +156,20 @@ __global__ void __launch_bounds__(256, 2) jag_fwd_kernel(JagArgs a, int64_t unit
       p[e >> 2][e & 3] = pack2<DT>(w[2 * e], w[2 * e + 1]);
       if (FINE) rest[e >> 2][e & 3] = left2<DT>(w[2 * e], w[2 * e + 1], p[e >> 2][e & 3]);
     }
-    if (!whole && odd_rows<DT, D, 4>(tv, col_at, 0)) add_cols_odd<DT, D, 4, FINE>(o, tv, col_at, 0, p, sees, rest);
-    else add_cols<DT, D, 4, FINE>(o, tv, col_at, 0, p, rest);
+    const bool careful = !whole && odd_rows<DT, D, 4>(tv, col_at, 0);
+    odd = odd || careful;
+    add_cols<DT, D, 4, FINE>(o, tv, col_at, 0, p, careful, rest);
+  }
+  if (__syncthreads_or(odd)) {
+#pragma unroll 1
+    for (int t = 0; t < keys.tiles; ++t) {
+      const int key = jag_key<KT>(keys, t);
+      load(t);
+      brought();
+      __syncthreads();
+      if (!unseen(key) && !all_seen(key)) mark_cols<DT, D, 4>(o, sv[t & 1], col_at, 0, [&](int j) { return sees(key + j); });
+      __syncthreads();
+    }
   }
 
   const float sum = l + __shfl_xor(l, 32);

@@ -169,6 +169,14 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   for (int d = 0; d < DD; ++d) dq[d] = zero16;
   const uint32_t row_at = Tile<D>::row_at(lane), col_at = Tile<D>::col_at(lane);
 
+  auto unseen = [&](int key) {  // (as in the forward pass)
+    return w0 >= s.nq || (a.causal && key > p_last) || (a.window > 0 && key + KT - 1 <= p_first - a.window && key >= a.sinks);
+  };
+  auto all_seen = [&](int key) {
+    return key + KT <= s.nk && (!a.causal || key + KT - 1 <= p_first) && (a.window == 0 || key > p_last - a.window || key + KT <= a.sinks);
+  };
+  auto sees = [&](int j) { return (uint32_t)(j - row_lo) < (uint32_t)row_n || j < row_first; };
+  bool odd = false;
   if (keys.tiles > 0) load(0);
 #pragma unroll 1
   for (int t = 0; t < keys.tiles; ++t) {
@@ -178,16 +186,14 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
     lds_barrier();  // the tile is there, and the one before it is done with
     if (t + 1 < keys.tiles) load(t + 1);
     if (GB && t > 0) gather(t - 1);
-    if (w0 >= s.nq || (a.causal && key > p_last) || (a.window > 0 && key + KT - 1 <= p_first - a.window && key >= a.sinks)) {
+    if (unseen(key)) {
 #pragma unroll
       for (int x = 0; x < XX; ++x)
         if (GB) win[t & 1][wave][x][lane] = 0.0f;
       continue;
     }
     const char *tk = sk[t & 1], *tv = sv[t & 1];
-    const bool whole = key + KT <= s.nk && (!a.causal || key + KT - 1 <= p_first) &&
-                       (a.window == 0 || key > p_last - a.window || key + KT <= a.sinks);
-    auto sees = [&](int j) { return (uint32_t)(key + j - row_lo) < (uint32_t)row_n || key + j < row_first; };
+    const bool whole = all_seen(key);
 #pragma unroll
     for (int x = 0; x < XX; ++x) {
       f32x16_t sc = zero16, dp = zero16;
@@ -206,7 +212,7 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
       }
       if (!whole) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) ds[e] = sees(32 * x + 4 * h + 8 * (e >> 2) + (e & 3)) ? ds[e] : 0.0f;
+        for (int e = 0; e < 16; ++e) ds[e] = sees(key + 32 * x + 4 * h + 8 * (e >> 2) + (e & 3)) ? ds[e] : 0.0f;
       }
       if (GB) {
         const int first = p_first - key - 32 * x - 31 - a.bias_start, last = first + 62;  // columns of the wave's pairs
@@ -247,8 +253,9 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
       u32x4_t w[2];
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e >> 2][e & 3] = DT == PDM_F16 ? pack2<DT>(ds[2 * e] * ahead, ds[2 * e + 1] * ahead) : pack2<DT>(ds[2 * e], ds[2 * e + 1]);
-      if (!whole && odd_rows<DT, D, 2>(tk, col_at, 32 * x)) add_cols_odd<DT, D, 2, false>(dq, tk, col_at, 32 * x, w, sees);
-      else add_cols<DT, D, 2>(dq, tk, col_at, 32 * x, w);
+      const bool careful = !whole && odd_rows<DT, D, 2>(tk, col_at, 32 * x);
+      odd = odd || careful;
+      add_cols<DT, D, 2>(dq, tk, col_at, 32 * x, w, careful);
     }
   }
   if (GB) {
@@ -261,6 +268,17 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
     if (lane == 0) ends[wave] = far, ends[4 + wave] = near;
     __syncthreads();
     if (tid < 2) part[cols + tid] = (ends[4 * tid] + ends[4 * tid + 1]) + (ends[4 * tid + 2] + ends[4 * tid + 3]);
+  }
+  if (__syncthreads_or(odd)) {
+#pragma unroll 1
+    for (int t = 0; t < keys.tiles; ++t) {
+      const int key = jag_key<KT>(keys, t);
+      load(t);
+      brought();
+      __syncthreads();
+      if (!unseen(key) && !all_seen(key)) mark_cols<DT, D, 2 * XX>(dq, sk[t & 1], col_at, 0, [&](int j) { return sees(key + j); });
+      __syncthreads();
+    }
   }
   if (!there) return;
 #pragma unroll
@@ -408,6 +426,18 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
   int power = 100;  // fp16: dk holds sums times 2^power
   const int64_t item0 = (int64_t)a.cu_q[b] / M + b;
 
+  // of 32 queries: none sees a key of this wave; each sees all of them (here); of a query: it sees this lane's key
+  auto unseen = [&](int i) {
+    const int p0 = off + i;
+    return i >= s.nq || jw >= s.nk || (SINK ? p0 + 31 < jw + a.window : (a.causal && p0 + 31 < jw) || (a.window > 0 && p0 >= jw + 31 + a.window));
+  };
+  auto all_seen = [&](int i) {
+    const int p0 = off + i;
+    return i + 32 <= s.nq && jw + 32 <= (SINK && a.sinks < s.nk ? a.sinks : s.nk) &&
+           (SINK ? p0 >= jw + 31 + a.window : (!a.causal || p0 >= jw + 31) && (a.window == 0 || p0 + 31 < jw + a.window));
+  };
+  auto sees = [&](int i) { return (uint32_t)(i - see_lo) < (uint32_t)see_n; };
+  bool odd = false;
   int hh = head_next, tt = tile_next;
   if (n1 > n0) load(n0);
 #pragma unroll 1
@@ -424,12 +454,9 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
     const char *tq = sq[n & 1], *tg = sg[n & 1];
 #pragma unroll
     for (int y0 = 0; y0 < (SINK ? 1 : QT / 32); ++y0) {
-      const int x = SINK ? wave : y0, i = i0 + 32 * x, p0 = off + i;
-      if (i >= s.nq || jw >= s.nk) continue;
-      if (SINK ? p0 + 31 < jw + a.window : (a.causal && p0 + 31 < jw) || (a.window > 0 && p0 >= jw + 31 + a.window)) continue;
-      const bool whole = i + 32 <= s.nq && jw + 32 <= (SINK ? a.sinks : s.nk) &&
-                         (SINK ? p0 >= jw + 31 + a.window : (!a.causal || p0 >= jw + 31) && (a.window == 0 || p0 + 31 < jw + a.window));
-      auto sees = [&](int r) { return (uint32_t)(i0 + r - see_lo) < (uint32_t)see_n; };
+      const int x = SINK ? wave : y0, i = i0 + 32 * x;
+      if (unseen(i)) continue;
+      const bool whole = all_seen(i);
       f32x16_t sc = zero16, dp = zero16;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
@@ -468,7 +495,7 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
       if (!whole) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const bool ok = sees(32 * x + 4 * h + 8 * (e >> 2) + (e & 3));
+          const bool ok = sees(i + 4 * h + 8 * (e >> 2) + (e & 3));
           p[e] = ok ? p[e] : 0.0f, ds[e] = ok ? ds[e] : 0.0f;
         }
       }
@@ -478,10 +505,28 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
         pw[e >> 2][e & 3] = pack2<DT>(p[2 * e], p[2 * e + 1]);
         dw[e >> 2][e & 3] = DT == PDM_F16 ? pack2<DT>(ds[2 * e] * ahead, ds[2 * e + 1] * ahead) : pack2<DT>(ds[2 * e], ds[2 * e + 1]);
       }
-      if (!whole && odd_rows<DT, D, 2>(tg, col_at, 32 * x)) add_cols_odd<DT, D, 2, false>(dv, tg, col_at, 32 * x, pw, sees);
-      else add_cols<DT, D, 2>(dv, tg, col_at, 32 * x, pw);
-      if (!whole && odd_rows<DT, D, 2>(tq, col_at, 32 * x)) add_cols_odd<DT, D, 2, false>(dk, tq, col_at, 32 * x, dw, sees);
-      else add_cols<DT, D, 2>(dk, tq, col_at, 32 * x, dw);
+      const bool careful = !whole && (odd_rows<DT, D, 2>(tg, col_at, 32 * x) || odd_rows<DT, D, 2>(tq, col_at, 32 * x));
+      odd = odd || careful;
+      add_cols<DT, D, 2>(dv, tg, col_at, 32 * x, pw, careful);
+      add_cols<DT, D, 2>(dk, tq, col_at, 32 * x, dw, careful);
+    }
+  }
+  if (__syncthreads_or(odd)) {
+    head_next = tiles ? n0 / tiles : 0, tile_next = tiles ? n0 % tiles : 0;
+#pragma unroll 1
+    for (int n = n0; n < n1; ++n) {
+      const int i0 = i_lo + tile_next * QT;
+      load(n);
+      brought();
+      __syncthreads();
+#pragma unroll 1
+      for (int y0 = 0; y0 < (SINK ? 1 : QT / 32); ++y0) {
+        const int x = SINK ? wave : y0, i = i0 + 32 * x;
+        if (unseen(i) || all_seen(i)) continue;
+        mark_cols<DT, D, 2>(dv, sg[n & 1], col_at, 32 * x, [&](int r) { return sees(i0 + r); });
+        mark_cols<DT, D, 2>(dk, sq[n & 1], col_at, 32 * x, [&](int r) { return sees(i0 + r); });
+      }
+      __syncthreads();
     }
   }
   const float back = DT == PDM_F16 ? pow2(-power) : 1.0f;
@@ -529,24 +574,23 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
     }
 }
 
-// Gradients of 32 sinks of a key head: their sums under the window and beyond it.
+// Gradients of 32 sinks of a key head, their sums under the window and beyond it: a thread an element.
 template <int DT, int D>
 __global__ void __launch_bounds__(256) jag_sinks_kernel(JagArgs a, int64_t units) {
-  const int64_t unit = linear_block();
+  constexpr int PARTS = 2 * D * 32 / 256;
+  const int64_t unit = linear_block() / PARTS;
   if (unit >= units) return;
-  const int kh = (int)(unit % a.hk);
+  const int kh = (int)(unit % a.hk), i = (int)(linear_block() % PARTS) * 256 + threadIdx.x;
   const int64_t x = unit / a.hk;
   const int j0 = (int)(x % a.sink_blocks) * 32, b = (int)(x / a.sink_blocks);
+  const int z = i / (D * 32), key = j0 + i % 32, d = i / 32 % D;
   JagSeq s;
-  if (!jag_seq(a, b, s)) return;
-  const float* from = a.sink_part + sink_slots(a, b, j0 / 32, kh) * (2 * D * 32);
-  for (int i = threadIdx.x; i < 2 * D * 32; i += 256) {
-    const int z = i / (D * 32), key = j0 + i % 32, d = i / 32 % D;
-    if (key >= s.nk) continue;
-    float sum = 0.0f;
-    for (int n = 0; n <= a.sink_shares; ++n) sum += from[(int64_t)n * (2 * D * 32) + i];
-    static_cast<uint16_t*>(z ? a.dv : a.dk)[((s.k0 + key) * a.hk + kh) * D + d] = (uint16_t)pack2<DT>(z ? sum : sum * a.scale, 0.0f);
-  }
+  if (!jag_seq(a, b, s) || key >= s.nk) return;
+  const float* from = a.sink_part + sink_slots(a, b, j0 / 32, kh) * (2 * D * 32) + i;
+  float sum = 0.0f;
+#pragma unroll 4
+  for (int n = 0; n <= a.sink_shares; ++n) sum += from[(int64_t)n * (2 * D * 32)];
+  static_cast<uint16_t*>(z ? a.dv : a.dk)[((s.k0 + key) * a.hk + kh) * D + d] = (uint16_t)pack2<DT>(z ? sum : sum * a.scale, 0.0f);
 }
 
 // ---- host -------------------------------------------------------------------------------
@@ -602,7 +646,7 @@ void launch(const JagArgs& a, hipStream_t st) {
     if (a.sink_blocks) {
       const int64_t blocks = (int64_t)a.seqs * a.sink_blocks * a.hk;
       jag_dkv_kernel<DT, D, BIAS, true><<<linear_grid(blocks * a.sink_shares), 256, 0, st>>>(a, blocks * a.sink_shares);
-      jag_sinks_kernel<DT, D><<<linear_grid(blocks), 256, 0, st>>>(a, blocks);
+      jag_sinks_kernel<DT, D><<<linear_grid(blocks * (2 * D * 32 / 256)), 256, 0, st>>>(a, blocks);
     }
   }
 }

@@ -214,15 +214,30 @@ struct Bring {
 __device__ __forceinline__ void brought() { __builtin_amdgcn_s_waitcnt(kWaitVmcnt0); }
 
 // ---- products with a tile's columns ------------------------------------------------------
+// A weight of a pair that is not seen is zero, and what it meets must not matter, though 0 times an infinity or NaN would.  So
+// where a tile is seen in part (`whole` says for a wave that it is not) and holds such elements (odd_rows), they are left out of
+// the product (`careful`), and after the walk over all tiles a second one brings them to the pairs that see them (mark_cols).
+
+// Zeros for the infinities and NaN of a pair of elements.
+template <int DT>
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+  const uint32_t n = odd2<DT>(w) >> 15;  // bits 0 and 16
+  return w & ~((n << 16) - n);
+}
+
 // acc[d] += columns of rows [y0, y0 + 16 Y) of the tile, times w (the weights of these rows, as a 32x32 product left them);
 // TWICE: and times rest.
 template <int DT, int D, int Y, bool TWICE = false>
-__device__ __forceinline__ void add_cols(f32x16_t* acc, const char* t, uint32_t at, int y0, const u32x4_t* w, const u32x4_t* rest = nullptr) {
+__device__ __forceinline__ void add_cols(f32x16_t* acc, const char* t, uint32_t at, int y0, const u32x4_t* w, bool careful, const u32x4_t* rest = nullptr) {
 #pragma unroll
   for (int y = 0; y < Y; ++y)
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) {
-      const u32x4_t f = Tile<D>::cols(t, at, y0 + 16 * y, d);
+      u32x4_t f = Tile<D>::cols(t, at, y0 + 16 * y, d);
+      if (careful) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = finite2<DT>(f[e]);
+      }
       acc[d] = mfma32<DT>(f, w[y], acc[d]);
       if constexpr (TWICE) acc[d] = mfma32<DT>(f, rest[y], acc[d]);
     }
@@ -242,50 +257,32 @@ __device__ __forceinline__ bool odd_rows(const char* t, uint32_t at, int y0) {
   return __any(odd != 0);
 }
 
-// add_cols where some weights belong to pairs that are not seen: they are zeros, and what they meet must not matter, though 0
-// times an infinity or NaN would.  Such elements are left out here, and brought to the pairs that are seen by products of ones:
-// +-infinity, and NaN as both.  sees(r): whether this lane's column sees row r of the tile.  Rare: a loop of little code.
-template <int DT, int D, int Y, bool TWICE, typename F>
-__device__ __forceinline__ void add_cols_odd(f32x16_t* acc, const char* t, uint32_t at, int y0, const u32x4_t* w, F sees, const u32x4_t* rest = nullptr) {
-  constexpr uint32_t one = DT == PDM_BF16 ? 0x3f80u : 0x3c00u, pos = DT == PDM_BF16 ? 0x7f80u : 0x7c00u, neg = pos | 0x8000u;
+// The second walk: products of 2^127 and 2, which no sum in fp32 holds, for pairs that are seen: +infinity, -infinity, and both for
+// NaN.  sees(r): whether this lane's column sees row r of the tile.
+template <int DT, int D, int Y, typename F>
+__device__ __forceinline__ void mark_cols(f32x16_t* acc, const char* t, uint32_t at, int y0, F sees) {
+  constexpr uint32_t pos = DT == PDM_BF16 ? 0x7f80u : 0x7c00u, neg = pos | 0x8000u;
   const int h4 = 4 * (threadIdx.x >> 5 & 1);
 #pragma unroll 1
   for (int y = 0; y < Y; ++y) {
-    u32x4_t seen, wy = w[0], ry = {0, 0, 0, 0};
-    if constexpr (TWICE) ry = rest[0];
-#pragma unroll
-    for (int i = 1; i < Y; ++i) {
-      wy = y == i ? w[i] : wy;
-      if constexpr (TWICE) ry = y == i ? rest[i] : ry;
-    }
+    u32x4_t seen;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int r = y0 + 16 * y + h4 + 8 * (e >> 1) + 2 * (e & 1);
-      seen[e] = (sees(r) ? one : 0u) | (sees(r + 1) ? one << 16 : 0u);
+      seen[e] = (sees(r) ? 0x4000u : 0u) | (sees(r + 1) ? 0x40000000u : 0u);  // bf16 2
     }
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) {
-      u32x4_t f = Tile<D>::cols(t, at, y0 + 16 * y, d), fp, fn;
+      const u32x4_t f = Tile<D>::cols(t, at, y0 + 16 * y, d);
+      u32x4_t up, down;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t full = (odd2<DT>(f[e]) >> 15) * 0xffffu, x = f[e] & 0xffffu, z = f[e] >> 16;
-        const uint32_t ones = full & (one | one << 16);
-        fp[e] = ones & ((x == neg ? 0u : 0xffffu) | (z == neg ? 0u : 0xffff0000u));
-        fn[e] = ones & ((x == pos ? 0u : 0xffffu) | (z == pos ? 0u : 0xffff0000u));
-        f[e] &= ~full;
+        const uint32_t n = odd2<DT>(f[e]) >> 15, full = (n << 16) - n, x = f[e] & 0xffffu, z = f[e] >> 16;
+        up[e] = full & ((x == neg ? 0u : 0x7f00u) | (z == neg ? 0u : 0x7f000000u));    // bf16 2^127
+        down[e] = full & ((x == pos ? 0u : 0xff00u) | (z == pos ? 0u : 0xff000000u));
       }
-      acc[d] = mfma32<DT>(f, wy, acc[d]);
-      if constexpr (TWICE) acc[d] = mfma32<DT>(f, ry, acc[d]);
-      constexpr f32x16_t zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-      __builtin_amdgcn_sched_barrier(0);
-      const f32x16_t up = mfma32<DT>(fp, seen, zero);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[d][e] += up[e] > 0.0f ? kInf : 0.0f;
-      __builtin_amdgcn_sched_barrier(0);
-      const f32x16_t down = mfma32<DT>(fn, seen, zero);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[d][e] -= down[e] > 0.0f ? kInf : 0.0f;
-      __builtin_amdgcn_sched_barrier(0);
+      acc[d] = mfma32x32x16(up, seen, acc[d]);
+      acc[d] = mfma32x32x16(down, seen, acc[d]);
     }
   }
 }
