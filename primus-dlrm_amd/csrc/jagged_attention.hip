@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(256, 2) jag_fwd_kernel(JagArgs a, int64_t unit
       if (a.rest) clear_row(a.rest, t * a.hq * D, a.hq * D);
       for (int h = threadIdx.x; h < a.hq; h += 256) {
         if (a.lse) a.lse[t * a.hq + h] = -kInf;
-        if (a.stats) a.stats[2 * (t * a.hq + h)] = 0.0f, a.stats[2 * (t * a.hq + h) + 1] = 0.0f;
+        if (a.stats) a.stats[2 * (t * a.hq + h)] = kNoKeys, a.stats[2 * (t * a.hq + h) + 1] = 0.0f;
       }
     });
     return;
@@ -102,6 +102,11 @@ __global__ void __launch_bounds__(256, 2) jag_fwd_kernel(JagArgs a, int64_t unit
   auto all_seen = [&](int key) {
     return key + KT <= s.nk && (!a.causal || key + KT - 1 <= p_first) && (a.window == 0 || key > p_last - a.window || key + KT <= a.sinks);
   };
+  // some pair of the workgroup's queries and the tile's keys is not seen (what lies behind the last key comes as zeros)
+  const int b_first = off + r0, b_last = off + (r0 + M < s.nq ? r0 + M : s.nq) - 1;
+  auto in_part = [&](int key) {
+    return (a.causal && key + KT - 1 > b_first) || (a.window > 0 && key <= b_last - a.window && key + KT > a.sinks);
+  };
   auto sees = [&](int j) { return (uint32_t)(j - row_lo) < (uint32_t)row_n || j < row_first; };
   bool odd = false;
   if (keys.tiles > 0) load(0);
@@ -110,18 +115,20 @@ __global__ void __launch_bounds__(256, 2) jag_fwd_kernel(JagArgs a, int64_t unit
     const int key = jag_key<KT>(keys, t);
     if (BIAS && tid < M + KT) sb[t & 1][tid] = bias_next;
     brought();
+    if (in_part(key) && clean_rows<DT, D, KT>(sv[t & 1], lane, wave)) odd = true;
     lds_barrier();  // the tile is there, and the one before it is done with
     if (t + 1 < keys.tiles) load(t + 1);
     const char *tk = sk[t & 1], *tv = sv[t & 1];
     if (unseen(key)) continue;
     const bool whole = all_seen(key);
-    f32x16_t sc[2];
+    f32x16_t sc[2] = {zero16, zero16};
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      sc[x] = zero16;
+    for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) sc[x] = mfma32<DT>(Tile<D>::rows(tk, row_at, 32 * x, kk), q[kk], sc[x]);
-    }
+      for (int x = 0; x < 2; ++x) sc[x] = mfma32<DT>(Tile<D>::rows(tk, row_at, 32 * x, kk), q[kk], sc[x]);
+    sched_mfma_ds_pipeline<2 * KK, 8>();
+    __builtin_amdgcn_sched_barrier(0);
     float w[32];
     const int bias_at = wave * 32 + c + KT - 1 - 4 * h;
 #pragma unroll
@@ -156,18 +163,18 @@ __global__ void __launch_bounds__(256, 2) jag_fwd_kernel(JagArgs a, int64_t unit
       p[e >> 2][e & 3] = pack2<DT>(w[2 * e], w[2 * e + 1]);
       if (FINE) rest[e >> 2][e & 3] = left2<DT>(w[2 * e], w[2 * e + 1], p[e >> 2][e & 3]);
     }
-    const bool careful = !whole && odd_rows<DT, D, 4>(tv, col_at, 0);
-    odd = odd || careful;
-    add_cols<DT, D, 4, FINE>(o, tv, col_at, 0, p, careful, rest);
+    add_cols<DT, D, 4, FINE>(o, tv, col_at, 0, p, rest);
+    __builtin_amdgcn_sched_barrier(0);
   }
   if (__syncthreads_or(odd)) {
 #pragma unroll 1
     for (int t = 0; t < keys.tiles; ++t) {
       const int key = jag_key<KT>(keys, t);
+      if (!in_part(key)) continue;
       load(t);
       brought();
       __syncthreads();
-      if (!unseen(key) && !all_seen(key)) mark_cols<DT, D, 4>(o, sv[t & 1], col_at, 0, [&](int j) { return sees(key + j); });
+      mark_cols<DT, D, 4, false>(o, sv[t & 1], col_at, 0, [&](int j) { return sees(key + j); });
       __syncthreads();
     }
   }
@@ -190,7 +197,7 @@ __global__ void __launch_bounds__(256, 2) jag_fwd_kernel(JagArgs a, int64_t unit
     // log2 of the sum: of its mantissa, and its exponent beside the reference, whose rounding it shares
     if (a.lse)
       a.lse[at] = sum != 0.0f ? ((m + (float)__builtin_amdgcn_frexp_expf(sum)) + __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(sum))) * kLn2 : -kInf;
-    if (a.stats) a.stats[2 * at] = sum != 0.0f ? m : 0.0f, a.stats[2 * at + 1] = inv;
+    if (a.stats) a.stats[2 * at] = sum != 0.0f ? m : kNoKeys, a.stats[2 * at + 1] = inv;
   }
 }
 

@@ -42,6 +42,7 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   __shared__ float win[2][GB ? 4 : 1][XX][GB ? 64 : 1];
   __shared__ float skew[GB ? 4 : 1][GB ? 32 : 1][64];
   __shared__ float ends[GB ? 8 : 1];
+  __shared__ int odd_keys[2][KT], odd_any[2][4];
 
   const int64_t unit = linear_block();
   if (unit >= units) {
@@ -175,6 +176,10 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   auto all_seen = [&](int key) {
     return key + KT <= s.nk && (!a.causal || key + KT - 1 <= p_first) && (a.window == 0 || key > p_last - a.window || key + KT <= a.sinks);
   };
+  const int b_first = off + r0, b_last = off + (r0 + M < s.nq ? r0 + M : s.nq) - 1;
+  auto in_part = [&](int key) {
+    return (a.causal && key + KT - 1 > b_first) || (a.window > 0 && key <= b_last - a.window && key + KT > a.sinks);
+  };
   auto sees = [&](int j) { return (uint32_t)(j - row_lo) < (uint32_t)row_n || j < row_first; };
   bool odd = false;
   if (keys.tiles > 0) load(0);
@@ -183,6 +188,12 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
     const int key = jag_key<KT>(keys, t);
     if (BIAS && tid < M + KT) sb[t & 1][tid] = bias_next;
     brought();
+    const bool part_seen = in_part(key);
+    if (part_seen) {
+      const bool bad = clean_rows<DT, D, KT>(sk[t & 1], lane, wave, odd_keys[t & 1]);
+      odd = odd || bad;
+      if (lane == 0) odd_any[t & 1][wave] = bad;
+    }
     lds_barrier();  // the tile is there, and the one before it is done with
     if (t + 1 < keys.tiles) load(t + 1);
     if (GB && t > 0) gather(t - 1);
@@ -209,6 +220,18 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
         const float w = BIAS ? __builtin_fmaf(sc[e], a.scale2, sb[t & 1][wave * 32 + local - j]) : sc[e] * a.scale2;
         const float p = __builtin_amdgcn_exp2f(w - m) * inv;
         ds[e] = p * (dp[e] - delta);
+      }
+      if (part_seen && (odd_any[t & 1][0] | odd_any[t & 1][1] | odd_any[t & 1][2] | odd_any[t & 1][3])) {
+        // a key that is not finite: scores of -inf, or rows of NaN
+#pragma unroll 1
+        for (int w = 0; w < 4; ++w) {
+          if (!odd_any[t & 1][w]) continue;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int j = 32 * x + 4 * h + 8 * (e >> 2) + (e & 3);
+            if (j / (KT / 4) == w && odd_keys[t & 1][j] && inv == inv) ds[e] = 0.0f;
+          }
+        }
       }
       if (!whole) {
 #pragma unroll
@@ -253,9 +276,7 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
       u32x4_t w[2];
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e >> 2][e & 3] = DT == PDM_F16 ? pack2<DT>(ds[2 * e] * ahead, ds[2 * e + 1] * ahead) : pack2<DT>(ds[2 * e], ds[2 * e + 1]);
-      const bool careful = !whole && odd_rows<DT, D, 2>(tk, col_at, 32 * x);
-      odd = odd || careful;
-      add_cols<DT, D, 2>(dq, tk, col_at, 32 * x, w, careful);
+      add_cols<DT, D, 2>(dq, tk, col_at, 32 * x, w);
     }
   }
   if (GB) {
@@ -273,10 +294,11 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
 #pragma unroll 1
     for (int t = 0; t < keys.tiles; ++t) {
       const int key = jag_key<KT>(keys, t);
+      if (!in_part(key)) continue;
       load(t);
       brought();
       __syncthreads();
-      if (!unseen(key) && !all_seen(key)) mark_cols<DT, D, 2 * XX>(dq, sk[t & 1], col_at, 0, [&](int j) { return sees(key + j); });
+      mark_cols<DT, D, 2 * XX, true>(dq, sk[t & 1], col_at, 0, [&](int j) { return sees(key + j); });
       __syncthreads();
     }
   }
@@ -436,6 +458,12 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
     return i + 32 <= s.nq && jw + 32 <= (SINK && a.sinks < s.nk ? a.sinks : s.nk) &&
            (SINK ? p0 >= jw + 31 + a.window : (!a.causal || p0 >= jw + 31) && (a.window == 0 || p0 + 31 < jw + a.window));
   };
+  // some pair of the tile's queries and the workgroup's keys is not seen (what lies behind the last query comes as zeros)
+  auto in_part = [&](int i) {
+    const int p0 = off + i;
+    if (SINK) return p0 < j1 + a.window || j1 >= a.sinks;
+    return (a.causal && p0 < j1) || (a.window > 0 && p0 + QT - 1 >= j0 + a.window);
+  };
   auto sees = [&](int i) { return (uint32_t)(i - see_lo) < (uint32_t)see_n; };
   bool odd = false;
   int hh = head_next, tt = tile_next;
@@ -449,6 +477,10 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
     for (int u = 0; u < (QT == 128 ? 2 : 1); ++u)
       if (tid + 256 * u < 3 * QT) (&ss[n & 1][0][0])[tid + 256 * u] = stat_next[u];
     brought();
+    if (in_part(i0)) {
+      if (clean_rows<DT, D, QT>(sq[n & 1], lane, wave)) odd = true;
+      if (clean_rows<DT, D, QT>(sg[n & 1], lane, wave)) odd = true;
+    }
     lds_barrier();  // the tile is there, and the one before it is done with
     if (n + 1 < n1) load(n + 1);
     const char *tq = sq[n & 1], *tg = sg[n & 1];
@@ -505,10 +537,8 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
         pw[e >> 2][e & 3] = pack2<DT>(p[2 * e], p[2 * e + 1]);
         dw[e >> 2][e & 3] = DT == PDM_F16 ? pack2<DT>(ds[2 * e] * ahead, ds[2 * e + 1] * ahead) : pack2<DT>(ds[2 * e], ds[2 * e + 1]);
       }
-      const bool careful = !whole && (odd_rows<DT, D, 2>(tg, col_at, 32 * x) || odd_rows<DT, D, 2>(tq, col_at, 32 * x));
-      odd = odd || careful;
-      add_cols<DT, D, 2>(dv, tg, col_at, 32 * x, pw, careful);
-      add_cols<DT, D, 2>(dk, tq, col_at, 32 * x, dw, careful);
+      add_cols<DT, D, 2>(dv, tg, col_at, 32 * x, pw);
+      add_cols<DT, D, 2>(dk, tq, col_at, 32 * x, dw);
     }
   }
   if (__syncthreads_or(odd)) {
@@ -521,10 +551,10 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
       __syncthreads();
 #pragma unroll 1
       for (int y0 = 0; y0 < (SINK ? 1 : QT / 32); ++y0) {
-        const int x = SINK ? wave : y0, i = i0 + 32 * x;
-        if (unseen(i) || all_seen(i)) continue;
-        mark_cols<DT, D, 2>(dv, sg[n & 1], col_at, 32 * x, [&](int r) { return sees(i0 + r); });
-        mark_cols<DT, D, 2>(dk, sq[n & 1], col_at, 32 * x, [&](int r) { return sees(i0 + r); });
+        const int x = SINK ? wave : y0;
+        if (!in_part(i0)) continue;
+        mark_cols<DT, D, 2, false>(dv, sg[n & 1], col_at, 32 * x, [&](int r) { return sees(i0 + r); });
+        mark_cols<DT, D, 2, true>(dk, sq[n & 1], col_at, 32 * x, [&](int r) { return sees(i0 + r); });
       }
       __syncthreads();
     }

@@ -35,6 +35,7 @@ struct JagArgs {
 };
 
 constexpr float kInf = __builtin_inff();
+constexpr float kNoKeys = 3e38f;  // the reference of a row without weights: none passes it
 constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.44269504088896341f;
 
 // ---- sequences -------------------------------------------------------------------
@@ -215,51 +216,63 @@ __device__ __forceinline__ void brought() { __builtin_amdgcn_s_waitcnt(kWaitVmcn
 
 // ---- products with a tile's columns ------------------------------------------------------
 // A weight of a pair that is not seen is zero, and what it meets must not matter, though 0 times an infinity or NaN would.  So
-// where a tile is seen in part (`whole` says for a wave that it is not) and holds such elements (odd_rows), they are left out of
-// the product (`careful`), and after the walk over all tiles a second one brings them to the pairs that see them (mark_cols).
+// where not every pair of a tile is seen, a wave looks at the rows that it brought, before the others read them, and puts zeros
+// for such elements (clean_rows); behind the walk over all tiles, a second one over those tiles as they are brings them to the
+// pairs that see them (mark_cols).
 
-// Zeros for the infinities and NaN of a pair of elements.
-template <int DT>
-__device__ __forceinline__ uint32_t finite2(uint32_t w) {
-  const uint32_t n = odd2<DT>(w) >> 15;  // bits 0 and 16
-  return w & ~((n << 16) - n);
+// True where rows that this wave brought held infinities or NaN; `rows`, where given, gets 1 for these (of ROWS) and 0 for its others.
+template <int DT, int D, int ROWS>
+__device__ __forceinline__ bool clean_rows(char* t, int lane, int wave, int* rows = nullptr) {
+  constexpr int N = Bring<D, ROWS>::N;
+  u32x4_t* p = reinterpret_cast<u32x4_t*>(t + wave * N * 1024 + lane * 16);
+  uint32_t odd = 0;
+  u32x4_t w[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) w[i] = p[64 * i];
+#pragma unroll
+  for (int i = 0; i < N; ++i) odd |= (odd2<DT>(w[i][0]) | odd2<DT>(w[i][1])) | (odd2<DT>(w[i][2]) | odd2<DT>(w[i][3]));
+  if (!__any(odd != 0)) return false;
+  if (rows && lane < N * Bring<D, ROWS>::R) rows[wave * N * Bring<D, ROWS>::R + lane] = 0;
+#pragma unroll 1
+  for (int i = 0; i < N; ++i) {
+    u32x4_t x = p[64 * i];
+    bool here = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t n = odd2<DT>(x[e]) >> 15;  // bits 0 and 16
+      here = here || n != 0;
+      x[e] &= ~((n << 16) - n);
+    }
+    p[64 * i] = x;
+    if (rows && here) rows[(wave * N + i) * Bring<D, ROWS>::R + lane / (D / 8)] = 1;
+  }
+  return true;
 }
 
 // acc[d] += columns of rows [y0, y0 + 16 Y) of the tile, times w (the weights of these rows, as a 32x32 product left them);
-// TWICE: and times rest.
+// TWICE: and times rest.  Fragments are read LEAD products ahead.
 template <int DT, int D, int Y, bool TWICE = false>
-__device__ __forceinline__ void add_cols(f32x16_t* acc, const char* t, uint32_t at, int y0, const u32x4_t* w, bool careful, const u32x4_t* rest = nullptr) {
+__device__ __forceinline__ void add_cols(f32x16_t* acc, const char* t, uint32_t at, int y0, const u32x4_t* w, const u32x4_t* rest = nullptr) {
+  constexpr int N = Y * (D / 32), LEAD = 4;
 #pragma unroll
-  for (int y = 0; y < Y; ++y)
+  for (int i = 0; i < N; ++i) {
+    const int y = i / (D / 32), d = i % (D / 32);
+    const u32x4_t f = Tile<D>::cols(t, at, y0 + 16 * y, d);
+    acc[d] = mfma32<DT>(f, w[y], acc[d]);
+    if constexpr (TWICE) acc[d] = mfma32<DT>(f, rest[y], acc[d]);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x100, 2 * LEAD, 0);  // two LDS reads a fragment
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d) {
-      u32x4_t f = Tile<D>::cols(t, at, y0 + 16 * y, d);
-      if (careful) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = finite2<DT>(f[e]);
-      }
-      acc[d] = mfma32<DT>(f, w[y], acc[d]);
-      if constexpr (TWICE) acc[d] = mfma32<DT>(f, rest[y], acc[d]);
-    }
-}
-
-// True where the tile's rows [y0, y0 + 16 Y) hold infinities or NaN (for the whole wave).
-template <int DT, int D, int Y>
-__device__ __forceinline__ bool odd_rows(const char* t, uint32_t at, int y0) {
-  uint32_t odd = 0;
-#pragma unroll 1
-  for (int y = 0; y < Y; ++y)
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d) {
-      const u32x4_t f = Tile<D>::cols(t, at, y0 + 16 * y, d);
-      odd |= (odd2<DT>(f[0]) | odd2<DT>(f[1])) | (odd2<DT>(f[2]) | odd2<DT>(f[3]));
-    }
-  return __any(odd != 0);
+  for (int i = 0; i < N - LEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, TWICE ? 2 : 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, LEAD * (TWICE ? 2 : 1), 0);
 }
 
 // The second walk: products of 2^127 and 2, which no sum in fp32 holds, for pairs that are seen: +infinity, -infinity, and both for
-// NaN.  sees(r): whether this lane's column sees row r of the tile.
-template <int DT, int D, int Y, typename F>
+// NaN, or for all of them (NANS: their weights are 0 or NaN).  sees(r): whether this lane's column sees row r of the tile.
+template <int DT, int D, int Y, bool NANS, typename F>
 __device__ __forceinline__ void mark_cols(f32x16_t* acc, const char* t, uint32_t at, int y0, F sees) {
   constexpr uint32_t pos = DT == PDM_BF16 ? 0x7f80u : 0x7c00u, neg = pos | 0x8000u;
   const int h4 = 4 * (threadIdx.x >> 5 & 1);
@@ -278,8 +291,8 @@ __device__ __forceinline__ void mark_cols(f32x16_t* acc, const char* t, uint32_t
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t n = odd2<DT>(f[e]) >> 15, full = (n << 16) - n, x = f[e] & 0xffffu, z = f[e] >> 16;
-        up[e] = full & ((x == neg ? 0u : 0x7f00u) | (z == neg ? 0u : 0x7f000000u));    // bf16 2^127
-        down[e] = full & ((x == pos ? 0u : 0xff00u) | (z == pos ? 0u : 0xff000000u));
+        up[e] = full & ((!NANS && x == neg ? 0u : 0x7f00u) | (!NANS && z == neg ? 0u : 0x7f000000u));    // bf16 2^127
+        down[e] = full & ((!NANS && x == pos ? 0u : 0xff00u) | (!NANS && z == pos ? 0u : 0xff000000u));
       }
       acc[d] = mfma32x32x16(up, seen, acc[d]);
       acc[d] = mfma32x32x16(down, seen, acc[d]);
