@@ -23,7 +23,7 @@ template <int DT> constexpr float kLift = DT == PDM_BF16 ? 30.0f : 0.0f;
 template <int DT> constexpr float kRoom = 8.0f - kLift<DT>;
 
 template <int DT, int D, bool BIAS, bool FINE>
-__global__ void __launch_bounds__(256, 2) jag_fwd_kernel(JagArgs a, int64_t units) {
+__global__ void __launch_bounds__(256, D == 64 ? 3 : 2) jag_fwd_kernel(JagArgs a, int64_t units) {
   constexpr int KK = D / 16, DD = D / 32;
   __shared__ alignas(1024) char sk[2][KT * Tile<D>::RS];
   __shared__ alignas(1024) char sv[2][KT * Tile<D>::RS];
@@ -63,7 +63,14 @@ __global__ void __launch_bounds__(256, 2) jag_fwd_kernel(JagArgs a, int64_t unit
     const uint16_t* x = static_cast<const uint16_t*>(a.q) + (s.q0 + row) * a.q_st + head * a.q_sh + 8 * h;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) q[kk] = load16(x + 16 * kk, row < s.nq);
+    if (a.scale2 < 0.0f) {  // the scale's sign goes into the queries
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[kk][e] ^= 0x80008000u;
+    }
   }
+  const float scale2 = fmaxf(fabsf(a.scale2), 0x1p-126f);  // not zero: a hidden score times it stays -inf
   if (row < s.nq) {
     const int hi = a.causal && pos + 1 < s.nk ? (pos + 1 > 0 ? pos + 1 : 0) : s.nk;
     row_lo = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
@@ -80,12 +87,13 @@ __global__ void __launch_bounds__(256, 2) jag_fwd_kernel(JagArgs a, int64_t unit
   bring_k.init(a.k_st, lane, wave);
   bring_v.init(a.v_st, lane, wave);
   float bias_next = 0.0f;
-  auto load = [&](int t) {
-    const int key = jag_key<KT>(keys, t);
-    bring_k.load(kp, a.k_st, key, s.nk, sk[t & 1], wave);
-    bring_v.load(vp, a.v_st, key, s.nk, sv[t & 1], wave);
-    // entry x: distance of query r0 + x - 63 from the tile's first key
-    if (BIAS && tid < M + KT) bias_next = bias2(a, brow, (int64_t)off + r0 + tid - (KT - 1) - key);
+  auto load_k = [&](int t) { bring_k.load(kp, a.k_st, jag_key<KT>(keys, t), s.nk, sk[t & 1], wave); };
+  auto load_v = [&](int t) { bring_v.load(vp, a.v_st, jag_key<KT>(keys, t), s.nk, sv[t & 1], wave); };
+  auto load_bias = [&](int t) {  // entry x: distance of query r0 + x - 63 from the tile's first key
+    if (BIAS && tid < M + KT) bias_next = bias2(a, brow, (int64_t)off + r0 + tid - (KT - 1) - jag_key<KT>(keys, t));
+  };
+  auto store_bias = [&](int t) {
+    if (BIAS && tid < M + KT) sb[t & 1][tid] = bias_next;
   };
 
   constexpr f32x16_t zero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
@@ -109,69 +117,95 @@ __global__ void __launch_bounds__(256, 2) jag_fwd_kernel(JagArgs a, int64_t unit
   };
   auto sees = [&](int j) { return (uint32_t)(j - row_lo) < (uint32_t)row_n || j < row_first; };
   bool odd = false;
-  if (keys.tiles > 0) load(0);
-#pragma unroll 1
-  for (int t = 0; t < keys.tiles; ++t) {
-    const int key = jag_key<KT>(keys, t);
-    if (BIAS && tid < M + KT) sb[t & 1][tid] = bias_next;
-    brought();
-    if (in_part(key) && clean_rows<DT, D, KT>(sv[t & 1], lane, wave)) odd = true;
-    lds_barrier();  // the tile is there, and the one before it is done with
-    if (t + 1 < keys.tiles) load(t + 1);
-    const char *tk = sk[t & 1], *tv = sv[t & 1];
-    if (unseen(key)) continue;
-    const bool whole = all_seen(key);
-    f32x16_t sc[2] = {zero16, zero16};
+
+  // ---- the steps of a tile ----
+  f32x16_t sc[2];
+  u32x4_t p[4], rest[4];
+  auto scores = [&](int t) __attribute__((always_inline)) {
+    if (unseen(jag_key<KT>(keys, t))) return;
+    const char* tk = sk[t & 1];
     __builtin_amdgcn_sched_barrier(0);
+    sc[0] = zero16, sc[1] = zero16;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
       for (int x = 0; x < 2; ++x) sc[x] = mfma32<DT>(Tile<D>::rows(tk, row_at, 32 * x, kk), q[kk], sc[x]);
     sched_mfma_ds_pipeline<2 * KK, 8>();
     __builtin_amdgcn_sched_barrier(0);
-    float w[32];
-    const int bias_at = wave * 32 + c + KT - 1 - 4 * h;
+  };
+  auto weights = [&](int t) __attribute__((always_inline)) {
+    const int key = jag_key<KT>(keys, t);
+    if (unseen(key)) return;
+    // Without a bias the scale is left to the exponent's argument.
+    float f = scale2;
+    if constexpr (BIAS) {
+      const float* b = &sb[t & 1][wave * 32 + c + KT - 1 - 4 * h];
+      f = 1.0f;
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      const int j = 32 * (e >> 4) + 8 * ((e >> 2) & 3) + (e & 3);  // and 4 h: the element's key
-      w[e] = BIAS ? __builtin_fmaf(sc[e >> 4][e & 15], a.scale2, sb[t & 1][bias_at - j]) : sc[e >> 4][e & 15] * a.scale2;
+      for (int e = 0; e < 32; ++e)  // element e: key 32 (e / 16) + 8 (e / 4 % 4) + e % 4 + 4 h
+        sc[e >> 4][e & 15] = __builtin_fmaf(sc[e >> 4][e & 15], scale2, b[-(32 * (e >> 4) + 8 * ((e >> 2) & 3) + (e & 3))]);
     }
-    if (!whole) {
+    if (!all_seen(key)) {
 #pragma unroll
-      for (int e = 0; e < 32; ++e) w[e] = sees(key + 4 * h + 32 * (e >> 4) + 8 * ((e >> 2) & 3) + (e & 3)) ? w[e] : -kInf;
+      for (int e = 0; e < 32; ++e)
+        sc[e >> 4][e & 15] = sees(key + 4 * h + 32 * (e >> 4) + 8 * ((e >> 2) & 3) + (e & 3)) ? sc[e >> 4][e & 15] : -kInf;
     }
-    float top = w[0];
+    float top = sc[0][0];
 #pragma unroll
-    for (int e = 1; e < 32; ++e) top = fmaxf(top, w[e]);
+    for (int e = 1; e < 32; ++e) top = fmaxf(top, sc[e >> 4][e & 15]);
+    top *= f;
     if (__any(top > m + kRoom<DT>)) {
       top = fmaxf(top, __shfl_xor(top, 32));
       const float now = top > m + kRoom<DT> ? top + kLift<DT> : m;  // by row: other rows change nothing
-      const float f = now == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - now);
+      const float g = now == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - now);
       m = now;
-      l *= f;
+      l *= g;
 #pragma unroll
-      for (int d = 0; d < DD; ++d) o[d] *= f;
+      for (int d = 0; d < DD; ++d) o[d] *= g;
     }
     const float base = m == -kInf ? 0.0f : m;
 #pragma unroll
-    for (int e = 0; e < 32; ++e) w[e] = __builtin_amdgcn_exp2f(w[e] - base);
+    for (int y = 0; y < 4; ++y) {
+      float w[8];
 #pragma unroll
-    for (int e = 0; e < 32; e += 4) l += (w[e] + w[e + 1]) + (w[e + 2] + w[e + 3]);
-    u32x4_t p[4], rest[4];
+      for (int e = 0; e < 8; ++e) {
+        const float x = sc[y >> 1][8 * (y & 1) + e];
+        w[e] = __builtin_amdgcn_exp2f(BIAS ? x - base : __builtin_fmaf(x, f, -base));
+      }
+      l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      p[e >> 2][e & 3] = pack2<DT>(w[2 * e], w[2 * e + 1]);
-      if (FINE) rest[e >> 2][e & 3] = left2<DT>(w[2 * e], w[2 * e + 1], p[e >> 2][e & 3]);
+      for (int e = 0; e < 4; ++e) {
+        p[y][e] = pack2<DT>(w[2 * e], w[2 * e + 1]);
+        if (FINE) rest[y][e] = left2<DT>(w[2 * e], w[2 * e + 1], p[y][e]);
+      }
     }
-    add_cols<DT, D, 4, FINE>(o, tv, col_at, 0, p, rest);
+  };
+  auto values = [&](int t) __attribute__((always_inline)) {
+    if (unseen(jag_key<KT>(keys, t))) return;
     __builtin_amdgcn_sched_barrier(0);
+    add_cols<DT, D, 4, FINE>(o, sv[t & 1], col_at, 0, p, rest);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  const int tiles = keys.tiles;
+  if (tiles > 0) load_k(0), load_v(0), load_bias(0);
+#pragma unroll 1
+  for (int t = 0; t < tiles; ++t) {
+    store_bias(t);
+    brought();
+    if (in_part(jag_key<KT>(keys, t)) && clean_rows<DT, D, KT>(sv[t & 1], lane, wave)) odd = true;
+    lds_barrier();  // the tile is there, and the one before it is done with
+    if (t + 1 < tiles) load_k(t + 1), load_v(t + 1), load_bias(t + 1);
+    scores(t);
+    weights(t);
+    values(t);
   }
   if (__syncthreads_or(odd)) {
 #pragma unroll 1
     for (int t = 0; t < keys.tiles; ++t) {
       const int key = jag_key<KT>(keys, t);
       if (!in_part(key)) continue;
-      load(t);
+      load_v(t);
       brought();
       __syncthreads();
       mark_cols<DT, D, 4, false>(o, sv[t & 1], col_at, 0, [&](int j) { return sees(key + j); });
@@ -180,20 +214,10 @@ __global__ void __launch_bounds__(256, 2) jag_fwd_kernel(JagArgs a, int64_t unit
   }
 
   const float sum = l + __shfl_xor(l, 32);
-  if (row >= s.nq) return;
   const int64_t at = (s.q0 + row) * a.hq + head;
   const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-#pragma unroll
-  for (int d = 0; d < DD; ++d)
-#pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      const float y[4] = {o[d][e] * inv, o[d][e + 1] * inv, o[d][e + 2] * inv, o[d][e + 3] * inv};
-      const u32x2_t w = {pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
-      const int64_t x = at * D + 32 * d + 2 * e + 4 * h;
-      *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.out) + x) = w;
-      if (FINE) *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.rest) + x) = u32x2_t{left2<DT>(y[0], y[1], w[0]), left2<DT>(y[2], y[3], w[1])};
-    }
-  if (h == 0) {
+  store_column<DT, D, FINE>(o, inv, row < s.nq, a.out, a.rest, at * D);
+  if (h == 0 && row < s.nq) {
     // log2 of the sum: of its mantissa, and its exponent beside the reference, whose rounding it shares
     if (a.lse)
       a.lse[at] = sum != 0.0f ? ((m + (float)__builtin_amdgcn_frexp_expf(sum)) + __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(sum))) * kLn2 : -kInf;
@@ -243,7 +267,7 @@ int jag_args(const char* fn, const pdm_jagged_attention_desc* d, JagArgs& a) {
   a.q_st = d->q_stride_t, a.q_sh = d->q_stride_h, a.k_st = d->k_stride_t, a.k_sh = d->k_stride_h;
   a.v_st = d->v_stride_t, a.v_sh = d->v_stride_h;
   a.scale = d->scale, a.scale2 = d->scale * kLog2e;
-  a.items = d->num_seqs ? d->q_tokens / M + d->num_seqs : 0;
+  a.items = d->num_seqs ? d->q_tokens / 128 + d->num_seqs : 0;
   return PDM_OK;
 }
 

@@ -302,13 +302,7 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
       __syncthreads();
     }
   }
-  if (!there) return;
-#pragma unroll
-  for (int d = 0; d < DD; ++d)
-#pragma unroll
-    for (int e = 0; e < 16; e += 4)
-      *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.dq) + at * D + 32 * d + 2 * e + 4 * h) =
-          u32x2_t{pack2<DT>(dq[d][e] * back, dq[d][e + 1] * back), pack2<DT>(dq[d][e + 2] * back, dq[d][e + 3] * back)};
+  store_column<DT, D>(dq, back, there, a.dq, nullptr, at * D);
 }
 
 // Sums the partial gradients of a column over the blocks of queries, in 64 bits: a lane per column, the blocks dealt to 16 waves.
@@ -590,18 +584,9 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
       }
     return;
   }
-  if (!there) return;
-  const float f = a.scale * back;
   const int64_t at = ((s.k0 + key) * a.hk + kh) * D;
-#pragma unroll
-  for (int d = 0; d < DD; ++d)
-#pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      const int64_t x = at + 32 * d + 2 * e + 4 * h;
-      *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.dv) + x) = u32x2_t{pack2<DT>(dv[d][e], dv[d][e + 1]), pack2<DT>(dv[d][e + 2], dv[d][e + 3])};
-      *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.dk) + x) =
-          u32x2_t{pack2<DT>(dk[d][e] * f, dk[d][e + 1] * f), pack2<DT>(dk[d][e + 2] * f, dk[d][e + 3] * f)};
-    }
+  store_column<DT, D>(dk, a.scale * back, there, a.dk, nullptr, at);
+  store_column<DT, D>(dv, 1.0f, there, a.dv, nullptr, at);
 }
 
 // Gradients of 32 sinks of a key head, their sums under the window and beyond it: a thread an element.

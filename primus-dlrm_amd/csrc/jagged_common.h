@@ -223,7 +223,7 @@ __device__ __forceinline__ void brought() { __builtin_amdgcn_s_waitcnt(kWaitVmcn
 // True where rows that this wave brought held infinities or NaN; `rows`, where given, gets 1 for these (of ROWS) and 0 for its others.
 template <int DT, int D, int ROWS>
 __device__ __forceinline__ bool clean_rows(char* t, int lane, int wave, int* rows = nullptr) {
-  constexpr int N = Bring<D, ROWS>::N;
+  constexpr int N = Bring<D, ROWS>::N, R = 64 / (D / 8);
   u32x4_t* p = reinterpret_cast<u32x4_t*>(t + wave * N * 1024 + lane * 16);
   uint32_t odd = 0;
   u32x4_t w[N];
@@ -232,7 +232,7 @@ __device__ __forceinline__ bool clean_rows(char* t, int lane, int wave, int* row
 #pragma unroll
   for (int i = 0; i < N; ++i) odd |= (odd2<DT>(w[i][0]) | odd2<DT>(w[i][1])) | (odd2<DT>(w[i][2]) | odd2<DT>(w[i][3]));
   if (!__any(odd != 0)) return false;
-  if (rows && lane < N * Bring<D, ROWS>::R) rows[wave * N * Bring<D, ROWS>::R + lane] = 0;
+  if (rows && lane < N * R) rows[wave * N * R + lane] = 0;
 #pragma unroll 1
   for (int i = 0; i < N; ++i) {
     u32x4_t x = p[64 * i];
@@ -244,7 +244,7 @@ __device__ __forceinline__ bool clean_rows(char* t, int lane, int wave, int* row
       x[e] &= ~((n << 16) - n);
     }
     p[64 * i] = x;
-    if (rows && here) rows[(wave * N + i) * Bring<D, ROWS>::R + lane / (D / 8)] = 1;
+    if (rows && here) rows[(wave * N + i) * R + lane / (D / 8)] = 1;
   }
   return true;
 }
@@ -298,6 +298,40 @@ __device__ __forceinline__ void mark_cols(f32x16_t* acc, const char* t, uint32_t
       acc[d] = mfma32x32x16(down, seen, acc[d]);
     }
   }
+}
+
+// A lane's column of transposed sums, 8 bytes of every 16 beside those of the lane 32 on, to 16-bit elements of a row: the two
+// exchange every other piece and write 16 bytes each.  LEFT: what the rounding left, to a second place.
+template <int DT, int D, bool LEFT = false>
+__device__ __forceinline__ void store_column(const f32x16_t* acc, float f, bool there, void* base, void* left, int64_t at) {
+  const int h = threadIdx.x >> 5 & 1;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; e += 8) {
+      float y[8];
+      u32x4_t w, r;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = acc[d][e + i] * f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = pack2<DT>(y[2 * i], y[2 * i + 1]);
+      if constexpr (LEFT) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = left2<DT>(y[2 * i], y[2 * i + 1], w[i]);
+      }
+      auto swap = [&](u32x4_t x) {
+        const u32x2_t a = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
+        const u32x2_t b = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+        return u32x4_t{a[0], b[0], a[1], b[1]};
+      };
+      w = swap(w);
+      if constexpr (LEFT) r = swap(r);
+      const int64_t x = at + 32 * d + 2 * e + 8 * h;
+      if (there) {
+        *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(base) + x) = w;
+        if constexpr (LEFT) *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(left) + x) = r;
+      }
+    }
 }
 
 // ---- the bias by distance -----------------------------------------------------------------
