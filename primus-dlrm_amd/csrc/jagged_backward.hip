@@ -208,10 +208,14 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
 #pragma unroll
     for (int x = 0; x < XX; ++x) {
       f32x16_t sc = zero16, dp = zero16;
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) sc = mfma32<DT>(Tile<D>::rows(tk, row_at, 32 * x, kk), q[kk], sc);
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) dp = mfma32<DT>(Tile<D>::rows(tv, row_at, 32 * x, kk), g[kk], dp);
+      for (int kk = 0; kk < KK; ++kk) {
+        sc = mfma32<DT>(Tile<D>::rows(tk, row_at, 32 * x, kk), q[kk], sc);
+        dp = mfma32<DT>(Tile<D>::rows(tv, row_at, 32 * x, kk), g[kk], dp);
+      }
+      sched_mfma_ds_pipeline<2 * KK, 4>();
+      __builtin_amdgcn_sched_barrier(0);
       float ds[16];
       const int local = c - 32 * x - 4 * h + KT - 1;
 #pragma unroll
@@ -237,16 +241,19 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
 #pragma unroll
         for (int e = 0; e < 16; ++e) ds[e] = sees(key + 32 * x + 4 * h + 8 * (e >> 2) + (e & 3)) ? ds[e] : 0.0f;
       }
+      bool lines = false;
       if (GB) {
         const int first = p_first - key - 32 * x - 31 - a.bias_start, last = first + 62;  // columns of the wave's pairs
         const int col = pos - key - 32 * x - 4 * h - a.bias_start;
-        float along = 0.0f;
+        lines = true;
         if (first >= a.bias_last) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) far += ds[e];
+          lines = false;
         } else if (last < 0) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) near += ds[e];
+          lines = false;
         } else {
           float* line = &skew[wave][4 * h][c + 31 - 4 * h];
           if (first >= 0 && last < a.bias_last) {
@@ -261,22 +268,23 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
               line[j * 63] = y >= 0 && y < a.bias_last ? ds[e] : 0.0f;
             }
           }
-          __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-          __builtin_amdgcn_wave_barrier();
-          __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-#pragma unroll
-          for (int r = 0; r < 32; r += 4)
-            along += (skew[wave][r][lane] + skew[wave][r + 1][lane]) + (skew[wave][r + 2][lane] + skew[wave][r + 3][lane]);
-          __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-          __builtin_amdgcn_wave_barrier();
-          __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
         }
-        win[t & 1][wave][x][lane] = along;
       }
       u32x4_t w[2];
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e >> 2][e & 3] = DT == PDM_F16 ? pack2<DT>(ds[2 * e] * ahead, ds[2 * e + 1] * ahead) : pack2<DT>(ds[2 * e], ds[2 * e + 1]);
       add_cols<DT, D, 2>(dq, tk, col_at, 32 * x, w);
+      if (GB) {  // (a wave's LDS instructions take effect in order: what the compiler must keep is theirs)
+        float along = 0.0f;
+        if (lines) {
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+#pragma unroll
+          for (int r = 0; r < 32; r += 4)
+            along += (skew[wave][r][lane] + skew[wave][r + 1][lane]) + (skew[wave][r + 2][lane] + skew[wave][r + 3][lane]);
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+        }
+        win[t & 1][wave][x][lane] = along;
+      }
     }
   }
   if (GB) {
@@ -311,14 +319,24 @@ __global__ void __launch_bounds__(1024) jag_dbias_kernel(JagArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cols = (int)a.part_stride - 2;
   const int head = blockIdx.y, col = blockIdx.x * 64 + lane;
   double sum = 0.0;
-  for (int64_t i = wave; i < a.items; i += 16) {
-    const int lo = a.part_range[2 * i], hi = a.part_range[2 * i + 1];
-    if (lo > hi) continue;
-    const float* p = a.part + (i * a.hq + head) * a.part_stride;
-    const int64_t d = (int64_t)col + a.bias_start;
-    if (col < cols && col < a.bias_last && d >= lo && d <= hi) sum += p[col];
-    if (col == a.bias_last) sum += p[cols];
-    if (col == 0) sum += p[cols + 1];
+  const int64_t d = (int64_t)col + a.bias_start;
+  for (int64_t i0 = wave; i0 < a.items; i0 += 16 * 64) {  // 64 blocks' ranges at once, a lane's each
+    const int64_t mine = i0 + 16 * lane;
+    int lo = 1, hi = 0;
+    if (mine < a.items) lo = a.part_range[2 * mine], hi = a.part_range[2 * mine + 1];
+    const int n = a.items - i0 < 16 * 64 ? (int)((a.items - i0 + 15) / 16) : 64;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const int from = __builtin_amdgcn_readlane(lo, j), to = __builtin_amdgcn_readlane(hi, j);
+      const float* p = a.part + ((i0 + 16 * j) * a.hq + head) * a.part_stride;
+      float v = 0.0f;
+      if (from <= to) {
+        if (col < cols && col < a.bias_last && d >= from && d <= to) v = p[col];
+        if (col == a.bias_last) v = p[cols];
+        if (col == 0) v += p[cols + 1];
+      }
+      sum += v;
+    }
   }
   part[wave][lane] = sum;
   __syncthreads();
@@ -484,15 +502,17 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
       if (unseen(i)) continue;
       const bool whole = all_seen(i);
       f32x16_t sc = zero16, dp = zero16;
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         u32x4_t f;
         if constexpr (KL) f = Tile<D>::rows(sk, row_at, 32 * wave, kk);
         else f = kf[kk];
         sc = mfma32<DT>(Tile<D>::rows(tq, row_at, 32 * x, kk), f, sc);
+        dp = mfma32<DT>(Tile<D>::rows(tg, row_at, 32 * x, kk), vf[kk], dp);
       }
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) dp = mfma32<DT>(Tile<D>::rows(tg, row_at, 32 * x, kk), vf[kk], dp);
+      if constexpr (!KL) sched_mfma_ds_pipeline<2 * KK, 4>();
+      __builtin_amdgcn_sched_barrier(0);
       float ahead = 1.0f;
       if (DT == PDM_F16) {
         const int want = kOut - a.expo[((item0 + (i >> 7)) * 4 + (i >> 5 & 3)) * a.hq + head];
