@@ -45,10 +45,11 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) jag_fwd_kernel(JagArgs a
   }
   // the query heads of a key head one after the other: with 8 key heads each has its keys in the cache of one XCD
   const int hx = (int)(unit % a.hq), kh = hx % a.hk, head = kh * a.group + hx / a.hk;
-  const int64_t item = a.items - 1 - unit / a.hq;  // later queries see more keys: they begin first
+  const int64_t place = unit / a.hq;
   JagSeq s;
   int b, r0;
-  if (!jag_block<M>(a, a.cu_q, item, s, b, r0)) return;
+  // later queries see more keys: they begin first
+  if (!(a.seqs <= 64 ? jag_ranked_block<M>(a, false, place, s, b, r0) : jag_block<M>(a, a.cu_q, a.items - 1 - place, s, b, r0))) return;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, h = lane >> 5;

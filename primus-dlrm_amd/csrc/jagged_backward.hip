@@ -52,14 +52,14 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
     return;
   }
   const int hx = (int)(unit % a.hq), kh = hx % a.hk, head = kh * a.group + hx / a.hk;
-  const int64_t item = a.items - 1 - unit / a.hq;
+  const int64_t place = unit / a.hq;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   JagSeq s;
   int b, r0;
-  if (!jag_block<M>(a, a.cu_q, item, s, b, r0)) {
-    if (GB && hx == 0 && tid == 0) a.part_range[2 * item] = 1, a.part_range[2 * item + 1] = 0;
-    return;
-  }
+  if (GB && hx == 0 && !jag_block<M>(a, a.cu_q, place, s, b, r0) && tid == 0)  // no partial result of that number
+    a.part_range[2 * place] = 1, a.part_range[2 * place + 1] = 0;
+  if (!(a.seqs <= 64 ? jag_ranked_block<M>(a, false, place, s, b, r0) : jag_block<M>(a, a.cu_q, a.items - 1 - place, s, b, r0))) return;
+  const int64_t item = (s.q0 / M) + b + r0 / M;
   const int c = lane & 31, h = lane >> 5;
   const int off = s.nk - s.nq;
   const JagKeys keys = jag_keys<KT>(a, s, r0, (r0 + M < s.nq ? r0 + M : s.nq) - 1);
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
       return;
     }
     kh = (int)(unit % a.hk);
-    if (!jag_block<M>(a, a.cu_k, unit / a.hk, s, b, j0)) return;
+    if (!(a.seqs <= 64 ? jag_ranked_block<M>(a, true, unit / a.hk, s, b, j0) : jag_block<M>(a, a.cu_k, unit / a.hk, s, b, j0))) return;
   }
   const int off = s.nk - s.nq, jw = SINK ? j0 : j0 + wave * 32;
   // queries that see a key of the block

@@ -62,6 +62,41 @@ __device__ __forceinline__ bool jag_block(const JagArgs& a, const int32_t* cu, i
   return true;
 }
 
+// The same list with the blocks that take longest first, for batches of at most 64 sequences, whose workgroups are few beside the
+// places for them: a late long one would be waited for (training on 8 sequences of 1,001 to 2,777 tokens: 633 -> TTT us).  A
+// block's cost goes by its level: causal, its number in the sequence, from the other end for blocks of keys (`keys`); else its
+// sequence's length.  Every lane has a sequence; the level of a rank is found by halving over sums of the wave.
+template <int M>
+__device__ __forceinline__ bool jag_ranked_block(const JagArgs& a, bool keys, int64_t rank, JagSeq& s, int& b, int& r0) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;  // blocks of this lane's sequence
+  if (lane < a.seqs && jag_seq(a, lane, s)) n = ((keys ? s.nk : s.nq) + M - 1) / M;
+  auto above = [&](int level) {  // blocks of higher levels
+    int x = a.causal ? (n - 1 > level ? n - 1 - level : 0) : (n - 1 > level ? n : 0);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+    return (int64_t)__builtin_amdgcn_readfirstlane(x);
+  };
+  int top = n;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) top = max(top, __shfl_xor(top, o));
+  top = __builtin_amdgcn_readfirstlane(top);
+  if (rank >= above(-1)) return false;
+  int lo = 0, hi = top - 1;  // the level: the lowest with above(level) <= rank
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (above(mid) <= rank) hi = mid;
+    else lo = mid + 1;
+  }
+  const int at = (int)(rank - above(lo)), each = a.causal ? 1 : lo + 1;  // place in the level; blocks that a sequence has there
+  const unsigned long long in = __ballot(a.causal ? n > lo : n == lo + 1);
+  const int before = __builtin_popcountll(in & ((1ull << lane) - 1));
+  b = __builtin_ctzll(__ballot((in >> lane & 1) && before == at / each));
+  const int blocks = __builtin_amdgcn_readlane(n, b);
+  r0 = (a.causal ? (keys ? blocks - 1 - lo : lo) : at % each) * M;
+  return jag_seq(a, b, s);
+}
+
 // Rows [first, first + 256) of the batch that no sequence which fits covers are given to clear(row), one after the other, by
 // the whole block of 256 threads; sequences [first, first + 256) that do not fit set the flag.
 template <typename F>
