@@ -59,18 +59,6 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) jag_fwd_kernel(JagArgs a
   // this lane's query and the keys that it sees: [row_lo, row_lo + row_n) and those below row_first
   const int row = r0 + wave * 32 + c, pos = off + row;
   int row_lo = 0, row_n = 0, row_first = 0;
-  u32x4_t q[KK];
-  {
-    const uint16_t* x = static_cast<const uint16_t*>(a.q) + (s.q0 + row) * a.q_st + head * a.q_sh + 8 * h;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) q[kk] = load16(x + 16 * kk, row < s.nq);
-    if (a.scale2 < 0.0f) {  // the scale's sign goes into the queries
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[kk][e] ^= 0x80008000u;
-    }
-  }
   const float scale2 = fmaxf(fabsf(a.scale2), 0x1p-126f);  // not zero: a hidden score times it stays -inf
   if (row < s.nq) {
     const int hi = a.causal && pos + 1 < s.nk ? (pos + 1 > 0 ? pos + 1 : 0) : s.nk;
@@ -118,6 +106,22 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) jag_fwd_kernel(JagArgs a
   };
   auto sees = [&](int j) { return (uint32_t)(j - row_lo) < (uint32_t)row_n || j < row_first; };
   bool odd = false;
+
+  const int tiles = keys.tiles;
+  // the queries come beside the first tile, by way of the second's place
+  char* own = (wave < 2 ? sk[1] : sv[1]) + (wave & 1) * 32 * Tile<D>::RS;
+  bring_own<D>(static_cast<const uint16_t*>(a.q) + s.q0 * a.q_st + head * a.q_sh, a.q_st, w0, s.nq, own);
+  if (tiles > 0) load_k(0), load_v(0), load_bias(0);
+  brought();
+  u32x4_t q[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) q[kk] = Tile<D>::rows(own, row_at, 0, kk);
+  if (a.scale2 < 0.0f) {  // the scale's sign goes into the queries
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[kk][e] ^= 0x80008000u;
+  }
 
   // ---- the steps of a tile ----
   f32x16_t sc[2];
@@ -188,8 +192,6 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) jag_fwd_kernel(JagArgs a
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  const int tiles = keys.tiles;
-  if (tiles > 0) load_k(0), load_v(0), load_bias(0);
 #pragma unroll 1
   for (int t = 0; t < tiles; ++t) {
     store_bias(t);
@@ -217,7 +219,8 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) jag_fwd_kernel(JagArgs a
   const float sum = l + __shfl_xor(l, 32);
   const int64_t at = (s.q0 + row) * a.hq + head;
   const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-  store_column<DT, D, FINE>(o, inv, row < s.nq, a.out, a.rest, at * D);
+  if (w0 < s.nq)
+    store_own<DT, D, FINE>(o, inv, &sk[0][0] + wave * 32 * Tile<D>::RS, a.out, a.rest, ((s.q0 + w0) * a.hq + head) * D, (int64_t)a.hq * D, s.nq - w0);
   if (h == 0 && row < s.nq) {
     // log2 of the sum: of its mantissa, and its exponent beside the reference, whose rounding it shares
     if (a.lse)

@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   __shared__ alignas(1024) char sv[2][KT * Tile<D>::RS];
   __shared__ float sb[2][BIAS ? M + KT : 1];
   __shared__ float win[2][GB ? 4 : 1][XX][GB ? 64 : 1];
-  __shared__ float skew[GB ? 4 : 1][GB ? 32 : 1][64];
+  __shared__ alignas(1024) float lines[GB || D == 128 ? 4 : 1][GB || D == 128 ? 32 : 1][64];
   __shared__ float ends[GB ? 8 : 1];
   __shared__ int odd_keys[2][KT], odd_any[2][4];
 
@@ -68,33 +68,42 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   const bool there = row < s.nq;
   const int64_t at = (s.q0 + row) * a.hq + head;
   int row_lo = 0, row_n = 0, row_first = 0;
+  // the wave's rows of q and dout, then of out and its rest, by way of the places of the tiles
+  const int w0 = r0 + wave * 32, p_first = off + w0, p_last = off + (w0 + 31 < s.nq ? w0 + 31 : s.nq - 1);
+  char *own = D == 64 ? &sk[0][0] + wave * 32 * Tile<D>::RS : (wave < 2 ? sk[wave & 1] : sv[wave & 1]);
+  char *own2 = D == 64 ? &sv[0][0] + wave * 32 * Tile<D>::RS : reinterpret_cast<char*>(&lines[wave][0][0]);
+  uint32_t row_at = Tile<D>::row_at(lane), col_at = Tile<D>::col_at(lane);
+  const int64_t o_st = (int64_t)a.hq * D, o_at = s.q0 * o_st + head * D;
   u32x4_t q[KK], g[KK];
   float delta = 0.0f, most = 0.0f, m = 0.0f, inv = 0.0f;
-  {
-    const uint16_t* x = static_cast<const uint16_t*>(a.q) + (s.q0 + row) * a.q_st + head * a.q_sh + 8 * h;
-    const uint16_t *y = static_cast<const uint16_t*>(a.dout) + at * D + 8 * h, *z = static_cast<const uint16_t*>(a.out) + at * D + 8 * h;
-    const uint16_t* r = static_cast<const uint16_t*>(a.rest) + at * D + 8 * h;
+  bring_own<D>(static_cast<const uint16_t*>(a.q) + s.q0 * a.q_st + head * a.q_sh, a.q_st, w0, s.nq, own);
+  bring_own<D>(static_cast<const uint16_t*>(a.dout) + o_at, o_st, w0, s.nq, own2);
+  brought();
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      q[kk] = load16(x + 16 * kk, there);
-      g[kk] = load16(y + 16 * kk, there);
-      const u32x4_t o = load16(z + 16 * kk, there);
-      u32x4_t o2 = {0, 0, 0, 0};
-      if (GB) o2 = load16(r + 16 * kk, there);
+  for (int kk = 0; kk < KK; ++kk) q[kk] = Tile<D>::rows(own, row_at, 0, kk), g[kk] = Tile<D>::rows(own2, row_at, 0, kk);
+  lds_barrier();
+  bring_own<D>(static_cast<const uint16_t*>(a.out) + o_at, o_st, w0, s.nq, own);
+  if (GB) bring_own<D>(static_cast<const uint16_t*>(a.rest) + o_at, o_st, w0, s.nq, own2);
+  brought();
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float lo = lo_of<DT>(g[kk][e]), hi = hi_of<DT>(g[kk][e]);
-        delta = __builtin_fmaf(lo, lo_of<DT>(o[e]), delta);
-        delta = __builtin_fmaf(hi, hi_of<DT>(o[e]), delta);
-        if (GB) {
-          delta = __builtin_fmaf(lo, lo_of<DT>(o2[e]), delta);
-          delta = __builtin_fmaf(hi, hi_of<DT>(o2[e]), delta);
-        }
-        if (DT == PDM_F16) most = fmaxf(most, fmaxf(fabsf(lo) < kInf ? fabsf(lo) : 0.0f, fabsf(hi) < kInf ? fabsf(hi) : 0.0f));
+  for (int kk = 0; kk < KK; ++kk) {
+    const u32x4_t o = Tile<D>::rows(own, row_at, 0, kk);
+    u32x4_t o2 = {0, 0, 0, 0};
+    if (GB) o2 = Tile<D>::rows(own2, row_at, 0, kk);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float lo = lo_of<DT>(g[kk][e]), hi = hi_of<DT>(g[kk][e]);
+      delta = __builtin_fmaf(lo, lo_of<DT>(o[e]), delta);
+      delta = __builtin_fmaf(hi, hi_of<DT>(o[e]), delta);
+      if (GB) {
+        delta = __builtin_fmaf(lo, lo_of<DT>(o2[e]), delta);
+        delta = __builtin_fmaf(hi, hi_of<DT>(o2[e]), delta);
       }
+      if (DT == PDM_F16) most = fmaxf(most, fmaxf(fabsf(lo) < kInf ? fabsf(lo) : 0.0f, fabsf(hi) < kInf ? fabsf(hi) : 0.0f));
     }
-    delta += __shfl_xor(delta, 32);
   }
+  delta += __shfl_xor(delta, 32);
+  lds_barrier();
   float back = a.scale, ahead = 1.0f;  // fp16: the row's power of two
   if (DT == PDM_F16) {
     most = fmaxf(most, __shfl_xor(most, 32));
@@ -112,7 +121,6 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
     if (a.dlse) delta -= a.dlse[at];  // d lse / d s = P
     if (h == 0) a.delta[at] = delta;
   }
-  const int w0 = r0 + wave * 32, p_first = off + w0, p_last = off + (w0 + 31 < s.nq ? w0 + 31 : s.nq - 1);
 
   const uint16_t* kp = static_cast<const uint16_t*>(a.k) + s.k0 * a.k_st + kh * a.k_sh;
   const uint16_t* vp = static_cast<const uint16_t*>(a.v) + s.k0 * a.v_st + kh * a.v_sh;
@@ -156,7 +164,7 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
     }
   };
   if (GB) {
-    float* w = &skew[0][0][0];
+    float* w = &lines[0][0][0];
     for (int i = tid; i < 4 * 32 * 64; i += 256) w[i] = 0.0f;
     if (hx == 0 && tid == 0) {
       a.part_range[2 * item] = keys.tiles ? off + r0 - jag_key<KT>(keys, keys.tiles - 1) - (KT - 1) : 1;
@@ -168,7 +176,6 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   f32x16_t dq[DD];
 #pragma unroll
   for (int d = 0; d < DD; ++d) dq[d] = zero16;
-  const uint32_t row_at = Tile<D>::row_at(lane), col_at = Tile<D>::col_at(lane);
 
   auto unseen = [&](int key) {  // (as in the forward pass)
     return w0 >= s.nq || (a.causal && key > p_last) || (a.window > 0 && key + KT - 1 <= p_first - a.window && key >= a.sinks);
@@ -207,6 +214,7 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
     const bool whole = all_seen(key);
 #pragma unroll
     for (int x = 0; x < XX; ++x) {
+      if (D == 128) asm volatile("" : "+v"(row_at), "+v"(col_at));  // places are computed here, not held through the loop
       f32x16_t sc = zero16, dp = zero16;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -241,21 +249,21 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
 #pragma unroll
         for (int e = 0; e < 16; ++e) ds[e] = sees(key + 32 * x + 4 * h + 8 * (e >> 2) + (e & 3)) ? ds[e] : 0.0f;
       }
-      bool lines = false;
+      bool near_lines = false;
       if (GB) {
         const int first = p_first - key - 32 * x - 31 - a.bias_start, last = first + 62;  // columns of the wave's pairs
         const int col = pos - key - 32 * x - 4 * h - a.bias_start;
-        lines = true;
+        near_lines = true;
         if (first >= a.bias_last) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) far += ds[e];
-          lines = false;
+          near_lines = false;
         } else if (last < 0) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) near += ds[e];
-          lines = false;
+          near_lines = false;
         } else {
-          float* line = &skew[wave][4 * h][c + 31 - 4 * h];
+          float* line = &lines[wave][4 * h][c + 31 - 4 * h];
           if (first >= 0 && last < a.bias_last) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) line[(8 * (e >> 2) + (e & 3)) * 63] = ds[e];
@@ -274,14 +282,14 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e >> 2][e & 3] = DT == PDM_F16 ? pack2<DT>(ds[2 * e] * ahead, ds[2 * e + 1] * ahead) : pack2<DT>(ds[2 * e], ds[2 * e + 1]);
       add_cols<DT, D, 2>(dq, tk, col_at, 32 * x, w);
-      if (GB) {  // (a wave's LDS instructions take effect in order: what the compiler must keep is theirs)
+      if (GB) {
         float along = 0.0f;
-        if (lines) {
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+        if (near_lines) {
+          own_lds_order();
 #pragma unroll
           for (int r = 0; r < 32; r += 4)
-            along += (skew[wave][r][lane] + skew[wave][r + 1][lane]) + (skew[wave][r + 2][lane] + skew[wave][r + 3][lane]);
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+            along += (lines[wave][r][lane] + lines[wave][r + 1][lane]) + (lines[wave][r + 2][lane] + lines[wave][r + 3][lane]);
+          own_lds_order();
         }
         win[t & 1][wave][x][lane] = along;
       }
@@ -310,7 +318,8 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
       __syncthreads();
     }
   }
-  store_column<DT, D>(dq, back, there, a.dq, nullptr, at * D);
+  if (w0 < s.nq)
+    store_own<DT, D>(dq, back, D == 64 ? own : own2, a.dq, nullptr, o_at + w0 * o_st, o_st, s.nq - w0);
 }
 
 // Sums the partial gradients of a column over the blocks of queries, in 64 bits: a lane per column, the blocks dealt to 16 waves.
@@ -413,20 +422,28 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
     const int hi = !SINK && a.window > 0 && edge < s.nq ? edge : s.nq;
     see_n = hi > see_lo ? hi - see_lo : 0;
   }
+  uint32_t row_at = Tile<D>::row_at(lane), col_at = Tile<D>::col_at(lane);
+  // the wave's keys and values, by way of the places of the tiles
+  const int64_t k_at = s.k0 * a.k_st + kh * a.k_sh, v_at = s.k0 * a.v_st + kh * a.v_sh;
+  char* own = SINK || D == 64 ? &sq[0][0] + wave * 32 * Tile<D>::RS : (wave < 2 ? sq[wave & 1] : sg[wave & 1]);
   u32x4_t kf[KL ? 1 : KK], vf[KK];
-  {
-    const uint16_t* x = static_cast<const uint16_t*>(a.k) + (s.k0 + key) * a.k_st + kh * a.k_sh + 8 * h;
-    const uint16_t* y = static_cast<const uint16_t*>(a.v) + (s.k0 + key) * a.v_st + kh * a.v_sh + 8 * h;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      if constexpr (!KL) kf[kk] = load16(x + 16 * kk, there);
-      vf[kk] = load16(y + 16 * kk, there);
-    }
-  }
   if constexpr (KL) {
+    bring_own<D>(static_cast<const uint16_t*>(a.v) + v_at, a.v_st, jw, s.nk, own);
     Bring<D, KEYS> bring_k;
     bring_k.init(a.k_st, lane, wave);
-    bring_k.load(static_cast<const uint16_t*>(a.k) + s.k0 * a.k_st + kh * a.k_sh, a.k_st, j0, s.nk, sk, wave);
+    bring_k.load(static_cast<const uint16_t*>(a.k) + k_at, a.k_st, j0, s.nk, sk, wave);
+    brought();
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) vf[kk] = Tile<D>::rows(own, row_at, 0, kk);
+    lds_barrier();
+  } else {
+    char* own2 = &sg[0][0] + wave * 32 * Tile<D>::RS;
+    bring_own<D>(static_cast<const uint16_t*>(a.v) + v_at, a.v_st, jw, s.nk, own);
+    bring_own<D>(static_cast<const uint16_t*>(a.k) + k_at, a.k_st, jw, s.nk, own2);
+    brought();
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) vf[kk] = Tile<D>::rows(own, row_at, 0, kk), kf[kk] = Tile<D>::rows(own2, row_at, 0, kk);
+    lds_barrier();
   }
 
   Bring<D, QT> bring_q, bring_g;
@@ -456,7 +473,6 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
   f32x16_t dk[DD], dv[DD];
 #pragma unroll
   for (int d = 0; d < DD; ++d) dk[d] = zero16, dv[d] = zero16;
-  const uint32_t row_at = Tile<D>::row_at(lane), col_at = Tile<D>::col_at(lane);
   int power = 100;  // fp16: dk holds sums times 2^power
   const int64_t item0 = (int64_t)a.cu_q[b] / M + b;
 
@@ -501,6 +517,7 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
       const int x = SINK ? wave : y0, i = i0 + 32 * x;
       if (unseen(i)) continue;
       const bool whole = all_seen(i);
+      if (D == 128) asm volatile("" : "+v"(row_at), "+v"(col_at));  // places are computed here, not held through the loop
       f32x16_t sc = zero16, dp = zero16;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -604,9 +621,10 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
       }
     return;
   }
-  const int64_t at = ((s.k0 + key) * a.hk + kh) * D;
-  store_column<DT, D>(dk, a.scale * back, there, a.dk, nullptr, at);
-  store_column<DT, D>(dv, 1.0f, there, a.dv, nullptr, at);
+  if (jw >= s.nk) return;
+  const int64_t at = ((s.k0 + jw) * a.hk + kh) * D, st = (int64_t)a.hk * D;
+  store_own<DT, D>(dk, a.scale * back, own, a.dk, nullptr, at, st, s.nk - jw);
+  store_own<DT, D>(dv, 1.0f, own, a.dv, nullptr, at, st, s.nk - jw);
 }
 
 // Gradients of 32 sinks of a key head, their sums under the window and beyond it: a thread an element.

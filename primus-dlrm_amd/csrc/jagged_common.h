@@ -62,39 +62,46 @@ __device__ __forceinline__ bool jag_block(const JagArgs& a, const int32_t* cu, i
   return true;
 }
 
+// Sum over the wave, for all of it: shifts within rows of 16 lanes, then rows on rows.
+__device__ __forceinline__ int wave_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // from 1, 2, 4 and 8 lanes below
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the last lane of a row to the next
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to the upper rows
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
 // The same list with the blocks that take longest first, for batches of at most 64 sequences, whose workgroups are few beside the
-// places for them: a late long one would be waited for (training on 8 sequences of 1,001 to 2,777 tokens: 633 -> TTT us).  A
+// places for them: a late long one would be waited for (training on 8 sequences of 1,001 to 2,777 tokens: 633 -> 557 us).  A
 // block's cost goes by its level: causal, its number in the sequence, from the other end for blocks of keys (`keys`); else its
 // sequence's length.  Every lane has a sequence; the level of a rank is found by halving over sums of the wave.
 template <int M>
 __device__ __forceinline__ bool jag_ranked_block(const JagArgs& a, bool keys, int64_t rank, JagSeq& s, int& b, int& r0) {
   const int lane = threadIdx.x & 63;
+  JagSeq mine{};
   int n = 0;  // blocks of this lane's sequence
-  if (lane < a.seqs && jag_seq(a, lane, s)) n = ((keys ? s.nk : s.nq) + M - 1) / M;
-  auto above = [&](int level) {  // blocks of higher levels
-    int x = a.causal ? (n - 1 > level ? n - 1 - level : 0) : (n - 1 > level ? n : 0);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
-    return (int64_t)__builtin_amdgcn_readfirstlane(x);
-  };
-  int top = n;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) top = max(top, __shfl_xor(top, o));
-  top = __builtin_amdgcn_readfirstlane(top);
+  if (lane < a.seqs && jag_seq(a, lane, mine)) n = ((keys ? mine.nk : mine.nq) + M - 1) / M;
+  auto above = [&](int level) { return wave_sum(a.causal ? (n - 1 > level ? n - 1 - level : 0) : (n - 1 > level ? n : 0)); };  // blocks of higher levels
   if (rank >= above(-1)) return false;
-  int lo = 0, hi = top - 1;  // the level: the lowest with above(level) <= rank
+  int lo = 0, hi = 1;  // the level: the lowest with above(level) <= rank
+  while (__ballot(n > hi)) hi *= 2;
+  --hi;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (above(mid) <= rank) hi = mid;
     else lo = mid + 1;
   }
-  const int at = (int)(rank - above(lo)), each = a.causal ? 1 : lo + 1;  // place in the level; blocks that a sequence has there
+  const int at = (int)rank - above(lo), each = a.causal ? 1 : lo + 1;  // place in the level; blocks that a sequence has there
   const unsigned long long in = __ballot(a.causal ? n > lo : n == lo + 1);
   const int before = __builtin_popcountll(in & ((1ull << lane) - 1));
   b = __builtin_ctzll(__ballot((in >> lane & 1) && before == at / each));
   const int blocks = __builtin_amdgcn_readlane(n, b);
   r0 = (a.causal ? (keys ? blocks - 1 - lo : lo) : at % each) * M;
-  return jag_seq(a, b, s);
+  s.q0 = __builtin_amdgcn_readlane((int)mine.q0, b), s.k0 = __builtin_amdgcn_readlane((int)mine.k0, b);
+  s.nq = __builtin_amdgcn_readlane(mine.nq, b), s.nk = __builtin_amdgcn_readlane(mine.nk, b);
+  return true;
 }
 
 // Rows [first, first + 256) of the batch that no sequence which fits covers are given to clear(row), one after the other, by
@@ -249,6 +256,30 @@ struct Bring {
 // This wave's loads into LDS have landed.
 __device__ __forceinline__ void brought() { __builtin_amdgcn_s_waitcnt(kWaitVmcnt0); }
 
+// A wave's own 32 rows of a head, [row0, row0 + 32) of n, into 32 rows of a tile.  (Fragments loaded from memory take 32 bytes of
+// 32 lines an instruction, and lines fall out of the first cache between two of them.)
+template <int D>
+__device__ __forceinline__ void bring_own(const void* head, int64_t stride, int row0, int n, const char* tile) {
+  constexpr int R = 64 / (D / 8);
+  const int lane = threadIdx.x & 63, rows = n - row0 < 32 ? n - row0 : 32;
+  const uint32_t step = (uint32_t)stride * 2;
+  const uint64_t base = reinterpret_cast<uint64_t>(static_cast<const uint16_t*>(head) + row0 * stride);
+  typedef uint32_t u32x4s __attribute__((ext_vector_type(4)));
+  const u32x4s rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32) & 0xffffu),
+                       (uint32_t)__builtin_amdgcn_readfirstlane(rows > 0 ? (rows - 1) * step + 2 * D : 0), 0x00027000u};
+  const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)tile));
+#pragma unroll
+  for (int i = 0; i < 32 / R; ++i) {
+    const int r = i * R + lane / (D / 8);
+    const uint32_t v = r * step + 16 * ((lane % (D / 8)) ^ Tile<D>::turn(r));
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                 :: "v"(v), "s"(rsrc), "s"(lds + i * 1024) : "memory", "m0");
+  }
+}
+
+// What a wave writes to LDS and reads back itself: its LDS instructions take effect in order, the compiler must keep theirs.
+__device__ __forceinline__ void own_lds_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
+
 // ---- products with a tile's columns ------------------------------------------------------
 // A weight of a pair that is not seen is zero, and what it meets must not matter, though 0 times an infinity or NaN would.  So
 // where not every pair of a tile is seen, a wave looks at the rows that it brought, before the others read them, and puts zeros
@@ -335,38 +366,39 @@ __device__ __forceinline__ void mark_cols(f32x16_t* acc, const char* t, uint32_t
   }
 }
 
-// A lane's column of transposed sums, 8 bytes of every 16 beside those of the lane 32 on, to 16-bit elements of a row: the two
-// exchange every other piece and write 16 bytes each.  LEFT: what the rounding left, to a second place.
+// A wave's 32 columns of transposed sums, times f, to rows of 16-bit elements `stride` apart, of which n are there: through 32
+// rows of a tile, so that whole lines are written.  LEFT: what the rounding left, to `left`.
 template <int DT, int D, bool LEFT = false>
-__device__ __forceinline__ void store_column(const f32x16_t* acc, float f, bool there, void* base, void* left, int64_t at) {
-  const int h = threadIdx.x >> 5 & 1;
+__device__ __forceinline__ void store_own(const f32x16_t* acc, float f, char* tile, void* base, void* left, int64_t at, int64_t stride, int n) {
+  constexpr int R = 64 / (D / 8);
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
 #pragma unroll
-  for (int d = 0; d < D / 32; ++d)
+  for (int pass = 0; pass < (LEFT ? 2 : 1); ++pass) {
 #pragma unroll
-    for (int e = 0; e < 16; e += 8) {
-      float y[8];
-      u32x4_t w, r;
+    for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = acc[d][e + i] * f;
+      for (int e = 0; e < 16; e += 4) {
+        float y[4];
+        u32x2_t w;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = pack2<DT>(y[2 * i], y[2 * i + 1]);
-      if constexpr (LEFT) {
+        for (int i = 0; i < 4; ++i) y[i] = acc[d][e + i] * f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = left2<DT>(y[2 * i], y[2 * i + 1], w[i]);
+        for (int i = 0; i < 2; ++i) {
+          w[i] = pack2<DT>(y[2 * i], y[2 * i + 1]);
+          if (pass) w[i] = left2<DT>(y[2 * i], y[2 * i + 1], w[i]);
+        }
+        *reinterpret_cast<u32x2_t*>(tile + c * Tile<D>::RS + 16 * ((4 * d + e / 4) ^ Tile<D>::turn(c)) + 8 * h) = w;
       }
-      auto swap = [&](u32x4_t x) {
-        const u32x2_t a = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
-        const u32x2_t b = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
-        return u32x4_t{a[0], b[0], a[1], b[1]};
-      };
-      w = swap(w);
-      if constexpr (LEFT) r = swap(r);
-      const int64_t x = at + 32 * d + 2 * e + 8 * h;
-      if (there) {
-        *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(base) + x) = w;
-        if constexpr (LEFT) *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(left) + x) = r;
-      }
+    own_lds_order();
+    uint16_t* to = static_cast<uint16_t*>(pass ? left : base) + at;
+#pragma unroll
+    for (int i = 0; i < 32 / R; ++i) {
+      const int r = i * R + lane / (D / 8);
+      const u32x4_t w = *reinterpret_cast<const u32x4_t*>(tile + i * 1024 + lane * 16);
+      if (r < n) *reinterpret_cast<u32x4_t*>(to + r * stride + 8 * ((lane % (D / 8)) ^ Tile<D>::turn(r))) = w;
     }
+    own_lds_order();
+  }
 }
 
 // ---- the bias by distance -----------------------------------------------------------------
