@@ -35,11 +35,13 @@ __global__ void __launch_bounds__(1024) bucket_range_kernel(const int32_t* map, 
   __shared__ int lo[kBuckets], hi[kBuckets];
   for (int b = threadIdx.x; b < buckets; b += 1024) lo[b] = 0x7fffffff, hi[b] = -1;
   __syncthreads();
+  // a bucket's first and last column are ends of runs of one bucket, and these are few
+#pragma unroll 8
   for (int c = threadIdx.x; c < span; c += 1024) {
-    const int b = map[c];
+    const int b = map[c], before = c > 0 ? map[c - 1] : -1, behind = c + 1 < span ? map[c + 1] : -1;
     if ((uint32_t)b < (uint32_t)buckets) {
-      atomicMin(&lo[b], c);
-      atomicMax(&hi[b], c);
+      if (b != before) atomicMin(&lo[b], c);
+      if (b != behind) atomicMax(&hi[b], c);
     }
   }
   __syncthreads();

@@ -76,10 +76,11 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) jag_fwd_kernel(JagArgs a
   bring_k.init(a.k_st, lane, wave);
   bring_v.init(a.v_st, lane, wave);
   float bias_next = 0.0f;
+  const int bias_at = bias_from(a, (int64_t)off + r0 - (KT - 1));
   auto load_k = [&](int t) { bring_k.load(kp, a.k_st, jag_key<KT>(keys, t), s.nk, sk[t & 1], wave); };
   auto load_v = [&](int t) { bring_v.load(vp, a.v_st, jag_key<KT>(keys, t), s.nk, sv[t & 1], wave); };
   auto load_bias = [&](int t) {  // entry x: distance of query r0 + x - 63 from the tile's first key
-    if (BIAS && tid < M + KT) bias_next = bias2(a, brow, (int64_t)off + r0 + tid - (KT - 1) - jag_key<KT>(keys, t));
+    if (BIAS && tid < M + KT) bias_next = bias2(a, brow, bias_at - jag_key<KT>(keys, t) + tid);
   };
   auto store_bias = [&](int t) {
     if (BIAS && tid < M + KT) sb[t & 1][tid] = bias_next;

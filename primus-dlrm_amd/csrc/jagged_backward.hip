@@ -129,11 +129,12 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   bring_k.init(a.k_st, lane, wave);
   bring_v.init(a.v_st, lane, wave);
   float bias_next = 0.0f;
+  const int bias_at = bias_from(a, (int64_t)off + r0 - (KT - 1));
   auto load = [&](int t) {
     const int key = jag_key<KT>(keys, t);
     bring_k.load(kp, a.k_st, key, s.nk, sk[t & 1], wave);
     bring_v.load(vp, a.v_st, key, s.nk, sv[t & 1], wave);
-    if (BIAS && tid < M + KT) bias_next = bias2(a, brow, (int64_t)off + r0 + tid - (KT - 1) - key);
+    if (BIAS && tid < M + KT) bias_next = bias2(a, brow, bias_at - key + tid);
   };
 
   // the bias's gradient: columns 0 .. cols - 1 of the partial result, then what lies behind them and before them
@@ -456,7 +457,7 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
     const int head = kh * a.group + head_next, i = i_lo + tile_next * QT;
     bring_q.load(static_cast<const uint16_t*>(a.q) + s.q0 * a.q_st + head * a.q_sh, a.q_st, i, s.nq, sq[n & 1], wave);
     bring_g.load(static_cast<const uint16_t*>(a.dout) + s.q0 * g_st + head * D, g_st, i, s.nq, sg[n & 1], wave);
-    if (BIAS && tid < KEYS + QT) bias_next = bias2(a, a.bias + (int64_t)head * (a.bias_last + 1), (int64_t)off + i + tid - (KEYS - 1) - j0);
+    if (BIAS && tid < KEYS + QT) bias_next = bias2(a, a.bias + (int64_t)head * (a.bias_last + 1), bias_from(a, (int64_t)off + i - (KEYS - 1) - j0) + tid);
 #pragma unroll
     for (int u = 0; u < (QT == 128 ? 2 : 1); ++u) {
       const int x = tid + 256 * u, r = i + (x & (QT - 1));

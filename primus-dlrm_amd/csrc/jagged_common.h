@@ -402,10 +402,14 @@ __device__ __forceinline__ void store_own(const f32x16_t* acc, float f, char* ti
 }
 
 // ---- the bias by distance -----------------------------------------------------------------
-// Of distance d in units of log2, finite where the bias is.
-__device__ __forceinline__ float bias2(const JagArgs& a, const float* row, int64_t d) {
+// Columns of a run of distances from d on, as a column that fits 32 bits with any key taken off: held where it makes no difference.
+__device__ __forceinline__ int bias_from(const JagArgs& a, int64_t d) {
   const int64_t c = d - a.bias_start;
-  const float b = row[c < 0 ? 0 : c > a.bias_last ? a.bias_last : c], v = b * kLog2e;
+  return c < -(1 << 30) ? -(1 << 30) : c > 0x7fffff00 ? 0x7fffff00 : (int)c;
+}
+// Of column c (held within the bias) in units of log2, finite where the bias is.
+__device__ __forceinline__ float bias2(const JagArgs& a, const float* row, int c) {
+  const float b = row[(uint32_t)min(max(c, 0), a.bias_last)], v = b * kLog2e;
   return fabsf(b) < kInf ? __builtin_amdgcn_fmed3f(v, -3.402823466e38f, 3.402823466e38f) : v;
 }
 

@@ -922,6 +922,13 @@ __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
   else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
+// A group's 128 rows are 128 / group tokens of each of its heads; the bias that a tile of keys needs, the distances of these
+// tokens from these keys, is brought to LDS while the products run, for each head a line of near_line() floats: an odd multiple
+// of 8, which spreads the heads over the banks.  (Loaded from memory by every lane for itself, two prompts as above under a
+// window of 2,048 took 752 us instead of TTT; groups whose lines do not fit still do that.)
+constexpr int kNear = 1024;
+__device__ __forceinline__ int near_line(int group, int KT) { return ((127 / group + 1 + KT + 23) & ~31) + 8; }
+
 template <int DT, int D, int KT, int NG, bool EXT>
 __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kernel(AttnArgs a, int64_t items) {
   constexpr int M = 128 * NG;
@@ -932,6 +939,7 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
   constexpr int LEAD = 8;                  // fragments read ahead of their products
   constexpr bool FINE = DT == PDM_F16;     // weights as two bf16 numbers (see the head of the file)
   __shared__ ManyShared<D, KT> sh;
+  __shared__ float near[EXT ? NG : 1][EXT ? kNear : 1];  // a group's bias of a tile, see near_bias
 
   const int64_t unit = linear_block();
   const int split = (int)(unit % a.splits);
@@ -992,6 +1000,28 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
   const int tok0 = r0 / a.group;
   const float* brow = EXT ? a.bias + (int64_t)(row < rows ? head : kh * a.group) * (a.bias_last + 1) : nullptr;
   const int bcol = sq.len - sq.n + (row < rows ? tok : tok0) - a.bias_start;
+  const int line = near_line(a.group, KT), line0 = (r0 + grp * 128) / a.group;  // floats of a head; the group's first token
+  const bool in_lds = EXT && a.bias && a.group * line <= kNear;
+  float near_next[EXT ? kNear / 256 : 1];
+  // Element x: head x / line, distance of its first token from the tile's last key, and x % line.
+  auto near_bias = [&](int t) {
+    if (!in_lds) return;
+    const int64_t c = (int64_t)sq.len - sq.n + line0 - real(begin + t * KT) - (KT - 1) - a.bias_start;
+    const int c0 = c < -(1 << 30) ? -(1 << 30) : c > (1 << 30) ? 1 << 30 : (int)c;
+    const float inv = 1.0f / line;
+#pragma unroll
+    for (int u = 0; u < kNear / 256; ++u) {
+      const int x = tid + 256 * u, hd = (int)((x + 0.5f) * inv);
+      if (x < a.group * line)
+        near_next[u] = bias_in_log2(a.bias[(int64_t)(kh * a.group + hd) * (a.bias_last + 1) + bias_column(a, c0 + x - hd * line)]);
+    }
+  };
+  auto near_store = [&]() {
+    if (!in_lds) return;
+#pragma unroll
+    for (int u = 0; u < kNear / 256; ++u)
+      if (tid + 256 * u < a.group * line) near[grp][tid + 256 * u] = near_next[u];
+  };
   const int pos0 = sq.len - sq.n + tok0, pos1 = sq.len - sq.n + (r0 + M < rows ? r0 + M - 1 : rows - 1) / a.group;
   // keys that every row of this wave sees
   int all_lo = 0, all_hi = sq.hi;
@@ -1185,6 +1215,21 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
       if (a.bias) {  // scores with their scale and bias
         const int64_t low = (int64_t)pos0 - key - (KT - 1) - a.bias_start, high = (int64_t)pos1 - key - a.bias_start;
         const bool inside = low >= 0 && high <= a.bias_last, alike = low >= a.bias_last || high <= 0;
+        if (in_lds) {
+          const float* b = &near[grp][(head - kh * a.group) * line + (tok - line0) + KT - 1 - 4 * h];
+          if (alike) {
+            const float one = b[0];
+#pragma unroll
+            for (int x = 0; x < XX; ++x)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) s[x][e] = __builtin_fmaf(s[x][e], sc[2 * x + (e >> 3)], one);
+          } else {
+#pragma unroll
+            for (int x = 0; x < XX; ++x)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) s[x][e] = __builtin_fmaf(s[x][e], sc[2 * x + (e >> 3)], b[-(32 * x + 8 * (e >> 2) + (e & 3))]);
+          }
+        } else {
         const float one = alike ? bias_in_log2(brow[low >= a.bias_last ? a.bias_last : 0]) : 0.0f;
 #pragma unroll
         for (int x = 0; x < XX; ++x)
@@ -1203,6 +1248,7 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[x][4 * y + e] = __builtin_fmaf(s[x][4 * y + e], sc[2 * x + (y >> 1)], v[e]);
           }
+        }
 #pragma unroll
         for (int x = 0; x < 2 * XX; ++x) sc[x] = sc[x] == sc[x] ? 1.0f : sc[x];
       }
@@ -1302,7 +1348,9 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
       if (decltype(kv)::value == 2) lds_barrier();
       lds_barrier();
       load(last > 0 ? 1 : 0, kv);
+      near_bias(0);
       scores(0);
+      near_store();
       lds_barrier();
       keys(1);
       weights(0);
@@ -1311,11 +1359,13 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
       for (int t = 1; t < tiles; ++t) {
         lds_barrier();
         load(last < t + 1 ? last : t + 1, kv);
+        near_bias(t);
         __builtin_amdgcn_sched_barrier(0);
         values(t - 1);
         __builtin_amdgcn_sched_barrier(0);
         scores(t);
         __builtin_amdgcn_sched_barrier(0);
+        near_store();
         lds_barrier();
         __builtin_amdgcn_sched_barrier(0);
         keys(t + 1);
