@@ -925,7 +925,7 @@ __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
 // A group's 128 rows are 128 / group tokens of each of its heads; the bias that a tile of keys needs, the distances of these
 // tokens from these keys, is brought to LDS while the products run, for each head a line of near_line() floats: an odd multiple
 // of 8, which spreads the heads over the banks.  (Loaded from memory by every lane for itself, two prompts as above under a
-// window of 2,048 took 752 us instead of TTT; groups whose lines do not fit still do that.)
+// window of 2,048 took 752 us instead of 491; groups whose lines do not fit still do that.)
 constexpr int kNear = 1024;
 __device__ __forceinline__ int near_line(int group, int KT) { return ((127 / group + 1 + KT + 23) & ~31) + 8; }
 
