@@ -258,7 +258,8 @@ int jag_args(const char* fn, const pdm_jagged_attention_desc* d, JagArgs& a) {
   if (d->q_tokens < 0 || d->k_tokens < 0 || d->q_tokens >= (1 << 30) || d->k_tokens >= (1 << 30)) return bad("tokens must lie in [0, 2^30)");
   if (d->q_tokens * d->n_q_heads >= (int64_t(1) << 31) || d->k_tokens * d->n_kv_heads >= (int64_t(1) << 31)) return bad("tokens * heads must be below 2^31");
   if (d->window < 0 || d->sinks < 0) return bad("window and sinks must not be negative");
-  if (!(d->scale - d->scale == 0.0f)) return bad("scale must be finite");
+  const float scale2 = d->scale * kLog2e;
+  if (!(scale2 - scale2 == 0.0f)) return bad("scale must be finite, and so must scale / ln 2");
   auto far = [](int64_t st) { return st < 0 || st >= (1 << 24); };
   if (far(d->q_stride_t) || far(d->k_stride_t) || far(d->v_stride_t)) return bad("token strides must lie in [0, 2^24)");
   if (d->bias_span < 0 || d->bias_span > (1 << 30)) return bad("bias_span must lie in [0, 2^30]");
@@ -271,7 +272,7 @@ int jag_args(const char* fn, const pdm_jagged_attention_desc* d, JagArgs& a) {
   a.bias_start = d->bias_start, a.bias_last = d->bias_span - 1;
   a.q_st = d->q_stride_t, a.q_sh = d->q_stride_h, a.k_st = d->k_stride_t, a.k_sh = d->k_stride_h;
   a.v_st = d->v_stride_t, a.v_sh = d->v_stride_h;
-  a.scale = d->scale, a.scale2 = d->scale * kLog2e;
+  a.scale = d->scale, a.scale2 = scale2;
   a.items = d->num_seqs ? d->q_tokens / 128 + d->num_seqs : 0;
   return PDM_OK;
 }

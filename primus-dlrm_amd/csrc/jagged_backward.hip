@@ -7,8 +7,9 @@
 // query, a key) and passes them on to the next product as the first leaves them.
 //
 // P and dS are rounded to the type of the operands for their products; the bias's gradient takes dS in 32 bits.  fp16 would
-// lose small dS (below 2^-14): its dS are multiplied by a power of two that brings dO to 2^-6, of each query for dQ, and of
-// 32 queries for dK, whose sums so far are brought to it.  (What is not finite does not count.)
+// lose small dS (below 2^-14): its dS are multiplied by a power of two that brings the larger of dO and the gradient of lse to
+// 2^-6, of each query for dQ, and of 32 queries for dK, whose sums so far are brought to it.  (What is not finite does not count.
+// dS of 2^20 times the largest |dO|, for which 64 values of 2^14 would have to point along dO, overflow.)
 #include <type_traits>
 
 #include "jagged_common.h"
@@ -22,7 +23,7 @@ int jag_inputs(const char* fn, JagArgs& a, const pdm_jagged_attention_desc* d, c
 namespace {
 
 constexpr int M = 128;
-constexpr int kOut = -5;     // |dO| below 2^kOut after its power of two
+constexpr int kOut = -5;     // |dO| and |dlse| below 2^kOut after their power of two
 constexpr int kNone = -100;  // exponent of rows of zeros
 
 __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
@@ -104,6 +105,11 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   }
   delta += __shfl_xor(delta, 32);
   lds_barrier();
+  if (there && a.dlse) {  // d lse / d s = P
+    const float x = a.dlse[at];
+    delta -= x;
+    if (DT == PDM_F16 && fabsf(x) < kInf) most = fmaxf(most, fabsf(x));
+  }
   float back = a.scale, ahead = 1.0f;  // fp16: the row's power of two
   if (DT == PDM_F16) {
     most = fmaxf(most, __shfl_xor(most, 32));
@@ -118,7 +124,6 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
     row_n = hi > row_lo ? hi - row_lo : 0;
     row_first = a.sinks < hi ? a.sinks : hi;
     m = a.stats[2 * at], inv = a.stats[2 * at + 1];
-    if (a.dlse) delta -= a.dlse[at];  // d lse / d s = P
     if (h == 0) a.delta[at] = delta;
   }
 
@@ -152,7 +157,10 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
       mine = base + rel;
     } else if (mine != base + rel) {
       put(mine, sum);
-      for (mine -= 256; mine > base + rel; mine -= 256) put(mine, 0.0f);
+      mine -= 256;
+      const int over = mine - (a.bias_start + cols - 1);  // distances of no column: passed at once
+      if (over > 0) mine -= min(mine - base - rel, (over + 255) & ~255);
+      for (; mine > base + rel; mine -= 256) put(mine, 0.0f);
       sum = 0.0f;
     }
 #pragma unroll
@@ -667,6 +675,9 @@ void sinks_of(JagArgs& a) {
   a.sink_shares = (int32_t)(shares > 1 ? shares : 1);
 }
 
+// The sums of sinks take 16 KiB (D 128: 32) a block of 32 in each sequence: as many as this do not run out of memory.
+constexpr int kMostSinks = 1024;
+
 struct Space {
   int64_t delta, expo, range, part, sinks, total;
 };
@@ -715,6 +726,7 @@ extern "C" int64_t pdm_jagged_attention_bwd_workspace_size(const pdm_jagged_atte
   JagArgs a{};
   if (int e = jag_args(__func__, desc, a)) return e;
   PDM_CHECK_ARG(!with_grad_bias || desc->bias_span > 0, "grad_bias without a bias");
+  PDM_CHECK_ARG(a.sinks <= kMostSinks, "at most 1024 sinks in a backward pass");
   return space_of(a, desc->dtype, desc->head_dim, with_grad_bias != 0).total;
 }
 
@@ -727,6 +739,7 @@ extern "C" int pdm_jagged_attention_bwd(const pdm_jagged_attention_desc* desc, c
   JagArgs a{};
   if (int e = jag_args(__func__, desc, a)) return e;
   if (int e = jag_inputs(__func__, a, desc, q, k, v, cu_q, cu_k, bias)) return e;
+  PDM_CHECK_ARG(a.sinks <= kMostSinks, "at most 1024 sinks in a backward pass");
   PDM_CHECK_ARG(a.q_tokens == 0 || (out && stats && grad_out && grad_q), "null out / stats / grad_out / grad_q");
   PDM_CHECK_ARG(a.k_tokens == 0 || (grad_k && grad_v), "null grad_k / grad_v");
   PDM_CHECK_ARG(!grad_bias || (bias && (a.q_tokens == 0 || out_rest)), "grad_bias without bias or out_rest");

@@ -1327,6 +1327,8 @@ def jagged_attention_raw(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_s
     index = _gpu_index(q, k, v, cu_seqlens, cu_seqlens_k, bias, err_flag)
     q, k, v = _even_heads(q), _even_heads(k), _even_heads(v)
     desc = _jagged_desc(q, k, v, cu_seqlens, cu_seqlens_k, bias, scale, causal, window, sinks, bias_start)
+    if keep and sinks > 1024 and k.shape[0] > 1024 and 0 < window < k.shape[0]:
+        raise ValueError(f"at most 1024 sinks where gradients are wanted, got {sinks}")
     T, hq = q.shape[:2]
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((T, hq), dtype=torch.float32, device=q.device) if return_lse else None

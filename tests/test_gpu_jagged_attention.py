@@ -172,6 +172,80 @@ def test_small_gradients_in_half_precision(pdm, dev):
     c.check_grads((dq, dk, dv, db), w)
 
 
+def test_gradients_of_lse_in_half_precision(pdm, dev):
+    """Of lse alone, and much larger than those of out."""
+    for size, mask in ((0.0, dict(causal=True)), (2.0 ** -20, dict(causal=True, window=60, sinks=4))):
+        c = Case([150, 20], [150, 70], 2, 1, 64, H, 12, seed=23)
+        c.go = (c.go.float() * size).to(H)
+        w = c.want(True, gl=True, **mask)
+        _, grads = c.grads(pdm, dev, gl=True, **mask)
+        # half a step of dS and of the result, each of its own size
+        for g, want in zip((grads[0], grads[1], grads[3]), (w.dq, w.dk, w.dbias)):
+            assert float((g.cpu().double() - want).norm() / want.norm()) < 2 * HALF[H]
+        assert size or (grads[2] == 0).all()
+
+
+@pytest.mark.parametrize("D,hk,group,dtype", [(64, 1, 4, B), (128, 2, 1, H), (64, 2, 1, H), (128, 1, 2, B)])
+def test_more_than_64_sequences(pdm, dev, D, hk, group, dtype):
+    g = torch.Generator().manual_seed(24)
+    lens = torch.randint(0, 60, (70,), generator=g).tolist()
+    lens[40], lens[41] = 400, 0
+    new = [min(n, x) for n, x in zip(lens, torch.randint(1, 500, (70,), generator=g).tolist())]
+    for span, start, mask in ((0, 0, dict(causal=False)), (30, 0, dict(causal=True, window=45, sinks=33)), (90, -40, dict(causal=False, window=20))):
+        c = Case(new, lens, hk * group, hk, D, dtype, span, start, seed=25)
+        w = c.want(True, **mask)
+        got, grads = c.grads(pdm, dev, **mask)
+        c.check(got, w)
+        c.check_grads(grads, w)
+
+
+@pytest.mark.parametrize("D,dtype", [(64, H), (128, B)])
+def test_sinks_of_long_sequences(pdm, dev, D, dtype):
+    """Queries beyond the window that are dealt to several workgroups; distances between the window and the sinks that no column
+    of the bias has, or that it has and no pair."""
+    for window, sinks, span, start in ((40, 2, 600, -100), (70, 100, 45, 0), (300, 33, 2600, 0), (40, 2, 100, 1900)):
+        c = Case([2600, 3], [2600, 2100], 4, 1, D, dtype, span, start, seed=window)
+        mask = dict(causal=True, window=window, sinks=sinks)
+        w = c.want(True, **mask)
+        got, grads = c.grads(pdm, dev, **mask)
+        c.check(got, w)
+        c.check_grads(grads, w)
+
+
+def test_two_graphs_on_two_streams(pdm, dev):
+    """Captured steps of different sizes, replayed at once and in turn."""
+    cases = [Case([700, 20], [700, 20], 2, 1, 64, H, 40, seed=26), Case([300], [300], 4, 2, 128, B, 90, seed=27)]
+    mask = dict(window=50, sinks=5)
+    want, graphs, made = [], [], []
+    for c in cases:
+        (out, _), grads = c.grads(pdm, dev, **mask)
+        want.append([out.detach().clone(), *[g.clone() for g in grads]])
+    del out, grads
+    for c in cases:
+        x, go, cu, cu_k = c.inputs(dev, True), c.go.to(dev), _t(c.cu_q, dev), _t(c.cu_k, dev)
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            out = pdm.jagged_attention(*x[:3], cu, cu_k, bias=x[3], **mask)
+            grads = torch.autograd.grad(out, x, go)
+        graphs.append(graph)
+        made.append([x, go, cu, cu_k, out.detach(), *grads])
+        del out, grads
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for turn in range(4):
+        for m in made:
+            for t in m[4:]:
+                t.fill_(math.nan)
+        torch.cuda.synchronize()
+        for i in (0, 1) if turn % 2 else (1, 0):
+            with torch.cuda.stream(side[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for m, wanted in zip(made, want):
+            assert all(torch.equal(a, b) for a, b in zip(wanted, m[4:]))
+        cases[0].run(pdm, dev)
+
+
 def test_values_up_to_the_largest(pdm, dev):
     c = Case([300], [300], 2, 1, 64, B, seed=7)
     c.v = (torch.sign(c.v.float()) * 3.3e38).to(B)

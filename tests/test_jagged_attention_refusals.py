@@ -59,6 +59,12 @@ def test_arguments(pdm, as_gpu):
     f(ValueError, "err_flag", err_flag=torch.zeros(1))
 
 
+def test_sinks_of_a_backward_pass(pdm, as_gpu):
+    q, k, v = (t.requires_grad_() for t in _qkv(T=1030))
+    with pytest.raises(ValueError, match="1024 sinks"):
+        pdm.jagged_attention(q, k, v, CU, window=5, sinks=1025)
+
+
 def test_gradients_that_do_not_fit(pdm, as_gpu):
     q, k, v = _qkv()
     out, stats = torch.zeros_like(q), torch.zeros(8, 4, 2)
@@ -152,6 +158,10 @@ def test_c_entries(pdm):
                      (dict(k_stride_t=1 << 24), "strides"), (dict(bias_start=1 << 30), "bias_start"), (dict(n_q_heads=65536 * 2), "65535")):
         assert lib.pdm_jagged_attention_workspace_size(desc(**kw)) == L.PDM_ERR_INVALID and text in L.last_error(), kw
         assert size(desc(**kw), 0) == L.PDM_ERR_INVALID
+    sinks = dict(k_tokens=5000, window=10, sinks=1025)
+    assert lib.pdm_jagged_attention_workspace_size(desc(**sinks)) == 0 and size(desc(**sinks), 0) == L.PDM_ERR_INVALID
+    assert "1024 sinks" in L.last_error() and size(desc(**{**sinks, "window": 5000}), 0) > 0
+    assert size(desc(scale=3e38), 0) == L.PDM_ERR_INVALID and "scale" in L.last_error()
     assert size(desc(), 1) == L.PDM_ERR_INVALID and "without a bias" in L.last_error()
     assert size(None, 0) == L.PDM_ERR_INVALID and "null" in L.last_error()
     fwd, bwd = lib.pdm_jagged_attention_fwd, lib.pdm_jagged_attention_bwd
