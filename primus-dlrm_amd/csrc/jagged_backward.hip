@@ -43,6 +43,10 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   __shared__ float win[2][GB ? 4 : 1][XX][GB ? 64 : 1];
   __shared__ alignas(1024) float lines[GB || D == 128 ? 4 : 1][GB || D == 128 ? 32 : 1][64];
   __shared__ float ends[GB ? 8 : 1];
+  // Where registers are short the last fragment of the queries stays in LDS: the compiler had put one into scratch memory, whose load
+  // in every tile waited for the next tile's to land (HOLDTEXT).
+  constexpr int HOLD = GB && D == 128 ? 2 : 0;
+  __shared__ u32x4_t held[HOLD ? 4 * HOLD : 1][HOLD ? 64 : 1];
   __shared__ int odd_keys[2][KT], odd_any[2][4];
 
   const int64_t unit = linear_block();
@@ -68,7 +72,6 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   const int row = r0 + wave * 32 + c, pos = off + row;
   const bool there = row < s.nq;
   const int64_t at = (s.q0 + row) * a.hq + head;
-  int row_lo = 0, row_n = 0, row_first = 0;
   // the wave's rows of q and dout, then of out and its rest, by way of the places of the tiles
   const int w0 = r0 + wave * 32, p_first = off + w0, p_last = off + (w0 + 31 < s.nq ? w0 + 31 : s.nq - 1);
   char *own = D == 64 ? &sk[0][0] + wave * 32 * Tile<D>::RS : (wave < 2 ? sk[wave & 1] : sv[wave & 1]);
@@ -82,6 +85,8 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   brought();
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) q[kk] = Tile<D>::rows(own, row_at, 0, kk), g[kk] = Tile<D>::rows(own2, row_at, 0, kk);
+#pragma unroll
+  for (int i = 0; i < HOLD; ++i) held[wave * HOLD + i][lane] = q[i];
   lds_barrier();
   bring_own<D>(static_cast<const uint16_t*>(a.out) + o_at, o_st, w0, s.nq, own);
   if (GB) bring_own<D>(static_cast<const uint16_t*>(a.rest) + o_at, o_st, w0, s.nq, own2);
@@ -119,10 +124,6 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
     if (e != kNone) ahead = pow2(kOut - e), back = a.scale * pow2(e - kOut);
   }
   if (there) {
-    const int hi = a.causal && pos + 1 < s.nk ? (pos + 1 > 0 ? pos + 1 : 0) : s.nk;
-    row_lo = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
-    row_n = hi > row_lo ? hi - row_lo : 0;
-    row_first = a.sinks < hi ? a.sinks : hi;
     m = a.stats[2 * at], inv = a.stats[2 * at + 1];
     if (h == 0) a.delta[at] = delta;
   }
@@ -196,7 +197,20 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   auto in_part = [&](int key) {
     return (a.causal && key + KT - 1 > b_first) || (a.window > 0 && key <= b_last - a.window && key + KT > a.sinks);
   };
-  auto sees = [&](int j) { return (uint32_t)(j - row_lo) < (uint32_t)row_n || j < row_first; };
+  struct Seen {  // keys that a query sees: [lo, lo + n) and those below first
+    int lo, n, first;
+    __device__ __forceinline__ bool operator()(int j) const { return (uint32_t)(j - lo) < (uint32_t)n || j < first; }
+  };
+  auto seen_from = [&](int p) {  // position p
+    Seen x{0, 0, 0};
+    if (p - off < s.nq) {
+      const int hi = a.causal && p + 1 < s.nk ? (p + 1 > 0 ? p + 1 : 0) : s.nk;
+      x.lo = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
+      x.n = hi > x.lo ? hi - x.lo : 0;
+      x.first = a.sinks < hi ? a.sinks : hi;
+    }
+    return x;
+  };
   bool odd = false;
   if (keys.tiles > 0) load(0);
 #pragma unroll 1
@@ -228,7 +242,7 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
-        sc = mfma32<DT>(Tile<D>::rows(tk, row_at, 32 * x, kk), q[kk], sc);
+        sc = mfma32<DT>(Tile<D>::rows(tk, row_at, 32 * x, kk), kk < HOLD ? held[wave * HOLD + kk][lane] : q[kk], sc);
         dp = mfma32<DT>(Tile<D>::rows(tv, row_at, 32 * x, kk), g[kk], dp);
       }
       sched_mfma_ds_pipeline<2 * KK, 4>();
@@ -255,6 +269,9 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
         }
       }
       if (!whole) {
+        int p = pos;
+        if (D == 128) asm volatile("" : "+v"(p));  // not held through the loop
+        const Seen sees = seen_from(p);
 #pragma unroll
         for (int e = 0; e < 16; ++e) ds[e] = sees(key + 32 * x + 4 * h + 8 * (e >> 2) + (e & 3)) ? ds[e] : 0.0f;
       }
@@ -316,6 +333,7 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
     if (tid < 2) part[cols + tid] = (ends[4 * tid] + ends[4 * tid + 1]) + (ends[4 * tid + 2] + ends[4 * tid + 3]);
   }
   if (__syncthreads_or(odd)) {
+    const Seen sees = seen_from(pos);
 #pragma unroll 1
     for (int t = 0; t < keys.tiles; ++t) {
       const int key = jag_key<KT>(keys, t);
