@@ -43,8 +43,8 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   __shared__ float win[2][GB ? 4 : 1][XX][GB ? 64 : 1];
   __shared__ alignas(1024) float lines[GB || D == 128 ? 4 : 1][GB || D == 128 ? 32 : 1][64];
   __shared__ float ends[GB ? 8 : 1];
-  // Where registers are short the last fragment of the queries stays in LDS: the compiler had put one into scratch memory, whose load
-  // in every tile waited for the next tile's to land (HOLDTEXT).
+  // Where registers are short two fragments of the queries stay in LDS: the compiler had put one into scratch memory, whose load in
+  // every tile waited for the next tile's to land (fp16, 24 heads of 8,134 tokens under a window of 512: 258 us instead of 234).
   constexpr int HOLD = GB && D == 128 ? 2 : 0;
   __shared__ u32x4_t held[HOLD ? 4 * HOLD : 1][HOLD ? 64 : 1];
   __shared__ int odd_keys[2][KT], odd_any[2][4];
@@ -401,7 +401,8 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
   __shared__ alignas(1024) char sg[2][QT * Tile<D>::RS];
   __shared__ alignas(1024) char sk[KL ? KEYS * Tile<D>::RS : 16];
   __shared__ float sb[2][BIAS ? KEYS + QT : 1];
-  __shared__ float ss[2][3][QT];
+  __shared__ alignas(16) float ss[2][3 * QT + 4];  // of the tile's queries: reference, 1 / sum, delta; fp16: the exponents of each 32
+  constexpr int STATS = 3 * QT + (DT == PDM_F16 ? QT / 32 : 0);
 
   const int64_t unit = linear_block();
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -474,11 +475,13 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
   }
 
   Bring<D, QT> bring_q, bring_g;
-  const int64_t g_st = (int64_t)a.hq * D;
+  const int64_t g_st = (int64_t)a.hq * D, item0 = s.q0 / M + b;
   bring_q.init(a.q_st, lane, wave);
   bring_g.init(g_st, lane, wave);
   float bias_next = 0.0f, stat_next[QT == 128 ? 2 : 1];
   int head_next = tiles ? n0 / tiles : 0, tile_next = tiles ? n0 % tiles : 0;
+  // (No load from memory may stand between these and their use: it would wait for them.  The exponents, read where they were needed,
+  // cost 236 us instead of 227.)
   auto load = [&](int n) {  // the head and tile at which the next load stands
     const int head = kh * a.group + head_next, i = i_lo + tile_next * QT;
     bring_q.load(static_cast<const uint16_t*>(a.q) + s.q0 * a.q_st + head * a.q_sh, a.q_st, i, s.nq, sq[n & 1], wave);
@@ -486,12 +489,13 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
     if (BIAS && tid < KEYS + QT) bias_next = bias2(a, a.bias + (int64_t)head * (a.bias_last + 1), bias_from(a, (int64_t)off + i - (KEYS - 1) - j0) + tid);
 #pragma unroll
     for (int u = 0; u < (QT == 128 ? 2 : 1); ++u) {
-      const int x = tid + 256 * u, r = i + (x & (QT - 1));
+      const int x = tid + 256 * u, r = i + (x & (QT - 1)), g = i + 32 * (x - 3 * QT);
       stat_next[u] = 0.0f;
       if (x < 3 * QT && r < s.nq) {
         const int64_t at = (s.q0 + r) * a.hq + head;
         stat_next[u] = x < QT ? a.stats[2 * at] : x < 2 * QT ? a.stats[2 * at + 1] : a.delta[at];
       }
+      if (x >= 3 * QT && x < STATS && g < s.nq) stat_next[u] = __int_as_float(a.expo[((item0 + (g >> 7)) * 4 + (g >> 5 & 3)) * a.hq + head]);
     }
     if (++tile_next == tiles) tile_next = 0, ++head_next;
   };
@@ -501,7 +505,6 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
 #pragma unroll
   for (int d = 0; d < DD; ++d) dk[d] = zero16, dv[d] = zero16;
   int power = 100;  // fp16: dk holds sums times 2^power
-  const int64_t item0 = (int64_t)a.cu_q[b] / M + b;
 
   // of 32 queries: none sees a key of this wave; each sees all of them (here); of a query: it sees this lane's key
   auto unseen = [&](int i) {
@@ -521,16 +524,16 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
   };
   auto sees = [&](int i) { return (uint32_t)(i - see_lo) < (uint32_t)see_n; };
   bool odd = false;
-  int hh = head_next, tt = tile_next;
+  int tt = tile_next;
   if (n1 > n0) load(n0);
 #pragma unroll 1
   for (int n = n0; n < n1; ++n) {
-    const int i0 = i_lo + tt * QT, head = kh * a.group + hh;
-    if (++tt == tiles) tt = 0, ++hh;
+    const int i0 = i_lo + tt * QT;
+    if (++tt == tiles) tt = 0;
     if (BIAS && tid < KEYS + QT) sb[n & 1][tid] = bias_next;
 #pragma unroll
     for (int u = 0; u < (QT == 128 ? 2 : 1); ++u)
-      if (tid + 256 * u < 3 * QT) (&ss[n & 1][0][0])[tid + 256 * u] = stat_next[u];
+      if (tid + 256 * u < STATS) ss[n & 1][tid + 256 * u] = stat_next[u];
     brought();
     if (in_part(i0)) {
       if (clean_rows<DT, D, QT>(sq[n & 1], lane, wave)) odd = true;
@@ -559,7 +562,7 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
       __builtin_amdgcn_sched_barrier(0);
       float ahead = 1.0f;
       if (DT == PDM_F16) {
-        const int want = kOut - a.expo[((item0 + (i >> 7)) * 4 + (i >> 5 & 3)) * a.hq + head];
+        const int want = kOut - __builtin_amdgcn_readfirstlane(__float_as_int(ss[n & 1][3 * QT + x]));
         if (want < power) {  // larger gradients than any before
           const float f = pow2(want - power);
           power = want;
@@ -572,8 +575,8 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         const int r = 32 * x + 8 * y + 4 * h;
-        const f32x4_t m = *reinterpret_cast<const f32x4_t*>(&ss[n & 1][0][r]), inv = *reinterpret_cast<const f32x4_t*>(&ss[n & 1][1][r]);
-        const f32x4_t delta = *reinterpret_cast<const f32x4_t*>(&ss[n & 1][2][r]);
+        const f32x4_t m = *reinterpret_cast<const f32x4_t*>(&ss[n & 1][r]), inv = *reinterpret_cast<const f32x4_t*>(&ss[n & 1][QT + r]);
+        const f32x4_t delta = *reinterpret_cast<const f32x4_t*>(&ss[n & 1][2 * QT + r]);
 #pragma unroll
         for (int z = 0; z < 4; ++z) {
           const int e = 4 * y + z;
