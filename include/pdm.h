@@ -727,7 +727,8 @@ int pdm_kv_attention_biased_fwd(const pdm_kv_attention_desc* desc,
  * the keys j with j <= p (causal) and, with window > 0, j > p - window or
  * j < sinks.  Its score of key j is
  *   scale * q . k_j + bias[h][c],  c = p - j - bias_start held within [0, bias_span)
- * Tokens < 2^30, tokens * heads < 2^31, num_seqs <= 2^24. */
+ * q, k and v are 16-byte aligned, their strides multiples of 8, those of tokens
+ * < 2^24.  Tokens < 2^30, tokens * heads < 2^31, num_seqs <= 2^24. */
 typedef struct {
   int32_t dtype;      /* PDM_F16 | PDM_BF16: q, k, v, out and their gradients */
   int32_t n_q_heads;  /* a multiple of n_kv_heads, at most 65535 */
@@ -773,8 +774,10 @@ int pdm_jagged_attention_fwd(const pdm_jagged_attention_desc* desc,
  * are zeros) and, where grad_bias is not NULL, of the bias (fp32, summed over
  * sequences and pairs).  out, out_rest (with grad_bias), stats: of the forward
  * pass; grad_out: contiguous, 16-byte aligned; grad_lse: optional, of lse.  Sums
- * run in one fixed order: the same inputs give the same bits.
- * |bias_start| < 2^30. */
+ * run in one fixed order: the same inputs give the same bits.  At most 1,024
+ * sinks (where window < k_tokens).  workspace: 256-byte aligned; with grad_bias it
+ * holds min(bias_span, k_tokens - bias_start) floats for every head and 128
+ * queries.  |bias_start| < 2^30. */
 int64_t pdm_jagged_attention_bwd_workspace_size(const pdm_jagged_attention_desc* desc, int32_t with_grad_bias);
 
 int pdm_jagged_attention_bwd(const pdm_jagged_attention_desc* desc,

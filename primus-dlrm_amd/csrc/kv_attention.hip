@@ -15,6 +15,11 @@
 // of their outputs goes from 1.7e-3, of the output's own rounding, to 2.1e-3, at 794 us instead of 1,048.  The running sum
 // takes weights before any rounding.
 //
+// Sinks and a bias by distance (EXT) are instances of their own, which leave the plain ones their registers.  Keys between the
+// sinks and the window are skipped in whole tiles.  A tile whose distances all have one column reads it once; 16 rows do not feel
+// the bias (64 sequences of 128 to 8,192: 66 us with it, 63 without), 17 to 32 rows of heads of 64 do (256 sequences of 300 to
+// 1,500: 68 and 45: its fragments are read when the tile is there, and do not fit the registers earlier).
+//
 // The simplest kernel, a wave for each (row, head), took 289 us for one sequence of 1,000 tokens, 4,764 for 64 of 128 to 8,192
 // and 110,493 for two prompts of 4,000 tokens behind 4,000 (32 query heads, 8 key heads of 128); these take 9.6, 65 and 786.
 #include <type_traits>
