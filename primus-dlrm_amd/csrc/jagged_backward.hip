@@ -13,8 +13,8 @@
 // dS of 2^20 times the largest |dO|, for which 64 values of 2^14 would have to point along dO, overflow.)
 //
 // Bound by latency at two waves a SIMD (matrix units 20 to 30 %, vector units 30 to 45, LDS 20 to 40 % of the time busy): 8
-// sequences of 1,001 to 2,777 tokens, 8 heads of 64, both sides: 195 us by queries, of which the bias's gradient takes about
-// half, and 182 by keys (0.59 PFLOP/s); 8,134 tokens, 24 heads of 128 on 6, window 512 with 4 sinks, fp16: 233, 227 and 46 for
+// sequences of 1,001 to 2,777 tokens, 8 heads of 64, both sides: 211 us by queries, of which the bias's gradient takes about
+// half, and 197 by keys (0.55 PFLOP/s); 8,134 tokens, 24 heads of 128 on 6, window 512 with 4 sinks, fp16: 234, 228 and 46 for
 // the sinks.
 #include <type_traits>
 
