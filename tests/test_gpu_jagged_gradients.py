@@ -1,0 +1,67 @@
+"""Gradients of jagged_attention where the definition leaves no room: rows that see one key."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_jagged_attention import B, H, HALF, Case
+
+pytestmark = pytest.mark.gpu
+
+KINDS = [(64, 3, 1, B), (128, 1, 4, B), (64, 2, 2, H), (128, 2, 1, H)]
+
+
+def _new(c, dtype):
+    """The case's gradients of a batch of its own seed: of any size, as training has them."""
+    c.go = (c.go.float() * 3).to(dtype)
+    return c
+
+
+# ---- rows that see one key ------------------------------------------------------------------
+# The softmax of one score is 1 whatever the score, so dS is 0: q, k and the bias get no gradient at all, and v that of the output.
+
+@pytest.mark.parametrize("D,hk,group,dtype", KINDS)
+@pytest.mark.parametrize("span,start", [(0, 0), (1, 0), (40, -3)])
+@pytest.mark.parametrize("lens,mask", [([1] * 130, dict(causal=True)), ([1] * 9, dict(causal=False)), ([100, 33, 1], dict(causal=True, window=1)),
+                                       ([700], dict(causal=True, window=1)), ([1] * 70, dict(causal=True, window=5, sinks=2))])
+def test_rows_that_see_one_key(pdm, dev, D, hk, group, dtype, span, start, lens, mask):
+    c = _new(Case(lens, lens, hk * group, hk, D, dtype, span, start, seed=len(lens) + D), dtype)
+    (out, _), grads = c.grads(pdm, dev, **mask)
+    assert torch.equal(out.cpu(), c.v.repeat_interleave(group, 1))
+    dq, dk, dv, *db = (g.cpu() for g in grads)
+    assert not dq.any() and not dk.any() and not (db and db[0].any())
+    want = c.go.double().view(-1, hk, group, D).sum(2)
+    # the sum over the group in fp32, rounded once
+    assert ((dv.double() - want).abs() <= HALF[dtype] * want.abs() + 4 * 2.0 ** -24 * c.go.double().abs().view(-1, hk, group, D).sum(2)).all()
+
+
+@pytest.mark.parametrize("D,hk,group,dtype", KINDS)
+@pytest.mark.parametrize("span", [0, 25])
+def test_rows_that_see_one_key_beside_others(pdm, dev, D, hk, group, dtype, span):
+    """The first query of a causal sequence; the first one that has a key at all; queries before their window's sink."""
+    for new, lens, mask, rows in (([150, 1, 40], [150, 90, 40], dict(causal=True), [0, 151]), ([70, 5], [30, 5], dict(causal=True), [40, 70]),
+                                  ([90], [90], dict(causal=True, window=1, sinks=1), [0])):
+        c = _new(Case(new, lens, hk * group, hk, D, dtype, span, seed=D), dtype)
+        got, grads = c.grads(pdm, dev, **mask)
+        assert not grads[0][rows].any() and grads[0].any()
+        w = c.want(True, **mask)
+        c.check(got, w)
+        c.check_grads(grads, w)
+
+
+def test_rows_that_see_one_key_through_lse(pdm, dev):
+    """lse is the score then, and its gradient the score's."""
+    for D, dtype, span in ((64, B, 0), (128, H, 30), (64, H, 0), (128, B, 30)):
+        c = Case([90, 1], [90, 1], 2, 1, D, dtype, span, seed=D)
+        c.go = torch.zeros_like(c.go)
+        _, (dq, dk, dv, *db) = c.grads(pdm, dev, gl=True, window=1)
+        gl, scale = c.gl.double()[..., None], D ** -0.5
+        for got, want in ((dq, gl * scale * c.k.double()), (dk, (gl * scale * c.q.double()).sum(1, keepdim=True))):
+            # half a step of dS, of the result
+            slack = 2 * HALF[dtype] * (gl.abs() * scale * (c.k if got is dq else c.q).double().abs())
+            slack = slack if got is dq else slack.sum(1, keepdim=True)
+            assert ((got.cpu().double() - want).abs() <= slack + 2.0 ** -24).all()
+        assert not dv.any()
+        if span:
+            assert ((db[0].cpu().double()[:, 0] - c.gl.double().sum(0)).abs() <= 91 * 2.0 ** -24 * c.gl.double().abs().sum(0)).all()
+            assert not db[0][:, 1:].any()
