@@ -291,27 +291,29 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
       if (GB) {
         const int first = p_first - key - 32 * x - 31 - a.bias_start, last = first + 62;  // columns of the wave's pairs
         const int col = pos - key - 32 * x - 4 * h - a.bias_start;
-        near_lines = true;
-        if (first >= a.bias_last) {
+        near_lines = first < a.bias_last && last >= 0;
+        // Rows that are not there stay out of these sums (their places in the lines stay zero): nothing holds their weights, which
+        // are the bias's alone, and infinity times 0 for a large one.
+        if (there) {
+          if (first >= a.bias_last) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) far += ds[e];
-          near_lines = false;
-        } else if (last < 0) {
+            for (int e = 0; e < 16; ++e) far += ds[e];
+          } else if (last < 0) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) near += ds[e];
-          near_lines = false;
-        } else {
-          float* line = &lines[wave][4 * h][c + 31 - 4 * h];
-          if (first >= 0 && last < a.bias_last) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) line[(8 * (e >> 2) + (e & 3)) * 63] = ds[e];
+            for (int e = 0; e < 16; ++e) near += ds[e];
           } else {
+            float* line = &lines[wave][4 * h][c + 31 - 4 * h];
+            if (first >= 0 && last < a.bias_last) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int j = 8 * (e >> 2) + (e & 3), y = col - j;
-              far += y >= a.bias_last ? ds[e] : 0.0f;
-              near += y < 0 ? ds[e] : 0.0f;
-              line[j * 63] = y >= 0 && y < a.bias_last ? ds[e] : 0.0f;
+              for (int e = 0; e < 16; ++e) line[(8 * (e >> 2) + (e & 3)) * 63] = ds[e];
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const int j = 8 * (e >> 2) + (e & 3), y = col - j;
+                far += y >= a.bias_last ? ds[e] : 0.0f;
+                near += y < 0 ? ds[e] : 0.0f;
+                line[j * 63] = y >= 0 && y < a.bias_last ? ds[e] : 0.0f;
+              }
             }
           }
         }

@@ -1,4 +1,4 @@
-"""Gradients of jagged_attention where the definition leaves no room: rows that see one key."""
+"""Gradients of jagged_attention where the definition leaves no room: rows that see one key; rows behind the last query, columns that no pair has."""
 import math
 
 import pytest
@@ -65,3 +65,44 @@ def test_rows_that_see_one_key_through_lse(pdm, dev):
         if span:
             assert ((db[0].cpu().double()[:, 0] - c.gl.double().sum(0)).abs() <= 91 * 2.0 ** -24 * c.gl.double().abs().sum(0)).all()
             assert not db[0][:, 1:].any()
+
+
+# ---- rows behind a sequence's last query -------------------------------------------------------
+# A block holds 32 queries, of which the last ones may not be there.  What the bias holds at their distances is nobody's.
+
+@pytest.mark.parametrize("D,dtype", [(64, B), (128, H)])
+@pytest.mark.parametrize("new,lens", [([100], [300]), ([1, 33], [65, 400]), ([150], [150])])
+def test_a_bias_of_any_size(pdm, dev, D, dtype, new, lens):
+    """A constant added to a head's bias changes no gradient, however large the weights of it alone would be."""
+    for mask, span in ((dict(causal=True), 350), (dict(causal=True), 20), (dict(causal=False), 30), (dict(causal=True, window=70, sinks=3), 350)):
+        c = Case(new, lens, 2, 1, D, dtype, span, -100 if not mask["causal"] else 0, seed=span)
+        c.bias[0] += 100.0
+        c.bias[1] += 1000.0
+        w = c.want(True, **mask)
+        got, grads = c.grads(pdm, dev, **mask)
+        c.check(got, w)
+        c.check_grads(grads, w)
+
+
+@pytest.mark.parametrize("D,dtype", [(64, B), (128, H)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, 3e38])
+def test_columns_that_no_seen_pair_has(pdm, dev, D, dtype, bad):
+    for new, lens, mask, span, first in (([100], [300], dict(causal=True, window=80), 300, 80), ([33, 70], [33, 300], dict(causal=True), 400, 300),
+                                         ([40], [140], dict(causal=False, window=100), 250, 100 + 139)):
+        c = Case(new, lens, 2, 1, D, dtype, span, 0 if mask["causal"] else -139, seed=3)
+        w = c.want(True, **mask)
+        c.bias[:, first:] = bad
+        got, grads = c.grads(pdm, dev, **mask)
+        c.check(got, w)
+        assert not grads[3][:, first:].any()
+        c.check_grads(grads, w)
+
+
+def test_a_key_that_is_not_finite_reaches_seen_columns_alone(pdm, dev):
+    for D, dtype in ((64, B), (128, H)):
+        c = Case([70], [300], 2, 1, D, dtype, 400, seed=4)
+        c.k[200, 0, 3] = math.inf
+        _, grads = c.grads(pdm, dev)
+        # (a row whose score of that key is -inf does without it)
+        finite = torch.isfinite(c.want(True).dbias)
+        assert not finite.all() and torch.equal(torch.isfinite(grads[3]).cpu(), finite) and not grads[3][:, 300:].any()
