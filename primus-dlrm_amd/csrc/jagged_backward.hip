@@ -9,7 +9,8 @@
 //
 // P and dS are rounded to the type of the operands for their products; the bias's gradient takes dS in 32 bits.  fp16 would
 // lose small dS (below 2^-14): its dS are multiplied by a power of two that brings the larger of dO and the gradient of lse to
-// 2^-6, of each query for dQ, and of 32 queries for dK, whose sums so far are brought to it.  (What is not finite does not count.
+// 2^-6, of each query for dQ, and of 32 queries for dK, whose sums so far are brought to it.  Weights for dV go in times 2^15, so
+// that those down to 2^-29 keep all their bits; a larger dO would not bring them back.  (What is not finite does not count.
 // dS of 2^20 times the largest |dO|, for which 64 values of 2^14 would have to point along dO, overflow.)
 //
 // Bound by latency at two waves a SIMD (matrix units 20 to 30 %, vector units 30 to 45, LDS 20 to 40 % of the time busy): 8
@@ -31,6 +32,7 @@ namespace {
 constexpr int M = 128;
 constexpr int kOut = -5;     // |dO| and |dlse| below 2^kOut after their power of two
 constexpr int kNone = -100;  // exponent of rows of zeros
+constexpr float kLarge = 0x1p15f;  // fp16: weights, 1 at most, go into dV's product times this
 
 __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
 
@@ -547,7 +549,7 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
     if (BIAS && tid < KEYS + QT) sb[n & 1][tid] = bias_next;
 #pragma unroll
     for (int u = 0; u < (QT == 128 ? 2 : 1); ++u)
-      if (tid + 256 * u < STATS) ss[n & 1][tid + 256 * u] = stat_next[u];
+      if (const int x = tid + 256 * u; x < STATS) ss[n & 1][x] = DT == PDM_F16 && x >= QT && x < 2 * QT ? stat_next[u] * kLarge : stat_next[u];
     brought();
     if (in_part(i0)) {
       if (clean_rows<DT, D, QT>(sq[n & 1], lane, wave)) odd = true;
@@ -583,9 +585,9 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
 #pragma unroll
           for (int d = 0; d < DD; ++d) dk[d] *= f;
         }
-        ahead = pow2(power);
+        ahead = pow2(power) / kLarge;
       }
-      float p[16], ds[16];
+      float p[16], ds[16];  // fp16: times kLarge
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         const int r = 32 * x + 8 * y + 4 * h;
@@ -634,7 +636,7 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
       __syncthreads();
     }
   }
-  const float back = DT == PDM_F16 ? pow2(-power) : 1.0f;
+  const float back = DT == PDM_F16 ? pow2(-power) : 1.0f, back_v = DT == PDM_F16 ? 1.0f / kLarge : 1.0f;
   // sums of a sink's block in fp32: [dk, dv][d][32 keys]
   auto sums_of = [&](int block, int slot) { return a.sink_part + (sink_slots(a, b, block, kh) + slot) * (2 * D * 32); };
   if constexpr (SINK) {
@@ -646,7 +648,7 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
 #pragma unroll
       for (int d = 0; d < DD; ++d)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mine[(32 * d + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + c] = z ? dv[d][e] : dk[d][e] * back;
+        for (int e = 0; e < 16; ++e) mine[(32 * d + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + c] = z ? dv[d][e] * back_v : dk[d][e] * back;
       __syncthreads();
       for (int x = tid; x < D * 32; x += 256)
         to[z * D * 32 + x] = (reinterpret_cast<const float*>(sq[0])[x] + reinterpret_cast<const float*>(sq[1])[x]) +
@@ -661,14 +663,14 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int x = (32 * d + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + c;
-        to[x] = dk[d][e] * back, to[D * 32 + x] = dv[d][e];
+        to[x] = dk[d][e] * back, to[D * 32 + x] = dv[d][e] * back_v;
       }
     return;
   }
   if (jw >= s.nk) return;
   const int64_t at = ((s.k0 + jw) * a.hk + kh) * D, st = (int64_t)a.hk * D;
   store_own<DT, D>(dk, a.scale * back, own, a.dk, nullptr, at, st, s.nk - jw);
-  store_own<DT, D>(dv, 1.0f, own, a.dv, nullptr, at, st, s.nk - jw);
+  store_own<DT, D>(dv, back_v, own, a.dv, nullptr, at, st, s.nk - jw);
 }
 
 // Gradients of 32 sinks of a key head, their sums under the window and beyond it: a thread an element.

@@ -1,4 +1,4 @@
-"""Gradients of jagged_attention where the definition leaves no room: rows that see one key; rows behind the last query, columns that no pair has."""
+"""Gradients of jagged_attention where the definition leaves no room: rows that see one key; rows behind the last query, columns that no pair has; small weights."""
 import math
 
 import pytest
@@ -106,3 +106,37 @@ def test_a_key_that_is_not_finite_reaches_seen_columns_alone(pdm, dev):
         # (a row whose score of that key is -inf does without it)
         finite = torch.isfinite(c.want(True).dbias)
         assert not finite.all() and torch.equal(torch.isfinite(grads[3]).cpu(), finite) and not grads[3][:, 300:].any()
+
+
+# ---- small weights in fp16 --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("gap", [9.0, 13.0, 17.0, 19.5])
+@pytest.mark.parametrize("mask", [dict(causal=False), dict(causal=True, window=60, sinks=40)])
+def test_small_weights_in_half_precision(pdm, dev, D, gap, mask):
+    """One key takes nearly all of every row; the others' gradients, of weights about e^-gap and a scaled gradient of the output,
+    are as exact as large ones.  p <= 1 meets dO as p 2^15: half a step of it down to 2^-29, 2^-40 below."""
+    n, scale = 200, D ** -0.5
+    c = Case([n], [n], 1, 1, D, H, seed=int(gap))
+    u = torch.ones(D) / math.sqrt(D)
+    c.q = (u + torch.randn(n, 1, D, generator=torch.Generator().manual_seed(1)) * 0.02).to(H)
+    c.k = (c.k.float() * 0.02).to(H)
+    c.k[0, 0] = (u * gap / scale).to(H)
+    c.go = (c.go.float() * 500).to(H)
+    q, k, go = c.q[:, 0].double(), c.k[:, 0].double(), c.go[:, 0].double()
+    seen = torch.ones(n, n, dtype=torch.bool)
+    if mask["causal"]:
+        i, j = torch.arange(n)[:, None], torch.arange(n)[None]
+        seen = (j <= i) & ((j > i - 60) | (j < 40))
+    p = torch.softmax((q @ k.T * scale).masked_fill(~seen, -math.inf), -1)
+    assert p[100, 1:][seen[100, 1:]].max() < 2.0 ** -11
+    want, size = p.T @ go, p.T @ go.abs()
+    serr = float((q.abs() @ k.abs().T * scale).max())
+    e_w = 2 * (D + 8) * 2.0 ** -24 * serr + 2.0 ** -20 + n * 2.0 ** -24
+    tol = (HALF[H] + e_w) * size + 2.0 ** -40 * go.abs().sum(0)
+    _, (_, _, dv) = c.grads(pdm, dev, **mask)
+    bad = (dv[:, 0].cpu().double() - want).abs() - tol - HALF[H] * (want.abs() + tol) - 2.0 ** -25
+    assert bad.max().item() <= 0, f"dv over by {bad.max().item():.3e}"
+    # (a result below 2^-14 is off by 2^-25)
+    rest = want[1:]
+    assert float((dv[1:, 0].cpu().double() - rest).norm() / rest.norm()) < 2 * HALF[H] + 2.0 ** -25 * math.sqrt(rest.numel()) / float(rest.norm())
