@@ -17,6 +17,7 @@
 // sequences of 1,001 to 2,777 tokens, 8 heads of 64, both sides: 211 us by queries, of which the bias's gradient takes about
 // half, and 197 by keys (0.55 PFLOP/s); 8,134 tokens, 24 heads of 128 on 6, window 512 with 4 sinks, fp16: 234, 228 and 46 for
 // the sinks.
+#include <algorithm>
 #include <type_traits>
 
 #include "jagged_common.h"
@@ -404,8 +405,34 @@ __global__ void __launch_bounds__(1024) jag_dbias_kernel(JagArgs a) {
 // First tokens that stay visible (SINK) have many more queries than other keys: those beyond the window are a kernel of their
 // own, a workgroup per 32 such keys and a share of these queries, which its waves take in turn.  Both leave sums in fp32, which
 // jag_sinks_kernel joins and rounds.
-__device__ __forceinline__ int64_t sink_slots(const JagArgs& a, int b, int block, int kh) {
-  return (((int64_t)b * a.sink_blocks + block) * a.hk + kh) * (a.sink_shares + 1);
+//
+// Only a sequence longer than the window has such queries, and only for its first nk - window keys.  The host does not know the
+// lengths: blocks are listed, and have rows for their sums, by sequence (sink_cell 0), or, where that is less, by cells of window + 1
+// keys of the batch.  A sequence of nk > window keys from k0 on has the nk / (window + 1) cells from number k0 / (window + 1) on
+// to itself, and its sums fit into min(sinks, window + 1) rows of each.  (16,384 sequences of 100 tokens, 8 key heads of 128, a
+// window of 1,024 with 4 sinks: 0.1 GB and not 8.6.)
+__device__ __forceinline__ int sinks_with_far_queries(const JagArgs& a, const JagSeq& s) {
+  return a.sink_blocks ? max(0, min(a.sinks, s.nk - a.window)) : 0;
+}
+
+// Block x of the list: keys [j0, j0 + n) of sequence b, n <= 32.  False for one without keys.
+__device__ __forceinline__ bool sink_block(const JagArgs& a, int64_t x, JagSeq& s, int& b, int& j0, int& n) {
+  int64_t block = x % a.sink_blocks;
+  x /= a.sink_blocks;
+  b = a.sink_cell ? find_sequence(a.seqs, (x + 1) * a.sink_cell - 1, [&](int i) { return (int64_t)a.cu_k[i]; }) : (int)x;
+  if (!jag_seq(a, b, s)) return false;
+  if (a.sink_cell) block += (x - s.k0 / a.sink_cell) * a.sink_blocks;
+  const int rows = sinks_with_far_queries(a, s);
+  if (block < 0 || block * 32 >= rows) return false;
+  j0 = (int)block * 32, n = min(32, rows - j0);
+  return true;
+}
+
+// The sums of such a block and key head: [shares + 1][dk, dv][D][n], the last for the queries under the window.
+template <int D>
+__device__ __forceinline__ float* sink_sums(const JagArgs& a, const JagSeq& s, int b, int j0, int n, int kh) {
+  const int64_t row = (a.sink_cell ? s.k0 / a.sink_cell : b) * a.sink_rows + j0;
+  return a.sink_part + (row * a.hk + kh * n) * (a.sink_shares + 1) * (2 * D);
 }
 
 template <int DT, int D, bool BIAS, bool SINK>
@@ -424,14 +451,13 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
   JagSeq s;
-  int b, j0, kh, share = 0;
+  int b, j0, kh, share = 0, keys_n = 0;  // SINK: its share of the queries, its keys
   if constexpr (SINK) {
     if (unit >= units) return;
     share = (int)(unit % a.sink_shares);
-    int64_t x = unit / a.sink_shares;
-    kh = (int)(x % a.hk), x /= a.hk;
-    j0 = (int)(x % a.sink_blocks) * KEYS, b = (int)(x / a.sink_blocks);
-    if (!jag_seq(a, b, s) || j0 >= s.nk) return;
+    const int64_t x = unit / a.sink_shares;
+    kh = (int)(x % a.hk);
+    if (!sink_block(a, x / a.hk, s, b, j0, keys_n)) return;
   } else {
     if (unit >= units) {
       const int64_t first = (unit - units) * 256;
@@ -637,10 +663,8 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
     }
   }
   const float back = DT == PDM_F16 ? pow2(-power) : 1.0f, back_v = DT == PDM_F16 ? 1.0f / kLarge : 1.0f;
-  // sums of a sink's block in fp32: [dk, dv][d][32 keys]
-  auto sums_of = [&](int block, int slot) { return a.sink_part + (sink_slots(a, b, block, kh) + slot) * (2 * D * 32); };
   if constexpr (SINK) {
-    float* to = sums_of(j0 / 32, share);
+    float* to = sink_sums<D>(a, s, b, j0, keys_n, kh) + (int64_t)share * (2 * D) * keys_n;
     float* mine = reinterpret_cast<float*>(wave < 2 ? sq[wave & 1] : sg[wave & 1]);  // QT rows of a tile: D x 32 floats and more
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
@@ -650,22 +674,24 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
 #pragma unroll
         for (int e = 0; e < 16; ++e) mine[(32 * d + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + c] = z ? dv[d][e] * back_v : dk[d][e] * back;
       __syncthreads();
-      for (int x = tid; x < D * 32; x += 256)
-        to[z * D * 32 + x] = (reinterpret_cast<const float*>(sq[0])[x] + reinterpret_cast<const float*>(sq[1])[x]) +
-                             (reinterpret_cast<const float*>(sg[0])[x] + reinterpret_cast<const float*>(sg[1])[x]);
+      for (int i = tid; i < D * keys_n; i += 256) {
+        const int d = i / keys_n, x = 32 * d + (i - d * keys_n);
+        to[z * D * keys_n + i] = (reinterpret_cast<const float*>(sq[0])[x] + reinterpret_cast<const float*>(sq[1])[x]) +
+                                 (reinterpret_cast<const float*>(sg[0])[x] + reinterpret_cast<const float*>(sg[1])[x]);
+      }
     }
     return;
   }
-  if (a.sink_blocks > jw / 32 && jw < s.nk) {
-    float* to = sums_of(jw / 32, a.sink_shares);
+  const int n = min(32, sinks_with_far_queries(a, s) - jw);
+  if (c < n) {  // jag_sinks_kernel writes over what these rows get below
+    float* to = sink_sums<D>(a, s, b, jw, n, kh) + (int64_t)a.sink_shares * (2 * D) * n;
 #pragma unroll
     for (int d = 0; d < DD; ++d)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int x = (32 * d + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + c;
-        to[x] = dk[d][e] * back, to[D * 32 + x] = dv[d][e] * back_v;
+        const int x = (32 * d + 8 * (e >> 2) + 4 * h + (e & 3)) * n + c;
+        to[x] = dk[d][e] * back, to[D * n + x] = dv[d][e] * back_v;
       }
-    return;
   }
   if (jw >= s.nk) return;
   const int64_t at = ((s.k0 + jw) * a.hk + kh) * D, st = (int64_t)a.hk * D;
@@ -673,23 +699,24 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
   store_own<DT, D>(dv, back_v, own, a.dv, nullptr, at, st, s.nk - jw);
 }
 
-// Gradients of 32 sinks of a key head, their sums under the window and beyond it: a thread an element.
+// Gradients of a block of sinks of a key head, their sums under the window and beyond it: a thread an element at a time, `parts`
+// workgroups.
 template <int DT, int D>
-__global__ void __launch_bounds__(256) jag_sinks_kernel(JagArgs a, int64_t units) {
-  constexpr int PARTS = 2 * D * 32 / 256;
-  const int64_t unit = linear_block() / PARTS;
+__global__ void __launch_bounds__(256) jag_sinks_kernel(JagArgs a, int64_t units, int parts) {
+  const int64_t unit = linear_block() / parts;
   if (unit >= units) return;
-  const int kh = (int)(unit % a.hk), i = (int)(linear_block() % PARTS) * 256 + threadIdx.x;
-  const int64_t x = unit / a.hk;
-  const int j0 = (int)(x % a.sink_blocks) * 32, b = (int)(x / a.sink_blocks);
-  const int z = i / (D * 32), key = j0 + i % 32, d = i / 32 % D;
+  const int kh = (int)(unit % a.hk);
   JagSeq s;
-  if (!jag_seq(a, b, s) || key >= s.nk) return;
-  const float* from = a.sink_part + sink_slots(a, b, j0 / 32, kh) * (2 * D * 32) + i;
-  float sum = 0.0f;
+  int b, j0, n;
+  if (!sink_block(a, unit / a.hk, s, b, j0, n)) return;
+  const float* from = sink_sums<D>(a, s, b, j0, n, kh);
+  for (int i = (int)(linear_block() % parts) * 256 + threadIdx.x; i < 2 * D * n; i += parts * 256) {
+    const int z = i / (D * n), d = i / n % D, key = j0 + i % n;
+    float sum = 0.0f;
 #pragma unroll 4
-  for (int n = 0; n <= a.sink_shares; ++n) sum += from[(int64_t)n * (2 * D * 32)];
-  static_cast<uint16_t*>(z ? a.dv : a.dk)[((s.k0 + key) * a.hk + kh) * D + d] = (uint16_t)pack2<DT>(z ? sum : sum * a.scale, 0.0f);
+    for (int x = 0; x <= a.sink_shares; ++x) sum += from[(int64_t)x * (2 * D) * n + i];
+    static_cast<uint16_t*>(z ? a.dv : a.dk)[((s.k0 + key) * a.hk + kh) * D + d] = (uint16_t)pack2<DT>(z ? sum : sum * a.scale, 0.0f);
+  }
 }
 
 // ---- host -------------------------------------------------------------------------------
@@ -701,18 +728,24 @@ int64_t part_cols(const JagArgs& a) {
   return reach < 0 ? 0 : reach < a.bias_last ? reach : a.bias_last;
 }
 
-// Blocks of 32 sinks of a sequence, and the shares that the queries beyond the window are dealt to: about 1,024 workgroups, each
-// of 8 tiles and more on average.
+// The list of blocks of 32 sinks (jag_dkv_kernel), and the shares that the queries beyond the window are dealt to: about 1,024
+// workgroups, each of 8 tiles and more on average.
+int64_t sink_lists(const JagArgs& a) { return a.sink_cell ? a.k_tokens / a.sink_cell : a.seqs; }
 void sinks_of(JagArgs& a) {
-  a.sink_blocks = a.seqs && a.q_tokens ? (a.sinks + 31) / 32 : 0;
-  if (!a.sink_blocks) return;
-  const int64_t units = (int64_t)a.seqs * a.sink_blocks * a.hk, most = a.group * (a.q_tokens / a.seqs) / (8 * 128);
+  a.sink_blocks = 0;
+  if (!a.seqs || !a.q_tokens || !a.sinks) return;
+  const int cell = a.window + 1, rows = a.sinks < cell ? a.sinks : cell;
+  const bool cells = a.k_tokens / cell * rows < (int64_t)a.seqs * a.sinks;
+  a.sink_cell = cells ? cell : 0, a.sink_rows = cells ? rows : a.sinks;
+  const int64_t lists = sink_lists(a), blocks = (a.sink_rows + 31) / 32, units = lists * blocks * a.hk;
+  const int64_t most = a.group * (a.q_tokens / (lists < a.seqs ? lists : a.seqs)) / (8 * 128);
   int64_t shares = 1024 / units;
   shares = shares < most ? shares : most;
   a.sink_shares = (int32_t)(shares > 1 ? shares : 1);
+  a.sink_blocks = (int32_t)blocks;
 }
 
-// The sums of sinks take 16 KiB (D 128: 32) a block of 32 in each sequence: as many as this do not run out of memory.
+// A limit of the interface: first tokens that stay visible are few.
 constexpr int kMostSinks = 1024;
 
 struct Space {
@@ -725,7 +758,7 @@ Space space_of(JagArgs& a, int dtype, int head_dim, bool gb) {
   s.range = s.expo + round256(dtype == PDM_F16 ? a.items * 16 * a.hq : 0);
   s.part = s.range + round256(gb ? a.items * 8 : 0);
   s.sinks = s.part + round256(gb ? a.items * a.hq * (part_cols(a) + 2) * 4 : 0);
-  s.total = s.sinks + (int64_t)a.seqs * a.sink_blocks * a.hk * (a.sink_shares + 1) * 2 * head_dim * 32 * 4;
+  s.total = s.sinks + (a.sink_blocks ? sink_lists(a) * a.sink_rows * a.hk * (a.sink_shares + 1) * 2 * head_dim * 4 : 0);
   return s;
 }
 
@@ -746,9 +779,12 @@ void launch(const JagArgs& a, hipStream_t st) {
     const int64_t items = a.seqs ? a.k_tokens / M + a.seqs : 0, units = items * a.hk, most = a.k_tokens > a.seqs ? a.k_tokens : a.seqs;
     jag_dkv_kernel<DT, D, BIAS, false><<<linear_grid(units + (most + 255) / 256), 256, 0, st>>>(a, units);
     if (a.sink_blocks) {
-      const int64_t blocks = (int64_t)a.seqs * a.sink_blocks * a.hk;
+      const int64_t blocks = sink_lists(a) * a.sink_blocks * a.hk;
+      // a workgroup for 256 elements while these are few (512 sequences of 300 tokens with 512 sinks, none of them beyond the window
+      // of 1,024, as 610,304 workgroups: the pass took 1,896 us instead of 1,065)
+      const int most = (2 * D * (a.sinks < 32 ? a.sinks : 32) + 255) / 256, parts = (int)std::max<int64_t>(1, std::min<int64_t>(most, 8192 / blocks));
       jag_dkv_kernel<DT, D, BIAS, true><<<linear_grid(blocks * a.sink_shares), 256, 0, st>>>(a, blocks * a.sink_shares);
-      jag_sinks_kernel<DT, D><<<linear_grid(blocks * (2 * D * 32 / 256)), 256, 0, st>>>(a, blocks);
+      jag_sinks_kernel<DT, D><<<linear_grid(blocks * parts), 256, 0, st>>>(a, blocks, parts);
     }
   }
 }

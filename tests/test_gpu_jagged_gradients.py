@@ -1,4 +1,4 @@
-"""Gradients of jagged_attention where the definition leaves no room: rows that see one key; rows behind the last query, columns that no pair has; small weights."""
+"""Gradients of jagged_attention where the definition leaves no room: rows that see one key; rows behind the last query, columns that no pair has; small weights; sinks of many sequences."""
 import math
 
 import pytest
@@ -140,3 +140,46 @@ def test_small_weights_in_half_precision(pdm, dev, D, gap, mask):
     # (a result below 2^-14 is off by 2^-25)
     rest = want[1:]
     assert float((dv[1:, 0].cpu().double() - rest).norm() / rest.norm()) < 2 * HALF[H] + 2.0 ** -25 * math.sqrt(rest.numel()) / float(rest.norm())
+
+
+# ---- sinks of many sequences ------------------------------------------------------------------------
+# Queries beyond the window are those of sequences longer than it, and so are the sums kept for them.
+
+@pytest.mark.parametrize("D,hk,group,dtype", KINDS)
+@pytest.mark.parametrize("window,sinks", [(30, 4), (7, 33), (1, 1), (5, 200), (40, 41), (100, 3), (33, 32)])
+def test_sinks_of_many_sequences(pdm, dev, D, hk, group, dtype, window, sinks):
+    """Mostly short ones, some of about the window's length, a few long; empty ones; with queries for all of the keys or for some."""
+    g = torch.Generator().manual_seed(window)
+    lens = torch.randint(0, 12, (200,), generator=g).tolist()
+    for at, n in ((3, window), (4, window + 1), (5, window), (50, window + 2), (51, window + 1), (52, 2 * window + 2), (120, 150), (121, 0), (122, 129), (199, window + 33)):
+        lens[at] = n
+    for new in (lens, [min(n, x) for n, x in zip(lens, torch.randint(0, 60, (200,), generator=g).tolist())]):
+        c = Case(new, lens, hk * group, hk, D, dtype, 20, seed=sinks)
+        mask = dict(causal=True, window=window, sinks=sinks)
+        w = c.want(True, **mask)
+        got, grads = c.grads(pdm, dev, **mask)
+        c.check(got, w)
+        c.check_grads(grads, w)
+
+
+def test_many_short_sequences_with_sinks(pdm, dev):
+    """40,000 sequences of 50 tokens, none of which has a query beyond the window, and one that has: the bits that the same
+    sequences have without sinks, within memory of the size of the batch's."""
+    n, length = 40_000, 50
+    g = torch.Generator(device=dev).manual_seed(5)
+    cu = torch.cat((torch.arange(n + 1) * length, torch.tensor([n * length + 400]))).int().to(dev)
+    T = n * length + 400
+    x = [torch.randn(T, 1, 64, generator=g, device=dev).to(B).requires_grad_(True) for _ in range(3)]
+    go = torch.randn(T, 1, 64, generator=g, device=dev).to(B)
+    torch.cuda.synchronize()
+    grads = []
+    for sinks in (0, 4):
+        out = pdm.jagged_attention(*x, cu, window=300, sinks=sinks)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        held = torch.cuda.memory_allocated()
+        grads.append(torch.autograd.grad(out, x, go))
+        torch.cuda.synchronize()
+        assert torch.cuda.max_memory_allocated() - held < 6 * T * 64 * 2
+    for a, b in zip(*grads):
+        assert torch.equal(a[:n * length], b[:n * length]) and not torch.equal(a[n * length:], b[n * length:])
