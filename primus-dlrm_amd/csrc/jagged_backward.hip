@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
 __global__ void __launch_bounds__(1024) jag_dbias_kernel(JagArgs a) {
   __shared__ double part[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cols = (int)a.part_stride - 2;
-  const int head = blockIdx.y, col = blockIdx.x * 64 + lane;
+  const int head = blockIdx.y, col = (int)(blockIdx.z * gridDim.x + blockIdx.x) * 64 + lane;
   double sum = 0.0;
   const int64_t d = (int64_t)col + a.bias_start;
   for (int64_t i0 = wave; i0 < a.items; i0 += 16 * 64) {  // 64 blocks' ranges at once, a lane's each
@@ -774,7 +774,10 @@ void launch(const JagArgs& a, hipStream_t st) {
       jag_dq_kernel<DT, D, false, false><<<grid, 256, 0, st>>>(a, units);
     }
   }
-  if (a.dbias) jag_dbias_kernel<<<dim3(a.bias_last / 64 + 1, a.hq), 1024, 0, st>>>(a);
+  if (a.dbias) {
+    const dim3 grid = linear_grid(a.bias_last / 64 + 1, 1 << 21);  // of columns; heads in between
+    jag_dbias_kernel<<<dim3(grid.x, a.hq, grid.y), 1024, 0, st>>>(a);
+  }
   if (a.k_tokens > 0) {
     const int64_t items = a.seqs ? a.k_tokens / M + a.seqs : 0, units = items * a.hk, most = a.k_tokens > a.seqs ? a.k_tokens : a.seqs;
     jag_dkv_kernel<DT, D, BIAS, false><<<linear_grid(units + (most + 255) / 256), 256, 0, st>>>(a, units);

@@ -1,4 +1,5 @@
-"""Gradients of jagged_attention where the definition leaves no room: rows that see one key; rows behind the last query, columns that no pair has; small weights; sinks of many sequences."""
+"""Gradients of jagged_attention where the definition leaves no room: rows that see one key; rows behind the last query, columns that no
+pair has; small weights; sinks of many sequences; very wide biases."""
 import math
 
 import pytest
@@ -183,3 +184,21 @@ def test_many_short_sequences_with_sinks(pdm, dev):
         assert torch.cuda.max_memory_allocated() - held < 6 * T * 64 * 2
     for a, b in zip(*grads):
         assert torch.equal(a[:n * length], b[:n * length]) and not torch.equal(a[n * length:], b[n * length:])
+
+
+# ---- a bias of more columns than a dimension of a launch has threads -------------------------------------
+
+def test_gradient_of_a_very_wide_bias(pdm, dev):
+    c = Case([40], [40], 1, 1, 64, B, 50, seed=6)
+    w = c.want(True)
+    x, span = c.inputs(dev), 2 ** 28 + 100
+    wide = torch.zeros(1, span, device=dev)
+    wide[:, :50] = x[3]
+    held = torch.full_like(wide, math.nan)  # whose memory the gradient gets
+    del held
+    x = [t.detach().requires_grad_(True) for t in (*x[:3], wide)]
+    out, _ = c.call(pdm, dev, x)
+    grads = list(torch.autograd.grad(out, x, c.go.to(dev)))
+    assert not grads[3][:, 50:].any()
+    grads[3] = grads[3][:, :50]
+    c.check_grads(grads, w)
