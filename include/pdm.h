@@ -741,7 +741,7 @@ typedef struct {
   int32_t bias_start; /* distance of the first column */
   int32_t bias_span;  /* columns; 0: no bias */
   float scale;
-  int32_t reserved;
+  int32_t stats_planes; /* of stats, see below: 2, or 1 (as 0) */
   int64_t q_tokens, k_tokens;     /* rows of q; of k and v */
   int64_t q_stride_t, q_stride_h; /* element (t, h, d) of q at q[t * q_stride_t + h * q_stride_h + d] */
   int64_t k_stride_t, k_stride_h;
@@ -752,7 +752,10 @@ typedef struct {
  * bias: fp32 [n_q_heads, bias_span].
  * lse: optional fp32 [q_tokens, n_q_heads], log of the sum of exponentials.
  * For the backward pass: stats, fp32 [q_tokens, n_q_heads, 2], and, where the
- * bias's gradient is wanted, out_rest (as out: what its rounding left).
+ * bias's gradient is wanted, out_rest (as out: what its rounding left).  With
+ * out_rest and stats_planes = 2 stats is [2, q_tokens, n_q_heads, 2]: the second
+ * plane keeps a row's weights in the bias's last column and before its first,
+ * and the gradients of the two outer columns are corrected by them.
  * A row that sees no key, and a row that no sequence covers, is zeros with lse
  * -inf; so is one whose scores are all -inf.  Keys and values that a query does
  * not see do not reach it, whatever they hold.  Spans that decrease or leave

@@ -287,7 +287,7 @@ class JaggedAttentionDesc(ctypes.Structure):
         ("bias_start", ctypes.c_int32),
         ("bias_span", ctypes.c_int32),
         ("scale", ctypes.c_float),
-        ("reserved", ctypes.c_int32),
+        ("stats_planes", ctypes.c_int32),
         ("q_tokens", ctypes.c_int64),
         ("k_tokens", ctypes.c_int64),
         ("q_stride_t", ctypes.c_int64),

@@ -45,6 +45,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) jag_fwd_kernel(JagArgs a
       for (int h = threadIdx.x; h < a.hq; h += 256) {
         if (a.lse) a.lse[t * a.hq + h] = -kInf;
         if (a.stats) a.stats[2 * (t * a.hq + h)] = kNoKeys, a.stats[2 * (t * a.hq + h) + 1] = 0.0f;
+        if (FINE && a.outer) a.outer[2 * (t * a.hq + h)] = a.outer[2 * (t * a.hq + h) + 1] = 0.0f;
       }
     });
     return;
@@ -93,7 +94,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) jag_fwd_kernel(JagArgs a
   };
 
   constexpr f32x16_t zero16 = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  float m = -kInf, l = 0.0f;
+  float m = -kInf, l = 0.0f, l_far = 0.0f, l_near = 0.0f;  // FINE: sums of the weights in and behind the bias's last column, before its first
   f32x16_t o[DD];
 #pragma unroll
   for (int d = 0; d < DD; ++d) o[d] = zero16;
@@ -172,10 +173,12 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) jag_fwd_kernel(JagArgs a
       const float g = now == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - now);
       m = now;
       l *= g;
+      if (FINE) l_far *= g, l_near *= g;
 #pragma unroll
       for (int d = 0; d < DD; ++d) o[d] *= g;
     }
     const float base = m == -kInf ? 0.0f : m;
+    float of_tile = 0.0f;
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
       float w[8];
@@ -184,12 +187,35 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) jag_fwd_kernel(JagArgs a
         const float x = sc[y >> 1][8 * (y & 1) + e];
         w[e] = __builtin_amdgcn_exp2f(BIAS ? x - base : __builtin_fmaf(x, f, -base));
       }
-      l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+      const float of_keys = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+      l += of_keys;
+      if (FINE) of_tile += of_keys;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         p[y][e] = pack2<DT>(w[2 * e], w[2 * e + 1]);
         if (FINE) rest[y][e] = left2<DT>(w[2 * e], w[2 * e + 1], p[y][e]);
       }
+    }
+    if constexpr (FINE) {
+      // columns of the wave's pairs, but for those of keys ahead or behind the window
+      const int from = p_first - key - (KT - 1), to = p_last - key;
+      const int first = (a.causal && from < 0 ? 0 : from) - a.bias_start;
+      const int last = (a.window > 0 && key >= a.sinks && to >= a.window ? a.window - 1 : to) - a.bias_start;
+      float far = first >= a.bias_last ? of_tile : 0.0f, near = last < 0 ? of_tile : 0.0f;
+      if ((first < 0 && last >= 0) || (first < a.bias_last && last >= a.bias_last)) {
+        const int col0 = pos - a.bias_start - key - 4 * h;
+        far = near = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const int col = col0 - (32 * (e >> 4) + 8 * ((e >> 2) & 3) + (e & 3));
+          uint32_t w = p[e >> 3][e >> 1 & 3], r = rest[e >> 3][e >> 1 & 3];
+          asm volatile("" : "+v"(w), "+v"(r));  // else what they were made of is kept for this
+          const float x = e & 1 ? hi_of<DT>(w) + hi_of<DT>(r) : lo_of<DT>(w) + lo_of<DT>(r);
+          far += col >= a.bias_last ? x : 0.0f;
+          near += col < 0 ? x : 0.0f;
+        }
+      }
+      l_far += far, l_near += near;
     }
   };
   auto values = [&](int t) __attribute__((always_inline)) {
@@ -234,6 +260,11 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) jag_fwd_kernel(JagArgs a
       a.lse[at] = sum != 0.0f ? ((m + (float)__builtin_amdgcn_frexp_expf(sum)) + __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(sum))) * kLn2 : -kInf;
     if (a.stats) a.stats[2 * at] = sum != 0.0f ? m : kNoKeys, a.stats[2 * at + 1] = inv;
   }
+  if constexpr (FINE) {
+    const float far = l_far + __shfl_xor(l_far, 32), near = l_near + __shfl_xor(l_near, 32);
+    float* outer = late_args()->outer;
+    if (outer && h == 0 && row < s.nq) outer[2 * at] = far * inv, outer[2 * at + 1] = near * inv;
+  }
 }
 
 template <int DT, int D>
@@ -264,6 +295,7 @@ int jag_args(const char* fn, const pdm_jagged_attention_desc* d, JagArgs& a) {
   if (d->q_tokens < 0 || d->k_tokens < 0 || d->q_tokens >= (1 << 30) || d->k_tokens >= (1 << 30)) return bad("tokens must lie in [0, 2^30)");
   if (d->q_tokens * d->n_q_heads >= (int64_t(1) << 31) || d->k_tokens * d->n_kv_heads >= (int64_t(1) << 31)) return bad("tokens * heads must be below 2^31");
   if (d->window < 0 || d->sinks < 0) return bad("window and sinks must not be negative");
+  if (d->stats_planes < 0 || d->stats_planes > 2) return bad("stats_planes must lie in [0, 2]");
   const float scale2 = d->scale * kLog2e;
   if (!(scale2 - scale2 == 0.0f)) return bad("scale must be finite, and so must scale / ln 2");
   auto far = [](int64_t st) { return st < 0 || st >= (1 << 24); };
@@ -322,7 +354,9 @@ extern "C" int pdm_jagged_attention_fwd(const pdm_jagged_attention_desc* desc, c
   PDM_CHECK_ARG(out, "null out");
   PDM_CHECK_ARG(!out_rest || bias, "out_rest without a bias");
   PDM_CHECK_ARG(((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_rest)) & 15) == 0, "out and out_rest must be 16-byte aligned");
+  PDM_CHECK_ARG(!out_rest || stats, "out_rest without stats");
   a.out = out, a.rest = out_rest, a.lse = lse, a.stats = stats, a.err = err_flag;
+  if (out_rest && desc->stats_planes == 2) a.outer = stats + 2 * a.q_tokens * a.hq;
   const bool bf16 = desc->dtype == PDM_BF16;
   if (desc->head_dim == 64) bf16 ? launch<PDM_BF16, 64>(a, stream) : launch<PDM_F16, 64>(a, stream);
   else bf16 ? launch<PDM_BF16, 128>(a, stream) : launch<PDM_F16, 128>(a, stream);

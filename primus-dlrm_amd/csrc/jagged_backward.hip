@@ -35,6 +35,13 @@ constexpr int kOut = -5;     // |dO| and |dlse| below 2^kOut after their power o
 constexpr int kNone = -100;  // exponent of rows of zeros
 constexpr float kLarge = 0x1p15f;  // fp16: weights, 1 at most, go into dV's product times this
 
+__device__ __forceinline__ float sum16(const float* x) {  // four chains
+  float s[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[i] = (x[i] + x[i + 4]) + (x[i + 8] + x[i + 12]);
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
 __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
 
 // ---- by queries -----------------------------------------------------------------------
@@ -52,11 +59,13 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   __shared__ float win[2][GB ? 4 : 1][XX][GB ? 64 : 1];
   __shared__ alignas(1024) float lines[GB || D == 128 ? 4 : 1][GB || D == 128 ? 32 : 1][64];
   __shared__ float ends[GB ? 8 : 1];
-  // Where registers are short two fragments of the queries stay in LDS: the compiler had put one into scratch memory, whose load in
-  // every tile waited for the next tile's to land (fp16, 24 heads of 8,134 tokens under a window of 512: 258 us instead of 234).
-  constexpr int HOLD = GB && D == 128 ? 2 : 0;
+  // Where registers are short three fragments of the queries stay in LDS: the compiler puts what does not fit into scratch memory,
+  // whose load in every tile waits for the next tile's to land (fp16, 24 heads of 8,134 tokens under a window of 512: 256 us with
+  // two, 240 with three; a fourth would leave LDS for one workgroup on a CU).
+  constexpr int HOLD = GB && D == 128 ? 3 : 0;
   __shared__ u32x4_t held[HOLD ? 4 * HOLD : 1][HOLD ? 64 : 1];
-  __shared__ int odd_keys[2][KT], odd_any[2][4];
+  __shared__ uint8_t odd_keys[2][KT];
+  __shared__ int odd_any[2][4];
 
   const int64_t unit = linear_block();
   if (unit >= units) {
@@ -176,7 +185,7 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   // the bias's gradient: columns 0 .. cols - 1 of the partial result, then what lies behind them and before them
   const int cols = (int)a.part_stride - 2;
   float* part = GB ? a.part + (item * a.hq + head) * a.part_stride : nullptr;
-  float far = 0.0f, near = 0.0f, sum = 0.0f;
+  float far = 0.0f, near = 0.0f, all = 0.0f, sum = 0.0f;  // all: of this row's dS
   int mine = 0;  // the distance that this thread sums
   auto put = [&](int d, float v) {
     const int x = d - a.bias_start;
@@ -290,6 +299,7 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
 #pragma unroll
         for (int e = 0; e < 16; ++e) ds[e] = sees(key + 32 * x + 4 * h + 8 * (e >> 2) + (e & 3)) ? ds[e] : 0.0f;
       }
+      if (GB) all += sum16(ds);
       bool near_lines = false;
       if (GB) {
         const int first = p_first - key - 32 * x - 31 - a.bias_start, last = first + 62;  // columns of the wave's pairs
@@ -299,11 +309,9 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
         // are the bias's alone, and infinity times 0 for a large one.
         if (there) {
           if (first >= a.bias_last) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) far += ds[e];
+            far += sum16(ds);
           } else if (last < 0) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) near += ds[e];
+            near += sum16(ds);
           } else {
             float* line = &lines[wave][4 * h][c + 31 - 4 * h];
             if (first >= 0 && last < a.bias_last) {
@@ -344,6 +352,18 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
       gather(keys.tiles - 1);
       put(mine, sum);
     }
+    // A row's dS add up to the gradient of its lse.  What they are off by is delta's error, which each has by its weight: little beside
+    // its own size, but a column of nearly all weights of every row has a sum that cancels to far less than its terms.  So the two
+    // columns that stand for many distances are put right (a bias of two columns, 980 tokens: off by 1.2e-5 to 8.6e-5 of the
+    // gradient, now by 1.5e-6 to 1.2e-5).
+    // A bias of one column has all of a row, whose sum is known.
+    const float sum_of_row = all + __shfl_xor(all, 32);
+    const LateArgs late = late_args();
+    if (late->outer && there && fabsf(sum_of_row) < kInf) {
+      const float right = late->dlse ? late->dlse[at] : 0.0f, p_far = late->outer[2 * at], p_near = late->outer[2 * at + 1];
+      if (a.bias_last == 0) far = h == 0 && p_far + p_near > 0.5f ? right : 0.0f, near = 0.0f;
+      else if (h == 0) far -= (sum_of_row - right) * p_far, near -= (sum_of_row - right) * p_near;
+    }
     far = group_sum(far, 64), near = group_sum(near, 64);
     if (lane == 0) ends[wave] = far, ends[4 + wave] = near;
     __syncthreads();
@@ -363,7 +383,7 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
     }
   }
   if (w0 < s.nq)
-    store_own<DT, D>(dq, back, D == 64 ? own : own2, a.dq, nullptr, o_at + w0 * o_st, o_st, s.nq - w0);
+    store_own<DT, D>(dq, back, D == 64 ? own : own2, late_args()->dq, nullptr, o_at + w0 * o_st, o_st, s.nq - w0);
 }
 
 // Sums the partial gradients of a column over the blocks of queries, in 64 bits: a lane per column, the blocks dealt to 16 waves.
@@ -829,6 +849,7 @@ extern "C" int pdm_jagged_attention_bwd(const pdm_jagged_attention_desc* desc, c
   PDM_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "workspace must be 256-byte aligned");
   char* ws = static_cast<char*>(workspace);
   a.out = const_cast<void*>(out), a.rest = const_cast<void*>(out_rest), a.stats = const_cast<float*>(stats);
+  if (grad_bias && desc->stats_planes == 2) a.outer = a.stats + 2 * a.q_tokens * a.hq;
   a.dout = grad_out, a.dlse = grad_lse, a.dq = grad_q, a.dk = grad_k, a.dv = grad_v, a.dbias = grad_bias;
   a.delta = reinterpret_cast<float*>(ws), a.expo = reinterpret_cast<int32_t*>(ws + sp.expo);
   a.part_range = reinterpret_cast<int32_t*>(ws + sp.range), a.part = reinterpret_cast<float*>(ws + sp.part);

@@ -17,6 +17,7 @@ struct JagArgs {
   int32_t* err;
   void *out, *rest;                  // forward; rest: what rounding out left (may be null)
   float *lse, *stats;                // stats: a row's reference (log2) and 1 / the sum of its weights
+  float* outer;                      // a row's weights of the bias's last column and of what lies before its first, or null
   const void* dout;                  // backward
   const float* dlse;
   void *dq, *dk, *dv;
@@ -37,6 +38,15 @@ struct JagArgs {
 constexpr float kInf = __builtin_inff();
 constexpr float kNoKeys = 3e38f;  // the reference of a row without weights: none passes it
 constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.44269504088896341f;
+
+// A kernel's arguments, read again: those that its end alone needs else take scalar registers all the way, and others are held in
+// lanes for them.  (JagArgs is every kernel's first argument.)
+typedef const __attribute__((address_space(4))) JagArgs* LateArgs;
+__device__ __forceinline__ LateArgs late_args() {
+  LateArgs p = (LateArgs)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
 
 // ---- sequences -------------------------------------------------------------------
 struct JagSeq {
@@ -108,7 +118,7 @@ __device__ __forceinline__ bool jag_ranked_block(const JagArgs& a, bool keys, in
 // the whole block of 256 threads; sequences [first, first + 256) that do not fit set the flag.
 template <typename F>
 __device__ __forceinline__ void jag_guard(const JagArgs& a, const int32_t* cu, int64_t tokens, int64_t first, F clear) {
-  __shared__ int bad[256];
+  __shared__ uint8_t bad[256];
   const int64_t t = first + threadIdx.x;
   JagSeq s;
   if (t < a.seqs && !jag_seq(a, (int)t, s) && a.err) *a.err = 1;
@@ -288,7 +298,7 @@ __device__ __forceinline__ void own_lds_order() { __builtin_amdgcn_fence(__ATOMI
 
 // True where rows that this wave brought held infinities or NaN; `rows`, where given, gets 1 for these (of ROWS) and 0 for its others.
 template <int DT, int D, int ROWS>
-__device__ __forceinline__ bool clean_rows(char* t, int lane, int wave, int* rows = nullptr) {
+__device__ __forceinline__ bool clean_rows(char* t, int lane, int wave, uint8_t* rows = nullptr) {
   constexpr int N = Bring<D, ROWS>::N, R = 64 / (D / 8);
   u32x4_t* p = reinterpret_cast<u32x4_t*>(t + wave * N * 1024 + lane * 16);
   uint32_t odd = 0;

@@ -1288,7 +1288,7 @@ def _check_bias(bias: Optional[torch.Tensor], heads: int, bias_start: int) -> in
     return bias.shape[1]
 
 
-def _jagged_desc(q, k, v, cu_seqlens, cu_seqlens_k, bias, scale, causal, window, sinks, bias_start) -> "L.JaggedAttentionDesc":
+def _jagged_desc(q, k, v, cu_seqlens, cu_seqlens_k, bias, scale, causal, window, sinks, bias_start, planes) -> "L.JaggedAttentionDesc":
     T, hq, D, q_st, q_sh, code = _check_heads("q", q)
     kT, hk, kD, k_st, k_sh, k_code = _check_heads("k", k)
     _, _, _, v_st, v_sh, v_code = _check_heads("v", v)
@@ -1312,7 +1312,7 @@ def _jagged_desc(q, k, v, cu_seqlens, cu_seqlens_k, bias, scale, causal, window,
             raise ValueError(f"{n} must lie in [0, 2^31), got {x}")
     span = _check_bias(bias, hq, bias_start)
     # (a dimension of one entry may have any stride)
-    return L.JaggedAttentionDesc(code, hq, hk, D, seqs, int(causal), window, sinks, bias_start, span, scale, 0, T, kT,
+    return L.JaggedAttentionDesc(code, hq, hk, D, seqs, int(causal), window, sinks, bias_start, span, scale, planes, T, kT,
                                  q_st if T > 1 else 0, q_sh if hq > 1 else 0, k_st if kT > 1 else 0, k_sh if hk > 1 else 0,
                                  v_st if kT > 1 else 0, v_sh if hk > 1 else 0)
 
@@ -1322,18 +1322,20 @@ def jagged_attention_raw(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_s
                          window: int = 0, sinks: int = 0, bias_start: int = 0, return_lse: bool = False, keep: int = 0,
                          err_flag: Optional[torch.Tensor] = None):
     """Launches pdm_jagged_attention_fwd on q [T, Hq, D], k and v [S, Hk, D]: (out, lse, stats, rest), None where not wanted.
-    ``keep``: what a backward pass needs, 1 the rows' statistics, 2 what the rounding of out left too (for the bias's gradient)."""
+    ``keep``: what a backward pass needs, 1 the rows' statistics, 2 what the rounding of out left too (for the bias's gradient), and
+    the weights of its outer columns (a second plane of the statistics)."""
     _check_err_flag(err_flag)
     index = _gpu_index(q, k, v, cu_seqlens, cu_seqlens_k, bias, err_flag)
     q, k, v = _even_heads(q), _even_heads(k), _even_heads(v)
-    desc = _jagged_desc(q, k, v, cu_seqlens, cu_seqlens_k, bias, scale, causal, window, sinks, bias_start)
+    planes = 2 if keep > 1 and bias is not None else 1
+    desc = _jagged_desc(q, k, v, cu_seqlens, cu_seqlens_k, bias, scale, causal, window, sinks, bias_start, planes)
     if keep and sinks > 1024 and k.shape[0] > 1024 and 0 < window < k.shape[0]:
         raise ValueError(f"at most 1024 sinks where gradients are wanted, got {sinks}")
     T, hq = q.shape[:2]
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((T, hq), dtype=torch.float32, device=q.device) if return_lse else None
-    stats = torch.empty((T, hq, 2), dtype=torch.float32, device=q.device) if keep else None
-    rest = torch.empty_like(out) if keep > 1 and bias is not None else None
+    stats = torch.empty((planes, T, hq, 2), dtype=torch.float32, device=q.device) if keep else None
+    rest = torch.empty_like(out) if planes > 1 else None
     lib = L.lib()
     ws_bytes = int(lib.pdm_jagged_attention_workspace_size(ctypes.byref(desc)))
     if ws_bytes < 0:
@@ -1361,7 +1363,8 @@ def jagged_attention_backward_raw(q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     if grad_lse is not None and (grad_lse.shape != q.shape[:2] or grad_lse.dtype != torch.float32):
         raise ValueError(f"grad_lse must be float32 {tuple(q.shape[:2])}, got {grad_lse.dtype} {tuple(grad_lse.shape)}")
     q, k, v, grad_out, grad_lse = _even_heads(q), _even_heads(k), _even_heads(v), _even(grad_out), _even(grad_lse)
-    desc = _jagged_desc(q, k, v, cu_seqlens, cu_seqlens_k, bias, scale, causal, window, sinks, bias_start)
+    desc = _jagged_desc(q, k, v, cu_seqlens, cu_seqlens_k, bias, scale, causal, window, sinks, bias_start,
+                        2 if stats.dim() == 4 and len(stats) == 2 else 1)
     gq, gk, gv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     gb = torch.empty_like(bias) if rest is not None else None
     lib = L.lib()
@@ -1392,7 +1395,7 @@ def jagged_attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_se
 def _(q, k, v, cu_seqlens, cu_seqlens_k, bias, scale, causal, window, sinks, bias_start, keep):
     T, hq, _ = q.shape
     return (q.new_empty(q.shape), q.new_empty((T, hq), dtype=torch.float32),
-            q.new_empty((T, hq, 2) if keep else (0,), dtype=torch.float32),
+            q.new_empty((2 if keep > 1 and bias is not None else 1, T, hq, 2) if keep else (0,), dtype=torch.float32),
             q.new_empty(q.shape if keep > 1 and bias is not None else (0,)))
 
 

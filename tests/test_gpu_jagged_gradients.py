@@ -1,5 +1,5 @@
 """Gradients of jagged_attention where the definition leaves no room: rows that see one key; rows behind the last query, columns that no
-pair has; small weights; sinks of many sequences; very wide biases."""
+pair has; small weights; sinks of many sequences; very wide biases; columns of nearly all weights."""
 import math
 
 import pytest
@@ -202,3 +202,78 @@ def test_gradient_of_a_very_wide_bias(pdm, dev):
     assert not grads[3][:, 50:].any()
     grads[3] = grads[3][:, :50]
     c.check_grads(grads, w)
+
+
+# ---- columns of nearly all weights -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("D,dtype", [(64, B), (128, B), (64, H), (128, H)])
+@pytest.mark.parametrize("span,start,mask", [(2, 0, dict(causal=True)), (3, 5000, dict(causal=False)), (70, -900, dict(causal=True, window=1000, sinks=4))])
+@pytest.mark.parametrize("gl", [False, True])
+def test_columns_of_nearly_all_weights(pdm, dev, D, dtype, span, start, mask, gl):
+    """The dS of a row add up to the gradient of its lse, and so does what such a column has of it, but for the few others: terms far
+    larger than their sum.  What is left of delta's error (2^-19 of |dO| |out|, in every row) would be ten times what fp32 sums
+    are off by.  These: an addition by 2^-25 of what has been summed, half of a row's sizes at most; a row's are summed in
+    blocks of 32 keys.  As a root mean square over the heads, twice that (another part is the products', of the same size)."""
+    n, length, heads = 200, 1200, 16
+    c = Case([n], [length], heads, heads, D, dtype, span, start, seed=D, spread=3.0)
+    c.bias[:, 0] = -8.0 if span == 2 else 0.0
+    if not gl:
+        c.gl = torch.zeros_like(c.gl)
+    _, (_, _, _, db) = c.grads(pdm, dev, gl=True, **mask)
+    i, j = torch.arange(length - n, length)[:, None], torch.arange(length)[None]
+    seen = (j <= i) if mask["causal"] else torch.ones(n, length, dtype=torch.bool)
+    if "window" in mask:
+        seen = seen & ((j > i - mask["window"]) | (j < mask["sinks"]))
+    col = (i - j - start).clamp(0, span - 1)
+    errors, sizes = [], []
+    for h in range(heads):
+        q, k, v, go = (t[:, h].double() for t in (c.q, c.k, c.v, c.go))
+        s = q @ k.T * D ** -0.5 + c.bias[h].double()[col]
+        p = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
+        ds = p * (go @ v.T - (go * (p @ v)).sum(-1, keepdim=True) + c.gl[:, h, None].double())
+        mass = torch.zeros(span, dtype=torch.float64).index_add_(0, col.flatten(), p.flatten())
+        most = int(mass.argmax())
+        assert mass[most] > 0.99 * n and most in (0, span - 1)
+        errors.append(float(db[h, most]) - float(ds[col == most].sum()))
+        sizes.append(float(ds.abs().sum(-1).square().sum()) * length / 32)
+    rms = lambda x: math.sqrt(sum(x) / heads)  # noqa: E731
+    assert rms([e * e for e in errors]) <= 2 * 2.0 ** -25 * rms(sizes)
+
+
+@pytest.mark.parametrize("D,hk,group,dtype", KINDS)
+def test_a_bias_of_one_column(pdm, dev, D, hk, group, dtype):
+    """It moves all scores of a row alike: its gradient is that of the lse, of the rows that see a key."""
+    for new, lens, mask, start in (([300, 5], [300, 90], dict(causal=True), 0), ([70, 40], [30, 40], dict(causal=True, window=20, sinks=3), 7),
+                                   ([90], [200], dict(causal=False), -50)):
+        c = Case(new, lens, hk * group, hk, D, dtype, 1, start, seed=D)
+        _, (*_, db) = c.grads(pdm, dev, **mask)
+        assert not db.any()
+        got, (*_, db) = c.grads(pdm, dev, gl=True, **mask)
+        gl = torch.where(torch.isinf(got[1].detach().cpu()), 0.0, c.gl).double()
+        # sums of 128 rows in fp32, of those in 64 bits
+        assert ((db.cpu().double()[:, 0] - gl.sum(0)).abs() <= 10 * 2.0 ** -24 * gl.abs().sum(0)).all()
+
+
+def test_one_plane_of_statistics(pdm, dev):
+    """Callers of the C entries that keep one plane: the same outputs and gradients, but for the outer columns' correction."""
+    import ctypes
+
+    L, ops = pdm._lib, pdm.ops
+    c = Case([90, 20], [90, 120], 4, 2, 64, B, 12, seed=9)
+    q, k, v, bias = c.inputs(dev)
+    cu = [torch.tensor(x, dtype=torch.int32, device=dev) for x in (c.cu_q, c.cu_k)]
+    args = (0.125, True, 0, 0, 0)
+    out, _, stats, rest = ops.jagged_attention_raw(q, k, v, *cu, bias, *args, keep=2)
+    assert stats.shape == (2, 110, 4, 2)
+    out1, rest1, stats1 = torch.empty_like(out), torch.empty_like(out), torch.full((2, 110, 4, 2), 7.0, device=dev)
+    desc = ops._jagged_desc(q, k, v, *cu, bias, *args, 1)
+    L.check(L.lib().pdm_jagged_attention_fwd(ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), cu[0].data_ptr(), cu[1].data_ptr(),
+                                             bias.data_ptr(), out1.data_ptr(), rest1.data_ptr(), None, stats1.data_ptr(), None, 0, None,
+                                             L.raw_stream(0)), "pdm_jagged_attention_fwd")
+    assert torch.equal(out, out1) and torch.equal(rest, rest1) and torch.equal(stats[0], stats1[0]) and (stats1[1] == 7).all()
+    both = ops.jagged_attention_backward_raw(q, k, v, *cu, bias, out, stats, rest, c.go.to(dev), None, *args)
+    one = ops.jagged_attention_backward_raw(q, k, v, *cu, bias, out, stats[0], rest, c.go.to(dev), None, *args)
+    assert all(torch.equal(a, b) for a, b in zip(both[:3], one[:3])) and torch.equal(both[3][:, 1:-1], one[3][:, 1:-1])
+    w = c.want(True)
+    c.check_grads(both, w)
+    c.check_grads(one, w)

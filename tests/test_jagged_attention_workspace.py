@@ -1,4 +1,4 @@
-"""Memory that a backward pass of jagged_attention asks for, from the C entry alone."""
+"""Memory that a backward pass of jagged_attention asks for, from the C entry alone; the planes of its statistics."""
 import ctypes
 
 import pytest
@@ -32,3 +32,15 @@ def test_sinks_of_few_sequences(pdm):
 def test_no_more_than_for_every_token(pdm):
     for seqs, tokens, window, sinks in ((1_000, 100_000, 1, 1_024), (10, 100_000, 7, 1_024), (5_000, 5_000, 3, 9)):
         assert _size(pdm, seqs, tokens, window, sinks) <= _size(pdm, seqs, tokens, window, 0) + tokens * 2 * 2 * 4 * 8 * 128
+
+
+def test_planes_of_the_statistics(pdm):
+    L = pdm._lib
+    for planes in (-1, 0, 1, 2, 3):
+        d = L.JaggedAttentionDesc(L.PDM_BF16, 2, 1, 64, 1, 1, 0, 0, 0, 4, 0.125, planes, 8, 8, 128, 64, 64, 64, 64, 64)
+        size = L.lib().pdm_jagged_attention_bwd_workspace_size(ctypes.byref(d), 1)
+        assert size > 0 if 0 <= planes <= 2 else size == L.PDM_ERR_INVALID and "stats_planes" in L.last_error()
+    p = 1 << 20  # never read
+    d = L.JaggedAttentionDesc(L.PDM_BF16, 2, 1, 64, 1, 1, 0, 0, 0, 4, 0.125, 2, 8, 8, 128, 64, 64, 64, 64, 64)
+    assert L.lib().pdm_jagged_attention_fwd(ctypes.byref(d), p, p, p, p, p, p, p, p, None, None, None, 0, None, None) == L.PDM_ERR_INVALID
+    assert "out_rest without stats" in L.last_error()
