@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) jag_fwd_kernel(JagArgs a
     return (a.causal && key + KT - 1 > b_first) || (a.window > 0 && key <= b_last - a.window && key + KT > a.sinks);
   };
   auto sees = [&](int j) { return (uint32_t)(j - row_lo) < (uint32_t)row_n || j < row_first; };
-  bool odd = false;
+  bool odd = false, large = false;  // large: scores are multiplied by the scale and rounded, as the reference is
 
   const int tiles = keys.tiles;
   // the queries come beside the first tile, by way of the second's place
@@ -176,6 +176,12 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) jag_fwd_kernel(JagArgs a
       if (FINE) l_far *= g, l_near *= g;
 #pragma unroll
       for (int d = 0; d < DD; ++d) o[d] *= g;
+      if (!BIAS && __any(fabsf(m) > kLargeScore)) large = true;
+    }
+    if (!BIAS && large) {  // what rounding left of the largest score would count as 2^32 and more from 2^30 on
+#pragma unroll
+      for (int e = 0; e < 32; ++e) sc[e >> 4][e & 15] *= f;
+      f = 1.0f;
     }
     const float base = m == -kInf ? 0.0f : m;
     float of_tile = 0.0f;
@@ -262,7 +268,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) jag_fwd_kernel(JagArgs a
   }
   if constexpr (FINE) {
     const float far = l_far + __shfl_xor(l_far, 32), near = l_near + __shfl_xor(l_near, 32);
-    float* outer = late_args()->outer;
+    float* outer = late_args().outer;
     if (outer && h == 0 && row < s.nq) outer[2 * at] = far * inv, outer[2 * at + 1] = near * inv;
   }
 }

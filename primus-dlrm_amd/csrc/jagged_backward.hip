@@ -35,6 +35,13 @@ constexpr int kOut = -5;     // |dO| and |dlse| below 2^kOut after their power o
 constexpr int kNone = -100;  // exponent of rows of zeros
 constexpr float kLarge = 0x1p15f;  // fp16: weights, 1 at most, go into dV's product times this
 
+// Rounded before the row's reference is taken off, which is a rounded score: the difference of the largest is 0, and not what rounding
+// left of it, which from 2^30 on would count as 2^32 and more.
+__device__ __forceinline__ float scaled(float score, float scale2) {
+#pragma clang fp contract(off)
+  return score * scale2;
+}
+
 __device__ __forceinline__ float sum16(const float* x) {  // four chains
   float s[4];
 #pragma unroll
@@ -276,8 +283,8 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int j = 8 * (e >> 2) + (e & 3);
-        const float w = BIAS ? __builtin_fmaf(sc[e], a.scale2, sb[t & 1][wave * 32 + local - j]) : sc[e] * a.scale2;
-        const float p = __builtin_amdgcn_exp2f(w - m) * inv;
+        const float w = BIAS ? __builtin_fmaf(sc[e], a.scale2, sb[t & 1][wave * 32 + local - j]) - m : scaled(sc[e], a.scale2) - m;
+        const float p = __builtin_amdgcn_exp2f(w) * inv;
         ds[e] = p * (dp[e] - delta);
       }
       if (part_seen && (odd_any[t & 1][0] | odd_any[t & 1][1] | odd_any[t & 1][2] | odd_any[t & 1][3])) {
@@ -358,9 +365,9 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
     // gradient, now by 1.5e-6 to 1.2e-5).
     // A bias of one column has all of a row, whose sum is known.
     const float sum_of_row = all + __shfl_xor(all, 32);
-    const LateArgs late = late_args();
-    if (late->outer && there && fabsf(sum_of_row) < kInf) {
-      const float right = late->dlse ? late->dlse[at] : 0.0f, p_far = late->outer[2 * at], p_near = late->outer[2 * at + 1];
+    const JagArgs& late = late_args();
+    if (late.outer && there && fabsf(sum_of_row) < kInf) {
+      const float right = late.dlse ? late.dlse[at] : 0.0f, p_far = late.outer[2 * at], p_near = late.outer[2 * at + 1];
       if (a.bias_last == 0) far = h == 0 && p_far + p_near > 0.5f ? right : 0.0f, near = 0.0f;
       else if (h == 0) far -= (sum_of_row - right) * p_far, near -= (sum_of_row - right) * p_near;
     }
@@ -383,7 +390,7 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
     }
   }
   if (w0 < s.nq)
-    store_own<DT, D>(dq, back, D == 64 ? own : own2, late_args()->dq, nullptr, o_at + w0 * o_st, o_st, s.nq - w0);
+    store_own<DT, D>(dq, back, D == 64 ? own : own2, late_args().dq, nullptr, o_at + w0 * o_st, o_st, s.nq - w0);
 }
 
 // Sums the partial gradients of a column over the blocks of queries, in 64 bits: a lane per column, the blocks dealt to 16 waves.
@@ -642,8 +649,8 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
 #pragma unroll
         for (int z = 0; z < 4; ++z) {
           const int e = 4 * y + z;
-          const float w = BIAS ? __builtin_fmaf(sc[e], a.scale2, sb[n & 1][r + z - (jw - j0) - c + KEYS - 1]) : sc[e] * a.scale2;
-          p[e] = __builtin_amdgcn_exp2f(w - m[z]) * inv[z];
+          const float w = BIAS ? __builtin_fmaf(sc[e], a.scale2, sb[n & 1][r + z - (jw - j0) - c + KEYS - 1]) - m[z] : scaled(sc[e], a.scale2) - m[z];
+          p[e] = __builtin_amdgcn_exp2f(w) * inv[z];
           ds[e] = p[e] * (dp[e] - delta[z]);
         }
       }
@@ -682,9 +689,10 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
       __syncthreads();
     }
   }
+  const JagArgs& late = late_args();
   const float back = DT == PDM_F16 ? pow2(-power) : 1.0f, back_v = DT == PDM_F16 ? 1.0f / kLarge : 1.0f;
   if constexpr (SINK) {
-    float* to = sink_sums<D>(a, s, b, j0, keys_n, kh) + (int64_t)share * (2 * D) * keys_n;
+    float* to = sink_sums<D>(late, s, b, j0, keys_n, kh) + (int64_t)share * (2 * D) * keys_n;
     float* mine = reinterpret_cast<float*>(wave < 2 ? sq[wave & 1] : sg[wave & 1]);  // QT rows of a tile: D x 32 floats and more
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
@@ -702,9 +710,9 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
     }
     return;
   }
-  const int n = min(32, sinks_with_far_queries(a, s) - jw);
+  const int n = min(32, sinks_with_far_queries(late, s) - jw);
   if (c < n) {  // jag_sinks_kernel writes over what these rows get below
-    float* to = sink_sums<D>(a, s, b, jw, n, kh) + (int64_t)a.sink_shares * (2 * D) * n;
+    float* to = sink_sums<D>(late, s, b, jw, n, kh) + (int64_t)late.sink_shares * (2 * D) * n;
 #pragma unroll
     for (int d = 0; d < DD; ++d)
 #pragma unroll
@@ -714,9 +722,9 @@ __global__ void __launch_bounds__(256, SINK ? 1 : 2) jag_dkv_kernel(JagArgs a, i
       }
   }
   if (jw >= s.nk) return;
-  const int64_t at = ((s.k0 + jw) * a.hk + kh) * D, st = (int64_t)a.hk * D;
-  store_own<DT, D>(dk, a.scale * back, own, a.dk, nullptr, at, st, s.nk - jw);
-  store_own<DT, D>(dv, back_v, own, a.dv, nullptr, at, st, s.nk - jw);
+  const int64_t at = ((s.k0 + jw) * late.hk + kh) * D, st = (int64_t)late.hk * D;
+  store_own<DT, D>(dk, late.scale * back, own, late.dk, nullptr, at, st, s.nk - jw);
+  store_own<DT, D>(dv, back_v, own, late.dv, nullptr, at, st, s.nk - jw);
 }
 
 // Gradients of a block of sinks of a key head, their sums under the window and beyond it: a thread an element at a time, `parts`

@@ -37,15 +37,16 @@ struct JagArgs {
 
 constexpr float kInf = __builtin_inff();
 constexpr float kNoKeys = 3e38f;  // the reference of a row without weights: none passes it
+constexpr float kLargeScore = 0x1p12f;
 constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.44269504088896341f;
 
 // A kernel's arguments, read again: those that its end alone needs else take scalar registers all the way, and others are held in
 // lanes for them.  (JagArgs is every kernel's first argument.)
-typedef const __attribute__((address_space(4))) JagArgs* LateArgs;
-__device__ __forceinline__ LateArgs late_args() {
-  LateArgs p = (LateArgs)__builtin_amdgcn_kernarg_segment_ptr();
+__device__ __forceinline__ const JagArgs& late_args() {
+  typedef const __attribute__((address_space(4))) JagArgs* Constant;
+  Constant p = (Constant)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(p));
-  return p;
+  return *(const JagArgs*)p;
 }
 
 // ---- sequences -------------------------------------------------------------------
