@@ -1206,6 +1206,7 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
     sched_mfma_ds_pipeline<XX * KK, LEAD>();
   };
   // the running maximum, and P from the scores
+  bool large = false;  // scores are multiplied by their scales and rounded, as the reference is
   u32x4_t p[2 * XX], rest[2 * XX];
   auto weights = [&](int t) __attribute__((always_inline)) {
     const int key = real(begin + t * KT);
@@ -1295,6 +1296,15 @@ __global__ void __launch_bounds__(256 * NG, D == 256 ? 1 : 2) kv_attn_many_kerne
       l *= f;
 #pragma unroll
       for (int d = 0; d < DD; ++d) o[d] *= f;
+      if (__any(fabsf(m) > 0x1p12f)) large = true;
+    }
+    if (large) {  // what rounding left of the largest product would count, as 2^32 and more from 2^30 on
+#pragma unroll
+      for (int x = 0; x < 2 * XX; ++x) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[x >> 1][8 * (x & 1) + e] *= sc[x];
+        sc[x] = 1.0f;
+      }
     }
     const float base = m == -kInf ? 0.0f : m;
 #pragma unroll
