@@ -355,9 +355,9 @@ extern "C" int pdm_jagged_attention_fwd(const pdm_jagged_attention_desc* desc, c
   clear_error();
   JagArgs a{};
   if (int e = jag_args(__func__, desc, a)) return e;
-  if (a.q_tokens == 0) return PDM_OK;
+  if (a.q_tokens == 0 && (!err_flag || !a.seqs)) return PDM_OK;
   if (int e = jag_inputs(__func__, a, desc, q, k, v, cu_q, cu_k, bias)) return e;
-  PDM_CHECK_ARG(out, "null out");
+  PDM_CHECK_ARG(out || !a.q_tokens, "null out");
   PDM_CHECK_ARG(!out_rest || bias, "out_rest without a bias");
   PDM_CHECK_ARG(((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_rest)) & 15) == 0, "out and out_rest must be 16-byte aligned");
   PDM_CHECK_ARG(!out_rest || stats, "out_rest without stats");

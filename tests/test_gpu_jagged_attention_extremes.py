@@ -1,4 +1,4 @@
-"""jagged_attention at the ends of its types: scores far beyond any softmax's need."""
+"""jagged_attention at its ends: scores far beyond any softmax's need, spans of a batch without queries."""
 import math
 
 import pytest
@@ -43,3 +43,14 @@ def test_scores_of_the_largest_inputs(pdm, dev, D, dtype, power, span):
             assert ((lse[:, h].detach().cpu().double() - want).abs() <= 4 * 2.0 ** -24 * want.abs()).all()
         want, mag = sum(p.T @ go[:, h] for h in range(2)), sum(p.T @ go[:, h].abs() for h in range(2))
         assert ((dv[:, 0].cpu().double() - want).abs() <= e * mag + HALF[dtype] * want.abs() + 2.0 ** -25).all()
+
+
+def test_spans_of_a_batch_without_queries(pdm, dev):
+    """There is nothing to compute, and spans that do not fit are told all the same."""
+    q, k = torch.zeros(0, 2, 64, dtype=B, device=dev), torch.randn(20, 1, 64, device=dev).to(B)
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    for cu_q, cu_k, bad in (([0, 0, 0], [0, 10, 20], 0), ([0, 0, 0], [0, 10, 21], 1), ([0, 0, 0], [0, 10, 5], 1), ([0, 1, 1], [0, 10, 20], 1), ([0] * 300, [0] * 299 + [21], 1),
+                            ([0] * 300, [0] * 300, 0), ([0], [0], 0)):
+        flag = torch.zeros(1, dtype=torch.int32, device=dev)
+        out = pdm.jagged_attention(q, k, k, t(cu_q), t(cu_k), err_flag=flag)
+        assert out.shape == (0, 2, 64) and flag.item() == bad
