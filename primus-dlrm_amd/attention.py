@@ -70,6 +70,9 @@ def jagged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     key (or only scores of -inf) and rows that no sequence covers are zeros, with lse -inf, and have and give no gradient.
     ``err_flag`` (int32, never cleared) is set where spans decrease or leave the batch; outputs then hold nothing of use.
 
+    Where the bias wants a gradient, weights meet the values in two parts: outputs are nearer to exact ones than without, and not
+    the same bits.  A recomputation that has to give the same bits runs with the same tensors requiring gradients.
+
     Before a backward pass is captured into a HIP graph, let go of eager outputs of the same leaves: torch accumulates their
     gradients on the stream that those were made on, which a capture does not survive."""
     _no_tangent("jagged_attention", q, k, v, bias)

@@ -3,7 +3,8 @@
 // Bound by the bytes of the [heads, span] side and, when small, by launches.  Forward: a thread per column and 4 heads.  Backward:
 // a workgroup per (bucket, head) sums the columns that are its own, in a fixed order and in 64 bits; in large maps one workgroup
 // finds the first and last column of every bucket before (a bucket's columns are neighbours in all but odd maps).  Eight reads of
-// the map are on their way before the first is looked at: 65,536 columns of 64 heads took 80 us instead of 54.
+// the map are on their way before the first is looked at: 65,536 columns of 64 heads in one bucket take 40 us instead of 71 (both
+// launches, back to back), in 320 logarithmic ones 32 either way (13.8 for the ranges, 23.4 for the sums, by themselves).
 #include "pdm_common.h"
 
 namespace pdm {

@@ -8,11 +8,12 @@
 //
 // Weights are rounded to the type of the values for the product, half a step of each, as the outputs are; where the gradient
 // of a bias is wanted (`rest`), which is a sum of many small differences in 32 bits, they go in as two numbers and what the
-// rounding of the outputs left is kept for the backward pass.
+// rounding of the outputs left is kept for the backward pass, with each row's weights in the bias's outer columns (151 -> 158 us
+// for the 8,134 tokens of jagged_backward.hip, 132 -> 144 for its sequences on both sides).
 //
-// Bound by the softmax beside the products: of a dense causal batch of 16,384 tokens heads of 128 reach 1.07 to 1.17 PFLOP/s and
-// heads of 64, with as many exponentials for half the products, 0.87 (a large library product on the same card 1.24).  Under a
-// window of 1,024 the tiles at both of its ends are whole and half used: 8,192 tokens, 32 heads of 128 on 8, 4 sinks: 180 us, 0.72
+// Bound by the softmax beside the products: 16,384 tokens, 16 heads on 8, causal and on both sides: heads of 128 1,082 and 2,135 us, 1.02
+// and 1.03 PFLOP/s; heads of 64, with as many exponentials for half the products, 685 and 1,229 us, 0.80 and 0.89 (a large
+// library product on such a card 1.24).  Under a window of 1,024 the tiles at both of its ends are whole and half used: 8,192 tokens, 32 heads of 128 on 8, 4 sinks: 180 us, 0.72
 // PFLOP/s of what is seen.  128 queries a workgroup: 64 would bring every tile twice as often, and 256 leave half of the CUs idle
 // in ordinary batches; three waves a SIMD for heads of 64, two for 128, whose sums take 64 registers.
 #include "jagged_common.h"

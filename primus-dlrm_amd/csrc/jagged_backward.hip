@@ -4,8 +4,8 @@
 //   dS = P (dP - delta),  dV = P^T dO,  dQ = scale dS K,  dK = scale dS^T Q,  dbias[c] = sum of dS over the pairs of column c.
 // Two kernels compute S and dP again, one by blocks of queries (dQ, delta, the bias's gradient), one by blocks of keys (dK, dV):
 // 7 products where one kernel would need 5 and sums of dQ over its workgroups, by atomics, whose order changes the result, or
-// once more through memory in fp32.  In both a lane holds scores of one column (a
-// query, a key) and passes them on to the next product as the first leaves them.
+// once more through memory in fp32.  In both a lane holds scores of one column (a query, a key) and passes them on to the next
+// product as the first leaves them.
 //
 // P and dS are rounded to the type of the operands for their products; the bias's gradient takes dS in 32 bits.  fp16 would
 // lose small dS (below 2^-14): its dS are multiplied by a power of two that brings the larger of dO and the gradient of lse to
@@ -14,9 +14,9 @@
 // dS of 2^20 times the largest |dO|, for which 64 values of 2^14 would have to point along dO, overflow.)
 //
 // Bound by latency at two waves a SIMD (matrix units 20 to 30 %, vector units 30 to 45, LDS 20 to 40 % of the time busy): 8
-// sequences of 1,001 to 2,777 tokens, 8 heads of 64, both sides: 211 us by queries, of which the bias's gradient takes about
-// half, and 197 by keys (0.55 PFLOP/s); 8,134 tokens, 24 heads of 128 on 6, window 512 with 4 sinks, fp16: 234, 228 and 46 for
-// the sinks.
+// sequences of 1,001 to 2,777 tokens, 8 heads of 64, both sides: 223 us by queries, of which the bias's gradient takes about
+// half (sums of rows for its outer columns 12), and 196 by keys (0.55 PFLOP/s); 8,134 tokens, 24 heads of 128 on 6, window 512 with
+// 4 sinks, fp16: 249, 230 and 46 for the sinks.
 #include <algorithm>
 #include <type_traits>
 
@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   __shared__ float ends[GB ? 8 : 1];
   // Where registers are short three fragments of the queries stay in LDS: the compiler puts what does not fit into scratch memory,
   // whose load in every tile waits for the next tile's to land (fp16, 24 heads of 8,134 tokens under a window of 512: 256 us with
-  // two, 240 with three; a fourth would leave LDS for one workgroup on a CU).
+  // two, 240 with three).  bf16 still has one fragment there; a fourth would leave LDS for one workgroup on a CU.
   constexpr int HOLD = GB && D == 128 ? 3 : 0;
   __shared__ u32x4_t held[HOLD ? 4 * HOLD : 1][HOLD ? 64 : 1];
   __shared__ uint8_t odd_keys[2][KT];

@@ -15,7 +15,9 @@
 // of their outputs goes from 1.7e-3, of the output's own rounding, to 2.1e-3, at 794 us instead of 1,048.  The running sum
 // takes weights before any rounding.
 //
-// Sinks and a bias by distance (EXT) are instances of their own, which leave the plain ones their registers.  Keys between the
+// Sinks and a bias by distance (EXT) are instances of their own, which leave the plain ones their registers and run short of them
+// themselves: 17 to 32 rows of heads of 64 keep 16 in scratch memory, many rows of heads of 128 11 (bf16) and 25 to 28 (fp16), few rows of
+// 128 and 256 two and seven, and many rows of heads of 64 in bf16 two waves a SIMD instead of three.  Keys between the
 // sinks and the window are skipped in whole tiles.  A tile whose distances all have one column reads it once; 16 rows do not feel
 // the bias (64 sequences of 128 to 8,192: 66 us with it, 63 without), 17 to 32 rows of heads of 64 do (256 sequences of 300 to
 // 1,500: 68 and 45: its fragments are read when the tile is there, and do not fit the registers earlier).
