@@ -752,7 +752,8 @@ typedef struct {
  * bias: fp32 [n_q_heads, bias_span].
  * lse: optional fp32 [q_tokens, n_q_heads], log of the sum of exponentials.
  * For the backward pass: stats, fp32 [q_tokens, n_q_heads, 2], and, where the
- * bias's gradient is wanted, out_rest (as out: what its rounding left).  With
+ * bias's gradient is wanted, out_rest (as out: what its rounding left, 16 bits
+ * an element, to be handed to the backward pass as they are).  With
  * out_rest and stats_planes = 2 stats is [2, q_tokens, n_q_heads, 2]: the second
  * plane keeps a row's weights in the bias's last column and before its first,
  * and the gradients of the two outer columns are corrected by them.

@@ -8,7 +8,7 @@
 //
 // Weights are rounded to the type of the values for the product, half a step of each, as the outputs are; where the gradient
 // of a bias is wanted (`rest`), which is a sum of many small differences in 32 bits, they go in as two numbers and what the
-// rounding of the outputs left is kept for the backward pass, with each row's weights in the bias's outer columns (151 -> 158 us
+// rounding of the outputs left is kept for the backward pass (rest2), with each row's weights in the bias's outer columns (151 -> 158 us
 // for the 8,134 tokens of jagged_backward.hip, 132 -> 144 for its sequences on both sides).
 //
 // Bound by the softmax beside the products: 16,384 tokens, 16 heads on 8, causal and on both sides: heads of 128 1,082 and 2,135 us, 1.02

@@ -142,14 +142,14 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
   const bool one_key = mine_seen.n + min(mine_seen.first, mine_seen.lo) == 1;
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) {
-    u32x4_t o2 = {0, 0, 0, 0};
-    if (GB) o2 = Tile<D>::rows(own2, row_at, 0, kk);
+    u32x4_t o = {0, 0, 0, 0}, o2 = {0, 0, 0, 0};
+    if (GB) o = Tile<D>::rows(own, row_at, 0, kk), o2 = Tile<D>::rows(own2, row_at, 0, kk);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float lo = lo_of<DT>(g[kk][e]), hi = hi_of<DT>(g[kk][e]);
       if (GB && !one_key) {
-        delta = __builtin_fmaf(lo, lo_of<DT>(o2[e]), delta);
-        delta = __builtin_fmaf(hi, hi_of<DT>(o2[e]), delta);
+        delta = __builtin_fmaf(lo, rest_lo<DT>(o[e], o2[e]), delta);
+        delta = __builtin_fmaf(hi, rest_hi<DT>(o[e], o2[e]), delta);
       }
       if (DT == PDM_F16) most = fmaxf(most, fmaxf(fabsf(lo) < kInf ? fabsf(lo) : 0.0f, fabsf(hi) < kInf ? fabsf(hi) : 0.0f));
     }
@@ -361,8 +361,8 @@ __global__ void __launch_bounds__(256, 2) jag_dq_kernel(JagArgs a, int64_t units
     }
     // A row's dS add up to the gradient of its lse.  What they are off by is delta's error, which each has by its weight: little beside
     // its own size, but a column of nearly all weights of every row has a sum that cancels to far less than its terms.  So the two
-    // columns that stand for many distances are put right (a bias of two columns, 980 tokens: off by 1.2e-5 to 8.6e-5 of the
-    // gradient, now by 1.5e-6 to 1.2e-5).
+    // columns that stand for many distances are put right (a bias of two columns, 980 tokens, and this and what rest2 keeps left
+    // out: off by 1.2e-5 to 8.6e-5 of the gradient, with both by 9e-7 to 2.8e-6).
     // A bias of one column has all of a row, whose sum is known.
     const float sum_of_row = all + __shfl_xor(all, 32);
     const JagArgs& late = late_args();

@@ -15,7 +15,7 @@ struct JagArgs {
   const int32_t *cu_q, *cu_k;
   const float* bias;                 // [hq, bias_last + 1] or null
   int32_t* err;
-  void *out, *rest;                  // forward; rest: what rounding out left (may be null)
+  void *out, *rest;                  // forward; rest: what rounding out left, see rest2 (may be null)
   float *lse, *stats;                // stats: a row's reference (log2) and 1 / the sum of its weights
   float* outer;                      // a row's weights of the bias's last column and of what lies before its first, or null
   const void* dout;                  // backward
@@ -190,6 +190,27 @@ template <int DT>
 __device__ __forceinline__ uint32_t left2(float lo, float hi, uint32_t w) {  // what rounding the pair to w left
   return pack2<DT>(lo - lo_of<DT>(w), hi - hi_of<DT>(w));
 }
+// What rounding a pair to w left, in 16 bits an element: fp16's remainders; of bf16 the lower halves of the fp32 bits, which lose
+// nothing (a remainder in bf16 leaves 2^-18, which would be most of the error of the bias's gradient).  Of halves of 0x8000 w does not
+// tell which way they were rounded: these are moved by one.
+template <int DT>
+__device__ __forceinline__ uint32_t rest2(float lo, float hi, uint32_t w) {
+  if constexpr (DT == PDM_F16) return left2<DT>(lo, hi, w);
+  auto half = [](uint32_t bits) {
+    const uint32_t x = bits & 0xffffu;
+    return x == 0x8000u ? 0x7fffu + 2 * (bits >> 16 & 1) : x;
+  };
+  return half(__float_as_uint(lo)) | half(__float_as_uint(hi)) << 16;
+}
+// The remainder of the lower (upper) element of w.
+template <int DT>
+__device__ __forceinline__ float rest_lo(uint32_t w, uint32_t rest) {
+  if constexpr (DT == PDM_F16) return lo_of<DT>(rest);
+  const uint32_t r = rest & 0xffffu;
+  return __uint_as_float(((w << 16) - ((r >> 15) << 16)) | r) - lo_of<DT>(w);
+}
+template <int DT>
+__device__ __forceinline__ float rest_hi(uint32_t w, uint32_t rest) { return rest_lo<DT>(w >> 16, rest >> 16); }
 // Bits 15 and 31: the element there is infinite or NaN.
 template <int DT>
 __device__ __forceinline__ uint32_t odd2(uint32_t w) {
@@ -396,7 +417,7 @@ __device__ __forceinline__ void store_own(const f32x16_t* acc, float f, char* ti
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           w[i] = pack2<DT>(y[2 * i], y[2 * i + 1]);
-          if (pass) w[i] = left2<DT>(y[2 * i], y[2 * i + 1], w[i]);
+          if (pass) w[i] = rest2<DT>(y[2 * i], y[2 * i + 1], w[i]);
         }
         *reinterpret_cast<u32x2_t*>(tile + c * Tile<D>::RS + 16 * ((4 * d + e / 4) ^ Tile<D>::turn(c)) + 8 * h) = w;
       }

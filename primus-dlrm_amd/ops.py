@@ -1323,7 +1323,7 @@ def jagged_attention_raw(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_s
                          err_flag: Optional[torch.Tensor] = None):
     """Launches pdm_jagged_attention_fwd on q [T, Hq, D], k and v [S, Hk, D]: (out, lse, stats, rest), None where not wanted.
     ``keep``: what a backward pass needs, 1 the rows' statistics, 2 what the rounding of out left too (for the bias's gradient), and
-    the weights of its outer columns (a second plane of the statistics)."""
+    the weights of its outer columns (a second plane of the statistics).  ``rest`` holds bits, int16, for the backward pass."""
     _check_err_flag(err_flag)
     index = _gpu_index(q, k, v, cu_seqlens, cu_seqlens_k, bias, err_flag)
     q, k, v = _even_heads(q), _even_heads(k), _even_heads(v)
@@ -1335,7 +1335,7 @@ def jagged_attention_raw(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_s
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((T, hq), dtype=torch.float32, device=q.device) if return_lse else None
     stats = torch.empty((planes, T, hq, 2), dtype=torch.float32, device=q.device) if keep else None
-    rest = torch.empty_like(out) if planes > 1 else None
+    rest = torch.empty(out.shape, dtype=torch.int16, device=q.device) if planes > 1 else None
     lib = L.lib()
     ws_bytes = int(lib.pdm_jagged_attention_workspace_size(ctypes.byref(desc)))
     if ws_bytes < 0:
@@ -1388,7 +1388,7 @@ def jagged_attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_se
     out, lse, stats, rest = jagged_attention_raw(q, k, v, cu_seqlens, cu_seqlens_k, bias, scale, causal, window, sinks,
                                                  bias_start, True, keep)
     return (out, lse, q.new_empty(0, dtype=torch.float32) if stats is None else stats,
-            q.new_empty(0) if rest is None else rest)
+            q.new_empty(0, dtype=torch.int16) if rest is None else rest)
 
 
 @jagged_attention_op.register_fake
@@ -1396,7 +1396,7 @@ def _(q, k, v, cu_seqlens, cu_seqlens_k, bias, scale, causal, window, sinks, bia
     T, hq, _ = q.shape
     return (q.new_empty(q.shape), q.new_empty((T, hq), dtype=torch.float32),
             q.new_empty((2 if keep > 1 and bias is not None else 1, T, hq, 2) if keep else (0,), dtype=torch.float32),
-            q.new_empty(q.shape if keep > 1 and bias is not None else (0,)))
+            q.new_empty(q.shape if keep > 1 and bias is not None else (0,), dtype=torch.int16))
 
 
 @torch.library.custom_op("pdm::jagged_attention_backward", mutates_args=())

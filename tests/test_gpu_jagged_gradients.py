@@ -240,6 +240,28 @@ def test_columns_of_nearly_all_weights(pdm, dev, D, dtype, span, start, mask, gl
     assert rms([e * e for e in errors]) <= 2 * 2.0 ** -25 * rms(sizes)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,span", [(100, 128), (500, 128), (300, 400)])
+def test_precision_of_the_bias_gradient(pdm, dev, D, n, span):
+    """What is left of delta's error in bf16 is that of weights in two parts, outputs being kept whole.  The second part is off by half
+    a step of bf16 of the first's error, which lies anywhere in half a step: 2^-19.6 of a weight as a root mean square (2^-18 at most).
+    A row's delta is off by the mean of dP that these make, and a column by the rows' by its weights.  Beside it scores and sums of
+    fp32, 2^-22 of the result."""
+    c = Case([n], [n], 8, 8, D, B, span, seed=n)
+    db = c.grads(pdm, dev)[1][3].cpu().double()
+    w = c.want(True)
+    i, j = torch.arange(n)[:, None], torch.arange(n)[None]
+    col = (i - j).clamp(0, span - 1)
+    square = 0.0
+    for h in range(8):
+        q, k, v, go = (t[:, h].double() for t in (c.q, c.k, c.v, c.go))
+        p = torch.softmax((q @ k.T * D ** -0.5 + c.bias[h].double()[col]).masked_fill(j > i, -math.inf), -1)
+        of_row = (p * (go @ v.T)).square().sum(-1, keepdim=True)
+        in_column = torch.zeros(n, span, dtype=torch.float64).scatter_add_(1, col, p)
+        square += float((in_column.square() * of_row).sum())
+    assert float((db - w.dbias).norm()) < 2.0 ** -19.6 * math.sqrt(square) + 2.0 ** -22 * float(w.dbias.norm())
+
+
 @pytest.mark.parametrize("D,hk,group,dtype", KINDS)
 def test_a_bias_of_one_column(pdm, dev, D, hk, group, dtype):
     """It moves all scores of a row alike: its gradient is that of the lse, of the rows that see a key."""
@@ -265,7 +287,7 @@ def test_one_plane_of_statistics(pdm, dev):
     args = (0.125, True, 0, 0, 0)
     out, _, stats, rest = ops.jagged_attention_raw(q, k, v, *cu, bias, *args, keep=2)
     assert stats.shape == (2, 110, 4, 2)
-    out1, rest1, stats1 = torch.empty_like(out), torch.empty_like(out), torch.full((2, 110, 4, 2), 7.0, device=dev)
+    out1, rest1, stats1 = torch.empty_like(out), torch.empty_like(rest), torch.full((2, 110, 4, 2), 7.0, device=dev)
     desc = ops._jagged_desc(q, k, v, *cu, bias, *args, 1)
     L.check(L.lib().pdm_jagged_attention_fwd(ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), cu[0].data_ptr(), cu[1].data_ptr(),
                                              bias.data_ptr(), out1.data_ptr(), rest1.data_ptr(), None, stats1.data_ptr(), None, 0, None,
