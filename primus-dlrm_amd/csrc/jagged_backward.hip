@@ -434,9 +434,10 @@ __global__ void __launch_bounds__(1024) jag_dbias_kernel(JagArgs a) {
 // jag_sinks_kernel joins and rounds.
 //
 // Only a sequence longer than the window has such queries, and only for its first nk - window keys.  The host does not know the
-// lengths: blocks are listed, and have rows for their sums, by sequence (sink_cell 0), or, where that is less, by cells of window + 1
-// keys of the batch.  A sequence of nk > window keys from k0 on has the nk / (window + 1) cells from number k0 / (window + 1) on
-// to itself, and its sums fit into min(sinks, window + 1) rows of each.  (16,384 sequences of 100 tokens, 8 key heads of 128, a
+// lengths: blocks are listed (sink_list), and have rows for their sums (sink_cell), by sequence (0), or by cells of window + 1 keys of
+// the batch, either where it is less.  A sequence of nk > window keys from k0 on has the nk / (window + 1) cells from number
+// k0 / (window + 1) on to itself, and its sums fit into min(sinks, window + 1) rows of each.  (1,000 sequences of 100 tokens, a window
+// of 1 with 200 sinks, listed by cells: the pass took 4,970 us instead of 3,058.  16,384 sequences of 100 tokens, 8 key heads of 128, a
 // window of 1,024 with 4 sinks: 0.1 GB and not 8.6.)
 __device__ __forceinline__ int sinks_with_far_queries(const JagArgs& a, const JagSeq& s) {
   return a.sink_blocks ? max(0, min(a.sinks, s.nk - a.window)) : 0;
@@ -446,9 +447,9 @@ __device__ __forceinline__ int sinks_with_far_queries(const JagArgs& a, const Ja
 __device__ __forceinline__ bool sink_block(const JagArgs& a, int64_t x, JagSeq& s, int& b, int& j0, int& n) {
   int64_t block = x % a.sink_blocks;
   x /= a.sink_blocks;
-  b = a.sink_cell ? find_sequence(a.seqs, (x + 1) * a.sink_cell - 1, [&](int i) { return (int64_t)a.cu_k[i]; }) : (int)x;
+  b = a.sink_list ? find_sequence(a.seqs, (x + 1) * a.sink_list - 1, [&](int i) { return (int64_t)a.cu_k[i]; }) : (int)x;
   if (!jag_seq(a, b, s)) return false;
-  if (a.sink_cell) block += (x - s.k0 / a.sink_cell) * a.sink_blocks;
+  if (a.sink_list) block += (x - s.k0 / a.sink_list) * a.sink_blocks;
   const int rows = sinks_with_far_queries(a, s);
   if (block < 0 || block * 32 >= rows) return false;
   j0 = (int)block * 32, n = min(32, rows - j0);
@@ -758,14 +759,16 @@ int64_t part_cols(const JagArgs& a) {
 
 // The list of blocks of 32 sinks (jag_dkv_kernel), and the shares that the queries beyond the window are dealt to: about 1,024
 // workgroups, each of 8 tiles and more on average.
-int64_t sink_lists(const JagArgs& a) { return a.sink_cell ? a.k_tokens / a.sink_cell : a.seqs; }
+int64_t sink_lists(const JagArgs& a) { return a.sink_list ? a.k_tokens / a.sink_list : a.seqs; }
 void sinks_of(JagArgs& a) {
   a.sink_blocks = 0;
   if (!a.seqs || !a.q_tokens || !a.sinks) return;
   const int cell = a.window + 1, rows = a.sinks < cell ? a.sinks : cell;
-  const bool cells = a.k_tokens / cell * rows < (int64_t)a.seqs * a.sinks;
-  a.sink_cell = cells ? cell : 0, a.sink_rows = cells ? rows : a.sinks;
-  const int64_t lists = sink_lists(a), blocks = (a.sink_rows + 31) / 32, units = lists * blocks * a.hk;
+  const int64_t cells = a.k_tokens / cell;
+  const bool fewer_rows = cells * rows < (int64_t)a.seqs * a.sinks, fewer_blocks = cells * ((rows + 31) / 32) < (int64_t)a.seqs * ((a.sinks + 31) / 32);
+  a.sink_cell = fewer_rows ? cell : 0, a.sink_rows = fewer_rows ? rows : a.sinks;
+  a.sink_list = fewer_blocks ? cell : 0;
+  const int64_t lists = sink_lists(a), blocks = ((fewer_blocks ? rows : a.sinks) + 31) / 32, units = lists * blocks * a.hk;
   const int64_t most = a.group * (a.q_tokens / (lists < a.seqs ? lists : a.seqs)) / (8 * 128);
   int64_t shares = 1024 / units;
   shares = shares < most ? shares : most;
@@ -786,7 +789,7 @@ Space space_of(JagArgs& a, int dtype, int head_dim, bool gb) {
   s.range = s.expo + round256(dtype == PDM_F16 ? a.items * 16 * a.hq : 0);
   s.part = s.range + round256(gb ? a.items * 8 : 0);
   s.sinks = s.part + round256(gb ? a.items * a.hq * (part_cols(a) + 2) * 4 : 0);
-  s.total = s.sinks + (a.sink_blocks ? sink_lists(a) * a.sink_rows * a.hk * (a.sink_shares + 1) * 2 * head_dim * 4 : 0);
+  s.total = s.sinks + (a.sink_blocks ? (a.sink_cell ? a.k_tokens / a.sink_cell : a.seqs) * a.sink_rows * a.hk * (a.sink_shares + 1) * 2 * head_dim * 4 : 0);
   return s;
 }
 

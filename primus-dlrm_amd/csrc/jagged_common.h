@@ -27,7 +27,7 @@ struct JagArgs {
   float* part;                       // partial gradients of the bias, [items of 128 rows, hq, part_stride]
   int32_t* part_range;               // [items, 2]: the distances that a partial gradient holds
   float* sink_part;                  // sums of the gradients of sinks, see jag_dkv_kernel
-  int32_t sink_cell, sink_rows, sink_blocks, sink_shares;
+  int32_t sink_cell, sink_rows, sink_list, sink_blocks, sink_shares;
   int64_t part_stride;
   int64_t q_tokens, k_tokens, items;
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;

@@ -147,7 +147,7 @@ def test_small_weights_in_half_precision(pdm, dev, D, gap, mask):
 # Queries beyond the window are those of sequences longer than it, and so are the sums kept for them.
 
 @pytest.mark.parametrize("D,hk,group,dtype", KINDS)
-@pytest.mark.parametrize("window,sinks", [(30, 4), (7, 33), (1, 1), (5, 200), (40, 41), (100, 3), (33, 32)])
+@pytest.mark.parametrize("window,sinks", [(30, 4), (7, 33), (1, 1), (1, 200), (5, 200), (40, 41), (100, 3), (33, 32)])
 def test_sinks_of_many_sequences(pdm, dev, D, hk, group, dtype, window, sinks):
     """Mostly short ones, some of about the window's length, a few long; empty ones; with queries for all of the keys or for some."""
     g = torch.Generator().manual_seed(window)
